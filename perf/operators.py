@@ -179,6 +179,13 @@ def prepare(case, seed):
         form=case["format"], page=page, k_pages=kc, v_pages=vc, k_scale=ks, v_scale=vs, table=table,
         lengths=torch.tensor(total, dtype=torch.int32, device=DEVICE), reads=_starts(total), read_rows=sum(total),
     )
+    if own:
+        # The handles that a serving program keeps: checked pointers and sizes of its pool and of a batch.
+        from pir2_b200 import kv_cache
+
+        state["pages"] = kv_cache.KVPages(kc, vc, ks, vs)
+        state["batch"] = kv_cache.Sequences(state["starts"], state["lengths"], table)
+        state["whole"] = kv_cache.Sequences(state["reads"], state["lengths"], table)
     return state
 
 
@@ -289,12 +296,11 @@ def run(state):
 
     if s["op"] == "prompt":
         return ops.prompt_attention(s["q"], s["k"], s["v"], s["starts"])
-    pages = (s["k_pages"], s["v_pages"], s["k_scale"], s["v_scale"])
     if s["op"] == "cache":
-        ops.cache_write(s["k"], s["v"], pages, s["table"], s["starts"], s["lengths"])
-        k, v = ops.cache_read(pages, s["table"], s["reads"], s["read_rows"])
+        ops.cache_write(s["k"], s["v"], s["pages"], s["batch"])
+        k, v = ops.cache_read(s["pages"], s["whole"], s["read_rows"])
         return _cache_outputs(s, k, v)
-    return ops.cache_attention(s["q"], pages, s["table"], s["starts"], s["lengths"])
+    return ops.cache_attention(s["q"], s["pages"], s["batch"])
 
 
 def work(case):
