@@ -397,6 +397,85 @@ int pir2b_attention_causal(const void *q, const void *k, const void *v, int64_t 
                            int64_t tokens, int hq, int hk, int head_dim, float scale, void *out,
                            int64_t ldo, void *stream);
 
+/* ---- ragged batches and the paged K/V cache of the text layers ----------
+ *
+ * The reference prefills one observation per robot and keeps no K/V cache
+ * (coexecution/optimization/groot/vlm.py:312-313 checks for transformers'
+ * "sdpa" attention); the entry points below serve several robots whose
+ * prompts differ in length, and text decoding after them.
+ *
+ * A batch is packed: the rows of sequence b are starts[b] .. starts[b+1]-1 of
+ * the [rows, heads, head_dim] tensors (starts: int32 [batch + 1] on the
+ * device, not decreasing), with no padding rows.  Rows of no sequence are
+ * left alone.  q, k, v are bf16 views with unit stride along head_dim and any
+ * row and head strides that are multiples of 8 elements (slices of a merged
+ * projection, or [heads, rows, head_dim] storage), 16-byte aligned.
+ * head_dim is 64 or 128; query head h reads kv head h / (hq / hk). */
+
+/* Cache formats: bf16 rows, or int8 / E4M3 codes with one fp32 scale per
+ * token and head, quantised as the activation packs (symmetric-row-v1,
+ * coexecution/kernels/ampere_ada/integer.py): s = max|v| * f32(1/L), 1 for a
+ * row of zeros, L = 127 / 448, code = v / s rounded to nearest even and
+ * clamped.  The maximum is over the finite values; an infinity becomes the
+ * largest code, a NaN code 0 (int8) or the E4M3 NaN. */
+#define PIR2B_CACHE_BF16 16
+#define PIR2B_CACHE_INT8 8
+#define PIR2B_CACHE_E4M3 9
+
+/* A pool of pages, each holding `page_size` (16, 32, 64 or 128) consecutive
+ * tokens of one sequence: k, v [pages, kv_heads, page_size, head_dim], 16-byte
+ * aligned; scales fp32 [pages, kv_heads, page_size] (null with bf16).  The
+ * page strides are in elements (multiples of 16 for k and v). */
+typedef struct pir2b_kv_pages {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int64_t k_page_stride, v_page_stride;
+  int64_t k_scale_page_stride, v_scale_page_stride;
+  int32_t pages, page_size, kv_heads, head_dim, format;
+} pir2b_kv_pages;
+
+/* The sequences of a batch: packed rows (starts), tokens each has after them
+ * (lengths, int32 [batch]; the rows are its last tokens) and the pages of its
+ * positions (table int32 [batch, table_width]: position p is in page
+ * table[b, p / page_size]).  All on the device; every index is checked there:
+ * a position outside the table or a page outside the pool is neither read nor
+ * written and sets the status word to PIR2B_STATUS_BAD_PAGE. */
+typedef struct pir2b_sequences {
+  const int32_t *starts, *lengths, *table;
+  int64_t table_stride;
+  int32_t batch, table_width;
+} pir2b_sequences;
+
+#define PIR2B_STATUS_BAD_PAGE 0x201
+
+/* Causal grouped-query attention over packed prompts: row i of a prompt sees
+ * its rows 0 .. i.  out: bf16 [rows, hq * head_dim], row stride ldo. */
+int pir2b_prompt_attention(const void *q, int64_t q_row, int64_t q_head, const void *k,
+                           int64_t k_row, int64_t k_head, const void *v, int64_t v_row,
+                           int64_t v_head, const int32_t *starts, int64_t batch, int64_t rows,
+                           int hq, int hk, int head_dim, float scale, void *out, int64_t ldo,
+                           void *stream);
+
+/* Writes the rows k, v [rows, kv_heads, head_dim] of each sequence to its
+ * last positions in the pages. */
+int pir2b_cache_write(const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row,
+                      int64_t v_head, int64_t rows, const pir2b_kv_pages *pages,
+                      const pir2b_sequences *sequences, void *stream);
+
+/* Reads positions 0, 1, ... of each sequence back as bf16(code * scale), into
+ * contiguous k_out, v_out [rows, kv_heads, head_dim]: starts gives the packed
+ * rows (lengths is not used). */
+int pir2b_cache_read(const pir2b_kv_pages *pages, const pir2b_sequences *sequences, int64_t rows,
+                     void *k_out, void *v_out, void *stream);
+
+/* Attention of each sequence's last rows over its pages: row i of n new rows
+ * of a sequence of L tokens sees positions 0 .. L - n + i (none when that is
+ * negative: zeros).  8-bit caches enter the products as their codes, which
+ * bf16 holds exactly; the scales multiply scores and weights in fp32. */
+int pir2b_cache_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int hq,
+                          const pir2b_kv_pages *pages, const pir2b_sequences *sequences,
+                          float scale, void *out, int64_t ldo, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,10 +22,33 @@ OUT_INT8, OUT_INT4, OUT_NVFP4 = 8, 4, 16
 OUT_FP8_VALUES = 32   # FP8 producers' first pass: bf16 values + fp32 row maxima
 STATUS_TIMEOUT_PROBE = 0x105   # device status word left by pir2b_wait_probe
 
+STATUS_BAD_PAGE = 0x201        # device status word left by an index outside a K/V pool or table
+CACHE_BF16, CACHE_INT8, CACHE_E4M3 = 16, 8, 9
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _F = ctypes.c_float
+
+
+class KVPagesStruct(ctypes.Structure):
+    """pir2b_kv_pages."""
+
+    _fields_ = [
+        ("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P),
+        ("k_page_stride", _I64), ("v_page_stride", _I64),
+        ("k_scale_page_stride", _I64), ("v_scale_page_stride", _I64),
+        ("pages", _I), ("page_size", _I), ("kv_heads", _I), ("head_dim", _I), ("format", _I),
+    ]
+
+
+class SequencesStruct(ctypes.Structure):
+    """pir2b_sequences."""
+
+    _fields_ = [
+        ("starts", _P), ("lengths", _P), ("table", _P), ("table_stride", _I64), ("batch", _I), ("table_width", _I),
+    ]
+
 
 # Exported entry points and their argument types, in header order.
 SIGNATURES = {
@@ -58,6 +81,12 @@ SIGNATURES = {
     "pir2b_attention_rows": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I, _I, _F, _P],
     "pir2b_unpack_int4": [_P, _I64, _I64, _P, _P],
     "pir2b_attention_causal": [_P, _P, _P, _I64, _I64, _I, _I, _I, _F, _P, _I64, _P],
+    "pir2b_prompt_attention": [
+        _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _I, _I, _F, _P, _I64, _P,
+    ],
+    "pir2b_cache_write": [_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P],
+    "pir2b_cache_read": [_P, _P, _I64, _P, _P, _P],
+    "pir2b_cache_attention": [_P, _I64, _I64, _I64, _I, _P, _P, _F, _P, _I64, _P],
     "pir2b_qk_norm_rope": [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I, _I, _I, _F, _P, _P, _P, _P],
 }
 

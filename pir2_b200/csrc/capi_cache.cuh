@@ -1,0 +1,271 @@
+// C ABI of the ragged-batch operators (packed prompts, paged K/V cache):
+// argument checks and launches.
+#pragma once
+#include "attention_ragged.cuh"
+#include "capi.cuh"
+#include "kv_cache.cuh"
+
+namespace pir2b {
+
+// Rows view [rows, heads, d] of bf16: strides in elements.
+static int check_view(const char *what, const void *p, int64_t row, int64_t head) {
+  if (p == nullptr)
+    return fail(PIR2B_EINVAL, "%s must be non-null", what);
+  if (!aligned(p, 16) || row % 8 != 0 || head % 8 != 0 || row < 0 || head < 0)
+    return fail(PIR2B_EALIGN, "%s must be 16-byte aligned with row and head strides that are multiples of 8", what);
+  return PIR2B_OK;
+}
+
+static int check_heads(const char *what, int hq, int hk, int d) {
+  if (hk < 1 || hq < 1 || hq % hk != 0 || hq > 1024 || (d != 64 && d != 128))
+    return fail(PIR2B_EINVAL, "%s: hq must be a multiple of hk (at most 1024 heads), head_dim 64 or 128", what);
+  return PIR2B_OK;
+}
+
+static int check_out(const char *what, const void *out, int64_t ldo, int64_t width) {
+  if (out == nullptr || ldo < width)
+    return fail(PIR2B_EINVAL, "%s: output missing or its row stride below its width", what);
+  if (!aligned(out, 16) || ldo % 8 != 0)
+    return fail(PIR2B_EALIGN, "%s: output must be 16-byte aligned with a row stride that is a multiple of 8", what);
+  return PIR2B_OK;
+}
+
+static int check_sequences(const char *what, const pir2b_sequences *s, int64_t rows, bool lengths) {
+  if (s == nullptr || s->starts == nullptr || s->batch < 1 || s->table_width < 0 || s->table_stride < s->table_width ||
+      (lengths && s->lengths == nullptr) || (s->table_width > 0 && s->table == nullptr))
+    return fail(PIR2B_EINVAL, "%s: sequences need starts, lengths, a table and batch >= 1", what);
+  if (rows < 0 || rows > 0x7fffffff)
+    return fail(PIR2B_EINVAL, "%s: rows out of range", what);
+  return PIR2B_OK;
+}
+
+static int make_pages(const char *what, const pir2b_kv_pages *p, const pir2b_sequences *s, CachePages *out) {
+  if (p == nullptr || p->k == nullptr || p->v == nullptr || p->pages < 1 || p->kv_heads < 1 || p->kv_heads > 1024)
+    return fail(PIR2B_EINVAL, "%s: a pool needs k, v, pages >= 1 and 1 to 1024 kv heads", what);
+  if (p->page_size != 16 && p->page_size != 32 && p->page_size != 64 && p->page_size != 128)
+    return fail(PIR2B_EINVAL, "%s: page_size must be 16, 32, 64 or 128", what);
+  if (p->head_dim != 64 && p->head_dim != 128)
+    return fail(PIR2B_EINVAL, "%s: head_dim must be 64 or 128", what);
+  if (p->format != PIR2B_CACHE_BF16 && p->format != PIR2B_CACHE_INT8 && p->format != PIR2B_CACHE_E4M3)
+    return fail(PIR2B_EINVAL, "%s: unknown cache format %d", what, p->format);
+  const int64_t tokens = int64_t(p->kv_heads) * p->page_size;
+  if (p->k_page_stride < tokens * p->head_dim || p->v_page_stride < tokens * p->head_dim)
+    return fail(PIR2B_EINVAL, "%s: page strides below a page's size", what);
+  if (!aligned(p->k, 16) || !aligned(p->v, 16) || p->k_page_stride % 16 != 0 || p->v_page_stride % 16 != 0)
+    return fail(PIR2B_EALIGN, "%s: pages must be 16-byte aligned", what);
+  if (p->format != PIR2B_CACHE_BF16 &&
+      (p->k_scale == nullptr || p->v_scale == nullptr || !aligned(p->k_scale, 16) || !aligned(p->v_scale, 16) ||
+       p->k_scale_page_stride < tokens || p->v_scale_page_stride < tokens || p->k_scale_page_stride % 4 != 0 ||
+       p->v_scale_page_stride % 4 != 0))
+    return fail(PIR2B_EINVAL, "%s: 8-bit pages need 16-byte aligned fp32 scales", what);
+  out->k = p->k;
+  out->v = p->v;
+  out->ks = p->k_scale;
+  out->vs = p->v_scale;
+  out->k_page = p->k_page_stride;
+  out->v_page = p->v_page_stride;
+  out->ks_page = p->k_scale_page_stride;
+  out->vs_page = p->v_scale_page_stride;
+  out->table = s->table;
+  out->ldt = s->table_stride;
+  out->width = s->table_width;
+  out->pages = p->pages;
+  out->shift = p->page_size == 16 ? 4 : p->page_size == 32 ? 5 : p->page_size == 64 ? 6 : 7;
+  out->hk = p->kv_heads;
+  return PIR2B_OK;
+}
+
+// A launch that may start while its predecessor drains (every kernel here
+// begins with griddepcontrol.wait).
+template <typename Args>
+static int launch_cache(const char *what, void (*kernel)(Args), int64_t grid, int threads, size_t smem,
+                        const Args &a, void *stream) {
+  if (grid > 0x7fffffff)
+    return fail(PIR2B_EINVAL, "%s: too many rows", what);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(grid), 1, 1);
+  cfg.blockDim = dim3(unsigned(threads), 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, a), what);
+}
+
+template <int kFormat>
+static int launch_rows(bool write, int d, const CacheRowsArgs &a, void *stream) {
+  const int64_t grid = (a.rows * 2 * a.c.hk * (d / 8) + kCacheThreads - 1) / kCacheThreads;
+  if (write)
+    return launch_cache("cache_write launch", d == 64 ? cache_write_kernel<kFormat, 64> : cache_write_kernel<kFormat, 128>,
+                        grid, kCacheThreads, 0, a, stream);
+  return launch_cache("cache_read launch", d == 64 ? cache_read_kernel<kFormat, 64> : cache_read_kernel<kFormat, 128>,
+                      grid, kCacheThreads, 0, a, stream);
+}
+
+static int launch_rows(bool write, int format, int d, const CacheRowsArgs &a, void *stream) {
+  switch (format) {
+  case kCacheInt8: return launch_rows<kCacheInt8>(write, d, a, stream);
+  case kCacheE4m3: return launch_rows<kCacheE4m3>(write, d, a, stream);
+  default: return launch_rows<kCacheBf16>(write, d, a, stream);
+  }
+}
+
+template <int kSource>
+static int launch_ragged(const char *what, int d, const RaggedArgs &a, void *stream) {
+  return launch_cache(what, d == 64 ? ragged_simple_kernel<kSource, 64> : ragged_simple_kernel<kSource, 128>,
+                      (a.rows * a.hq + 3) / 4, 128, 0, a, stream);
+}
+
+} // namespace pir2b
+
+using namespace pir2b;
+
+extern "C" {
+
+int pir2b_prompt_attention(const void *q, int64_t q_row, int64_t q_head, const void *k,
+                           int64_t k_row, int64_t k_head, const void *v, int64_t v_row,
+                           int64_t v_head, const int32_t *starts, int64_t batch, int64_t rows,
+                           int hq, int hk, int head_dim, float scale, void *out, int64_t ldo,
+                           void *stream) {
+  const char *what = "prompt_attention";
+  if (int r = check_heads(what, hq, hk, head_dim))
+    return r;
+  if (rows < 0 || rows > 0x7fffffff || batch < 1 || batch > 0x7fffffff || starts == nullptr)
+    return fail(PIR2B_EINVAL, "prompt_attention: need starts, batch >= 1 and rows >= 0");
+  if (!(scale > 0.f) || !(scale < 3.0e38f))
+    return fail(PIR2B_EINVAL, "prompt_attention: scale must be positive and finite");
+  if (rows == 0)
+    return PIR2B_OK;
+  if (int r = check_view("prompt_attention q", q, q_row, q_head))
+    return r;
+  if (int r = check_view("prompt_attention k", k, k_row, k_head))
+    return r;
+  if (int r = check_view("prompt_attention v", v, v_row, v_head))
+    return r;
+  if (int r = check_out(what, out, ldo, int64_t(hq) * head_dim))
+    return r;
+  DeviceInfo *dev = nullptr;
+  if (int r = device_info(&dev))
+    return r;
+  RaggedArgs a = {};
+  a.q = static_cast<const __nv_bfloat16 *>(q);
+  a.q_row = q_row;
+  a.q_head = q_head;
+  a.k = static_cast<const __nv_bfloat16 *>(k);
+  a.k_row = k_row;
+  a.k_head = k_head;
+  a.v = static_cast<const __nv_bfloat16 *>(v);
+  a.v_row = v_row;
+  a.v_head = v_head;
+  a.starts = starts;
+  a.out = static_cast<__nv_bfloat16 *>(out);
+  a.ldo = ldo;
+  a.rows = rows;
+  a.batch = int(batch);
+  a.hq = hq;
+  a.hk = hk;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  return launch_ragged<kSourceRows>("prompt_attention launch", head_dim, a, stream);
+}
+
+int pir2b_cache_write(const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row,
+                      int64_t v_head, int64_t rows, const pir2b_kv_pages *pages,
+                      const pir2b_sequences *sequences, void *stream) {
+  const char *what = "cache_write";
+  CacheRowsArgs a = {};
+  if (int r = check_sequences(what, sequences, rows, true))
+    return r;
+  if (int r = make_pages(what, pages, sequences, &a.c))
+    return r;
+  if (rows == 0)
+    return PIR2B_OK;
+  if (int r = check_view("cache_write k", k, k_row, k_head))
+    return r;
+  if (int r = check_view("cache_write v", v, v_row, v_head))
+    return r;
+  DeviceInfo *dev = nullptr;
+  if (int r = device_info(&dev))
+    return r;
+  a.k = static_cast<const __nv_bfloat16 *>(k);
+  a.v = static_cast<const __nv_bfloat16 *>(v);
+  a.k_row = k_row;
+  a.k_head = k_head;
+  a.v_row = v_row;
+  a.v_head = v_head;
+  a.starts = sequences->starts;
+  a.lengths = sequences->lengths;
+  a.batch = sequences->batch;
+  a.rows = rows;
+  return launch_rows(true, pages->format, pages->head_dim, a, stream);
+}
+
+int pir2b_cache_read(const pir2b_kv_pages *pages, const pir2b_sequences *sequences, int64_t rows,
+                     void *k_out, void *v_out, void *stream) {
+  const char *what = "cache_read";
+  CacheRowsArgs a = {};
+  if (int r = check_sequences(what, sequences, rows, false))
+    return r;
+  if (int r = make_pages(what, pages, sequences, &a.c))
+    return r;
+  if (rows == 0)
+    return PIR2B_OK;
+  if (k_out == nullptr || v_out == nullptr)
+    return fail(PIR2B_EINVAL, "cache_read outputs must be non-null");
+  if (!aligned(k_out, 16) || !aligned(v_out, 16))
+    return fail(PIR2B_EALIGN, "cache_read outputs must be 16-byte aligned");
+  DeviceInfo *dev = nullptr;
+  if (int r = device_info(&dev))
+    return r;
+  a.k_out = static_cast<__nv_bfloat16 *>(k_out);
+  a.v_out = static_cast<__nv_bfloat16 *>(v_out);
+  a.starts = sequences->starts;
+  a.batch = sequences->batch;
+  a.rows = rows;
+  return launch_rows(false, pages->format, pages->head_dim, a, stream);
+}
+
+int pir2b_cache_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int hq,
+                          const pir2b_kv_pages *pages, const pir2b_sequences *sequences,
+                          float scale, void *out, int64_t ldo, void *stream) {
+  const char *what = "cache_attention";
+  RaggedArgs a = {};
+  if (int r = check_sequences(what, sequences, rows, true))
+    return r;
+  if (int r = make_pages(what, pages, sequences, &a.c))
+    return r;
+  if (int r = check_heads(what, hq, pages->kv_heads, pages->head_dim))
+    return r;
+  if (!(scale > 0.f) || !(scale < 3.0e38f))
+    return fail(PIR2B_EINVAL, "cache_attention: scale must be positive and finite");
+  if (rows == 0)
+    return PIR2B_OK;
+  if (int r = check_view("cache_attention q", q, q_row, q_head))
+    return r;
+  if (int r = check_out(what, out, ldo, int64_t(hq) * pages->head_dim))
+    return r;
+  DeviceInfo *dev = nullptr;
+  if (int r = device_info(&dev))
+    return r;
+  a.q = static_cast<const __nv_bfloat16 *>(q);
+  a.q_row = q_row;
+  a.q_head = q_head;
+  a.starts = sequences->starts;
+  a.lengths = sequences->lengths;
+  a.out = static_cast<__nv_bfloat16 *>(out);
+  a.ldo = ldo;
+  a.rows = rows;
+  a.batch = sequences->batch;
+  a.hq = hq;
+  a.hk = pages->kv_heads;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  switch (pages->format) {
+  case kCacheInt8: return launch_ragged<kCacheInt8>("cache_attention launch", pages->head_dim, a, stream);
+  case kCacheE4m3: return launch_ragged<kCacheE4m3>("cache_attention launch", pages->head_dim, a, stream);
+  default: return launch_ragged<kCacheBf16>("cache_attention launch", pages->head_dim, a, stream);
+  }
+}
+
+} // extern "C"

@@ -628,3 +628,110 @@ def attention_rows(q, k, v, *, batch, heads, head_dim, scale=None, out=None):
     )
     _lib.check(status, "pir2b_attention_rows")
     return out
+
+
+def _head_rows(x, what):
+    """(rows, heads, head_dim, row stride, head stride) of a packed bf16
+    [rows, heads, head_dim] view with unit stride along head_dim."""
+    if x.ndim != 3 or x.dtype != torch.bfloat16 or not x.is_cuda or x.stride(2) != 1:
+        raise ValueError(f"{what} must be CUDA bf16 [rows, heads, head_dim] with unit stride along head_dim")
+    rows, heads, d = x.shape
+    return rows, heads, d, x.stride(0) if rows > 1 else heads * d, x.stride(1) if heads > 1 else d
+
+
+def _attention_out(out, q, rows, width):
+    if out is None:
+        return torch.empty((rows, width), device=q.device, dtype=torch.bfloat16)
+    if out.shape != (rows, width) or out.dtype != torch.bfloat16 or out.device != q.device or out.stride(1) != 1:
+        raise ValueError("out must be bf16 [rows, heads * head_dim] on q's device with unit column stride")
+    return out
+
+
+def prompt_attention(q, k, v, starts, *, scale=None, out=None):
+    """Causal grouped-query attention over packed prompts of different lengths.
+
+    q: bf16 [rows, hq, head_dim]; k, v: bf16 [rows, hk, head_dim] (views with
+    any row and head strides that are multiples of 8, e.g. slices of merged
+    projection rows); starts: int32 [prompts + 1] on the device: prompt b is
+    rows starts[b] .. starts[b+1]-1, row i of it sees its rows 0 .. i.
+    head_dim 64 or 128; scale defaults to head_dim ** -0.5.  Returns bf16
+    [rows, hq * head_dim], the o_proj input; rows of no prompt are not
+    written.
+    """
+    rows, hq, d, q_row, q_head = _head_rows(q, "prompt_attention: q")
+    k_rows, hk, k_d, k_row, k_head = _head_rows(k, "prompt_attention: k")
+    *v_shape, v_row, v_head = _head_rows(v, "prompt_attention: v")
+    if v_shape != [rows, hk, d] or k_rows != rows or k_d != d:
+        raise ValueError("prompt_attention: k and v must be [rows, hk, head_dim] with q's rows and head_dim")
+    index = q.get_device()
+    if k.get_device() != index or v.get_device() != index or starts.get_device() != index:
+        raise ValueError("prompt_attention: all tensors must be on one device")
+    if starts.dtype != torch.int32 or starts.ndim != 1 or starts.numel() < 2 or not starts.is_contiguous():
+        raise ValueError("prompt_attention: starts must be contiguous int32 [prompts + 1]")
+    out = _attention_out(out, q, rows, hq * d)
+    status = _lib.lib().pir2b_prompt_attention(
+        q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
+        starts.data_ptr(), starts.numel() - 1, rows, hq, hk, d, d**-0.5 if scale is None else scale, out.data_ptr(),
+        out.stride(0) if rows > 1 else hq * d, _stream(index),
+    )
+    _lib.check(status, "pir2b_prompt_attention")
+    return out
+
+
+def cache_write(k, v, pages, sequences):
+    """Quantises (in the pool's format) the new rows k, v: bf16 [rows,
+    kv_heads, head_dim] views and writes them to the last positions of their
+    sequences.  `pages`: kv_cache.KVPages, `sequences`: kv_cache.Sequences."""
+    rows, hk, d, k_row, k_head = _head_rows(k, "cache_write: k")
+    *v_shape, v_row, v_head = _head_rows(v, "cache_write: v")
+    if v_shape != [rows, hk, d] or hk != pages.kv_heads or d != pages.head_dim:
+        raise ValueError("cache_write: k and v must be [rows, kv_heads, head_dim] of the pool's heads")
+    index = k.get_device()
+    if v.get_device() != index or pages.index != index or sequences.index != index:
+        raise ValueError("cache_write: rows, pages and sequences must be on one device")
+    status = _lib.lib().pir2b_cache_write(
+        k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, rows, pages.address, sequences.address,
+        _stream(index),
+    )
+    _lib.check(status, "pir2b_cache_write")
+
+
+def cache_read(pages, sequences, rows):
+    """Positions 0, 1, ... of each sequence as packed bf16 rows: (k, v), each
+    [rows, kv_heads, head_dim]; sequence b is rows starts[b] ..
+    starts[b+1]-1 (`rows` = starts[-1], which the host knows)."""
+    index = pages.index
+    if sequences.index != index:
+        raise ValueError("cache_read: pages and sequences must be on one device")
+    if rows < 0:
+        raise ValueError("cache_read: rows must not be negative")
+    k, v = torch.empty((2, rows, pages.kv_heads, pages.head_dim), device=pages.device, dtype=torch.bfloat16)
+    status = _lib.lib().pir2b_cache_read(
+        pages.address, sequences.address, rows, k.data_ptr(), v.data_ptr(), _stream(index)
+    )
+    _lib.check(status, "pir2b_cache_read")
+    return k, v
+
+
+def cache_attention(q, pages, sequences, *, scale=None, out=None):
+    """Attention of each sequence's newest rows over its pages.
+
+    q: bf16 [rows, hq, head_dim] view, packed as sequences.starts says; row i
+    of a sequence's n rows sees positions 0 .. length - n + i of it (its own
+    key, and those before it, are in the pages already: `cache_write` first).
+    A row that sees no position gives zeros.  Returns bf16 [rows,
+    hq * head_dim]; scale defaults to head_dim ** -0.5.
+    """
+    rows, hq, d, q_row, q_head = _head_rows(q, "cache_attention: q")
+    if d != pages.head_dim or hq % pages.kv_heads:
+        raise ValueError("cache_attention: q must be [rows, hq, head_dim], hq a multiple of the pool's kv_heads")
+    index = q.get_device()
+    if pages.index != index or sequences.index != index:
+        raise ValueError("cache_attention: q, pages and sequences must be on one device")
+    out = _attention_out(out, q, rows, hq * d)
+    status = _lib.lib().pir2b_cache_attention(
+        q.data_ptr(), q_row, q_head, rows, hq, pages.address, sequences.address, d**-0.5 if scale is None else scale,
+        out.data_ptr(), out.stride(0) if rows > 1 else hq * d, _stream(index),
+    )
+    _lib.check(status, "pir2b_cache_attention")
+    return out
