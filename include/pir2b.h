@@ -416,8 +416,9 @@ int pir2b_attention_causal(const void *q, const void *k, const void *v, int64_t 
  * token and head, quantised as the activation packs (symmetric-row-v1,
  * coexecution/kernels/ampere_ada/integer.py): s = max|v| * f32(1/L), 1 for a
  * row of zeros, L = 127 / 448, code = v / s rounded to nearest even and
- * clamped.  The maximum is over the finite values; an infinity becomes the
- * largest code, a NaN code 0 (int8) or the E4M3 NaN. */
+ * clamped.  The maximum is over the finite values and an infinity becomes the
+ * largest code; a row with a NaN gets codes of 0 and a NaN scale, so the codes
+ * are always numbers (attention takes no E4M3 NaN codes). */
 #define PIR2B_CACHE_BF16 16
 #define PIR2B_CACHE_INT8 8
 #define PIR2B_CACHE_E4M3 9
@@ -474,7 +475,12 @@ int pir2b_cache_read(const pir2b_kv_pages *pages, const pir2b_sequences *sequenc
  * bf16 holds exactly; the scales multiply scores and weights in fp32. */
 int pir2b_cache_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int hq,
                           const pir2b_kv_pages *pages, const pir2b_sequences *sequences,
-                          float scale, void *out, int64_t ldo, void *stream);
+                          float scale, void *out, int64_t ldo, void *workspace, void *stream);
+
+/* Bytes of workspace (16-byte aligned, uninitialised, written and read by the
+ * call alone) that pir2b_cache_attention needs for these shapes; may be 0. */
+int64_t pir2b_cache_attention_workspace(int64_t rows, int hq, const pir2b_kv_pages *pages,
+                                        const pir2b_sequences *sequences);
 
 #ifdef __cplusplus
 }

@@ -86,7 +86,8 @@ SIGNATURES = {
     ],
     "pir2b_cache_write": [_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P],
     "pir2b_cache_read": [_P, _P, _I64, _P, _P, _P],
-    "pir2b_cache_attention": [_P, _I64, _I64, _I64, _I, _P, _P, _F, _P, _I64, _P],
+    "pir2b_cache_attention": [_P, _I64, _I64, _I64, _I, _P, _P, _F, _P, _I64, _P, _P],
+    "pir2b_cache_attention_workspace": [_I64, _I, _P, _P],
     "pir2b_qk_norm_rope": [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I, _I, _I, _F, _P, _P, _P, _P],
 }
 
@@ -110,7 +111,10 @@ def lib():
     for name, argtypes in SIGNATURES.items():
         fn = getattr(handle, name)
         fn.argtypes = argtypes
-        fn.restype = {"pir2b_last_error": ctypes.c_char_p, "pir2b_dit_ffn_workspace": _I64}.get(name, _I)
+        fn.restype = {
+            "pir2b_last_error": ctypes.c_char_p, "pir2b_dit_ffn_workspace": _I64,
+            "pir2b_cache_attention_workspace": _I64,
+        }.get(name, _I)
     return handle
 
 

@@ -1,0 +1,501 @@
+// Attention of a few new rows per sequence over the paged K/V cache.
+//
+// A unit is up to 8 kNT rows (query token x head of one kv head's group) of
+// one sequence; a CTA streams a range of the unit's keys once, eight warps
+// taking 16-key steps in turn.  Few rows cannot fill a 128-row tensor tile
+// and the work is reading the cache, so the products run on warp-level MMAs
+// (m16n8k16, bf16, fp32 sums) with the keys as the M rows:
+//   S^T [16 keys x 8 rows]  = K [16 x D] Q^T,
+//   O^T [D x 8 rows]       += V^T [D x 16 keys] P^T,
+// and cache bytes go from global memory to the MMA registers with no shared
+// memory between: the order of D inside a product is free, so each lane takes
+// whole 16-byte runs of a row (K: its quarter of D; V: its eighth) and q is
+// read in the same order.  8-bit codes become bf16 exactly in registers; the
+// scales multiply scores and weights in fp32.  P is transposed between the
+// products by movmatrix.  The running maximum of a row moves only when a
+// score passes it by more than 8 (in log2), so that most steps have one vote
+// and no rescaling; sums and maxima are fp32.
+#pragma once
+#include "attention_ragged.cuh"
+
+namespace pir2b {
+
+constexpr int kFewWarps = 8;
+
+// Two bf16 pairs from a word of four 8-bit codes, exactly.
+// int8: with u the low seven bits and s the sign bit of a byte, 0x43'u is
+// 128 + u and 0x43's0 is 128 or 256, so their difference is u - 128 s.
+// E4M3: sign and magnitude bits moved to bf16's places hold value * 2^-120
+// (subnormals included).  The pool holds no E4M3 NaN (cache_write puts a NaN
+// into the scale).
+template <int kFormat>
+__device__ __forceinline__ void codes_to_bf16(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  auto sub = [](uint32_t x, uint32_t y) {
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&x), *reinterpret_cast<__nv_bfloat162 *>(&y));
+    return *reinterpret_cast<const uint32_t *>(&d);
+  };
+  if constexpr (kFormat == kCacheInt8) {
+    const uint32_t a = __byte_perm(w, 0x43434343u, 0x4140), b = __byte_perm(w, 0x43434343u, 0x4342);
+    lo = sub(a & 0xff7fff7fu, a & 0xff80ff80u);
+    hi = sub(b & 0xff7fff7fu, b & 0xff80ff80u);
+  } else {
+    const __nv_bfloat162 up = __halves2bfloat162(__ushort_as_bfloat16(0x7b80), __ushort_as_bfloat16(0x7b80));  // 2^120
+    const uint32_t a = __byte_perm(w, 0, 0x1404), b = __byte_perm(w, 0, 0x3424);
+    uint32_t x = (a & 0x80008000u) | ((a & 0x7f007f00u) >> 4), y = (b & 0x80008000u) | ((b & 0x7f007f00u) >> 4);
+    const __nv_bfloat162 m = __hmul2(*reinterpret_cast<__nv_bfloat162 *>(&x), up);
+    const __nv_bfloat162 n = __hmul2(*reinterpret_cast<__nv_bfloat162 *>(&y), up);
+    lo = *reinterpret_cast<const uint32_t *>(&m);
+    hi = *reinterpret_cast<const uint32_t *>(&n);
+  }
+}
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// `kWords` consecutive words (2, 4, 8 or 16) read once.
+template <int kWords>
+__device__ __forceinline__ void load_words(const void *p, uint32_t (&w)[kWords]) {
+  if constexpr (kWords == 2) {
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4)
+      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
+                   : "l"(static_cast<const uint32_t *>(p) + i));
+  }
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Whether a packed bf16 pair holds a NaN or an infinity.
+__device__ __forceinline__ bool pair_not_finite(uint32_t w) {
+  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+
+// Tokens of sequence b in the cache, at most what the table names.
+__device__ __forceinline__ int cache_length(const CachePages &c, const int *lengths, int b) {
+  const int64_t length = __ldg(lengths + b), capacity = int64_t(c.width) << c.shift;
+  if (length > capacity)
+    record_status(kStatusBadPage);
+  return int(max(int64_t(0), min(length, capacity)));
+}
+
+// Position of the first of its n new rows (negative when it has fewer tokens).
+__device__ __forceinline__ int first_new_position(const int *lengths, int b, int n) {
+  return int(max(int64_t(__ldg(lengths + b)) - n, -(int64_t(1) << 30)));
+}
+
+// The unit of a slot: sequences are given floor(starts[b] * group / tile) + b
+// as their first slot, which leaves each of them ceil(rows * group / tile) at
+// least and takes floor(rows * group / tile) + batch in all, so the host can
+// size the grid without the lengths.  Returns the sequence, or -1.
+__device__ __forceinline__ int unit_of(const RaggedArgs &a, int group, int tile_log2, int slot, int &tile) {
+  int lo = 0, hi = a.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (((int64_t(__ldg(a.starts + mid)) * group) >> tile_log2) + mid <= slot)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const int64_t s0 = max(__ldg(a.starts + lo), 0), s1 = min(int64_t(__ldg(a.starts + lo + 1)), a.rows);
+  tile = slot - int((s0 * group) >> tile_log2) - lo;
+  return (tile >= 0 && (int64_t(tile) << tile_log2) < (s1 - s0) * group) ? lo : -1;
+}
+
+template <int D, int kNT>
+constexpr int few_smem() {
+  return kFewWarps * kNT * 8 * (D + 4 + 2) * 4;
+}
+
+template <int kFormat, int D, int kNT>
+__global__ void __launch_bounds__(kFewWarps * 32, kNT == 1 ? 2 : 1) attention_few_kernel(const RaggedArgs a) {
+  constexpr bool kBf16 = kFormat == kCacheBf16;
+  constexpr int kRows = 8 * kNT, kRowsLog2 = kNT == 1 ? 3 : 4;
+  constexpr int KS = D / 16;                       // K steps of S, and M tiles of O
+  constexpr int KW = kBf16 ? D / 8 : D / 16;       // words of a lane's quarter of a K row
+  constexpr int VW = kBf16 ? D / 16 : D / 32;      // words of a lane's eighth of a V row
+  constexpr int kBytes = kBf16 ? 2 : 1;
+  extern __shared__ __align__(16) float few_sm[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q4 = lane & 3;
+  const int kvh = blockIdx.y, split = blockIdx.z;
+  const int group = a.hq / a.hk;
+  pdl_wait();
+  pdl_launch_dependents();
+  int tile;
+  const int b = unit_of(a, group, kRowsLog2, blockIdx.x, tile);
+  if (b < 0)
+    return;
+  const int64_t begin = max(__ldg(a.starts + b), 0);
+  const int n = int(min(int64_t(__ldg(a.starts + b + 1)), a.rows) - begin);
+  const int r0 = tile << kRowsLog2;
+  const int r1 = min(r0 + kRows, n * group);       // the unit's rows: r = token * group + head
+  // Row r sees positions 0 .. first_new + r / group.
+  const int length = cache_length(a.c, a.lengths, b);
+  const int first_new = first_new_position(a.lengths, b, n);
+  const int keys = max(0, min(length, first_new + (r1 - 1) / group + 1));
+  const int all_see = min(length, first_new + r0 / group + 1);   // every row sees positions below this
+  // This split's 16-key steps.
+  const int steps = (keys + 15) >> 4;
+  const int per = (((steps + a.splits - 1) / a.splits) + kFewWarps - 1) / kFewWarps * kFewWarps;
+  const int step_end = min(steps, (split + 1) * per);
+
+  uint32_t qf[kNT][KS][2];
+  int limit[kNT][2];
+#pragma unroll
+  for (int t = 0; t < kNT; ++t) {
+    const int r = r0 + t * 8 + g;
+    uint32_t w[D / 8] = {};
+    if (r < r1) {
+      const __nv_bfloat16 *src = a.q + (begin + r / group) * a.q_row + (kvh * group + r % group) * a.q_head + q4 * (D / 4);
+      load_words<D / 8>(src, w);
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      qf[t][s][0] = w[2 * s];
+      qf[t][s][1] = w[2 * s + 1];
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int rr = r0 + t * 8 + 2 * q4 + e;
+      limit[t][e] = rr < r1 ? first_new + rr / group : -1;
+    }
+  }
+
+  float o[kNT][KS][4] = {};
+  float l[kNT][2] = {}, mu[kNT][2] = {};           // mu: the maximum subtracted (0 while none)
+  float top[kNT][2];                               // the running maximum
+#pragma unroll
+  for (int t = 0; t < kNT; ++t)
+    top[t][0] = top[t][1] = -INFINITY;
+
+  const uint8_t *kbase = static_cast<const uint8_t *>(a.c.k), *vbase = static_cast<const uint8_t *>(a.c.v);
+  uint32_t kr[2][KW];
+  float ksc[2] = {1.f, 1.f};
+  const int page_mask = (1 << a.c.shift) - 1;
+  auto load_k = [&](int page, int step) {
+    const int64_t slot = (int64_t(kvh) << a.c.shift) + ((step << 4) & page_mask) + g;
+    const int64_t at = int64_t(page) * a.c.k_page + slot * D + q4 * (D / 4);
+    load_words<KW>(kbase + at * kBytes, kr[0]);
+    load_words<KW>(kbase + (at + 8 * D) * kBytes, kr[1]);
+    if constexpr (!kBf16) {
+      const float *s = a.c.ks + page * a.c.ks_page + slot;
+      ksc[0] = __ldg(s);
+      ksc[1] = __ldg(s + 8);
+    }
+  };
+
+  int step = split * per + warp;
+  int pages_of_lane = -1;
+  auto page_at = [&](int i) { return __shfl_sync(0xffffffffu, pages_of_lane, i & 31); };
+  auto fetch_pages = [&](int first) {               // the pages of this warp's next 32 steps
+    const int64_t s = int64_t(first) + lane * kFewWarps;
+    pages_of_lane = s < step_end ? page_of(a.c, b, s << 4) : -1;
+  };
+  int page = -1;
+  if (step < step_end) {
+    fetch_pages(step);
+    page = page_at(0);
+    if (page >= 0)
+      load_k(page, step);
+  }
+  for (int i = 0; step < step_end; ++i, step += kFewWarps) {
+    const int page_now = page;
+    const int next = step + kFewWarps;
+    if (((i + 1) & 31) == 0 && next < step_end)
+      fetch_pages(next);
+    page = next < step_end ? page_at(i + 1) : -1;
+    if (page_now < 0) {                             // no such page: its keys are hidden
+      if (page >= 0)
+        load_k(page, next);
+      continue;
+    }
+    uint32_t vr[4][VW];                             // keys 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
+    float vsc[2] = {1.f, 1.f};
+    {
+      const int64_t slot = (int64_t(kvh) << a.c.shift) + ((step << 4) & page_mask);
+      const int64_t at = int64_t(page_now) * a.c.v_page + (slot + 2 * q4) * D + g * (D / 8);
+      load_words<VW>(vbase + at * kBytes, vr[0]);
+      load_words<VW>(vbase + (at + D) * kBytes, vr[1]);
+      load_words<VW>(vbase + (at + 8 * D) * kBytes, vr[2]);
+      load_words<VW>(vbase + (at + 9 * D) * kBytes, vr[3]);
+      if constexpr (!kBf16) {
+        const float *s = a.c.vs + page_now * a.c.vs_page + slot + g;
+        vsc[0] = __ldg(s);
+        vsc[1] = __ldg(s + 8);
+      }
+    }
+    float sc[kNT][4] = {};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      uint32_t af[4];
+      if constexpr (kBf16) {
+        af[0] = kr[0][2 * s], af[1] = kr[1][2 * s], af[2] = kr[0][2 * s + 1], af[3] = kr[1][2 * s + 1];
+      } else {
+        codes_to_bf16<kFormat>(kr[0][s], af[0], af[2]);
+        codes_to_bf16<kFormat>(kr[1][s], af[1], af[3]);
+      }
+#pragma unroll
+      for (int t = 0; t < kNT; ++t)
+        mma_bf16_16816(sc[t], af, qf[t][s][0], qf[t][s][1]);
+    }
+    const float k_lo = ksc[0] * a.scale_log2, k_hi = ksc[1] * a.scale_log2;
+    if (page >= 0)
+      load_k(page, next);
+    const int key0 = step << 4;
+    const bool masked = key0 + 16 > all_see;
+    bool raise = false;
+#pragma unroll
+    for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = sc[t][e] * (e < 2 ? k_lo : k_hi);
+        if (masked && key0 + g + (e & 2) * 4 > limit[t][e & 1])
+          v = -INFINITY;
+        sc[t][e] = v;
+        raise |= v > top[t][e & 1] + 8.f;
+      }
+    }
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float m = fmaxf(top[t][e], fmaxf(sc[t][e], sc[t][e + 2]));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+          const float keep = top[t][e] == -INFINITY ? 1.f : exp2_fast(top[t][e] - m);   // nothing summed yet: keep it
+          top[t][e] = m;
+          mu[t][e] = m == -INFINITY ? 0.f : m;
+          l[t][e] *= keep;
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            o[t][s][e] *= keep;
+            o[t][s][e + 2] *= keep;
+          }
+        }
+      }
+    }
+    uint32_t pf[kNT][2];
+#pragma unroll
+    for (int t = 0; t < kNT; ++t) {
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float w = exp2_fast(sc[t][e] - mu[t][e & 1]);
+        l[t][e & 1] += w;
+        p[e] = kBf16 ? w : w * vsc[e >> 1];
+        if (!kBf16 && masked && sc[t][e] == -INFINITY)   // a hidden key's scale may be anything
+          p[e] = 0.f;
+      }
+      pf[t][0] = transpose_8x8(pack_bf16x2(p[0], p[1]));
+      pf[t][1] = transpose_8x8(pack_bf16x2(p[2], p[3]));
+    }
+    // Pairs (key, key + 1) of a column for the two halves of an M tile pair.
+    auto product = [&](const uint32_t (&pp)[kNT][2]) {
+#pragma unroll
+      for (int j = 0; j < VW; ++j) {
+        if constexpr (kBf16) {
+          const uint32_t af[4] = {__byte_perm(vr[0][j], vr[1][j], 0x5410), __byte_perm(vr[0][j], vr[1][j], 0x7632),
+                                  __byte_perm(vr[2][j], vr[3][j], 0x5410), __byte_perm(vr[2][j], vr[3][j], 0x7632)};
+#pragma unroll
+          for (int t = 0; t < kNT; ++t)
+            mma_bf16_16816(o[t][j], af, pp[t][0], pp[t][1]);
+        } else {
+          uint32_t af[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {   // keys 2 q4 .. and 2 q4 + 8 ..
+            const uint32_t x = __byte_perm(vr[2 * h][j], vr[2 * h + 1][j], 0x5140);
+            const uint32_t y = __byte_perm(vr[2 * h][j], vr[2 * h + 1][j], 0x7362);
+            codes_to_bf16<kFormat>(x, af[0][2 * h], af[0][2 * h + 1]);
+            codes_to_bf16<kFormat>(y, af[1][2 * h], af[1][2 * h + 1]);
+          }
+#pragma unroll
+          for (int t = 0; t < kNT; ++t) {
+            mma_bf16_16816(o[t][2 * j], af[0], pp[t][0], pp[t][1]);
+            mma_bf16_16816(o[t][2 * j + 1], af[1], pp[t][0], pp[t][1]);
+          }
+        }
+      }
+    };
+    if constexpr (kBf16) {
+      if (masked) {
+        // Hidden values must not enter a product, not even times 0: positions
+        // no row sees become 0 here, and where a position hidden from some
+        // rows holds a value that is not finite the rows go one at a time.
+        bool spoiled = false;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int key = key0 + 2 * q4 + (x & 1) + (x & 2) * 4;
+#pragma unroll
+          for (int j = 0; j < VW; ++j) {
+            if (key >= keys)
+              vr[x][j] = 0;
+            else if (key >= all_see)
+              spoiled |= pair_not_finite(vr[x][j]);
+          }
+        }
+        if (__any_sync(0xffffffffu, spoiled)) {
+          uint32_t kept[4][VW];
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int j = 0; j < VW; ++j)
+              kept[x][j] = vr[x][j];
+#pragma unroll 1
+          for (int r = 0; r < kRows; ++r) {
+            const int last = r0 + r < r1 ? first_new + (r0 + r) / group : -1;
+            uint32_t one[kNT][2];
+#pragma unroll
+            for (int t = 0; t < kNT; ++t) {
+              one[t][0] = t * 8 + g == r ? pf[t][0] : 0;
+              one[t][1] = t * 8 + g == r ? pf[t][1] : 0;
+            }
+            // The product runs on columns of zeros for the other rows, so a
+            // value that this row sees must not reach them either: it is
+            // added to this row alone, below.
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int key = key0 + 2 * q4 + (x & 1) + (x & 2) * 4;
+#pragma unroll
+              for (int j = 0; j < VW; ++j)
+                vr[x][j] = key > last ? 0 : kept[x][j];
+            }
+            float saved[kNT][KS][4];
+#pragma unroll
+            for (int t = 0; t < kNT; ++t)
+#pragma unroll
+              for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  saved[t][s][e] = o[t][s][e];
+            product(one);
+            // Columns of O^T are rows: keep the new sums of row r only.
+#pragma unroll
+            for (int t = 0; t < kNT; ++t)
+#pragma unroll
+              for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (t * 8 + 2 * q4 + (e & 1) != r)
+                    o[t][s][e] = saved[t][s][e];
+          }
+          continue;
+        }
+      }
+    }
+    product(pf);
+  }
+
+  // The warps' partial sums, added in warp order.
+  float *so = few_sm;                                          // [warps][rows][D + 4]
+  float *sm = so + kFewWarps * kRows * (D + 4), *sl = sm + kFewWarps * kRows;
+#pragma unroll
+  for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = l[t][e];
+      x += __shfl_xor_sync(0xffffffffu, x, 4);
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      const int r = t * 8 + 2 * q4 + e;
+      if (g == 0) {
+        sm[warp * kRows + r] = top[t][e];
+        sl[warp * kRows + r] = x;
+      }
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {                           // d = g D/8 + 2 s + (0, 1)
+        const float2 pair = make_float2(o[t][s][e], o[t][s][e + 2]);
+        *reinterpret_cast<float2 *>(so + (warp * kRows + r) * (D + 4) + g * (D / 8) + 2 * s) = pair;
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kRows * (D / 4); i += kFewWarps * 32) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    if (r0 + r >= r1)
+      continue;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w)
+      m = fmaxf(m, sm[w * kRows + r]);
+    float total = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      const float mw = sm[w * kRows + r];
+      const float f = mw == m ? 1.f : exp2_fast(mw - m);       // equal, -inf too: the sums as they are
+      const float4 x = *reinterpret_cast<const float4 *>(so + (w * kRows + r) * (D + 4) + d);
+      total += f * sl[w * kRows + r];
+      sum.x += f * x.x, sum.y += f * x.y, sum.z += f * x.z, sum.w += f * x.w;
+    }
+    const int64_t row = begin + (r0 + r) / group;
+    const int h = kvh * group + (r0 + r) % group;
+    if (a.splits == 1) {
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      *reinterpret_cast<uint2 *>(a.out + row * a.ldo + h * D + d) =
+          make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+    } else {
+      const int64_t at = (int64_t(split) * a.rows + row) * a.hq + h;
+      *reinterpret_cast<float4 *>(a.part_o + at * D + d) = sum;
+      if (d == 0)
+        a.part_ml[at] = make_float2(m, total);
+    }
+  }
+}
+
+// Joins the splits of each (row, head), in split order: a warp per row and
+// head, D / 32 values per lane.
+template <int D>
+__global__ void __launch_bounds__(256) attention_join_kernel(const RaggedArgs a) {
+  constexpr int E = D / 32;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t item = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const int64_t row = item / a.hq;
+  const int h = int(item % a.hq);
+  if (row >= a.rows || sequence_of(a.starts, a.batch, row) < 0)
+    return;
+  const int64_t apart = a.rows * a.hq;
+  // At most 32 splits: a lane per split holds its maximum and sum.
+  const float2 ml = lane < a.splits ? a.part_ml[lane * apart + item] : make_float2(-INFINITY, 0.f);
+  float m = ml.x;
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1)
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+  const float f = ml.x == m ? 1.f : exp2_fast(ml.x - m);
+  float total = f * ml.y;
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1)
+    total += __shfl_xor_sync(0xffffffffu, total, x);
+  float sum[E] = {};
+  for (int s = 0; s < a.splits; ++s) {
+    const float fs = __shfl_sync(0xffffffffu, f, s);
+    const float *p = a.part_o + (s * apart + item) * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      sum[e] += fs * p[e];
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  uint32_t w[E / 2];
+#pragma unroll
+  for (int e = 0; e < E; e += 2)
+    w[e / 2] = pack_bf16x2(sum[e] * inv, sum[e + 1] * inv);
+  __nv_bfloat16 *out = a.out + row * a.ldo + h * D + lane * E;
+  if constexpr (E == 4)
+    *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
+  else
+    *reinterpret_cast<uint32_t *>(out) = w[0];
+}
+
+} // namespace pir2b

@@ -22,14 +22,15 @@ struct RaggedArgs {
   int64_t rows;
   int batch, hq, hk;
   float scale_log2;             // scale * log2(e)
+  int splits;                   // CTAs along the keys of a unit, at most 32
+  float *part_o;                // [splits, rows, hq, D] sums, where splits > 1,
+  float2 *part_ml;              // [splits, rows, hq] and their (maximum, sum of weights)
 };
-
-constexpr int kSourceRows = 0;  // else a cache format (kCacheBf16, ...)
 
 // The plain form: a warp per (row, head), D / 32 dimensions per lane, one key
 // at a time with the running maximum and sum.
-template <int kSource, int D>
-__global__ void __launch_bounds__(128) ragged_simple_kernel(const RaggedArgs a) {
+template <int D>
+__global__ void __launch_bounds__(128) prompt_simple_kernel(const RaggedArgs a) {
   constexpr int E = D / 32;
   pdl_wait();
   pdl_launch_dependents();
@@ -43,15 +44,7 @@ __global__ void __launch_bounds__(128) ragged_simple_kernel(const RaggedArgs a) 
   if (b < 0)
     return;
   const int64_t begin = max(__ldg(a.starts + b), 0);
-  int64_t keys = row - begin + 1;
-  if constexpr (kSource != kSourceRows) {
-    const int64_t length = __ldg(a.lengths + b);
-    keys = length - __ldg(a.starts + b + 1) + row + 1;
-    if (keys > int64_t(a.c.width) << a.c.shift) {   // the table names fewer positions
-      keys = int64_t(a.c.width) << a.c.shift;
-      record_status(kStatusBadPage);
-    }
-  }
+  const int64_t keys = row - begin + 1;
   float q[E], o[E];
   const __nv_bfloat16 *qp = a.q + row * a.q_row + h * a.q_head + lane * E;
 #pragma unroll
@@ -61,45 +54,14 @@ __global__ void __launch_bounds__(128) ragged_simple_kernel(const RaggedArgs a) 
   }
   float m = -INFINITY, l = 0.f;
   for (int64_t j = 0; j < keys; ++j) {
-    float kv[E], vv[E], ks = 1.f, vs = 1.f;
-    if constexpr (kSource == kSourceRows) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        kv[e] = __bfloat162float(a.k[(begin + j) * a.k_row + kvh * a.k_head + lane * E + e]);
-        vv[e] = __bfloat162float(a.v[(begin + j) * a.v_row + kvh * a.v_head + lane * E + e]);
-      }
-    } else {
-      const int page = page_of(a.c, b, j);
-      if (page < 0)
-        continue;
-      const int64_t slot = (int64_t(kvh) << a.c.shift) + (j & ((1 << a.c.shift) - 1));
-      const int64_t ak = page * a.c.k_page + slot * D + lane * E, av = page * a.c.v_page + slot * D + lane * E;
-      if constexpr (kSource == kCacheBf16) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          kv[e] = __bfloat162float(static_cast<const __nv_bfloat16 *>(a.c.k)[ak + e]);
-          vv[e] = __bfloat162float(static_cast<const __nv_bfloat16 *>(a.c.v)[av + e]);
-        }
-      } else {
-        ks = a.c.ks[page * a.c.ks_page + slot];
-        vs = a.c.vs[page * a.c.vs_page + slot];
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          const float2 fk = code_values<kSource>(*reinterpret_cast<const uint16_t *>(static_cast<const uint8_t *>(a.c.k) + ak + e));
-          const float2 fv = code_values<kSource>(*reinterpret_cast<const uint16_t *>(static_cast<const uint8_t *>(a.c.v) + av + e));
-          kv[e] = fk.x, kv[e + 1] = fk.y;
-          vv[e] = fv.x, vv[e + 1] = fv.y;
-        }
-      }
-    }
     float s = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      s += q[e] * kv[e];
+      s += q[e] * __bfloat162float(a.k[(begin + j) * a.k_row + kvh * a.k_head + lane * E + e]);
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1)
       s += __shfl_xor_sync(0xffffffffu, s, x);
-    s *= ks * a.scale_log2;
+    s *= a.scale_log2;
     const float top = fmaxf(m, s);
     const float keep = m == -INFINITY ? 1.f : exp2f(m - top);   // nothing summed yet: keep 0 (or a NaN)
     const float p = s == -INFINITY ? 0.f : exp2f(s - top);   // NaN and +inf scores give NaN
@@ -107,7 +69,7 @@ __global__ void __launch_bounds__(128) ragged_simple_kernel(const RaggedArgs a) 
     l = l * keep + p;
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      o[e] = o[e] * keep + p * vs * vv[e];
+      o[e] = o[e] * keep + p * __bfloat162float(a.v[(begin + j) * a.v_row + kvh * a.v_head + lane * E + e]);
   }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll

@@ -51,6 +51,7 @@ struct DeviceInfo {
   int sms = 0;
   int max_smem = 0;
   bool attrs_set = false;
+  bool cache_attrs_set = false;  // attributes of the paged-cache kernels
   void *ffn_scratch = nullptr;   // device address of g_ffn_scratch (set on first use)
 };
 

@@ -1,6 +1,7 @@
 // C ABI of the ragged-batch operators (packed prompts, paged K/V cache):
 // argument checks and launches.
 #pragma once
+#include "attention_few.cuh"
 #include "attention_ragged.cuh"
 #include "capi.cuh"
 #include "kv_cache.cuh"
@@ -78,12 +79,12 @@ static int make_pages(const char *what, const pir2b_kv_pages *p, const pir2b_seq
 // A launch that may start while its predecessor drains (every kernel here
 // begins with griddepcontrol.wait).
 template <typename Args>
-static int launch_cache(const char *what, void (*kernel)(Args), int64_t grid, int threads, size_t smem,
-                        const Args &a, void *stream) {
+static int launch_cache(const char *what, void (*kernel)(Args), int64_t grid, int grid_y, int grid_z, int threads,
+                        size_t smem, const Args &a, void *stream) {
   if (grid > 0x7fffffff)
     return fail(PIR2B_EINVAL, "%s: too many rows", what);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(grid), 1, 1);
+  cfg.gridDim = dim3(unsigned(grid), unsigned(grid_y), unsigned(grid_z));
   cfg.blockDim = dim3(unsigned(threads), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
@@ -100,9 +101,9 @@ static int launch_rows(bool write, int d, const CacheRowsArgs &a, void *stream) 
   const int64_t grid = (a.rows * 2 * a.c.hk * (d / 8) + kCacheThreads - 1) / kCacheThreads;
   if (write)
     return launch_cache("cache_write launch", d == 64 ? cache_write_kernel<kFormat, 64> : cache_write_kernel<kFormat, 128>,
-                        grid, kCacheThreads, 0, a, stream);
+                        grid, 1, 1, kCacheThreads, 0, a, stream);
   return launch_cache("cache_read launch", d == 64 ? cache_read_kernel<kFormat, 64> : cache_read_kernel<kFormat, 128>,
-                      grid, kCacheThreads, 0, a, stream);
+                      grid, 1, 1, kCacheThreads, 0, a, stream);
 }
 
 static int launch_rows(bool write, int format, int d, const CacheRowsArgs &a, void *stream) {
@@ -113,10 +114,60 @@ static int launch_rows(bool write, int format, int d, const CacheRowsArgs &a, vo
   }
 }
 
-template <int kSource>
-static int launch_ragged(const char *what, int d, const RaggedArgs &a, void *stream) {
-  return launch_cache(what, d == 64 ? ragged_simple_kernel<kSource, 64> : ragged_simple_kernel<kSource, 128>,
-                      (a.rows * a.hq + 3) / 4, 128, 0, a, stream);
+constexpr int kFewWaves = 2;
+
+// How the few-row kernel covers a call: rows per unit, grid slots and splits.
+struct FewPlan {
+  int nt;          // 8 nt rows per unit
+  int64_t slots;
+  int splits;
+};
+
+static FewPlan plan_few(int64_t rows, int hq, int hk, int batch, int64_t positions, int sms) {
+  FewPlan p;
+  const int group = hq / hk;
+  p.nt = (rows + batch - 1) / batch * group <= 8 ? 1 : 2;
+  p.slots = rows * group / (8 * p.nt) + batch;
+  // Two CTAs fit an SM; a split reads at least 128 keys.
+  const int64_t want = (int64_t(kFewWaves) * 2 * sms + p.slots * hk - 1) / (p.slots * hk);
+  p.splits = int(std::max<int64_t>(1, std::min<int64_t>({want, positions / (16 * kFewWarps), 32})));
+  return p;
+}
+
+template <int kFormat, int D, int kNT>
+static int launch_attention_few(const FewPlan &p, const RaggedArgs &a, void *stream) {
+  return launch_cache("cache_attention launch", attention_few_kernel<kFormat, D, kNT>, p.slots, a.hk, p.splits,
+                      kFewWarps * 32, few_smem<D, kNT>(), a, stream);
+}
+
+template <int kFormat>
+static int launch_attention_few(const FewPlan &p, int d, const RaggedArgs &a, void *stream) {
+  if (d == 64)
+    return p.nt == 1 ? launch_attention_few<kFormat, 64, 1>(p, a, stream) : launch_attention_few<kFormat, 64, 2>(p, a, stream);
+  return p.nt == 1 ? launch_attention_few<kFormat, 128, 1>(p, a, stream) : launch_attention_few<kFormat, 128, 2>(p, a, stream);
+}
+
+static int launch_join(int d, const RaggedArgs &a, void *stream) {
+  return launch_cache("cache_attention join launch", d == 64 ? attention_join_kernel<64> : attention_join_kernel<128>,
+                      (a.rows * a.hq + 7) / 8, 1, 1, 256, 0, a, stream);
+}
+
+// Dynamic shared memory above the default limit, once per device.
+static int cache_kernel_attributes(DeviceInfo *dev) {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  if (dev->cache_attrs_set)
+    return PIR2B_OK;
+  const std::pair<const void *, int> kernels[] = {
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheBf16, 128, 2>), few_smem<128, 2>()},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheInt8, 128, 2>), few_smem<128, 2>()},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 128, 2>), few_smem<128, 2>()},
+  };
+  for (const auto &k : kernels)
+    if (int r = cuda_status(cudaFuncSetAttribute(k.first, cudaFuncAttributeMaxDynamicSharedMemorySize, k.second),
+                            "cudaFuncSetAttribute"))
+      return r;
+  dev->cache_attrs_set = true;
+  return PIR2B_OK;
 }
 
 } // namespace pir2b
@@ -168,7 +219,8 @@ int pir2b_prompt_attention(const void *q, int64_t q_row, int64_t q_head, const v
   a.hq = hq;
   a.hk = hk;
   a.scale_log2 = scale * 1.4426950408889634f;
-  return launch_ragged<kSourceRows>("prompt_attention launch", head_dim, a, stream);
+  return launch_cache("prompt_attention launch", head_dim == 64 ? prompt_simple_kernel<64> : prompt_simple_kernel<128>,
+                      (a.rows * a.hq + 3) / 4, 1, 1, 128, 0, a, stream);
 }
 
 int pir2b_cache_write(const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row,
@@ -229,7 +281,7 @@ int pir2b_cache_read(const pir2b_kv_pages *pages, const pir2b_sequences *sequenc
 
 int pir2b_cache_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int hq,
                           const pir2b_kv_pages *pages, const pir2b_sequences *sequences,
-                          float scale, void *out, int64_t ldo, void *stream) {
+                          float scale, void *out, int64_t ldo, void *workspace, void *stream) {
   const char *what = "cache_attention";
   RaggedArgs a = {};
   if (int r = check_sequences(what, sequences, rows, true))
@@ -261,11 +313,35 @@ int pir2b_cache_attention(const void *q, int64_t q_row, int64_t q_head, int64_t 
   a.hq = hq;
   a.hk = pages->kv_heads;
   a.scale_log2 = scale * 1.4426950408889634f;
-  switch (pages->format) {
-  case kCacheInt8: return launch_ragged<kCacheInt8>("cache_attention launch", pages->head_dim, a, stream);
-  case kCacheE4m3: return launch_ragged<kCacheE4m3>("cache_attention launch", pages->head_dim, a, stream);
-  default: return launch_ragged<kCacheBf16>("cache_attention launch", pages->head_dim, a, stream);
+  const int d = pages->head_dim;
+  if (int r = cache_kernel_attributes(dev))
+    return r;
+  const FewPlan plan = plan_few(rows, hq, a.hk, a.batch, int64_t(a.c.width) << a.c.shift, dev->sms);
+  a.splits = plan.splits;
+  if (plan.splits > 1) {
+    if (workspace == nullptr || !aligned(workspace, 16))
+      return fail(PIR2B_EALIGN, "cache_attention: this shape needs a 16-byte aligned workspace");
+    a.part_o = static_cast<float *>(workspace);
+    a.part_ml = reinterpret_cast<float2 *>(a.part_o + int64_t(plan.splits) * rows * hq * d);
   }
+  int status = PIR2B_OK;
+  switch (pages->format) {
+  case kCacheInt8: status = launch_attention_few<kCacheInt8>(plan, d, a, stream); break;
+  case kCacheE4m3: status = launch_attention_few<kCacheE4m3>(plan, d, a, stream); break;
+  default: status = launch_attention_few<kCacheBf16>(plan, d, a, stream); break;
+  }
+  return status != PIR2B_OK || plan.splits == 1 ? status : launch_join(d, a, stream);
+}
+
+int64_t pir2b_cache_attention_workspace(int64_t rows, int hq, const pir2b_kv_pages *pages,
+                                        const pir2b_sequences *sequences) {
+  DeviceInfo *dev = nullptr;
+  if (pages == nullptr || sequences == nullptr || rows < 1 || pages->kv_heads < 1 || hq < pages->kv_heads ||
+      sequences->batch < 1 || device_info(&dev) != PIR2B_OK)
+    return 0;                                     // the call itself reports what is wrong
+  const FewPlan plan = plan_few(rows, hq, pages->kv_heads, sequences->batch,
+                                int64_t(sequences->table_width) * pages->page_size, dev->sms);
+  return plan.splits == 1 ? 0 : int64_t(plan.splits) * rows * hq * (pages->head_dim * 4 + 8);
 }
 
 } // extern "C"

@@ -8,7 +8,9 @@
 // [i * page, (i + 1) * page) of sequence b.  Rows are quantised as the
 // activation packs are (symmetric-row-v1, quant.cuh): s = max|v| * f32(1/L),
 // 1 for a row of zeros, L = 127 or 448; code = rint(v / s) clamped, or the
-// nearest E4M3 number.
+// nearest E4M3 number.  An infinity becomes the largest code.  A row with a
+// NaN gets codes of 0 and the NaN as its scale, so every reader of the row
+// sees it and the codes themselves are always numbers.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -77,33 +79,40 @@ __device__ __forceinline__ int page_of(const CachePages &c, int b, int64_t pos) 
   return page;
 }
 
-// Largest finite |value| of eight bf16.
-__device__ __forceinline__ float finite_max8(const uint4 &x) {
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+  return m;
+}
+
+// Largest |value| of eight bf16, infinities aside; a NaN where one is.
+__device__ __forceinline__ float row_max8(const uint4 &x) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
   float m = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float lo = fabsf(__uint_as_float(w[i] << 16)), hi = fabsf(__uint_as_float(w[i] & 0xffff0000u));
-    m = fmaxf(m, lo <= 3.3895314e38f ? lo : 0.f);
-    m = fmaxf(m, hi <= 3.3895314e38f ? hi : 0.f);
+    m = max_nan(m, lo == INFINITY ? 0.f : lo);
+    m = max_nan(m, hi == INFINITY ? 0.f : hi);
   }
   return m;
 }
 
-// Eight bf16 -> eight codes under scale s.  A NaN becomes code 0 (int8) or
-// the E4M3 NaN; an infinity the largest code.
+// Eight bf16 -> eight codes under scale s (0 under a NaN).
 template <int kFormat>
 __device__ __forceinline__ uint2 quantise8(const uint4 &x, float s) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
   uint32_t out[2] = {0, 0};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float lo = __fdiv_rn(__uint_as_float(w[i] << 16), s);
-    const float hi = __fdiv_rn(__uint_as_float(w[i] & 0xffff0000u), s);
+    float lo = __fdiv_rn(__uint_as_float(w[i] << 16), s);
+    float hi = __fdiv_rn(__uint_as_float(w[i] & 0xffff0000u), s);
+    lo = lo != lo ? 0.f : lo;
+    hi = hi != hi ? 0.f : hi;
     uint32_t pair;
     if constexpr (kFormat == kCacheInt8) {
-      const int a = lo != lo ? 0 : __float2int_rn(fminf(fmaxf(lo, -127.f), 127.f));
-      const int b = hi != hi ? 0 : __float2int_rn(fminf(fmaxf(hi, -127.f), 127.f));
+      const int a = __float2int_rn(fminf(fmaxf(lo, -127.f), 127.f));
+      const int b = __float2int_rn(fminf(fmaxf(hi, -127.f), 127.f));
       pair = (uint32_t(a) & 0xffu) | ((uint32_t(b) & 0xffu) << 8);
     } else {
       uint16_t e;
@@ -164,10 +173,10 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const CacheR
     if (page >= 0)
       *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(codes) + at) = x;
   } else {
-    float m = finite_max8(x);
+    float m = row_max8(x);
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1)
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float s = m == 0.f ? 1.f : __fmul_rn(m, kFormat == kCacheInt8 ? 1.0f / 127.0f : 1.0f / 448.0f);
     if (page >= 0) {
       *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(codes) + at) = quantise8<kFormat>(x, s);

@@ -729,9 +729,12 @@ def cache_attention(q, pages, sequences, *, scale=None, out=None):
     if pages.index != index or sequences.index != index:
         raise ValueError("cache_attention: q, pages and sequences must be on one device")
     out = _attention_out(out, q, rows, hq * d)
-    status = _lib.lib().pir2b_cache_attention(
+    lib = _lib.lib()
+    size = lib.pir2b_cache_attention_workspace(rows, hq, pages.address, sequences.address)
+    workspace = torch.empty(size, device=q.device, dtype=torch.uint8) if size > 0 else None
+    status = lib.pir2b_cache_attention(
         q.data_ptr(), q_row, q_head, rows, hq, pages.address, sequences.address, d**-0.5 if scale is None else scale,
-        out.data_ptr(), out.stride(0) if rows > 1 else hq * d, _stream(index),
+        out.data_ptr(), out.stride(0) if rows > 1 else hq * d, _ptr(workspace), _stream(index),
     )
     _lib.check(status, "pir2b_cache_attention")
     return out

@@ -52,17 +52,17 @@ def tolerance(out, mass):
 
 def quantise(x, dtype):
     """symmetric-row-v1 per row of the last dimension, in fp32 as defined:
-    (codes, scale)."""
+    (codes, scale).  A row with a NaN: codes of 0, the NaN as its scale."""
     x = x.float()
     if dtype == torch.bfloat16:
         return x.to(torch.bfloat16), None
     limit = INT8_LIMIT if dtype == torch.int8 else E4M3_LIMIT
-    most = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x)).amax(-1)
+    most = torch.where(torch.isinf(x), torch.zeros_like(x), x.abs()).amax(-1)
     scale = torch.where(most == 0, torch.ones_like(most), most * float(1.0 / torch.tensor(limit)))
-    y = x / scale[..., None]
+    y = torch.nan_to_num(x / scale[..., None], nan=0.0).clamp(-limit, limit)
     if dtype == torch.int8:
-        return torch.nan_to_num(torch.round(y.clamp(-limit, limit)), nan=0.0).to(torch.int8), scale
-    return y.clamp(-limit, limit).to(torch.float8_e4m3fn), scale
+        return torch.round(y).to(torch.int8), scale
+    return y.to(torch.float8_e4m3fn), scale
 
 
 def values(codes, scale):

@@ -76,11 +76,14 @@ def test_write_of_values_that_are_not_finite(dtype):
     page = int(table[0, 0])
     for x, c, s in ((k, kc, ks), (v, vc, vs)):
         codes, scale = quantise(x, dtype)
-        assert torch.equal(s[page, :, :4].T, scale)
-        got = c[page, :, :4].transpose(0, 1)
-        nan = torch.isnan(x)
-        assert torch.equal(got.float()[~nan], codes.float()[~nan])
-        assert (got.float()[nan] == 0).all() if dtype == torch.int8 else torch.isnan(got.float()[nan]).all()
+        assert torch.equal(torch.nan_to_num(s[page, :, :4].T, nan=-1.0), torch.nan_to_num(scale, nan=-1.0))
+        assert torch.isnan(scale).sum() == (1 if x is k else 0)
+        assert torch.equal(c[page, :, :4].transpose(0, 1).float(), codes.float())
+    # A reader of the row with the NaN sees it, the others do not.
+    q, _ = new_rows(1, 4, 128, seed=4)
+    for length, spoiled in ((1, True), (4, True)):
+        out = ops.cache_attention(q, KVPages(kc, vc, ks, vs), Sequences(starts_of([1]), ints([length]), table)).view(4, 128)
+        assert torch.isnan(out[:2]).all() == spoiled and torch.isfinite(out[2:]).all()
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "int8", "e4m3"])

@@ -27,7 +27,7 @@ def sequences(**changes):
 
 def attention(p, s, *, q=4096, q_row=2048, q_head=128, rows=2, hq=16, scale=1.0, out=4096, ldo=2048):
     return _lib.lib().pir2b_cache_attention(
-        q, q_row, q_head, rows, hq, ctypes.byref(p), ctypes.byref(s), scale, out, ldo, None
+        q, q_row, q_head, rows, hq, ctypes.byref(p), ctypes.byref(s), scale, out, ldo, None, None
     )
 
 
