@@ -3,6 +3,7 @@
 #pragma once
 #include "attention_few.cuh"
 #include "attention_ragged.cuh"
+#include "attention_tile.cuh"
 #include "capi.cuh"
 #include "kv_cache.cuh"
 
@@ -152,6 +153,41 @@ static int launch_join(int d, const RaggedArgs &a, void *stream) {
                       (a.rows * a.hq + 7) / 8, 1, 1, 256, 0, a, stream);
 }
 
+// 3-D map over packed bf16 rows [rows, heads, d], box of 128 rows of one head
+// and 64 columns in 128-byte swizzled rows.
+static int make_rows_map(CUtensorMap *map, const void *base, int64_t rows, int heads, int d, int64_t row, int64_t head) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr)
+    return fail(PIR2B_ECUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  const cuuint64_t dims[3] = {cuuint64_t(d), cuuint64_t(heads), cuuint64_t(rows)};
+  const cuuint64_t strides[2] = {cuuint64_t(head) * 2, cuuint64_t(row) * 2};
+  const cuuint32_t box[3] = {64, 1, kTileKeys};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? PIR2B_OK : fail(PIR2B_ECUDA, "cuTensorMapEncodeTiled (rows) failed (%d)", int(r));
+}
+
+template <int kSource, int D>
+static int launch_tile(const char *what, const RaggedArgs &a, const CUtensorMap &tm_k, const CUtensorMap &tm_v,
+                       void *stream) {
+  const int64_t grid = (a.rows * (a.hq / a.hk) / 256 + a.batch) * a.hk;
+  if (grid > 0x7fffffff)
+    return fail(PIR2B_EINVAL, "%s: too many rows", what);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(grid), 1, 1);
+  cfg.blockDim = dim3(kTileThreads, 1, 1);
+  cfg.dynamicSmemBytes = TileShape<D>::kSmem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, attention_tile_kernel<kSource, D>, a, tm_k, tm_v), what);
+}
+
 // Dynamic shared memory above the default limit, once per device.
 static int cache_kernel_attributes(DeviceInfo *dev) {
   std::lock_guard<std::mutex> lock(g_mutex);
@@ -161,6 +197,8 @@ static int cache_kernel_attributes(DeviceInfo *dev) {
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheBf16, 128, 2>), few_smem<128, 2>()},
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheInt8, 128, 2>), few_smem<128, 2>()},
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 128, 2>), few_smem<128, 2>()},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 64>), TileShape<64>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 128>), TileShape<128>::kSmem},
   };
   for (const auto &k : kernels)
     if (int r = cuda_status(cudaFuncSetAttribute(k.first, cudaFuncAttributeMaxDynamicSharedMemorySize, k.second),
@@ -219,8 +257,15 @@ int pir2b_prompt_attention(const void *q, int64_t q_row, int64_t q_head, const v
   a.hq = hq;
   a.hk = hk;
   a.scale_log2 = scale * 1.4426950408889634f;
-  return launch_cache("prompt_attention launch", head_dim == 64 ? prompt_simple_kernel<64> : prompt_simple_kernel<128>,
-                      (a.rows * a.hq + 3) / 4, 1, 1, 128, 0, a, stream);
+  if (int r = cache_kernel_attributes(dev))
+    return r;
+  CUtensorMap tm_k, tm_v;
+  if (int r = make_rows_map(&tm_k, k, rows, hk, head_dim, k_row, k_head))
+    return r;
+  if (int r = make_rows_map(&tm_v, v, rows, hk, head_dim, v_row, v_head))
+    return r;
+  return head_dim == 64 ? launch_tile<kSourceRows, 64>("prompt_attention launch", a, tm_k, tm_v, stream)
+                        : launch_tile<kSourceRows, 128>("prompt_attention launch", a, tm_k, tm_v, stream);
 }
 
 int pir2b_cache_write(const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row,
