@@ -97,14 +97,19 @@ __device__ __forceinline__ int first_new_position(const int *lengths, int b, int
 // as their first slot, which leaves each of them ceil(rows * group / tile) at
 // least and takes floor(rows * group / tile) + batch in all, so the host can
 // size the grid without the lengths.  Returns the sequence, or -1.
-// All lanes of a warp search together, 32 candidates at a time.
+// All lanes of a warp search together, 128 candidates at a time.
 __device__ __forceinline__ int unit_of(const RaggedArgs &a, int group, int tile_log2, int slot, int &tile) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = a.batch;
   do {
-    const int step = (hi - lo + 31) >> 5, at = lo + lane * step;
-    const bool before = at < hi && ((int64_t(max(__ldg(a.starts + at), 0)) * group) >> tile_log2) + at <= slot;
-    const int count = __popc(__ballot_sync(0xffffffffu, before));
+    const int step = (hi - lo + 127) >> 7;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = lo + (i * 32 + lane) * step;
+      const bool before = at < hi && ((int64_t(max(__ldg(a.starts + min(at, hi)), 0)) * group) >> tile_log2) + at <= slot;
+      count += __popc(__ballot_sync(0xffffffffu, before));
+    }
     if (count == 0)
       return -1;
     lo += (count - 1) * step;

@@ -22,6 +22,7 @@ struct RaggedArgs {
   int64_t rows;
   int batch, hq, hk;
   float scale_log2;             // scale * log2(e)
+  int q_by_tma;                 // q tiles are whole boxes: the group divides 128
   int splits;                   // CTAs along the keys of a unit, at most 32
   float *part_o;                // [splits, rows, hq, D] sums, where splits > 1,
   float2 *part_ml;              // [splits, rows, hq] and their (maximum, sum of weights)

@@ -1,22 +1,22 @@
 // Causal attention of many rows: 128-row tiles on the tensor cores
 // (tcgen05.mma), for packed prompts and for chunks over the paged cache.
 //
-// A CTA takes 256 rows (token x head of one kv head's group, token major, so
-// the heads that share a kv head share its K and V tiles) of one sequence as
-// two M = 128 tiles, and walks the keys in blocks of 128:
+// A CTA takes 128 kTiles rows (token x head of one kv head's group, token
+// major, so the heads that share a kv head share its K and V tiles) of one
+// sequence as M = 128 tiles, and walks the keys in blocks of 128:
 //   S = Q K^T  (Q, K in shared memory, 128-byte swizzle; S fp32 in TMEM),
-//   P = exp2(scale S - m), rounded to bf16, written over S in TMEM,
+//   P = exp2(scale S - m), rounded to bf16, written over half of S in TMEM,
 //   O += P V   (P from TMEM, V in shared memory as it lies: keys x D, the
 //               transposed B operand; O fp32 in TMEM).
-// Warps 0-3 and 4-7 are the softmax of the two tiles, one thread per row, so
-// row maxima and sums need no shuffles; warp 8 issues the MMAs; warp 9 loads
-// K and V by TMA into a ring; warps 10-11 mend V blocks that hold positions
-// some row must not see.  While one tile's softmax runs, the tensor core
-// works on the other's products.  The running maximum moves only when a score
+// Four warps per tile are its softmax, one thread per row, so row maxima and
+// sums need no shuffles; then one warp issues the MMAs, one loads K and V by
+// TMA into a ring, and two mend V blocks that hold positions some row must
+// not see.  While one tile's softmax runs, the tensor core works on the
+// other's products.  The running maximum moves only when a score
 // passes it by more than 8 (in log2): P stays below 2^8 and O is rescaled in
 // TMEM by the softmax warps only then.  Maxima, sums and O are fp32.
 //
-// TMEM columns: S/P of the tiles at 0 and 128, O at 256 and 384.
+// TMEM columns: S/P of each tile (128 each), then O of each.
 // Every wait is bounded; on expiry all roles leave their loops, the loader
 // waits for its copies in flight and TMEM is freed.
 #pragma once
@@ -25,19 +25,21 @@
 
 namespace pir2b {
 
-constexpr int kTileThreads = 384;
 constexpr int kSourceRows = 0;   // K and V source: packed rows, else a cache format
 constexpr int kTileKeys = 128;
 
-template <int D>
+// kTiles = 1 fits two CTAs on an SM: one's softmax, prologue and epilogue run
+// beside the other's products.
+template <int D, int kTiles>
 struct TileShape {
+  static constexpr int kThreads = kTiles * 128 + 128;
   static constexpr int kBytes = 128 * D * 2;            // a Q, K or V tile
-  static constexpr int kStages = D == 128 ? 5 : 8;
-  static constexpr int kSmem = (2 + kStages) * kBytes + 1024 /* alignment */ + 256 /* barriers */;
+  static constexpr int kStages = kTiles == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 2 : 5);
+  static constexpr int kSmem = (kTiles + kStages) * kBytes + 1024 /* alignment */ + 256 /* barriers */;
 };
 
 struct TileBarriers {
-  uint64_t full[8], empty[8], q_full[2], s_full[2], p_full[2], o_full[2], to_mend[3], mended[3];
+  uint64_t full[8], empty[8], q_full[2], s_full[2], p_full[2][2], o_full[2], to_mend[3], mended[3];
   uint32_t tmem;
   int spoiled;   // a V block held a value that is not finite at a position hidden from some row
 };
@@ -80,16 +82,19 @@ __device__ __forceinline__ uint64_t smem_desc_rows(uint32_t saddr, uint32_t bloc
   return d;
 }
 
-__device__ __forceinline__ void tmem_st_32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, "
-      "%25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
 }
 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -103,15 +108,6 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const void *tmap, uint64_
       : "memory");
 }
 
-template <int kRegisters>
-__device__ __forceinline__ void registers_up() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
-}
-template <int kRegisters>
-__device__ __forceinline__ void registers_down() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters));
-}
-
 // What a CTA works on.
 struct TileWork {
   int b;              // sequence
@@ -120,34 +116,41 @@ struct TileWork {
   int first;          // position of its first token (prompts: 0)
   int keys;           // positions any row sees
   int all_see;        // positions below this are seen by every row
-  int blocks0, blocks1;   // 128-key blocks of each tile
+  int keys0, keys1;   // positions any row of each tile sees
 
-  __device__ __forceinline__ int blocks(int u) const { return u ? blocks1 : blocks0; }
+  __device__ __forceinline__ int blocks(int u) const { return ((u ? keys1 : keys0) + kTileKeys - 1) / kTileKeys; }
+  // Keys of the tile in block j, in steps of 16 (the products' granularity).
+  __device__ __forceinline__ int steps(int u, int j) const {
+    return (min(kTileKeys, (u ? keys1 : keys0) - j * kTileKeys) + 15) >> 4;
+  }
 };
 
-template <int kSource, int D>
-__global__ void __launch_bounds__(kTileThreads, 1)
-    attention_tile_kernel(const RaggedArgs a, const __grid_constant__ CUtensorMap tm_k,
-                          const __grid_constant__ CUtensorMap tm_v) {
-  using Shape = TileShape<D>;
+template <int kSource, int D, int kTiles>
+__global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 1 : 2)
+    attention_tile_kernel(const RaggedArgs a, const __grid_constant__ CUtensorMap tm_q,
+                          const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+  using Shape = TileShape<D, kTiles>;
+  constexpr int kMmaWarp = kTiles * 4, kRows = kTiles * 128;
+  constexpr uint32_t kOCols = kTiles * 128;       // TMEM: S/P of the tiles, then O
   constexpr int kStages = Shape::kStages, kBytes = Shape::kBytes;
   constexpr int kHalves = D / 64;                 // 64-column blocks of a tile, 16 KB each
   extern __shared__ uint8_t tile_raw[];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tile_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *q_sm = sm, *ring = sm + 2 * kBytes;
+  uint8_t *q_sm = sm, *ring = sm + kTiles * kBytes;
   TileBarriers &bar = *reinterpret_cast<TileBarriers *>(ring + kStages * kBytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  if (warp == 8) {
+  if (warp == kMmaWarp) {
     if (lane == 0) {
       for (int i = 0; i < kStages; ++i) {
         mbar_init(&bar.full[i], 1);
         mbar_init(&bar.empty[i], 1);
       }
-      for (int u = 0; u < 2; ++u) {
-        mbar_init(&bar.q_full[u], 128);
+      for (int u = 0; u < kTiles; ++u) {
+        mbar_init(&bar.q_full[u], a.q_by_tma ? 1 : 128);
         mbar_init(&bar.s_full[u], 1);
-        mbar_init(&bar.p_full[u], 4);
+        mbar_init(&bar.p_full[u][0], 4);
+        mbar_init(&bar.p_full[u][1], 4);
         mbar_init(&bar.o_full[u], 1);
       }
       for (int i = 0; i < 3; ++i) {
@@ -158,10 +161,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       fence_barrier_init();
     }
     __syncwarp();
-    tmem_alloc(&bar.tmem, 512);
+    tmem_alloc(&bar.tmem, kTiles * 256);
     tmem_relinquish();
   }
-  if (warp == 9 && lane == 0) {
+  if (warp == kMmaWarp + 1 && lane == 0) {
+    tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
@@ -172,11 +176,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int kvh = int(blockIdx.x % a.hk), slot = int((gridDim.x - 1 - blockIdx.x) / a.hk);
   TileWork w = {};
   int tile;
-  w.b = unit_of(a, group, 8, slot, tile);
+  w.b = unit_of(a, group, kTiles == 2 ? 8 : 7, slot, tile);
   if (w.b >= 0) {
     w.begin = max(__ldg(a.starts + w.b), 0);
     const int n = int(min(int64_t(__ldg(a.starts + w.b + 1)), a.rows) - w.begin);
-    w.r0 = tile << 8;
+    w.r0 = tile * kRows;
     w.r1 = n * group;
     int length = n;
     if constexpr (kSource != kSourceRows) {
@@ -185,10 +189,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     w.all_see = max(0, min(length, w.first + w.r0 / group + 1));
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < kTiles; ++u) {
       const int last = min(w.r0 + 128 * (u + 1), w.r1) - 1;   // last row of the tile
       const int keys = last < w.r0 + 128 * u ? 0 : max(0, min(length, w.first + last / group + 1));
-      (u ? w.blocks1 : w.blocks0) = (keys + kTileKeys - 1) / kTileKeys;
+      (u ? w.keys1 : w.keys0) = keys;
       w.keys = max(w.keys, keys);
     }
   }
@@ -196,27 +200,38 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bar.tmem;
-  const int blocks = max(w.blocks0, w.blocks1);
+  const int blocks = max(w.blocks(0), w.blocks(1));
   // The rows' limits span at most 256 positions, so at most three blocks hold
   // positions hidden from some row; each has its barriers.
   const int first_mend = w.all_see / kTileKeys;
 
-  if (warp < 8) {
-    registers_up<208>();
+  if (warp < kMmaWarp) {
     const int u = warp >> 2, t = tid & 127;
     const uint32_t lanes = uint32_t(warp & 3) << 21;          // this warp's TMEM lanes
-    const uint32_t s_tm = tmem + lanes + u * 128, o_tm = tmem + lanes + 256 + u * 128;
+    const uint32_t s_tm = tmem + lanes + u * 128, o_tm = tmem + lanes + kOCols + u * 128;
     const int r = w.r0 + u * 128 + t;                         // this thread's row
     const bool valid = w.b >= 0 && r < w.r1;
-    const int limit = valid ? w.first + r / group : -1;       // it sees positions 0 .. limit
+    // Token and head of the CTA's i-th row, by a multiply: exact for i + rest
+    // below 2^21 / group (at most 256 + group, group at most 1024).
+    const int token0 = w.r0 / group;
+    const uint32_t rest = w.r0 - token0 * group, inverse = ((1u << 21) + group - 1) / group;
+    auto token_of = [&](int i, int &head) {
+      const int step = int(((rest + i) * inverse) >> 21);
+      head = kvh * group + int(rest) + i - step * group;
+      return token0 + step;
+    };
+    int my_head;
+    const int my_token = token_of(u * 128 + t, my_head);
+    const int limit = valid ? w.first + my_token : -1;       // it sees positions 0 .. limit
     bool ok = true;
-    if (w.blocks(u) > 0) {
+    if (w.blocks(u) > 0 && !a.q_by_tma) {
       for (int i = t; i < 128 * (D / 8); i += 128) {
         const int qr = i / (D / 8), c = i % (D / 8);
         uint8_t *dst = q_sm + u * kBytes + (c >> 3) * 16384 + qr * 128 + (((c & 7) ^ (qr & 7)) << 4);
-        const int rr = w.r0 + u * 128 + qr;
-        if (rr < w.r1)
-          cp_async_16(dst, a.q + (w.begin + rr / group) * a.q_row + (kvh * group + rr % group) * a.q_head + c * 8);
+        int head;
+        const int token = token_of(u * 128 + qr, head);
+        if (w.r0 + u * 128 + qr < w.r1)
+          cp_async_16(dst, a.q + (w.begin + token) * a.q_row + head * a.q_head + c * 8);
         else
           *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
       }
@@ -224,78 +239,124 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       fence_proxy_async_smem();
       mbar_arrive(&bar.q_full[u]);
     }
-    float top = -INFINITY, mu = 0.f, l = 0.f;
+    float top = -INFINITY, mu = 0.f;
+    float2 sum = make_float2(0.f, 0.f);
     for (int j = 0; j < w.blocks(u); ++j) {
       if (!mbar_wait(&bar.s_full[u], j & 1, kStatusTimeoutEpilogue)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        tmem_ld_32(s_tm + i * 32, s[i]);
-      tmem_ld_wait();
-      const int seen = limit - j * kTileKeys;                 // columns above this are hidden
-      if (__any_sync(0xffffffffu, seen < kTileKeys - 1)) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (i * 32 + c > seen)
-              s[i][c] = 0xff800000u;
+      // Columns above `seen` are hidden.  Only blocks past all_see have any,
+      // and a warp's rows differ in few positions: a chunk of 32 columns is
+      // mostly all seen or all hidden.
+      const int seen = limit - j * kTileKeys;
+      int seen_by_all = kTileKeys, seen_by_any = kTileKeys;
+      if ((j + 1) * kTileKeys > w.all_see) {
+        seen_by_all = __reduce_min_sync(0xffffffffu, seen);
+        seen_by_any = __reduce_max_sync(0xffffffffu, seen);
       }
+      // The scores are read 64 columns at a time, 0 .. 63 twice: once for the
+      // maximum, once for the weights (a row does not fit the registers).
+      uint32_t s[2][32];
       float most = -INFINITY;
+      auto load = [&](int half) {
+        tmem_ld_32(s_tm + half * 64, s[0]);
+        tmem_ld_32(s_tm + half * 64 + 32, s[1]);
+        tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
+          if (seen_by_all < half * 64 + i * 32 + 31) {
 #pragma unroll
-        for (int c = 0; c < 32; ++c)
-          most = fmaxf(most, __uint_as_float(s[i][c]));
+            for (int c = 0; c < 32; ++c)
+              if (half * 64 + i * 32 + c > seen)
+                s[i][c] = 0xff800000u;
+          }
+      };
+      auto maximum = [&]() {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            m0 = max3(m0, __uint_as_float(s[i][c]), __uint_as_float(s[i][c + 1]));
+            m1 = max3(m1, __uint_as_float(s[i][c + 2]), __uint_as_float(s[i][c + 3]));
+          }
+          most = max3(most, m0, m1);
+        }
+      };
+      load(0);
+      maximum();
+      if (seen_by_any >= 64) {
+        load(1);
+        maximum();
+      }
       most *= a.scale_log2;
       if (__any_sync(0xffffffffu, most > top + 8.f)) {
         const float m = fmaxf(top, most);
         const float keep = top == -INFINITY ? 1.f : exp2_fast(top - m);   // nothing summed yet: keep it
         top = m;
         mu = m == -INFINITY ? 0.f : m;
-        l *= keep;
+        sum.x *= keep;
+        sum.y *= keep;
         if (j > 0) {
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            uint32_t o[32];
-            tmem_ld_32(o_tm + i * 32, o);
+#pragma unroll 1
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t o[16];
+            tmem_ld_16(o_tm + i * 16, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
+            for (int c = 0; c < 16; ++c)
               o[c] = __float_as_uint(__uint_as_float(o[c]) * keep);
-            tmem_st_32(o_tm + i * 32, o);
+            tmem_st_16(o_tm + i * 16, o);
           }
         }
       }
+      const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), minus = make_float2(-mu, -mu);
+      // P goes over columns 64 .. 127 of S, which are in registers by then.
+      auto weights = [&](int half) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t p[32];
+        for (int i = 0; i < 2; ++i) {
+          uint32_t p[16];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float x = exp2_fast(__uint_as_float(s[2 * i + c / 16][c * 2 % 32]) * a.scale_log2 - mu);
-          const float y = exp2_fast(__uint_as_float(s[2 * i + c / 16][c * 2 % 32 + 1]) * a.scale_log2 - mu);
-          l += x + y;
-          p[c] = pack_bf16x2(x, y);
+          for (int c = 0; c < 16; ++c) {
+            const float2 x = __ffma2_rn(
+                make_float2(__uint_as_float(s[i][2 * c]), __uint_as_float(s[i][2 * c + 1])), scale2, minus);
+            const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+            sum = __fadd2_rn(sum, e);
+            p[c] = pack_bf16x2(e.x, e.y);
+          }
+          tmem_st_16(s_tm + 64 + half * 32 + i * 16, p);
         }
-        tmem_st_32(s_tm + i * 32, p);
+      };
+      auto ready = [&](int half) {
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&bar.p_full[u][half]);
+      };
+      if (seen_by_any >= 64) {
+        weights(1);
+        ready(1);
+        load(0);
+      } else {
+        const uint32_t none[16] = {};
+        tmem_st_16(s_tm + 96, none);
+        tmem_st_16(s_tm + 112, none);
+        ready(1);
       }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0)
-        mbar_arrive(&bar.p_full[u]);
+      weights(0);
+      ready(0);
     }
     if (ok && w.blocks(u) > 0)
       ok = mbar_wait(&bar.o_full[u], 0, kStatusTimeoutEpilogue);
     tc_fence_after();
     if (ok && w.b >= 0 && w.r0 + u * 128 < w.r1) {
+      const float l = sum.x + sum.y;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const bool spoiled = *reinterpret_cast<volatile int *>(&bar.spoiled) != 0;
-      __nv_bfloat16 *out = a.out + (w.begin + r / group) * a.ldo + (kvh * group + r % group) * D;
+      uint8_t *row_sm = q_sm + u * kBytes + t * (D * 2);
 #pragma unroll 1
       for (int i = 0; i < D / 32; ++i) {
         uint32_t o[32] = {};
@@ -319,34 +380,46 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
           }
         }
-        if (valid) {
+        // The row's 16-byte pieces into the tile that held Q (its products are
+        // done), rotated by row so that a warp's writes spread over the banks.
 #pragma unroll
-          for (int c = 0; c < 32; c += 8)
-            *reinterpret_cast<uint4 *>(out + i * 32 + c) =
-                make_uint4(pack_bf16x2(f[c], f[c + 1]), pack_bf16x2(f[c + 2], f[c + 3]), pack_bf16x2(f[c + 4], f[c + 5]),
-                           pack_bf16x2(f[c + 6], f[c + 7]));
-        }
+        for (int c = 0; c < 32; c += 8)
+          *reinterpret_cast<uint4 *>(row_sm + (((i * 4 + c / 8) ^ (t & 7)) << 4)) =
+              make_uint4(pack_bf16x2(f[c], f[c + 1]), pack_bf16x2(f[c + 2], f[c + 3]), pack_bf16x2(f[c + 4], f[c + 5]),
+                         pack_bf16x2(f[c + 6], f[c + 7]));
+      }
+      // Whole rows at a time to memory, this warp's own 32.
+      __syncwarp();
+      constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces;
+#pragma unroll 4
+      for (int i = 0; i < 32; i += kAtOnce) {
+        const int rr = (warp & 3) * 32 + i + lane / kPieces, piece = lane % kPieces;
+        int head;
+        const int token = token_of(u * 128 + rr, head);
+        const uint4 x = *reinterpret_cast<const uint4 *>(q_sm + u * kBytes + rr * (D * 2) + ((piece ^ (rr & 7)) << 4));
+        if (w.r0 + u * 128 + rr < w.r1)
+          *reinterpret_cast<uint4 *>(a.out + (w.begin + token) * a.ldo + head * D + piece * 8) = x;
       }
     }
   } else {
-    registers_down<80>();
-    if (warp == 8) {
+    if (warp == kMmaWarp) {
       if (elect_one_sync()) {
-        constexpr uint32_t kIdescS = idesc_bf16(128, kTileKeys, false), kIdescO = idesc_bf16(128, D, true);
+        constexpr uint32_t kIdescO = idesc_bf16(128, D, true);
         const uint32_t q_addr = smem_u32(q_sm), ring_addr = smem_u32(ring);
         auto wait = [&](uint64_t *b, int parity) { return mbar_wait(b, uint32_t(parity & 1), kStatusTimeoutMma); };
         auto scores = [&](int u, int item) {
           const uint32_t k_addr = ring_addr + (item % kStages) * kBytes;
+          const uint32_t idesc = idesc_bf16(128, w.steps(u, item / 2) * 16, false);
 #pragma unroll
           for (int s = 0; s < D / 16; ++s) {
             const uint32_t at = (s >> 2) * 16384 + (s & 3) * 32;
-            mma_bf16_ss(tmem + u * 128, smem_desc_sw128(q_addr + u * kBytes + at), smem_desc_sw128(k_addr + at), kIdescS,
+            mma_bf16_ss(tmem + u * 128, smem_desc_sw128(q_addr + u * kBytes + at), smem_desc_sw128(k_addr + at), idesc,
                         s > 0);
           }
           mma_commit(&bar.s_full[u]);
         };
         bool ok = blocks > 0 && wait(&bar.full[0], 0);
-        for (int u = 0; u < 2 && ok; ++u)
+        for (int u = 0; u < kTiles && ok; ++u)
           if (w.blocks(u) > 0) {
             ok = wait(&bar.q_full[u], 0);
             if (ok)
@@ -357,7 +430,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int j = 0; j < blocks && ok; ++j) {
           const int v_item = 2 * j + 1, k_item = 2 * j + 2;
           bool v_ready = false, k_ready = false;
-          for (int u = 0; u < 2 && ok; ++u) {
+          for (int u = 0; u < kTiles && ok; ++u) {
             if (j >= w.blocks(u))
               continue;
             if (!v_ready) {
@@ -367,15 +440,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 ok = wait(&bar.full[v_item % kStages], v_item / kStages);
               v_ready = true;
             }
-            ok = ok && wait(&bar.p_full[u], j);
+            const uint32_t v_addr = ring_addr + (v_item % kStages) * kBytes;
+            const int steps = w.steps(u, j);
+            // Keys 64 .. 127 of the block first: their weights are ready first.
+            bool begun = j > 0;
+            for (int half = 1; half >= 0; --half) {
+              ok = ok && wait(&bar.p_full[u][half], j);
+              if (!ok)
+                break;
+              tc_fence_after();
+#pragma unroll 1
+              for (int s = half * 4; s < min(steps, half * 4 + 4); ++s) {
+                mma_bf16_ts(tmem + kOCols + u * 128, tmem + u * 128 + 64 + s * 8, smem_desc_rows(v_addr + s * 2048, 16384),
+                            kIdescO, begun);
+                begun = true;
+              }
+            }
             if (!ok)
               break;
-            tc_fence_after();
-            const uint32_t v_addr = ring_addr + (v_item % kStages) * kBytes;
-#pragma unroll
-            for (int s = 0; s < kTileKeys / 16; ++s)
-              mma_bf16_ts(tmem + 256 + u * 128, tmem + u * 128 + s * 8, smem_desc_rows(v_addr + s * 2048, 16384), kIdescO,
-                          j > 0 || s > 0);
             if (j + 1 < w.blocks(u)) {
               if (!k_ready) {
                 ok = wait(&bar.full[k_item % kStages], k_item / kStages);
@@ -394,8 +476,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
         }
       }
-    } else if (warp == 9) {
+    } else if (warp == kMmaWarp + 1) {
       if (elect_one_sync()) {
+        if (a.q_by_tma) {
+          for (int u = 0; u < kTiles; ++u) {
+            if (w.blocks(u) == 0)
+              continue;
+            mbar_arrive_expect_tx(&bar.q_full[u], kBytes);
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+              tma_load_3d(q_sm + u * kBytes + h * 16384, &tm_q, &bar.q_full[u], h * 64, kvh * group,
+                          int(w.begin) + (w.r0 + u * 128) / group);
+          }
+        }
         int item = 0;
         for (; item < 2 * blocks; ++item) {
           const int stage = item % kStages;
@@ -413,6 +506,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // No copy is in flight when the CTA ends (at once, unless a wait gave up).
         for (int i = max(0, item - kStages); i < item; ++i)
           mbar_wait(&bar.full[i % kStages], uint32_t((i / kStages) & 1), kStatusTimeoutProducer);
+        if (a.q_by_tma)
+          for (int u = 0; u < kTiles; ++u)
+            if (w.blocks(u) > 0)
+              mbar_wait(&bar.q_full[u], 0, kStatusTimeoutProducer);
       }
     } else {
       // Positions some row of the tiles must not see: those past the keys
@@ -427,29 +524,47 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           break;
         uint8_t *v = ring + (item % kStages) * kBytes;
         const int from = max(0, w.all_see - j * kTileKeys), end = w.keys - j * kTileKeys;
-        bool found = false;
-        for (int i = (warp - 10) * 32 + lane; i < (kTileKeys - from) * (D / 8); i += 64) {
-          const int key = from + i / (D / 8), c = i % (D / 8);
-          uint4 *at = reinterpret_cast<uint4 *>(v + (c >> 3) * 16384 + key * 128 + (((c & 7) ^ (key & 7)) << 4));
+        const int used = min(kTileKeys, (end + 15) & ~15);   // rows the products read
+        auto chunk = [&](int i, int &key) {          // 16-byte chunks of the rows from `from` on
+          key = from + i / (D / 8);
+          const int c = i % (D / 8);
+          return reinterpret_cast<uint4 *>(v + (c >> 3) * 16384 + key * 128 + (((c & 7) ^ (key & 7)) << 4));
+        };
+        const int chunks = (used - from) * (D / 8), first_chunk = (warp - kMmaWarp - 2) * 32 + lane;
+        // 0 times a value that is not finite is NaN, and stays in the sum.
+        const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
+        __nv_bfloat162 sum = zero;
+#pragma unroll 4
+        for (int i = first_chunk; i < chunks; i += 64) {
+          int key;
+          uint4 *at = chunk(i, key);
           if (key >= end) {
             *at = make_uint4(0, 0, 0, 0);
           } else {
+            const uint4 x = *at;
+            const __nv_bfloat162 *pair = reinterpret_cast<const __nv_bfloat162 *>(&x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              sum = __hfma2(pair[e], zero, sum);
+          }
+        }
+        if (__any_sync(0xffffffffu, __hisnan2(sum).x != __nv_bfloat16(0.f) || __hisnan2(sum).y != __nv_bfloat16(0.f))) {
+          for (int i = first_chunk; i < chunks; i += 64) {
+            int key;
+            uint4 *at = chunk(i, key);
             uint4 x = *at;
             uint32_t *word = reinterpret_cast<uint32_t *>(&x);
-            bool bad = false;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               if ((word[e] & 0x7f80u) == 0x7f80u)
-                word[e] &= 0xffff0000u, bad = true;
+                word[e] &= 0xffff0000u;
               if ((word[e] & 0x7f800000u) == 0x7f800000u)
-                word[e] &= 0xffffu, bad = true;
+                word[e] &= 0xffffu;
             }
-            if (bad)
-              *at = x, found = true;
+            *at = x;
           }
-        }
-        if (found)
           *reinterpret_cast<volatile int *>(&bar.spoiled) = 1;
+        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0)
@@ -460,8 +575,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8)
-    tmem_dealloc(tmem, 512);
+  if (warp == kMmaWarp)
+    tmem_dealloc(tmem, kTiles * 256);
 }
 
 } // namespace pir2b

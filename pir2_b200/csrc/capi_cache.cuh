@@ -153,15 +153,16 @@ static int launch_join(int d, const RaggedArgs &a, void *stream) {
                       (a.rows * a.hq + 7) / 8, 1, 1, 256, 0, a, stream);
 }
 
-// 3-D map over packed bf16 rows [rows, heads, d], box of 128 rows of one head
-// and 64 columns in 128-byte swizzled rows.
-static int make_rows_map(CUtensorMap *map, const void *base, int64_t rows, int heads, int d, int64_t row, int64_t head) {
+// 3-D map over packed bf16 rows [rows, heads, d], box of 64 columns in
+// 128-byte swizzled rows.
+static int make_rows_map(CUtensorMap *map, const void *base, int64_t rows, int heads, int d, int64_t row, int64_t head,
+                         int box_heads, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr)
     return fail(PIR2B_ECUDA, "cuTensorMapEncodeTiled entry point unavailable");
   const cuuint64_t dims[3] = {cuuint64_t(d), cuuint64_t(heads), cuuint64_t(rows)};
   const cuuint64_t strides[2] = {cuuint64_t(head) * 2, cuuint64_t(row) * 2};
-  const cuuint32_t box[3] = {64, 1, kTileKeys};
+  const cuuint32_t box[3] = {64, cuuint32_t(box_heads), cuuint32_t(box_rows)};
   const cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -169,24 +170,39 @@ static int make_rows_map(CUtensorMap *map, const void *base, int64_t rows, int h
   return r == CUDA_SUCCESS ? PIR2B_OK : fail(PIR2B_ECUDA, "cuTensorMapEncodeTiled (rows) failed (%d)", int(r));
 }
 
-template <int kSource, int D>
-static int launch_tile(const char *what, const RaggedArgs &a, const CUtensorMap &tm_k, const CUtensorMap &tm_v,
-                       void *stream) {
-  const int64_t grid = (a.rows * (a.hq / a.hk) / 256 + a.batch) * a.hk;
+// A query tile is one box (its heads, then its tokens) when the group divides
+// 128; otherwise its rows are gathered.
+static int make_q_map(CUtensorMap *map, RaggedArgs *a, int d) {
+  const int group = a->hq / a->hk;
+  a->q_by_tma = 128 % group == 0;
+  return make_rows_map(map, a->q, a->rows, a->hq, d, a->q_row, a->q_head, a->q_by_tma ? group : 1,
+                       a->q_by_tma ? 128 / group : 128);
+}
+
+template <int kSource, int D, int kTiles>
+static int launch_tile(const char *what, const RaggedArgs &a, const CUtensorMap &tm_q, const CUtensorMap &tm_k,
+                       const CUtensorMap &tm_v, void *stream) {
+  const int64_t grid = (a.rows * (a.hq / a.hk) / (128 * kTiles) + a.batch) * a.hk;
   if (grid > 0x7fffffff)
     return fail(PIR2B_EINVAL, "%s: too many rows", what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(grid), 1, 1);
-  cfg.blockDim = dim3(kTileThreads, 1, 1);
-  cfg.dynamicSmemBytes = TileShape<D>::kSmem;
+  cfg.blockDim = dim3(TileShape<D, kTiles>::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = TileShape<D, kTiles>::kSmem;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, attention_tile_kernel<kSource, D>, a, tm_k, tm_v), what);
+  return cuda_status(cudaLaunchKernelEx(&cfg, attention_tile_kernel<kSource, D, kTiles>, a, tm_q, tm_k, tm_v), what);
 }
+
+// Tiles per CTA of the tile kernel.  One tile and two CTAs on an SM cover the
+// latencies of a CTA's start and end with another's products (64 prompts of
+// 280-816 tokens: 197 us against 218); two tiles read K and V half as often,
+// which carries long prompts (8192 tokens: 241 us against 255).
+static int tiles_per_cta(int64_t rows, int batch) { return rows / batch >= 2048 ? 2 : 1; }
 
 // Dynamic shared memory above the default limit, once per device.
 static int cache_kernel_attributes(DeviceInfo *dev) {
@@ -197,8 +213,10 @@ static int cache_kernel_attributes(DeviceInfo *dev) {
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheBf16, 128, 2>), few_smem<128, 2>()},
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheInt8, 128, 2>), few_smem<128, 2>()},
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 128, 2>), few_smem<128, 2>()},
-      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 64>), TileShape<64>::kSmem},
-      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 128>), TileShape<128>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 64, 1>), TileShape<64, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 128, 1>), TileShape<128, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 64, 2>), TileShape<64, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 128, 2>), TileShape<128, 2>::kSmem},
   };
   for (const auto &k : kernels)
     if (int r = cuda_status(cudaFuncSetAttribute(k.first, cudaFuncAttributeMaxDynamicSharedMemorySize, k.second),
@@ -259,13 +277,16 @@ int pir2b_prompt_attention(const void *q, int64_t q_row, int64_t q_head, const v
   a.scale_log2 = scale * 1.4426950408889634f;
   if (int r = cache_kernel_attributes(dev))
     return r;
-  CUtensorMap tm_k, tm_v;
-  if (int r = make_rows_map(&tm_k, k, rows, hk, head_dim, k_row, k_head))
+  CUtensorMap tm_q, tm_k, tm_v;
+  if (int r = make_rows_map(&tm_k, k, rows, hk, head_dim, k_row, k_head, 1, kTileKeys))
     return r;
-  if (int r = make_rows_map(&tm_v, v, rows, hk, head_dim, v_row, v_head))
+  if (int r = make_rows_map(&tm_v, v, rows, hk, head_dim, v_row, v_head, 1, kTileKeys))
     return r;
-  return head_dim == 64 ? launch_tile<kSourceRows, 64>("prompt_attention launch", a, tm_k, tm_v, stream)
-                        : launch_tile<kSourceRows, 128>("prompt_attention launch", a, tm_k, tm_v, stream);
+  if (int r = make_q_map(&tm_q, &a, head_dim))
+    return r;
+  const bool two = tiles_per_cta(rows, int(batch)) == 2;
+  return head_dim == 64 ? (two ? launch_tile<kSourceRows, 64, 2> : launch_tile<kSourceRows, 64, 1>)(what, a, tm_q, tm_k, tm_v, stream)
+                        : (two ? launch_tile<kSourceRows, 128, 2> : launch_tile<kSourceRows, 128, 1>)(what, a, tm_q, tm_k, tm_v, stream);
 }
 
 int pir2b_cache_write(const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row,
