@@ -482,7 +482,8 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const RaggedArgs a)
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1)
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-  const float f = ml.x == m ? 1.f : exp2_fast(ml.x - m);
+  // A split that saw nothing has a sum of 0 and may have written no values.
+  const float f = ml.y == 0.f ? 0.f : ml.x == m ? 1.f : exp2_fast(ml.x - m);
   float total = f * ml.y;
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1)
@@ -490,6 +491,8 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const RaggedArgs a)
   float sum[E] = {};
   for (int s = 0; s < a.splits; ++s) {
     const float fs = __shfl_sync(0xffffffffu, f, s);
+    if (fs == 0.f)
+      continue;
     const float *p = a.part_o + (s * apart + item) * D + lane * E;
 #pragma unroll
     for (int e = 0; e < E; ++e)

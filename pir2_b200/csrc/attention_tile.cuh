@@ -30,12 +30,18 @@ constexpr int kTileKeys = 128;
 
 // kTiles = 1 fits two CTAs on an SM: one's softmax, prologue and epilogue run
 // beside the other's products.
-template <int D, int kTiles>
+template <int kSource, int D, int kTiles>
 struct TileShape {
-  static constexpr int kThreads = kTiles * 128 + 128;
+  static constexpr bool kScaled = kSource == kCacheInt8 || kSource == kCacheE4m3;
+  static constexpr int kThreads = kTiles * 128 + 128 + (kScaled ? 128 : 0);
   static constexpr int kBytes = 128 * D * 2;            // a Q, K or V tile
-  static constexpr int kStages = kTiles == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 2 : 5);
-  static constexpr int kSmem = (kTiles + kStages) * kBytes + 1024 /* alignment */ + 256 /* barriers */;
+  static constexpr int kStages = kTiles == 2 ? (D == 128 ? (kScaled ? 4 : 5) : 8) : (D == 128 ? 2 : 5);
+  // Blocks whose scales are kept: the loader writes block j's when K item 2 j
+  // has a stage, which item 2 j - kStages has left; it must not be before V
+  // item 2 (j - kDepth) + 1 has.
+  static constexpr int kDepth = (kStages + 2) / 2;
+  static constexpr int kScaleBytes = kScaled ? kDepth * 2 * kTileKeys * 4 : 0;
+  static constexpr int kSmem = (kTiles + kStages) * kBytes + kScaleBytes + 1024 /* alignment */ + 256 /* barriers */;
 };
 
 struct TileBarriers {
@@ -100,6 +106,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 3-D and 4-D tiled loads into this CTA's shared memory.
+__device__ __forceinline__ void tma_load_4d(void *dst, const void *tmap, uint64_t *bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+          "r"(smem_u32(dst)),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
 __device__ __forceinline__ void tma_load_3d(void *dst, const void *tmap, uint64_t *bar, int x, int y, int z) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
@@ -108,12 +122,13 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const void *tmap, uint64_
       : "memory");
 }
 
-// What a CTA works on.
+// What a CTA works on.  Positions count from `base`, the first of its split.
 struct TileWork {
   int b;              // sequence
   int r0, r1;         // its rows [r0, min(r0 + 256, r1)) of the sequence's token x head rows
   int64_t begin;      // packed row of its first token
-  int first;          // position of its first token (prompts: 0)
+  int base;           // multiple of 128
+  int first;          // position of the sequence's first row's token
   int keys;           // positions any row sees
   int all_see;        // positions below this are seen by every row
   int keys0, keys1;   // positions any row of each tile sees
@@ -126,10 +141,11 @@ struct TileWork {
 };
 
 template <int kSource, int D, int kTiles>
-__global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 1 : 2)
+__global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTiles == 2 ? 1 : 2)
     attention_tile_kernel(const RaggedArgs a, const __grid_constant__ CUtensorMap tm_q,
                           const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
-  using Shape = TileShape<D, kTiles>;
+  using Shape = TileShape<kSource, D, kTiles>;
+  constexpr bool kScaled = Shape::kScaled, kPaged = kSource != kSourceRows;
   constexpr int kMmaWarp = kTiles * 4, kRows = kTiles * 128;
   constexpr uint32_t kOCols = kTiles * 128;       // TMEM: S/P of the tiles, then O
   constexpr int kStages = Shape::kStages, kBytes = Shape::kBytes;
@@ -137,13 +153,14 @@ __global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 
   extern __shared__ uint8_t tile_raw[];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tile_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *q_sm = sm, *ring = sm + kTiles * kBytes;
-  TileBarriers &bar = *reinterpret_cast<TileBarriers *>(ring + kStages * kBytes);
+  float *scales = reinterpret_cast<float *>(ring + kStages * kBytes);   // [kDepth][K, V][128]
+  TileBarriers &bar = *reinterpret_cast<TileBarriers *>(ring + kStages * kBytes + Shape::kScaleBytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (warp == kMmaWarp) {
     if (lane == 0) {
       for (int i = 0; i < kStages; ++i) {
-        mbar_init(&bar.full[i], 1);
+        mbar_init(&bar.full[i], kScaled ? 4 : 1);
         mbar_init(&bar.empty[i], 1);
       }
       for (int u = 0; u < kTiles; ++u) {
@@ -166,14 +183,17 @@ __global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 
   }
   if (warp == kMmaWarp + 1 && lane == 0) {
     tma_prefetch_desc(&tm_q);
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_v);
+    if (!kScaled) {
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+    }
   }
   pdl_wait();
   pdl_launch_dependents();
   const int group = a.hq / a.hk;
   // Later rows see more keys: they start first.
-  const int kvh = int(blockIdx.x % a.hk), slot = int((gridDim.x - 1 - blockIdx.x) / a.hk);
+  const int unit = int((gridDim.x - 1 - blockIdx.x) / a.splits), split = int(blockIdx.x % a.splits);
+  const int kvh = unit % a.hk, slot = unit / a.hk;
   TileWork w = {};
   int tile;
   w.b = unit_of(a, group, kTiles == 2 ? 8 : 7, slot, tile);
@@ -183,7 +203,7 @@ __global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 
     w.r0 = tile * kRows;
     w.r1 = n * group;
     int length = n;
-    if constexpr (kSource != kSourceRows) {
+    if constexpr (kPaged) {
       length = cache_length(a.c, a.lengths, w.b);
       w.first = first_new_position(a.lengths, w.b, n);
     }
@@ -195,6 +215,12 @@ __global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 
       (u ? w.keys1 : w.keys0) = keys;
       w.keys = max(w.keys, keys);
     }
+    const int per = ((w.keys + kTileKeys - 1) / kTileKeys + a.splits - 1) / a.splits * kTileKeys;   // of a split
+    w.base = split * per;
+    w.keys0 = max(0, min(w.keys0 - w.base, per));
+    w.keys1 = max(0, min(w.keys1 - w.base, per));
+    w.keys = max(w.keys0, w.keys1);
+    w.all_see = max(0, w.all_see - w.base);
   }
   tc_fence_before();
   __syncthreads();
@@ -222,7 +248,7 @@ __global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 
     };
     int my_head;
     const int my_token = token_of(u * 128 + t, my_head);
-    const int limit = valid ? w.first + my_token : -1;       // it sees positions 0 .. limit
+    const int limit = valid ? w.first + my_token - w.base : -1;   // it sees positions 0 .. limit
     bool ok = true;
     if (w.blocks(u) > 0 && !a.q_by_tma) {
       for (int i = t; i < 128 * (D / 8); i += 128) {
@@ -260,10 +286,24 @@ __global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 
       // maximum, once for the weights (a row does not fit the registers).
       uint32_t s[2][32];
       float most = -INFINITY;
+      const float *block_scales = scales + (j % Shape::kDepth) * 2 * kTileKeys;
       auto load = [&](int half) {
         tmem_ld_32(s_tm + half * 64, s[0]);
         tmem_ld_32(s_tm + half * 64 + 32, s[1]);
         tmem_ld_wait();
+        if constexpr (kScaled) {
+          const float4 *k_scale = reinterpret_cast<const float4 *>(block_scales + half * 64);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              const float4 x = k_scale[(i * 32 + c) / 4];
+              const float2 y = __fmul2_rn(make_float2(__uint_as_float(s[i][c]), __uint_as_float(s[i][c + 1])), make_float2(x.x, x.y));
+              const float2 z = __fmul2_rn(make_float2(__uint_as_float(s[i][c + 2]), __uint_as_float(s[i][c + 3])), make_float2(x.z, x.w));
+              s[i][c] = __float_as_uint(y.x), s[i][c + 1] = __float_as_uint(y.y);
+              s[i][c + 2] = __float_as_uint(z.x), s[i][c + 3] = __float_as_uint(z.y);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           if (seen_by_all < half * 64 + i * 32 + 31) {
@@ -322,8 +362,15 @@ __global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 
           for (int c = 0; c < 16; ++c) {
             const float2 x = __ffma2_rn(
                 make_float2(__uint_as_float(s[i][2 * c]), __uint_as_float(s[i][2 * c + 1])), scale2, minus);
-            const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+            float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
             sum = __fadd2_rn(sum, e);
+            if constexpr (kScaled) {
+              const float2 v = *reinterpret_cast<const float2 *>(block_scales + kTileKeys + half * 64 + i * 32 + 2 * c);
+              if (seen_by_all < half * 64 + i * 32 + 31)   // a hidden row's scale may be anything
+                e = make_float2(e.x == 0.f ? 0.f : e.x * v.x, e.y == 0.f ? 0.f : e.y * v.y);
+              else
+                e = __fmul2_rn(e, v);
+            }
             p[c] = pack_bf16x2(e.x, e.y);
           }
           tmem_st_16(s_tm + 64 + half * 32 + i * 16, p);
@@ -354,7 +401,10 @@ __global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 
     tc_fence_after();
     if (ok && w.b >= 0 && w.r0 + u * 128 < w.r1) {
       const float l = sum.x + sum.y;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = l == 0.f ? 0.f : a.splits > 1 ? 1.f : 1.f / l;   // splits are divided when joined
+      const int64_t part = (int64_t(split) * a.rows + w.begin + my_token) * a.hq + my_head;
+      if (a.splits > 1 && valid)
+        a.part_ml[part] = make_float2(top, l);
       const bool spoiled = *reinterpret_cast<volatile int *>(&bar.spoiled) != 0;
       uint8_t *row_sm = q_sm + u * kBytes + t * (D * 2);
 #pragma unroll 1
@@ -371,14 +421,29 @@ __global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 
         if (spoiled) {
           // Values that are not finite were left out of the products from
           // position all_see on: they go to the rows that see them.
-          for (int key = w.all_see; key <= limit; ++key) {
-            const __nv_bfloat16 *v = a.v + (w.begin + key) * a.v_row + kvh * a.v_head + i * 32;
+          for (int key = w.all_see; key <= min(limit, w.keys - 1); ++key) {
+            const __nv_bfloat16 *v;
+            if constexpr (kPaged) {
+              const int64_t page = max(0, page_of(a.c, w.b, w.base + key));
+              const int64_t slot = (int64_t(kvh) << a.c.shift) + (key & ((1 << a.c.shift) - 1));
+              v = static_cast<const __nv_bfloat16 *>(a.c.v) + page * a.c.v_page + slot * D + i * 32;
+            } else {
+              v = a.v + (w.begin + w.base + key) * a.v_row + kvh * a.v_head + i * 32;
+            }
             for (int c = 0; c < 32; ++c) {
               const float x = __bfloat162float(v[c]);
               if (!(fabsf(x) < INFINITY))
                 f[c] += x;
             }
           }
+        }
+        if (a.splits > 1) {
+          if (valid && w.blocks(u) > 0) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4)
+              *reinterpret_cast<float4 *>(a.part_o + part * D + i * 32 + c) = make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]);
+          }
+          continue;
         }
         // The row's 16-byte pieces into the tile that held Q (its products are
         // done), rotated by row so that a warp's writes spread over the banks.
@@ -392,7 +457,7 @@ __global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 
       __syncwarp();
       constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces;
 #pragma unroll 4
-      for (int i = 0; i < 32; i += kAtOnce) {
+      for (int i = a.splits > 1 ? 32 : 0; i < 32; i += kAtOnce) {
         const int rr = (warp & 3) * 32 + i + lane / kPieces, piece = lane % kPieces;
         int head;
         const int token = token_of(u * 128 + rr, head);
@@ -434,7 +499,7 @@ __global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 
             if (j >= w.blocks(u))
               continue;
             if (!v_ready) {
-              if ((j + 1) * kTileKeys > w.all_see)
+              if (!kScaled && (j + 1) * kTileKeys > w.all_see)
                 ok = wait(&bar.mended[j - first_mend], 0);
               else
                 ok = wait(&bar.full[v_item % kStages], v_item / kStages);
@@ -477,39 +542,139 @@ __global__ void __launch_bounds__(TileShape<D, kTiles>::kThreads, kTiles == 2 ? 
         }
       }
     } else if (warp == kMmaWarp + 1) {
-      if (elect_one_sync()) {
-        if (a.q_by_tma) {
-          for (int u = 0; u < kTiles; ++u) {
-            if (w.blocks(u) == 0)
-              continue;
-            mbar_arrive_expect_tx(&bar.q_full[u], kBytes);
+      if (a.q_by_tma && lane < kTiles && w.blocks(lane) > 0) {
+        mbar_arrive_expect_tx(&bar.q_full[lane], kBytes);
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h)
-              tma_load_3d(q_sm + u * kBytes + h * 16384, &tm_q, &bar.q_full[u], h * 64, kvh * group,
-                          int(w.begin) + (w.r0 + u * 128) / group);
+        for (int h = 0; h < kHalves; ++h)
+          tma_load_3d(q_sm + lane * kBytes + h * 16384, &tm_q, &bar.q_full[lane], h * 64, kvh * group,
+                      int(w.begin) + (w.r0 + lane * 128) / group);
+      }
+      // Item 2 j is block j's K, item 2 j + 1 its V.  From pages, a lane per
+      // page copies it (a bad page reads page 0: any values do).
+      int item = 0, page = 0;
+      bool mine = lane == 0;
+      for (; !kScaled && item < 2 * blocks; ++item) {
+        const int stage = item % kStages, j = item >> 1;
+        if constexpr (kPaged) {
+          if (!(item & 1)) {
+            const int at = j * kTileKeys + (lane << a.c.shift);
+            mine = (lane << a.c.shift) < kTileKeys && at < w.keys;
+            if (mine)
+              page = max(0, page_of(a.c, w.b, w.base + at));
           }
         }
-        int item = 0;
-        for (; item < 2 * blocks; ++item) {
-          const int stage = item % kStages;
-          if (item >= kStages && !mbar_wait(&bar.empty[stage], uint32_t((item / kStages - 1) & 1), kStatusTimeoutProducer))
-            break;
-          mbar_arrive_expect_tx(&bar.full[stage], kBytes);
+        const int copies = __popc(__ballot_sync(0xffffffffu, mine));
+        bool free_stage = true;
+        if (item >= kStages)
+          free_stage = mbar_wait(&bar.empty[stage], uint32_t((item / kStages - 1) & 1), kStatusTimeoutProducer);
+        if (!__all_sync(0xffffffffu, free_stage))
+          break;
+        if (lane == 0)
+          mbar_arrive_expect_tx(&bar.full[stage], kPaged ? (copies << a.c.shift) * D * 2 : kBytes);
+        __syncwarp();
+        if (mine) {
           const void *map = (item & 1) ? &tm_v : &tm_k;
 #pragma unroll
-          for (int h = 0; h < kHalves; ++h)
-            tma_load_3d(ring + stage * kBytes + h * 16384, map, &bar.full[stage], h * 64, kvh,
-                        int(w.begin) + (item >> 1) * kTileKeys);
-          if ((item & 1) && ((item >> 1) + 1) * kTileKeys > w.all_see)
-            mbar_arrive(&bar.to_mend[(item >> 1) - first_mend]);
+          for (int h = 0; h < kHalves; ++h) {
+            uint8_t *dst = ring + stage * kBytes + h * 16384;
+            if constexpr (kPaged)
+              tma_load_4d(dst + (lane << a.c.shift) * 128, map, &bar.full[stage], h * 64, 0, kvh, page);
+            else
+              tma_load_3d(dst, map, &bar.full[stage], h * 64, kvh, int(w.begin) + w.base + j * kTileKeys);
+          }
         }
-        // No copy is in flight when the CTA ends (at once, unless a wait gave up).
-        for (int i = max(0, item - kStages); i < item; ++i)
+        if (lane == 0 && (item & 1) && (j + 1) * kTileKeys > w.all_see)
+          mbar_arrive(&bar.to_mend[j - first_mend]);
+      }
+      // No copy is in flight when the CTA ends (at once, unless a wait gave up).
+      if (lane == 0) {
+        for (int i = max(0, item - kStages); !kScaled && i < item; ++i)
           mbar_wait(&bar.full[i % kStages], uint32_t((i / kStages) & 1), kStatusTimeoutProducer);
-        if (a.q_by_tma)
-          for (int u = 0; u < kTiles; ++u)
-            if (w.blocks(u) > 0)
-              mbar_wait(&bar.q_full[u], 0, kStatusTimeoutProducer);
+        for (int u = 0; u < kTiles && a.q_by_tma; ++u)
+          if (w.blocks(u) > 0)
+            mbar_wait(&bar.q_full[u], 0, kStatusTimeoutProducer);
+      }
+    } else if (kScaled) {
+      if constexpr (kScaled) {
+        // Four warps turn codes into bf16 tiles: 16-byte runs of a row, one
+        // item's loads in flight while the one before is converted.  Rows past
+        // the keys become 0.
+        constexpr int kRuns = D / 16, kLoads = kRuns * kTileKeys / 128, kRowStep = 128 / kRuns;
+        const int t = tid - (kMmaWarp + 4) * 32, run = t % kRuns, row0 = t / kRuns;
+        if (t >= 0) {
+          const uint8_t *codes[2] = {static_cast<const uint8_t *>(a.c.k), static_cast<const uint8_t *>(a.c.v)};
+          const int page_mask = (1 << a.c.shift) - 1;
+          uint4 held[2][kLoads];
+          int page = -1;                           // of the block's 16 (lane % 8) .. + 15
+          auto fetch = [&](int item) {
+            const int j = item >> 1, which = item & 1;
+            if (which == 0) {
+              const int at = j * kTileKeys + (lane & 7) * 16;
+              page = at < w.keys ? page_of(a.c, w.b, w.base + at) : -1;
+            }
+            const int64_t apart = which ? a.c.v_page : a.c.k_page;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+              const int row = row0 + i * kRowStep, key = j * kTileKeys + row;
+              const int64_t of = __shfl_sync(0xffffffffu, page, row >> 4);
+              uint4 x = make_uint4(0, 0, 0, 0);
+              if (of >= 0 && key < w.keys)
+                x = __ldg(reinterpret_cast<const uint4 *>(
+                    codes[which] + of * apart + ((int64_t(kvh) << a.c.shift) + (key & page_mask)) * D + run * 16));
+              held[which][i] = x;
+            }
+          };
+          auto store = [&](int item) {
+            const int stage = item % kStages;
+            uint8_t *dst = ring + stage * kBytes + (run >> 2) * 16384;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+              const int row = row0 + i * kRowStep;
+              const uint4 x = held[item & 1][i];
+              uint4 lo, hi;
+              codes_to_bf16<kSource>(x.x, lo.x, lo.y);
+              codes_to_bf16<kSource>(x.y, lo.z, lo.w);
+              codes_to_bf16<kSource>(x.z, hi.x, hi.y);
+              codes_to_bf16<kSource>(x.w, hi.z, hi.w);
+              const int piece = (run & 3) * 2;
+              *reinterpret_cast<uint4 *>(dst + row * 128 + ((piece ^ (row & 7)) << 4)) = lo;
+              *reinterpret_cast<uint4 *>(dst + row * 128 + (((piece + 1) ^ (row & 7)) << 4)) = hi;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0)
+              mbar_arrive(&bar.full[stage]);
+          };
+          auto wait_free = [&](int item) {
+            return item < kStages ||
+                   mbar_wait(&bar.empty[item % kStages], uint32_t((item / kStages - 1) & 1), kStatusTimeoutProducer);
+          };
+          if (blocks > 0)
+            fetch(0);
+          for (int j = 0; j < blocks; ++j) {
+            // The block's scales: a thread per row.
+            const int key = j * kTileKeys + t;
+            const int64_t of = __shfl_sync(0xffffffffu, page, (t >> 4) & 7);
+            float k_scale = 0.f, v_scale = 0.f;
+            if (of >= 0 && key < w.keys) {
+              const int64_t slot = (int64_t(kvh) << a.c.shift) + (key & page_mask);
+              k_scale = __ldg(a.c.ks + of * a.c.ks_page + slot);
+              v_scale = __ldg(a.c.vs + of * a.c.vs_page + slot);
+            }
+            fetch(2 * j + 1);
+            if (!__all_sync(0xffffffffu, wait_free(2 * j)))
+              break;
+            float *mine = scales + (j % Shape::kDepth) * 2 * kTileKeys;
+            mine[t] = k_scale;
+            mine[kTileKeys + t] = v_scale;
+            store(2 * j);
+            if (j + 1 < blocks)
+              fetch(2 * j + 2);
+            if (!__all_sync(0xffffffffu, wait_free(2 * j + 1)))
+              break;
+            store(2 * j + 1);
+          }
+        }
       }
     } else {
       // Positions some row of the tiles must not see: those past the keys

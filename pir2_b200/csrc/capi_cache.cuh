@@ -116,6 +116,7 @@ static int launch_rows(bool write, int format, int d, const CacheRowsArgs &a, vo
 }
 
 constexpr int kFewWaves = 2;
+constexpr int kFewRows = 32;   // rows a sequence has in a kv head, up to which the few-row kernel takes it
 
 // How the few-row kernel covers a call: rows per unit, grid slots and splits.
 struct FewPlan {
@@ -148,11 +149,6 @@ static int launch_attention_few(const FewPlan &p, int d, const RaggedArgs &a, vo
   return p.nt == 1 ? launch_attention_few<kFormat, 128, 1>(p, a, stream) : launch_attention_few<kFormat, 128, 2>(p, a, stream);
 }
 
-static int launch_join(int d, const RaggedArgs &a, void *stream) {
-  return launch_cache("cache_attention join launch", d == 64 ? attention_join_kernel<64> : attention_join_kernel<128>,
-                      (a.rows * a.hq + 7) / 8, 1, 1, 256, 0, a, stream);
-}
-
 // 3-D map over packed bf16 rows [rows, heads, d], box of 64 columns in
 // 128-byte swizzled rows.
 static int make_rows_map(CUtensorMap *map, const void *base, int64_t rows, int heads, int d, int64_t row, int64_t head,
@@ -182,13 +178,13 @@ static int make_q_map(CUtensorMap *map, RaggedArgs *a, int d) {
 template <int kSource, int D, int kTiles>
 static int launch_tile(const char *what, const RaggedArgs &a, const CUtensorMap &tm_q, const CUtensorMap &tm_k,
                        const CUtensorMap &tm_v, void *stream) {
-  const int64_t grid = (a.rows * (a.hq / a.hk) / (128 * kTiles) + a.batch) * a.hk;
+  const int64_t grid = (a.rows * (a.hq / a.hk) / (128 * kTiles) + a.batch) * a.hk * a.splits;
   if (grid > 0x7fffffff)
     return fail(PIR2B_EINVAL, "%s: too many rows", what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(grid), 1, 1);
-  cfg.blockDim = dim3(TileShape<D, kTiles>::kThreads, 1, 1);
-  cfg.dynamicSmemBytes = TileShape<D, kTiles>::kSmem;
+  cfg.blockDim = dim3(TileShape<kSource, D, kTiles>::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = TileShape<kSource, D, kTiles>::kSmem;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -204,6 +200,73 @@ static int launch_tile(const char *what, const RaggedArgs &a, const CUtensorMap 
 // which carries long prompts (8192 tokens: 241 us against 255).
 static int tiles_per_cta(int64_t rows, int batch) { return rows / batch >= 2048 ? 2 : 1; }
 
+// 4-D map over bf16 pages [pages, hk, page, d], box of one page of one head
+// and 64 columns in 128-byte swizzled rows.
+static int make_pages_map(CUtensorMap *map, const void *base, const CachePages &c, int d, int64_t page_stride) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr)
+    return fail(PIR2B_ECUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  const cuuint64_t page = cuuint64_t(1) << c.shift;
+  const cuuint64_t dims[4] = {cuuint64_t(d), page, cuuint64_t(c.hk), cuuint64_t(c.pages)};
+  const cuuint64_t strides[3] = {cuuint64_t(d) * 2, page * d * 2, cuuint64_t(page_stride) * 2};
+  const cuuint32_t box[4] = {64, cuuint32_t(page), 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? PIR2B_OK : fail(PIR2B_ECUDA, "cuTensorMapEncodeTiled (pages) failed (%d)", int(r));
+}
+
+// How a call of cache_attention runs: the few-row kernel (tiles = 0) or
+// 128-row tiles, and its splits along the keys.
+struct CachePlan {
+  int tiles;
+  FewPlan few;
+  int splits;
+};
+
+static CachePlan plan_cache(int64_t rows, int hq, int hk, int batch, int64_t positions, int format, int sms) {
+  CachePlan p = {};
+  const int64_t per_sequence = (rows + batch - 1) / batch * (hq / hk);
+  if (per_sequence <= kFewRows) {
+    p.few = plan_few(rows, hq, hk, batch, positions, sms);
+    p.splits = p.few.splits;
+    return p;
+  }
+  p.tiles = format != kCacheBf16 || per_sequence > 128 ? 2 : 1;
+  const int64_t ctas = batch * ((per_sequence + 128 * p.tiles - 1) / (128 * p.tiles)) * hk;
+  p.splits = int(std::max<int64_t>(1, std::min<int64_t>({sms * (3 - p.tiles) / ctas, positions / (4 * kTileKeys), 32})));
+  return p;
+}
+
+template <int kSource, int D>
+static int launch_cache_tile(const CachePlan &p, RaggedArgs a, void *stream) {
+  CUtensorMap tm_q, tm_k = {}, tm_v = {};
+  if (int r = make_q_map(&tm_q, &a, D))
+    return r;
+  if constexpr (kSource == kCacheBf16) {
+    if (int r = make_pages_map(&tm_k, a.c.k, a.c, D, a.c.k_page))
+      return r;
+    if (int r = make_pages_map(&tm_v, a.c.v, a.c, D, a.c.v_page))
+      return r;
+    if (p.tiles == 1)
+      return launch_tile<kSource, D, 1>("cache_attention launch", a, tm_q, tm_k, tm_v, stream);
+  }
+  return launch_tile<kSource, D, 2>("cache_attention launch", a, tm_q, tm_k, tm_v, stream);
+}
+
+template <int kFormat>
+static int launch_cache_attention(const CachePlan &p, int d, const RaggedArgs &a, void *stream) {
+  if (p.tiles == 0)
+    return launch_attention_few<kFormat>(p.few, d, a, stream);
+  return d == 64 ? launch_cache_tile<kFormat, 64>(p, a, stream) : launch_cache_tile<kFormat, 128>(p, a, stream);
+}
+
+static int launch_join(int d, const RaggedArgs &a, void *stream) {
+  return launch_cache("cache_attention join launch", d == 64 ? attention_join_kernel<64> : attention_join_kernel<128>,
+                      (a.rows * a.hq + 7) / 8, 1, 1, 256, 0, a, stream);
+}
+
 // Dynamic shared memory above the default limit, once per device.
 static int cache_kernel_attributes(DeviceInfo *dev) {
   std::lock_guard<std::mutex> lock(g_mutex);
@@ -213,10 +276,18 @@ static int cache_kernel_attributes(DeviceInfo *dev) {
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheBf16, 128, 2>), few_smem<128, 2>()},
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheInt8, 128, 2>), few_smem<128, 2>()},
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 128, 2>), few_smem<128, 2>()},
-      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 64, 1>), TileShape<64, 1>::kSmem},
-      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 128, 1>), TileShape<128, 1>::kSmem},
-      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 64, 2>), TileShape<64, 2>::kSmem},
-      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 128, 2>), TileShape<128, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 64, 1>), TileShape<kSourceRows, 64, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 64, 2>), TileShape<kSourceRows, 64, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 128, 1>), TileShape<kSourceRows, 128, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 128, 2>), TileShape<kSourceRows, 128, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kCacheBf16, 64, 1>), TileShape<kCacheBf16, 64, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kCacheBf16, 64, 2>), TileShape<kCacheBf16, 64, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kCacheBf16, 128, 1>), TileShape<kCacheBf16, 128, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kCacheBf16, 128, 2>), TileShape<kCacheBf16, 128, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kCacheInt8, 64, 2>), TileShape<kCacheInt8, 64, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kCacheInt8, 128, 2>), TileShape<kCacheInt8, 128, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kCacheE4m3, 64, 2>), TileShape<kCacheE4m3, 64, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kCacheE4m3, 128, 2>), TileShape<kCacheE4m3, 128, 2>::kSmem},
   };
   for (const auto &k : kernels)
     if (int r = cuda_status(cudaFuncSetAttribute(k.first, cudaFuncAttributeMaxDynamicSharedMemorySize, k.second),
@@ -275,6 +346,7 @@ int pir2b_prompt_attention(const void *q, int64_t q_row, int64_t q_head, const v
   a.hq = hq;
   a.hk = hk;
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.splits = 1;
   if (int r = cache_kernel_attributes(dev))
     return r;
   CUtensorMap tm_q, tm_k, tm_v;
@@ -382,7 +454,8 @@ int pir2b_cache_attention(const void *q, int64_t q_row, int64_t q_head, int64_t 
   const int d = pages->head_dim;
   if (int r = cache_kernel_attributes(dev))
     return r;
-  const FewPlan plan = plan_few(rows, hq, a.hk, a.batch, int64_t(a.c.width) << a.c.shift, dev->sms);
+  const CachePlan plan =
+      plan_cache(rows, hq, a.hk, a.batch, int64_t(a.c.width) << a.c.shift, pages->format, dev->sms);
   a.splits = plan.splits;
   if (plan.splits > 1) {
     if (workspace == nullptr || !aligned(workspace, 16))
@@ -392,9 +465,9 @@ int pir2b_cache_attention(const void *q, int64_t q_row, int64_t q_head, int64_t 
   }
   int status = PIR2B_OK;
   switch (pages->format) {
-  case kCacheInt8: status = launch_attention_few<kCacheInt8>(plan, d, a, stream); break;
-  case kCacheE4m3: status = launch_attention_few<kCacheE4m3>(plan, d, a, stream); break;
-  default: status = launch_attention_few<kCacheBf16>(plan, d, a, stream); break;
+  case kCacheInt8: status = launch_cache_attention<kCacheInt8>(plan, d, a, stream); break;
+  case kCacheE4m3: status = launch_cache_attention<kCacheE4m3>(plan, d, a, stream); break;
+  default: status = launch_cache_attention<kCacheBf16>(plan, d, a, stream); break;
   }
   return status != PIR2B_OK || plan.splits == 1 ? status : launch_join(d, a, stream);
 }
@@ -405,8 +478,8 @@ int64_t pir2b_cache_attention_workspace(int64_t rows, int hq, const pir2b_kv_pag
   if (pages == nullptr || sequences == nullptr || rows < 1 || pages->kv_heads < 1 || hq < pages->kv_heads ||
       sequences->batch < 1 || device_info(&dev) != PIR2B_OK)
     return 0;                                     // the call itself reports what is wrong
-  const FewPlan plan = plan_few(rows, hq, pages->kv_heads, sequences->batch,
-                                int64_t(sequences->table_width) * pages->page_size, dev->sms);
+  const CachePlan plan = plan_cache(rows, hq, pages->kv_heads, sequences->batch,
+                                    int64_t(sequences->table_width) * pages->page_size, pages->format, dev->sms);
   return plan.splits == 1 ? 0 : int64_t(plan.splits) * rows * hq * (pages->head_dim * 4 + 8);
 }
 
