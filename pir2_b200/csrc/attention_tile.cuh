@@ -35,17 +35,20 @@ struct TileShape {
   static constexpr bool kScaled = kSource == kCacheInt8 || kSource == kCacheE4m3;
   static constexpr int kThreads = kTiles * 128 + 128 + (kScaled ? 128 : 0);
   static constexpr int kBytes = 128 * D * 2;            // a Q, K or V tile
-  static constexpr int kStages = kTiles == 2 ? (D == 128 ? (kScaled ? 4 : 5) : 8) : (D == 128 ? 2 : 5);
-  // Blocks whose scales are kept: the loader writes block j's when K item 2 j
-  // has a stage, which item 2 j - kStages has left; it must not be before V
-  // item 2 (j - kDepth) + 1 has.
-  static constexpr int kDepth = (kStages + 2) / 2;
+  static constexpr int kStages = kTiles == 2 ? (D == 128 ? (kScaled ? 3 : 5) : (kScaled ? 6 : 8)) : (D == 128 ? 2 : 5);
+  // 8-bit caches: tiles of codes on their way to the converting warps, and
+  // blocks whose scales are kept.  The loader writes block j's scales when
+  // item 2 j - kRaw has been converted, so item 2 j - kRaw - kStages has been
+  // used; V item 2 (j - kDepth) + 1 must not come after that.
+  static constexpr int kRaw = kScaled ? 3 : 0, kRawBytes = 128 * D;
+  static constexpr int kDepth = (kStages + kRaw + 2) / 2;
   static constexpr int kScaleBytes = kScaled ? kDepth * 2 * kTileKeys * 4 : 0;
-  static constexpr int kSmem = (kTiles + kStages) * kBytes + kScaleBytes + 1024 /* alignment */ + 256 /* barriers */;
+  static constexpr int kSmem =
+      (kTiles + kStages) * kBytes + kRaw * kRawBytes + kScaleBytes + 1024 /* alignment */ + 512 /* barriers */;
 };
 
-struct TileBarriers {
-  uint64_t full[8], empty[8], q_full[2], s_full[2], p_full[2][2], o_full[2], to_mend[3], mended[3];
+struct TileBarriers {   // at most 512 bytes
+  uint64_t full[8], empty[8], raw_full[3], raw_empty[3], q_full[2], s_full[2], p_full[2][2], o_full[2], to_mend[3], mended[3];
   uint32_t tmem;
   int spoiled;   // a V block held a value that is not finite at a position hidden from some row
 };
@@ -153,8 +156,9 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
   extern __shared__ uint8_t tile_raw[];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tile_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *q_sm = sm, *ring = sm + kTiles * kBytes;
-  float *scales = reinterpret_cast<float *>(ring + kStages * kBytes);   // [kDepth][K, V][128]
-  TileBarriers &bar = *reinterpret_cast<TileBarriers *>(ring + kStages * kBytes + Shape::kScaleBytes);
+  uint8_t *raw = ring + kStages * kBytes;                               // [kRaw][128][D] codes
+  float *scales = reinterpret_cast<float *>(raw + Shape::kRaw * Shape::kRawBytes);   // [kDepth][K, V][128]
+  TileBarriers &bar = *reinterpret_cast<TileBarriers *>(reinterpret_cast<uint8_t *>(scales) + Shape::kScaleBytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (warp == kMmaWarp) {
@@ -174,6 +178,10 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
         mbar_init(&bar.to_mend[i], 1);
         mbar_init(&bar.mended[i], 2);
       }
+      for (int i = 0; i < Shape::kRaw; ++i) {
+        mbar_init(&bar.raw_full[i], 1);
+        mbar_init(&bar.raw_empty[i], 4);
+      }
       bar.spoiled = 0;
       fence_barrier_init();
     }
@@ -183,10 +191,8 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
   }
   if (warp == kMmaWarp + 1 && lane == 0) {
     tma_prefetch_desc(&tm_q);
-    if (!kScaled) {
-      tma_prefetch_desc(&tm_k);
-      tma_prefetch_desc(&tm_v);
-    }
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
   }
   pdl_wait();
   pdl_launch_dependents();
@@ -358,6 +364,8 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint32_t p[16];
+          const float4 *v_scale = reinterpret_cast<const float4 *>(block_scales + kTileKeys + half * 64 + i * 32);
+          float4 v4;
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             const float2 x = __ffma2_rn(
@@ -365,7 +373,9 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
             float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
             sum = __fadd2_rn(sum, e);
             if constexpr (kScaled) {
-              const float2 v = *reinterpret_cast<const float2 *>(block_scales + kTileKeys + half * 64 + i * 32 + 2 * c);
+              if (!(c & 1))
+                v4 = v_scale[c / 2];
+              const float2 v = (c & 1) ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
               if (seen_by_all < half * 64 + i * 32 + 31)   // a hidden row's scale may be anything
                 e = make_float2(e.x == 0.f ? 0.f : e.x * v.x, e.y == 0.f ? 0.f : e.y * v.y);
               else
@@ -550,11 +560,14 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
                       int(w.begin) + (w.r0 + lane * 128) / group);
       }
       // Item 2 j is block j's K, item 2 j + 1 its V.  From pages, a lane per
-      // page copies it (a bad page reads page 0: any values do).
+      // page copies it (a bad page reads page 0: any values do).  8-bit codes
+      // go to the converting warps' ring, with the block's scales.
+      constexpr int kRing = kScaled ? Shape::kRaw : kStages;
+      uint64_t *full = kScaled ? bar.raw_full : bar.full, *empty = kScaled ? bar.raw_empty : bar.empty;
       int item = 0, page = 0;
       bool mine = lane == 0;
-      for (; !kScaled && item < 2 * blocks; ++item) {
-        const int stage = item % kStages, j = item >> 1;
+      for (; item < 2 * blocks; ++item) {
+        const int stage = item % kRing, j = item >> 1;
         if constexpr (kPaged) {
           if (!(item & 1)) {
             const int at = j * kTileKeys + (lane << a.c.shift);
@@ -565,114 +578,81 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
         }
         const int copies = __popc(__ballot_sync(0xffffffffu, mine));
         bool free_stage = true;
-        if (item >= kStages)
-          free_stage = mbar_wait(&bar.empty[stage], uint32_t((item / kStages - 1) & 1), kStatusTimeoutProducer);
+        if (item >= kRing)
+          free_stage = mbar_wait(&empty[stage], uint32_t((item / kRing - 1) & 1), kStatusTimeoutProducer);
         if (!__all_sync(0xffffffffu, free_stage))
           break;
-        if (lane == 0)
-          mbar_arrive_expect_tx(&bar.full[stage], kPaged ? (copies << a.c.shift) * D * 2 : kBytes);
+        if (lane == 0) {
+          const int row_bytes = kScaled ? D + (item & 1 ? 0 : 8) : D * 2;
+          mbar_arrive_expect_tx(&full[stage], kPaged ? (copies << a.c.shift) * row_bytes : kBytes);
+        }
         __syncwarp();
         if (mine) {
           const void *map = (item & 1) ? &tm_v : &tm_k;
+          if constexpr (kScaled) {
+            const int row = lane << a.c.shift;
+            tma_load_4d(raw + stage * Shape::kRawBytes + row * D, map, &full[stage], 0, 0, kvh, page);
+            if (!(item & 1)) {
+              float *block_scales = scales + (j % Shape::kDepth) * 2 * kTileKeys + row;
+              const int64_t slot = int64_t(kvh) << a.c.shift;
+              bulk_load(block_scales, a.c.ks + page * a.c.ks_page + slot, 4u << a.c.shift, &full[stage]);
+              bulk_load(block_scales + kTileKeys, a.c.vs + page * a.c.vs_page + slot, 4u << a.c.shift, &full[stage]);
+            }
+          } else {
 #pragma unroll
-          for (int h = 0; h < kHalves; ++h) {
-            uint8_t *dst = ring + stage * kBytes + h * 16384;
-            if constexpr (kPaged)
-              tma_load_4d(dst + (lane << a.c.shift) * 128, map, &bar.full[stage], h * 64, 0, kvh, page);
-            else
-              tma_load_3d(dst, map, &bar.full[stage], h * 64, kvh, int(w.begin) + w.base + j * kTileKeys);
+            for (int h = 0; h < kHalves; ++h) {
+              uint8_t *dst = ring + stage * kBytes + h * 16384;
+              if constexpr (kPaged)
+                tma_load_4d(dst + (lane << a.c.shift) * 128, map, &full[stage], h * 64, 0, kvh, page);
+              else
+                tma_load_3d(dst, map, &full[stage], h * 64, kvh, int(w.begin) + w.base + j * kTileKeys);
+            }
           }
         }
-        if (lane == 0 && (item & 1) && (j + 1) * kTileKeys > w.all_see)
+        if (!kScaled && lane == 0 && (item & 1) && (j + 1) * kTileKeys > w.all_see)
           mbar_arrive(&bar.to_mend[j - first_mend]);
       }
       // No copy is in flight when the CTA ends (at once, unless a wait gave up).
       if (lane == 0) {
-        for (int i = max(0, item - kStages); !kScaled && i < item; ++i)
-          mbar_wait(&bar.full[i % kStages], uint32_t((i / kStages) & 1), kStatusTimeoutProducer);
+        for (int i = max(0, item - kRing); i < item; ++i)
+          mbar_wait(&full[i % kRing], uint32_t((i / kRing) & 1), kStatusTimeoutProducer);
         for (int u = 0; u < kTiles && a.q_by_tma; ++u)
           if (w.blocks(u) > 0)
             mbar_wait(&bar.q_full[u], 0, kStatusTimeoutProducer);
       }
     } else if (kScaled) {
       if constexpr (kScaled) {
-        // Four warps turn codes into bf16 tiles: 16-byte runs of a row, one
-        // item's loads in flight while the one before is converted.  Rows past
-        // the keys become 0.
-        constexpr int kRuns = D / 16, kLoads = kRuns * kTileKeys / 128, kRowStep = 128 / kRuns;
+        // Four warps turn tiles of codes into bf16 tiles, 16 bytes of a row at
+        // a time.  Rows past the keys hold old codes, which are numbers.
+        constexpr int kRuns = D / 16, kRowStep = 128 / kRuns;
         const int t = tid - (kMmaWarp + 4) * 32, run = t % kRuns, row0 = t / kRuns;
-        if (t >= 0) {
-          const uint8_t *codes[2] = {static_cast<const uint8_t *>(a.c.k), static_cast<const uint8_t *>(a.c.v)};
-          const int page_mask = (1 << a.c.shift) - 1;
-          uint4 held[2][kLoads];
-          int page = -1;                           // of the block's 16 (lane % 8) .. + 15
-          auto fetch = [&](int item) {
-            const int j = item >> 1, which = item & 1;
-            if (which == 0) {
-              const int at = j * kTileKeys + (lane & 7) * 16;
-              page = at < w.keys ? page_of(a.c, w.b, w.base + at) : -1;
-            }
-            const int64_t apart = which ? a.c.v_page : a.c.k_page;
+        for (int item = 0; t >= 0 && item < 2 * blocks; ++item) {
+          const int from = item % Shape::kRaw, stage = item % kStages;
+          bool go = mbar_wait(&bar.raw_full[from], uint32_t((item / Shape::kRaw) & 1), kStatusTimeoutConvert);
+          if (go && item >= kStages)
+            go = mbar_wait(&bar.empty[stage], uint32_t((item / kStages - 1) & 1), kStatusTimeoutConvert);
+          if (!__all_sync(0xffffffffu, go))
+            break;
+          const uint8_t *src = raw + from * Shape::kRawBytes + row0 * D + run * 16;
+          uint8_t *dst = ring + stage * kBytes + (run >> 2) * 16384;
+          const int piece = (run & 3) * 2;
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-              const int row = row0 + i * kRowStep, key = j * kTileKeys + row;
-              const int64_t of = __shfl_sync(0xffffffffu, page, row >> 4);
-              uint4 x = make_uint4(0, 0, 0, 0);
-              if (of >= 0 && key < w.keys)
-                x = __ldg(reinterpret_cast<const uint4 *>(
-                    codes[which] + of * apart + ((int64_t(kvh) << a.c.shift) + (key & page_mask)) * D + run * 16));
-              held[which][i] = x;
-            }
-          };
-          auto store = [&](int item) {
-            const int stage = item % kStages;
-            uint8_t *dst = ring + stage * kBytes + (run >> 2) * 16384;
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-              const int row = row0 + i * kRowStep;
-              const uint4 x = held[item & 1][i];
-              uint4 lo, hi;
-              codes_to_bf16<kSource>(x.x, lo.x, lo.y);
-              codes_to_bf16<kSource>(x.y, lo.z, lo.w);
-              codes_to_bf16<kSource>(x.z, hi.x, hi.y);
-              codes_to_bf16<kSource>(x.w, hi.z, hi.w);
-              const int piece = (run & 3) * 2;
-              *reinterpret_cast<uint4 *>(dst + row * 128 + ((piece ^ (row & 7)) << 4)) = lo;
-              *reinterpret_cast<uint4 *>(dst + row * 128 + (((piece + 1) ^ (row & 7)) << 4)) = hi;
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0)
-              mbar_arrive(&bar.full[stage]);
-          };
-          auto wait_free = [&](int item) {
-            return item < kStages ||
-                   mbar_wait(&bar.empty[item % kStages], uint32_t((item / kStages - 1) & 1), kStatusTimeoutProducer);
-          };
-          if (blocks > 0)
-            fetch(0);
-          for (int j = 0; j < blocks; ++j) {
-            // The block's scales: a thread per row.
-            const int key = j * kTileKeys + t;
-            const int64_t of = __shfl_sync(0xffffffffu, page, (t >> 4) & 7);
-            float k_scale = 0.f, v_scale = 0.f;
-            if (of >= 0 && key < w.keys) {
-              const int64_t slot = (int64_t(kvh) << a.c.shift) + (key & page_mask);
-              k_scale = __ldg(a.c.ks + of * a.c.ks_page + slot);
-              v_scale = __ldg(a.c.vs + of * a.c.vs_page + slot);
-            }
-            fetch(2 * j + 1);
-            if (!__all_sync(0xffffffffu, wait_free(2 * j)))
-              break;
-            float *mine = scales + (j % Shape::kDepth) * 2 * kTileKeys;
-            mine[t] = k_scale;
-            mine[kTileKeys + t] = v_scale;
-            store(2 * j);
-            if (j + 1 < blocks)
-              fetch(2 * j + 2);
-            if (!__all_sync(0xffffffffu, wait_free(2 * j + 1)))
-              break;
-            store(2 * j + 1);
+          for (int i = 0; i < kTileKeys / kRowStep; ++i) {
+            const int row = row0 + i * kRowStep;
+            const uint4 x = *reinterpret_cast<const uint4 *>(src + i * kRowStep * D);
+            uint4 lo, hi;
+            codes_to_bf16<kSource>(x.x, lo.x, lo.y);
+            codes_to_bf16<kSource>(x.y, lo.z, lo.w);
+            codes_to_bf16<kSource>(x.z, hi.x, hi.y);
+            codes_to_bf16<kSource>(x.w, hi.z, hi.w);
+            *reinterpret_cast<uint4 *>(dst + row * 128 + ((piece ^ (row & 7)) << 4)) = lo;
+            *reinterpret_cast<uint4 *>(dst + row * 128 + (((piece + 1) ^ (row & 7)) << 4)) = hi;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&bar.full[stage]);
+            mbar_arrive(&bar.raw_empty[from]);
           }
         }
       }

@@ -200,19 +200,20 @@ static int launch_tile(const char *what, const RaggedArgs &a, const CUtensorMap 
 // which carries long prompts (8192 tokens: 241 us against 255).
 static int tiles_per_cta(int64_t rows, int batch) { return rows / batch >= 2048 ? 2 : 1; }
 
-// 4-D map over bf16 pages [pages, hk, page, d], box of one page of one head
-// and 64 columns in 128-byte swizzled rows.
-static int make_pages_map(CUtensorMap *map, const void *base, const CachePages &c, int d, int64_t page_stride) {
+// 4-D map over pages [pages, hk, page, d], box of one page of one head: bf16
+// in 64 columns and 128-byte swizzled rows, codes in whole rows.
+static int make_pages_map(CUtensorMap *map, const void *base, const CachePages &c, int d, int64_t page_stride, int bytes) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr)
     return fail(PIR2B_ECUDA, "cuTensorMapEncodeTiled entry point unavailable");
   const cuuint64_t page = cuuint64_t(1) << c.shift;
   const cuuint64_t dims[4] = {cuuint64_t(d), page, cuuint64_t(c.hk), cuuint64_t(c.pages)};
-  const cuuint64_t strides[3] = {cuuint64_t(d) * 2, page * d * 2, cuuint64_t(page_stride) * 2};
-  const cuuint32_t box[4] = {64, cuuint32_t(page), 1, 1};
+  const cuuint64_t strides[3] = {cuuint64_t(d) * bytes, page * d * bytes, cuuint64_t(page_stride) * bytes};
+  const cuuint32_t box[4] = {bytes == 2 ? 64u : cuuint32_t(d), cuuint32_t(page), 1, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  CUresult r = fn(map, bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4,
+                  const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  bytes == 2 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? PIR2B_OK : fail(PIR2B_ECUDA, "cuTensorMapEncodeTiled (pages) failed (%d)", int(r));
 }
@@ -241,14 +242,15 @@ static CachePlan plan_cache(int64_t rows, int hq, int hk, int batch, int64_t pos
 
 template <int kSource, int D>
 static int launch_cache_tile(const CachePlan &p, RaggedArgs a, void *stream) {
-  CUtensorMap tm_q, tm_k = {}, tm_v = {};
+  constexpr int kBytes = kSource == kCacheBf16 ? 2 : 1;
+  CUtensorMap tm_q, tm_k, tm_v;
   if (int r = make_q_map(&tm_q, &a, D))
     return r;
+  if (int r = make_pages_map(&tm_k, a.c.k, a.c, D, a.c.k_page, kBytes))
+    return r;
+  if (int r = make_pages_map(&tm_v, a.c.v, a.c, D, a.c.v_page, kBytes))
+    return r;
   if constexpr (kSource == kCacheBf16) {
-    if (int r = make_pages_map(&tm_k, a.c.k, a.c, D, a.c.k_page))
-      return r;
-    if (int r = make_pages_map(&tm_v, a.c.v, a.c, D, a.c.v_page))
-      return r;
     if (p.tiles == 1)
       return launch_tile<kSource, D, 1>("cache_attention launch", a, tm_q, tm_k, tm_v, stream);
   }
