@@ -97,14 +97,25 @@ static int launch_cache(const char *what, void (*kernel)(Args), int64_t grid, in
   return cuda_status(cudaLaunchKernelEx(&cfg, kernel, a), what);
 }
 
+// Few tokens are spread over more warps, one row load each (8 tokens of 8 kv
+// heads: 2.1 us against 3.2, 862 tokens of 4: 2.3 against 3.2); many keep four
+// in flight and share the search for their sequence.
+template <int kFormat, int D>
+static int launch_rows(bool write, const CacheRowsArgs &a, void *stream) {
+  constexpr int kRows = 32 / (D / 16);                      // rows of a warp's load
+  const int64_t grid = (a.rows + kCacheWarps - 1) / kCacheWarps;
+  const int loads = (2 * a.c.hk + kRows - 1) / kRows;
+  if (!write)
+    return launch_cache("cache_read launch", cache_read_kernel<kFormat, D>, grid, 1, 1, kCacheWarps * 32, 0, a, stream);
+  if (a.rows * loads <= 4096)
+    return launch_cache("cache_write launch", cache_write_kernel<kFormat, D, 1>, grid, loads, 1, kCacheWarps * 32, 0, a, stream);
+  return launch_cache("cache_write launch", cache_write_kernel<kFormat, D, 4>, grid, (loads + 3) / 4, 1, kCacheWarps * 32, 0,
+                      a, stream);
+}
+
 template <int kFormat>
 static int launch_rows(bool write, int d, const CacheRowsArgs &a, void *stream) {
-  const int64_t grid = (a.rows * 2 * a.c.hk * (d / 8) + kCacheThreads - 1) / kCacheThreads;
-  if (write)
-    return launch_cache("cache_write launch", d == 64 ? cache_write_kernel<kFormat, 64> : cache_write_kernel<kFormat, 128>,
-                        grid, 1, 1, kCacheThreads, 0, a, stream);
-  return launch_cache("cache_read launch", d == 64 ? cache_read_kernel<kFormat, 64> : cache_read_kernel<kFormat, 128>,
-                      grid, 1, 1, kCacheThreads, 0, a, stream);
+  return d == 64 ? launch_rows<kFormat, 64>(write, a, stream) : launch_rows<kFormat, 128>(write, a, stream);
 }
 
 static int launch_rows(bool write, int format, int d, const CacheRowsArgs &a, void *stream) {

@@ -4,6 +4,7 @@ host tensors."""
 
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
@@ -103,3 +104,22 @@ def test_host_tensors_are_refused():
     x = torch.zeros(2, 1, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="CUDA"):
         ops.prompt_attention(x, x, x, torch.zeros(2, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("limit", [127, 448])
+def test_quotients_of_the_cache_quantiser_are_correctly_rounded(limit):
+    """The quantiser divides a bf16 x by s = f32(1/L) * (a bf16) as q = x y,
+    q + (x - q s) y with y = 1 / s: for every pair of significands and every
+    exponent whose code is not 0 that is the correctly rounded quotient
+    (fp64 holds x - q s exactly, as an FMA does)."""
+    f = np.float32
+    significand = f(1) + np.arange(128, dtype=f) / f(128)
+    s = significand * (f(1) / f(limit))
+    y = f(1) / s
+    for shift in range(20):
+        x = (significand * f(2.0**-shift))[:, None]
+        q = x * y
+        rest = (x.astype(np.float64) - q.astype(np.float64) * s).astype(f)
+        q = (q.astype(np.float64) + rest.astype(np.float64) * y).astype(f)
+        inside = x <= significand            # s belongs to the row's largest value
+        assert np.array_equal(np.broadcast_to(x / s, q.shape)[inside], q[inside])
