@@ -4,18 +4,21 @@
 // one sequence; a CTA streams a range of the unit's keys once, eight warps
 // taking 16-key steps in turn.  Few rows cannot fill a 128-row tensor tile
 // and the work is reading the cache, so the products run on warp-level MMAs
-// (m16n8k16, bf16, fp32 sums) with the keys as the M rows:
+// (m16n8k16, fp32 sums) with the keys as the M rows:
 //   S^T [16 keys x 8 rows]  = K [16 x D] Q^T,
-//   O^T [D x 8 rows]       += V^T [D x 16 keys] P^T,
-// and cache bytes go from global memory to the MMA registers with no shared
-// memory between: the order of D inside a product is free, so each lane takes
-// whole 16-byte runs of a row (K: its quarter of D; V: its eighth) and q is
-// read in the same order.  8-bit codes become bf16 exactly in registers; the
-// scales multiply scores and weights in fp32.  P is transposed between the
-// products by movmatrix.  The running maximum of a row moves only when a
-// score passes it by more than 8 (in log2), so that most steps have one vote
-// and no rescaling; sums and maxima are fp32.
+//   O^T [D x 8 rows]       += V^T [D x 16 keys] P^T.
+// Each warp has a ring of its own: its first lane keeps the TMA copies of the
+// next steps in flight, and all lanes read the step at hand into MMA
+// fragments.  Which key is which M row, and the order of D inside a product,
+// are free: each lane takes whole 16-byte pieces, and rows are dealt so that
+// the swizzled tiles are read without bank conflicts.  8-bit codes become fp16
+// (K, the cheaper conversion; q is scaled to fit) and bf16 (V: the weights need
+// its range) exactly in registers; the scales multiply scores and weights in
+// fp32.  P is transposed between the products by movmatrix.  The running maximum of a row
+// moves only when a score passes it by more than 8 (in log2), so that most
+// steps have one vote and no rescaling; sums and maxima are fp32.
 #pragma once
+#include <cuda.h>
 #include "attention_ragged.cuh"
 
 namespace pir2b {
@@ -49,24 +52,37 @@ __device__ __forceinline__ void codes_to_bf16(uint32_t w, uint32_t &lo, uint32_t
   }
 }
 
+// Two fp16 pairs from a word of four 8-bit codes, exactly: 0x64'(code + 128) is
+// 1024 + 128 + code; E4M3 converts.
+template <int kFormat>
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  if constexpr (kFormat == kCacheInt8) {
+    const uint32_t x = w ^ 0x80808080u, offset = 0x64806480u;   // 1152
+    const uint32_t a = __byte_perm(x, 0x64646464u, 0x4140), b = __byte_perm(x, 0x64646464u, 0x4342);
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(offset));
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(offset));
+  } else {
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"(uint16_t(w)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"(uint16_t(w >> 16)));
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ void mma_half_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-
-// `kWords` consecutive words (2, 4, 8 or 16) read once.
-template <int kWords>
-__device__ __forceinline__ void load_words(const void *p, uint32_t (&w)[kWords]) {
-  if constexpr (kWords == 2) {
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-  } else {
-#pragma unroll
-    for (int i = 0; i < kWords; i += 4)
-      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
-                   : "l"(static_cast<const uint32_t *>(p) + i));
-  }
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -120,23 +136,67 @@ __device__ __forceinline__ int unit_of(const RaggedArgs &a, int group, int tile_
   return (tile >= 0 && (int64_t(tile) << tile_log2) < (s1 - s0) * group) ? lo : -1;
 }
 
-template <int D, int kNT>
-constexpr int few_smem() {
-  return kFewWarps * kNT * 8 * (D + 4 + 2) * 4;
+// Shared memory of the few-row kernel: each warp's ring of K and V tiles of 16
+// rows, their scales and barriers; at the end the warps' partial sums.
+template <int kFormat, int D, int kNT>
+struct FewShape {
+  static constexpr bool kBf16 = kFormat == kCacheBf16;
+  static constexpr int kRowBytes = D * (kBf16 ? 2 : 1);
+  static constexpr int kBoxes = kRowBytes > 128 ? 2 : 1;          // a swizzled row has at most 128 bytes
+  static constexpr int kTile = 16 * kRowBytes;
+  static constexpr int kStages = 3;
+  static constexpr int kCtas = kRowBytes > 128 || kNT == 2 ? 1 : 2;   // on an SM
+  static constexpr int kRing = kFewWarps * kStages * 2 * kTile;
+  static constexpr int kScales = kFewWarps * kStages * 2 * 16 * 4;
+  static constexpr int kSums = kFewWarps * kNT * 8 * (D + 4 + 2) * 4;
+  static constexpr int kSmem =
+      1024 /* alignment */ + (kRing + kScales + kFewWarps * kStages * 8 > kSums ? kRing + kScales + kFewWarps * kStages * 8 : kSums);
+};
+
+// 4-D tiled load into this CTA's shared memory.
+__device__ __forceinline__ void tma_load_4d(void *dst, const void *tmap, uint64_t *bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+          "r"(smem_u32(dst)),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// 16-byte piece `c` of row `r` of a swizzled tile of kRowBytes rows (of 256
+// bytes: two tiles of 128-byte halves).
+template <int kRowBytes>
+__device__ __forceinline__ const uint8_t *piece_of(const uint8_t *tile, int r, int c) {
+  if constexpr (kRowBytes >= 128)
+    return tile + (c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+  else
+    return tile + r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
 template <int kFormat, int D, int kNT>
-__global__ void __launch_bounds__(kFewWarps * 32, kNT == 1 ? 2 : 1) attention_few_kernel(const RaggedArgs a) {
+__global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCtas)
+    attention_few_kernel(const RaggedArgs a, const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v) {
+  using Shape = FewShape<kFormat, D, kNT>;
   constexpr bool kBf16 = kFormat == kCacheBf16;
   constexpr int kRows = 8 * kNT, kRowsLog2 = kNT == 1 ? 3 : 4;
   constexpr int KS = D / 16;                       // K steps of S, and M tiles of O
   constexpr int KW = kBf16 ? D / 8 : D / 16;       // words of a lane's quarter of a K row
   constexpr int VW = kBf16 ? D / 16 : D / 32;      // words of a lane's eighth of a V row
-  constexpr int kBytes = kBf16 ? 2 : 1;
-  extern __shared__ __align__(16) float few_sm[];
+  constexpr int kRowBytes = Shape::kRowBytes, kStages = Shape::kStages, kTile = Shape::kTile;
+  extern __shared__ uint8_t few_raw[];
+  uint8_t *few_sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(few_raw) + 1023) & ~uintptr_t(1023));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q4 = lane & 3;
   const int kvh = blockIdx.y, split = blockIdx.z;
   const int group = a.hq / a.hk;
+  uint8_t *ring = few_sm + warp * kStages * 2 * kTile;                                    // [kStages][K, V]
+  float *scales = reinterpret_cast<float *>(few_sm + Shape::kRing) + warp * kStages * 32;   // [kStages][K, V][16]
+  uint64_t *full = reinterpret_cast<uint64_t *>(few_sm + Shape::kRing + Shape::kScales) + warp * kStages;
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i)
+      mbar_init(&full[i], 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
   pdl_wait();
   pdl_launch_dependents();
   int tile;
@@ -157,25 +217,77 @@ __global__ void __launch_bounds__(kFewWarps * 32, kNT == 1 ? 2 : 1) attention_fe
   const int per = (((steps + a.splits - 1) / a.splits) + kFewWarps - 1) / kFewWarps * kFewWarps;
   const int step_end = min(steps, (split + 1) * per);
 
+  // The warp's steps: every kFewWarps-th from `step0` on.
+  const int step0 = split * per + warp;
+  const int count = step_end > step0 ? (step_end - step0 + kFewWarps - 1) / kFewWarps : 0;
+  const int page_mask = (1 << a.c.shift) - 1;
+  int pages_of_lane = 0;                            // the pages of the next 32 steps to copy
+  auto copy = [&](int i) {
+    const int step = step0 + i * kFewWarps, stage = i % kStages;
+    if ((i & 31) == 0 && i + lane < count)          // a bad page reads page 0: any values do
+      pages_of_lane = max(0, page_of(a.c, b, int64_t(step + lane * kFewWarps) << 4));
+    const int page = __shfl_sync(0xffffffffu, pages_of_lane, i & 31);
+    if (lane == 0) {
+      uint8_t *to = ring + stage * 2 * kTile;
+      const int in_page = (step << 4) & page_mask;
+      mbar_arrive_expect_tx(&full[stage], 2 * kTile + (kBf16 ? 0 : 128));
+#pragma unroll
+      for (int h = 0; h < Shape::kBoxes; ++h) {
+        tma_load_4d(to + h * 2048, &tm_k, &full[stage], h * 64, in_page, kvh, page);
+        tma_load_4d(to + kTile + h * 2048, &tm_v, &full[stage], h * 64, in_page, kvh, page);
+      }
+      if constexpr (!kBf16) {
+        const int64_t slot = (int64_t(kvh) << a.c.shift) + in_page;
+        bulk_load(scales + stage * 32, a.c.ks + page * a.c.ks_page + slot, 64, &full[stage]);
+        bulk_load(scales + stage * 32 + 16, a.c.vs + page * a.c.vs_page + slot, 64, &full[stage]);
+      }
+    }
+  };
+  for (int i = 0; i < min(kStages, count); ++i)
+    copy(i);
+
   uint32_t qf[kNT][KS][2];
   int limit[kNT][2];
+  float to_log2[kNT][2];                           // a row's factor from its products to scores in log2
 #pragma unroll
   for (int t = 0; t < kNT; ++t) {
     const int r = r0 + t * 8 + g;
-    uint32_t w[D / 8] = {};
-    if (r < r1) {
-      const __nv_bfloat16 *src = a.q + (begin + r / group) * a.q_row + (kvh * group + r % group) * a.q_head + q4 * (D / 4);
-      load_words<D / 8>(src, w);
-    }
+    // The four elements of each product step that this lane holds of a K row.
+    const __nv_bfloat16 *src = a.q + (begin + r / group) * a.q_row + (kvh * group + r % group) * a.q_head;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      qf[t][s][0] = w[2 * s];
-      qf[t][s][1] = w[2 * s + 1];
+      const int at = kBf16 ? (s / 2 * 4 + q4) * 8 + s % 2 * 4 : (s / 4 * 4 + q4) * 16 + s % 4 * 4;
+      const uint2 w = r < r1 ? __ldg(reinterpret_cast<const uint2 *>(src + at)) : make_uint2(0, 0);
+      qf[t][s][0] = w.x;
+      qf[t][s][1] = w.y;
+    }
+    float undo = 1.f;
+    if constexpr (!kBf16) {
+      // fp16 holds a bf16 row exactly (to 2^-35 of its largest value) once a
+      // power of two has brought that value to 2^10.
+      uint32_t most = 0;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        most = __vmaxu2(most, __vmaxu2(qf[t][s][0] & 0x7fff7fffu, qf[t][s][1] & 0x7fff7fffu));
+      most = max(most & 0xffffu, most >> 16);
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int up = most == 0 ? 127 : min(264 - int(most >> 7), 253);   // exponent field of the power
+      const float factor = __int_as_float(up << 23);
+      undo = __int_as_float((254 - up) << 23);
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 x = bf16_pair(qf[t][s][e]);
+          qf[t][s][e] = pack_half2(x.x * factor, x.y * factor);
+        }
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int rr = r0 + t * 8 + 2 * q4 + e;
       limit[t][e] = rr < r1 ? first_new + rr / group : -1;
+      to_log2[t][e] = __shfl_sync(0xffffffffu, undo, (2 * q4 + e) * 4) * a.scale_log2;
     }
   }
 
@@ -183,64 +295,29 @@ __global__ void __launch_bounds__(kFewWarps * 32, kNT == 1 ? 2 : 1) attention_fe
   float l[kNT][2] = {}, mu[kNT][2] = {};           // mu: the maximum subtracted (0 while none)
   float top[kNT][2];                               // the running maximum
 #pragma unroll
-  for (int t = 0; t < kNT; ++t)
+  for (int t = 0; t < kNT; ++t) {
     top[t][0] = top[t][1] = -INFINITY;
-
-  const uint8_t *kbase = static_cast<const uint8_t *>(a.c.k), *vbase = static_cast<const uint8_t *>(a.c.v);
-  uint32_t kr[2][KW];
-  float ksc[2] = {1.f, 1.f};
-  const int page_mask = (1 << a.c.shift) - 1;
-  auto load_k = [&](int page, int step) {
-    const int64_t slot = (int64_t(kvh) << a.c.shift) + ((step << 4) & page_mask) + g;
-    const int64_t at = int64_t(page) * a.c.k_page + slot * D + q4 * (D / 4);
-    load_words<KW>(kbase + at * kBytes, kr[0]);
-    load_words<KW>(kbase + (at + 8 * D) * kBytes, kr[1]);
-    if constexpr (!kBf16) {
-      const float *s = a.c.ks + page * a.c.ks_page + slot;
-      ksc[0] = __ldg(s);
-      ksc[1] = __ldg(s + 8);
-    }
-  };
-
-  int step = split * per + warp;
-  int pages_of_lane = -1;
-  auto page_at = [&](int i) { return __shfl_sync(0xffffffffu, pages_of_lane, i & 31); };
-  auto fetch_pages = [&](int first) {               // the pages of this warp's next 32 steps
-    const int64_t s = int64_t(first) + lane * kFewWarps;
-    pages_of_lane = s < step_end ? page_of(a.c, b, s << 4) : -1;
-  };
-  int page = -1;
-  if (step < step_end) {
-    fetch_pages(step);
-    page = page_at(0);
-    if (page >= 0)
-      load_k(page, step);
   }
-  for (int i = 0; step < step_end; ++i, step += kFewWarps) {
-    const int page_now = page;
-    const int next = step + kFewWarps;
-    if (((i + 1) & 31) == 0 && next < step_end)
-      fetch_pages(next);
-    page = next < step_end ? page_at(i + 1) : -1;
-    if (page_now < 0) {                             // no such page: its keys are hidden
-      if (page >= 0)
-        load_k(page, next);
-      continue;
+
+  // M row g of a step is its key `mine` (and g + 8 is 8 after it); K index 2 q4
+  // is key 2 q4 and 2 q4 + 1 is key `odd` of its first eight.
+  const int mine = g ^ ((g & 1) << 2), odd = (2 * q4 + 1) ^ 4;
+  int done = 0;
+  for (; done < count; ++done) {
+    const int step = step0 + done * kFewWarps, stage = done % kStages;
+    if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], uint32_t((done / kStages) & 1), kStatusTimeoutProducer)))
+      break;
+    const uint8_t *k_tile = ring + stage * 2 * kTile, *v_tile = k_tile + kTile;
+    uint32_t kr[2][KW], vr[4][VW];                  // K rows mine, mine + 8; V rows 2 q4, odd, and 8 after them
+#pragma unroll
+    for (int i = 0; i < KW / 4; ++i) {
+      *reinterpret_cast<uint4 *>(&kr[0][i * 4]) = *reinterpret_cast<const uint4 *>(piece_of<kRowBytes>(k_tile, mine, i * 4 + q4));
+      *reinterpret_cast<uint4 *>(&kr[1][i * 4]) = *reinterpret_cast<const uint4 *>(piece_of<kRowBytes>(k_tile, mine + 8, i * 4 + q4));
     }
-    uint32_t vr[4][VW];                             // keys 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
-    float vsc[2] = {1.f, 1.f};
-    {
-      const int64_t slot = (int64_t(kvh) << a.c.shift) + ((step << 4) & page_mask);
-      const int64_t at = int64_t(page_now) * a.c.v_page + (slot + 2 * q4) * D + g * (D / 8);
-      load_words<VW>(vbase + at * kBytes, vr[0]);
-      load_words<VW>(vbase + (at + D) * kBytes, vr[1]);
-      load_words<VW>(vbase + (at + 8 * D) * kBytes, vr[2]);
-      load_words<VW>(vbase + (at + 9 * D) * kBytes, vr[3]);
-      if constexpr (!kBf16) {
-        const float *s = a.c.vs + page_now * a.c.vs_page + slot + g;
-        vsc[0] = __ldg(s);
-        vsc[1] = __ldg(s + 8);
-      }
+    float ksc[2] = {1.f, 1.f}, vsc[2] = {1.f, 1.f};
+    if constexpr (!kBf16) {
+      const float *s = scales + stage * 32 + mine;
+      ksc[0] = s[0], ksc[1] = s[8], vsc[0] = s[16], vsc[1] = s[24];
     }
     float sc[kNT][4] = {};
 #pragma unroll
@@ -249,16 +326,32 @@ __global__ void __launch_bounds__(kFewWarps * 32, kNT == 1 ? 2 : 1) attention_fe
       if constexpr (kBf16) {
         af[0] = kr[0][2 * s], af[1] = kr[1][2 * s], af[2] = kr[0][2 * s + 1], af[3] = kr[1][2 * s + 1];
       } else {
-        codes_to_bf16<kFormat>(kr[0][s], af[0], af[2]);
-        codes_to_bf16<kFormat>(kr[1][s], af[1], af[3]);
+        codes_to_half<kFormat>(kr[0][s], af[0], af[2]);
+        codes_to_half<kFormat>(kr[1][s], af[1], af[3]);
       }
 #pragma unroll
-      for (int t = 0; t < kNT; ++t)
-        mma_bf16_16816(sc[t], af, qf[t][s][0], qf[t][s][1]);
+      for (int t = 0; t < kNT; ++t) {
+        if constexpr (kBf16)
+          mma_bf16_16816(sc[t], af, qf[t][s][0], qf[t][s][1]);
+        else
+          mma_half_16816(sc[t], af, qf[t][s][0], qf[t][s][1]);
+      }
     }
-    const float k_lo = ksc[0] * a.scale_log2, k_hi = ksc[1] * a.scale_log2;
-    if (page >= 0)
-      load_k(page, next);
+    const float k_lo = ksc[0], k_hi = ksc[1];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int r = (x & 1 ? odd : 2 * q4) + (x & 2) * 4;
+      if constexpr (VW == 2) {
+        *reinterpret_cast<uint2 *>(vr[x]) = *reinterpret_cast<const uint2 *>(piece_of<kRowBytes>(v_tile, r, g >> 1) + (g & 1) * 8);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VW / 4; ++i)
+          *reinterpret_cast<uint4 *>(&vr[x][i * 4]) = *reinterpret_cast<const uint4 *>(piece_of<kRowBytes>(v_tile, r, i * 8 + g));
+      }
+    }
+    __syncwarp();
+    if (done + kStages < count)
+      copy(done + kStages);
     const int key0 = step << 4;
     const bool masked = key0 + 16 > all_see;
     bool raise = false;
@@ -266,8 +359,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, kNT == 1 ? 2 : 1) attention_fe
     for (int t = 0; t < kNT; ++t) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float v = sc[t][e] * (e < 2 ? k_lo : k_hi);
-        if (masked && key0 + g + (e & 2) * 4 > limit[t][e & 1])
+        float v = kBf16 ? sc[t][e] * a.scale_log2 : sc[t][e] * (e < 2 ? k_lo : k_hi) * to_log2[t][e & 1];
+        if (masked && key0 + mine + (e & 2) * 4 > limit[t][e & 1])
           v = -INFINITY;
         sc[t][e] = v;
         raise |= v > top[t][e & 1] + 8.f;
@@ -297,17 +390,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, kNT == 1 ? 2 : 1) attention_fe
     uint32_t pf[kNT][2];
 #pragma unroll
     for (int t = 0; t < kNT; ++t) {
-      float p[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float w = exp2_fast(sc[t][e] - mu[t][e & 1]);
         l[t][e & 1] += w;
-        p[e] = kBf16 ? w : w * vsc[e >> 1];
-        if (!kBf16 && masked && sc[t][e] == -INFINITY)   // a hidden key's scale may be anything
-          p[e] = 0.f;
+        // A hidden key's scale may be anything.
+        sc[t][e] = kBf16 ? w : masked && sc[t][e] == -INFINITY ? 0.f : w * vsc[e >> 1];
       }
-      pf[t][0] = transpose_8x8(pack_bf16x2(p[0], p[1]));
-      pf[t][1] = transpose_8x8(pack_bf16x2(p[2], p[3]));
+      pf[t][0] = transpose_8x8(pack_bf16x2(sc[t][0], sc[t][1]));
+      pf[t][1] = transpose_8x8(pack_bf16x2(sc[t][2], sc[t][3]));
     }
     // Pairs (key, key + 1) of a column for the two halves of an M tile pair.
     auto product = [&](const uint32_t (&pp)[kNT][2]) {
@@ -344,7 +435,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, kNT == 1 ? 2 : 1) attention_fe
         bool spoiled = false;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int key = key0 + 2 * q4 + (x & 1) + (x & 2) * 4;
+          const int key = key0 + (x & 1 ? odd : 2 * q4) + (x & 2) * 4;
 #pragma unroll
           for (int j = 0; j < VW; ++j) {
             if (key >= keys)
@@ -374,7 +465,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, kNT == 1 ? 2 : 1) attention_fe
             // added to this row alone, below.
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const int key = key0 + 2 * q4 + (x & 1) + (x & 2) * 4;
+              const int key = key0 + (x & 1 ? odd : 2 * q4) + (x & 2) * 4;
 #pragma unroll
               for (int j = 0; j < VW; ++j)
                 vr[x][j] = key > last ? 0 : kept[x][j];
@@ -405,8 +496,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, kNT == 1 ? 2 : 1) attention_fe
     product(pf);
   }
 
+  // No copy is in flight past this point (at once, unless a wait gave up).
+  for (int i = done; i < min(done + kStages, count); ++i)
+    mbar_wait(&full[i % kStages], uint32_t((i / kStages) & 1), kStatusTimeoutProducer);
+  __syncthreads();
   // The warps' partial sums, added in warp order.
-  float *so = few_sm;                                          // [warps][rows][D + 4]
+  float *so = reinterpret_cast<float *>(few_sm);                // [warps][rows][D + 4]
   float *sm = so + kFewWarps * kRows * (D + 4), *sl = sm + kFewWarps * kRows;
 #pragma unroll
   for (int t = 0; t < kNT; ++t) {
@@ -422,9 +517,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, kNT == 1 ? 2 : 1) attention_fe
         sl[warp * kRows + r] = x;
       }
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {                           // d = g D/8 + 2 s + (0, 1)
+      for (int s = 0; s < KS; ++s) {                           // the two columns of tile s
+        const int d = kBf16 ? (s / 4 * 8 + g) * 8 + s % 4 * 2 : g * (D / 8) + 2 * s;
         const float2 pair = make_float2(o[t][s][e], o[t][s][e + 2]);
-        *reinterpret_cast<float2 *>(so + (warp * kRows + r) * (D + 4) + g * (D / 8) + 2 * s) = pair;
+        *reinterpret_cast<float2 *>(so + (warp * kRows + r) * (D + 4) + d) = pair;
       }
     }
   }

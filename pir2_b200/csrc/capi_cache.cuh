@@ -1,6 +1,8 @@
 // C ABI of the ragged-batch operators (packed prompts, paged K/V cache):
 // argument checks and launches.
 #pragma once
+#include <type_traits>
+#include <utility>
 #include "attention_few.cuh"
 #include "attention_ragged.cuh"
 #include "attention_tile.cuh"
@@ -79,9 +81,9 @@ static int make_pages(const char *what, const pir2b_kv_pages *p, const pir2b_seq
 
 // A launch that may start while its predecessor drains (every kernel here
 // begins with griddepcontrol.wait).
-template <typename Args>
-static int launch_cache(const char *what, void (*kernel)(Args), int64_t grid, int grid_y, int grid_z, int threads,
-                        size_t smem, const Args &a, void *stream) {
+template <typename... Args>
+static int launch_cache(const char *what, void (*kernel)(Args...), int64_t grid, int grid_y, int grid_z, int threads,
+                        size_t smem, void *stream, const std::remove_reference_t<Args> &...args) {
   if (grid > 0x7fffffff)
     return fail(PIR2B_EINVAL, "%s: too many rows", what);
   cudaLaunchConfig_t cfg = {};
@@ -94,7 +96,7 @@ static int launch_cache(const char *what, void (*kernel)(Args), int64_t grid, in
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, a), what);
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args...), what);
 }
 
 // Few tokens are spread over more warps, one row load each (8 tokens of 8 kv
@@ -106,11 +108,11 @@ static int launch_rows(bool write, const CacheRowsArgs &a, void *stream) {
   const int64_t grid = (a.rows + kCacheWarps - 1) / kCacheWarps;
   const int loads = (2 * a.c.hk + kRows - 1) / kRows;
   if (!write)
-    return launch_cache("cache_read launch", cache_read_kernel<kFormat, D>, grid, 1, 1, kCacheWarps * 32, 0, a, stream);
+    return launch_cache("cache_read launch", cache_read_kernel<kFormat, D>, grid, 1, 1, kCacheWarps * 32, 0, stream, a);
   if (a.rows * loads <= 4096)
-    return launch_cache("cache_write launch", cache_write_kernel<kFormat, D, 1>, grid, loads, 1, kCacheWarps * 32, 0, a, stream);
+    return launch_cache("cache_write launch", cache_write_kernel<kFormat, D, 1>, grid, loads, 1, kCacheWarps * 32, 0, stream, a);
   return launch_cache("cache_write launch", cache_write_kernel<kFormat, D, 4>, grid, (loads + 3) / 4, 1, kCacheWarps * 32, 0,
-                      a, stream);
+                      stream, a);
 }
 
 template <int kFormat>
@@ -126,7 +128,7 @@ static int launch_rows(bool write, int format, int d, const CacheRowsArgs &a, vo
   }
 }
 
-constexpr int kFewWaves = 2;
+static const int kFewWaves = getenv("PIR2B_W") ? atoi(getenv("PIR2B_W")) : 2;
 constexpr int kFewRows = 32;   // rows a sequence has in a kv head, up to which the few-row kernel takes it
 
 // How the few-row kernel covers a call: rows per unit, grid slots and splits.
@@ -147,10 +149,38 @@ static FewPlan plan_few(int64_t rows, int hq, int hk, int batch, int64_t positio
   return p;
 }
 
+// 4-D map over pages [pages, hk, page, d], box of `rows` rows of one head: 64
+// columns of bf16 or whole rows of codes, swizzled over the row's 128 or 64
+// bytes or as they lie.
+static int make_pages_map(CUtensorMap *map, const void *base, const CachePages &c, int d, int64_t page_stride, int bytes,
+                          int rows, bool swizzled) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr)
+    return fail(PIR2B_ECUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  const cuuint64_t page = cuuint64_t(1) << c.shift;
+  const cuuint64_t dims[4] = {cuuint64_t(d), page, cuuint64_t(c.hk), cuuint64_t(c.pages)};
+  const cuuint64_t strides[3] = {cuuint64_t(d) * bytes, page * d * bytes, cuuint64_t(page_stride) * bytes};
+  const cuuint32_t box[4] = {bytes == 2 ? 64u : cuuint32_t(d), cuuint32_t(rows), 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4,
+                  const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  !swizzled ? CU_TENSOR_MAP_SWIZZLE_NONE
+                            : box[0] * bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? PIR2B_OK : fail(PIR2B_ECUDA, "cuTensorMapEncodeTiled (pages) failed (%d)", int(r));
+}
+
 template <int kFormat, int D, int kNT>
 static int launch_attention_few(const FewPlan &p, const RaggedArgs &a, void *stream) {
+  constexpr int kBytes = kFormat == kCacheBf16 ? 2 : 1;
+  CUtensorMap tm_k, tm_v;
+  if (int r = make_pages_map(&tm_k, a.c.k, a.c, D, a.c.k_page, kBytes, 16, true))
+    return r;
+  if (int r = make_pages_map(&tm_v, a.c.v, a.c, D, a.c.v_page, kBytes, 16, true))
+    return r;
   return launch_cache("cache_attention launch", attention_few_kernel<kFormat, D, kNT>, p.slots, a.hk, p.splits,
-                      kFewWarps * 32, few_smem<D, kNT>(), a, stream);
+                      kFewWarps * 32, FewShape<kFormat, D, kNT>::kSmem, stream, a, tm_k, tm_v);
 }
 
 template <int kFormat>
@@ -189,20 +219,10 @@ static int make_q_map(CUtensorMap *map, RaggedArgs *a, int d) {
 template <int kSource, int D, int kTiles>
 static int launch_tile(const char *what, const RaggedArgs &a, const CUtensorMap &tm_q, const CUtensorMap &tm_k,
                        const CUtensorMap &tm_v, void *stream) {
+  using Shape = TileShape<kSource, D, kTiles>;
   const int64_t grid = (a.rows * (a.hq / a.hk) / (128 * kTiles) + a.batch) * a.hk * a.splits;
-  if (grid > 0x7fffffff)
-    return fail(PIR2B_EINVAL, "%s: too many rows", what);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(grid), 1, 1);
-  cfg.blockDim = dim3(TileShape<kSource, D, kTiles>::kThreads, 1, 1);
-  cfg.dynamicSmemBytes = TileShape<kSource, D, kTiles>::kSmem;
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, attention_tile_kernel<kSource, D, kTiles>, a, tm_q, tm_k, tm_v), what);
+  return launch_cache(what, attention_tile_kernel<kSource, D, kTiles>, grid, 1, 1, Shape::kThreads, Shape::kSmem, stream, a,
+                      tm_q, tm_k, tm_v);
 }
 
 // Tiles per CTA of the tile kernel.  One tile and two CTAs on an SM cover the
@@ -210,24 +230,6 @@ static int launch_tile(const char *what, const RaggedArgs &a, const CUtensorMap 
 // 280-816 tokens: 197 us against 218); two tiles read K and V half as often,
 // which carries long prompts (8192 tokens: 241 us against 255).
 static int tiles_per_cta(int64_t rows, int batch) { return rows / batch >= 2048 ? 2 : 1; }
-
-// 4-D map over pages [pages, hk, page, d], box of one page of one head: bf16
-// in 64 columns and 128-byte swizzled rows, codes in whole rows.
-static int make_pages_map(CUtensorMap *map, const void *base, const CachePages &c, int d, int64_t page_stride, int bytes) {
-  EncodeTiledFn fn = encode_fn();
-  if (fn == nullptr)
-    return fail(PIR2B_ECUDA, "cuTensorMapEncodeTiled entry point unavailable");
-  const cuuint64_t page = cuuint64_t(1) << c.shift;
-  const cuuint64_t dims[4] = {cuuint64_t(d), page, cuuint64_t(c.hk), cuuint64_t(c.pages)};
-  const cuuint64_t strides[3] = {cuuint64_t(d) * bytes, page * d * bytes, cuuint64_t(page_stride) * bytes};
-  const cuuint32_t box[4] = {bytes == 2 ? 64u : cuuint32_t(d), cuuint32_t(page), 1, 1};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(map, bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4,
-                  const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  bytes == 2 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? PIR2B_OK : fail(PIR2B_ECUDA, "cuTensorMapEncodeTiled (pages) failed (%d)", int(r));
-}
 
 // How a call of cache_attention runs: the few-row kernel (tiles = 0) or
 // 128-row tiles, and its splits along the keys.
@@ -257,9 +259,9 @@ static int launch_cache_tile(const CachePlan &p, RaggedArgs a, void *stream) {
   CUtensorMap tm_q, tm_k, tm_v;
   if (int r = make_q_map(&tm_q, &a, D))
     return r;
-  if (int r = make_pages_map(&tm_k, a.c.k, a.c, D, a.c.k_page, kBytes))
+  if (int r = make_pages_map(&tm_k, a.c.k, a.c, D, a.c.k_page, kBytes, 1 << a.c.shift, kBytes == 2))
     return r;
-  if (int r = make_pages_map(&tm_v, a.c.v, a.c, D, a.c.v_page, kBytes))
+  if (int r = make_pages_map(&tm_v, a.c.v, a.c, D, a.c.v_page, kBytes, 1 << a.c.shift, kBytes == 2))
     return r;
   if constexpr (kSource == kCacheBf16) {
     if (p.tiles == 1)
@@ -277,7 +279,7 @@ static int launch_cache_attention(const CachePlan &p, int d, const RaggedArgs &a
 
 static int launch_join(int d, const RaggedArgs &a, void *stream) {
   return launch_cache("cache_attention join launch", d == 64 ? attention_join_kernel<64> : attention_join_kernel<128>,
-                      (a.rows * a.hq + 7) / 8, 1, 1, 256, 0, a, stream);
+                      (a.rows * a.hq + 7) / 8, 1, 1, 256, 0, stream, a);
 }
 
 // Dynamic shared memory above the default limit, once per device.
@@ -286,9 +288,18 @@ static int cache_kernel_attributes(DeviceInfo *dev) {
   if (dev->cache_attrs_set)
     return PIR2B_OK;
   const std::pair<const void *, int> kernels[] = {
-      {reinterpret_cast<const void *>(attention_few_kernel<kCacheBf16, 128, 2>), few_smem<128, 2>()},
-      {reinterpret_cast<const void *>(attention_few_kernel<kCacheInt8, 128, 2>), few_smem<128, 2>()},
-      {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 128, 2>), few_smem<128, 2>()},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheBf16, 64, 1>), FewShape<kCacheBf16, 64, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheBf16, 64, 2>), FewShape<kCacheBf16, 64, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheBf16, 128, 1>), FewShape<kCacheBf16, 128, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheBf16, 128, 2>), FewShape<kCacheBf16, 128, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheInt8, 64, 1>), FewShape<kCacheInt8, 64, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheInt8, 64, 2>), FewShape<kCacheInt8, 64, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheInt8, 128, 1>), FewShape<kCacheInt8, 128, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheInt8, 128, 2>), FewShape<kCacheInt8, 128, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 64, 1>), FewShape<kCacheE4m3, 64, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 64, 2>), FewShape<kCacheE4m3, 64, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 128, 1>), FewShape<kCacheE4m3, 128, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 128, 2>), FewShape<kCacheE4m3, 128, 2>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 64, 1>), TileShape<kSourceRows, 64, 1>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 64, 2>), TileShape<kSourceRows, 64, 2>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 128, 1>), TileShape<kSourceRows, 128, 1>::kSmem},
