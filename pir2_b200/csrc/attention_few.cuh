@@ -23,7 +23,7 @@
 
 namespace pir2b {
 
-constexpr int kFewWarps = 8;
+constexpr int kFewWarps = 4;
 
 // Two bf16 pairs from a word of four 8-bit codes, exactly.
 // int8: with u the low seven bits and s the sign bit of a byte, 0x43'u is
@@ -136,6 +136,9 @@ __device__ __forceinline__ int unit_of(const RaggedArgs &a, int group, int tile_
   return (tile >= 0 && (int64_t(tile) << tile_log2) < (s1 - s0) * group) ? lo : -1;
 }
 
+// CTAs that the registers and shared memory of an SM take.
+constexpr int few_ctas(int format, int d, int nt) { return nt == 2 || (format == kCacheBf16 && d == 128) ? 2 : 4; }
+
 // Shared memory of the few-row kernel: each warp's ring of K and V tiles of 16
 // rows, their scales and barriers; at the end the warps' partial sums.
 template <int kFormat, int D, int kNT>
@@ -145,10 +148,10 @@ struct FewShape {
   static constexpr int kBoxes = kRowBytes > 128 ? 2 : 1;          // a swizzled row has at most 128 bytes
   static constexpr int kTile = 16 * kRowBytes;
   static constexpr int kStages = 3;
-  static constexpr int kCtas = kRowBytes > 128 || kNT == 2 ? 1 : 2;   // on an SM
+  static constexpr int kCtas = few_ctas(kFormat, D, kNT);   // on an SM
   static constexpr int kRing = kFewWarps * kStages * 2 * kTile;
   static constexpr int kScales = kFewWarps * kStages * 2 * 16 * 4;
-  static constexpr int kSums = kFewWarps * kNT * 8 * (D + 4 + 2) * 4;
+  static constexpr int kSums = kFewWarps * kNT * 8 * (D + 4 + 2) * 4 + kNT * 8 * (D + 4) * 4;
   static constexpr int kSmem =
       1024 /* alignment */ + (kRing + kScales + kFewWarps * kStages * 8 > kSums ? kRing + kScales + kFewWarps * kStages * 8 : kSums);
 };
@@ -162,14 +165,104 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const void *tmap, uint64_
       : "memory");
 }
 
-// 16-byte piece `c` of row `r` of a swizzled tile of kRowBytes rows (of 256
-// bytes: two tiles of 128-byte halves).
+// Offset of 16-byte piece `c` (below 8) of row `r` in a swizzled tile of
+// kRowBytes rows (of 256 bytes: in the first of two boxes of 128-byte halves).
 template <int kRowBytes>
-__device__ __forceinline__ const uint8_t *piece_of(const uint8_t *tile, int r, int c) {
-  if constexpr (kRowBytes >= 128)
-    return tile + (c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+__device__ __forceinline__ int offset_of(int r, int c) {
+  return kRowBytes >= 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+}
+
+// Where sequences and kv heads are few, the work of a call is cut into pieces
+// that fill the SMs: pieces of about equal length, however the
+// lengths of the sequences differ: with s_b 16-key steps for each of a
+// sequence's units, W steps in all and `pieces` CTAs wanted, T is a little over
+// W / pieces and each unit has ceil(s_b / T) pieces, W / T + units at most in
+// all.  They are numbered sequence, kv head, unit, piece.
+struct FewPiece {
+  int b, kvh, tile;      // sequence (-1: none), kv head, unit of its rows
+  int index, count;      // piece of the unit
+};
+
+// Units of sequence b and the steps of each (one at least, to write zeros).
+__device__ __forceinline__ void units_of(const RaggedArgs &a, int group, int rows_log2, int b, uint32_t &units,
+                                         uint32_t &steps) {
+  const int64_t s0 = max(__ldg(a.starts + b), 0), s1 = min(int64_t(__ldg(a.starts + b + 1)), a.rows);
+  const int64_t length = min(int64_t(__ldg(a.lengths + b)), int64_t(a.c.width) << a.c.shift);
+  units = uint32_t((max(s1 - s0, int64_t(0)) * group + (1 << rows_log2) - 1) >> rows_log2);
+  steps = uint32_t(max(int64_t(1), (length + 15) >> 4));
+}
+
+// The block's piece: every warp searches by itself, a lane over every 32nd part
+// of the sequences.
+__device__ __forceinline__ FewPiece piece_of_block(const RaggedArgs &a, int group, int rows_log2) {
+  const int lane = threadIdx.x & 31, each = (a.batch + 31) >> 5;
+  const int b0 = lane * each, b1 = min(a.batch, b0 + each);
+  uint32_t units = 0, steps = 1;
+  float work = 0.f, whole = 0.f;
+  for (int b = b0; b < b1; ++b) {
+    units_of(a, group, rows_log2, b, units, steps);
+    work += float(units) * float(steps);
+    whole += float(units);
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) {
+    work += __shfl_xor_sync(0xffffffffu, work, x);
+    whole += __shfl_xor_sync(0xffffffffu, whole, x);
+  }
+  const float cuts = fmaxf(a.pieces - whole * a.c.hk, 0.5f * a.pieces);
+  const uint32_t length = max(uint32_t(kFewWarps), uint32_t(work * 1.0001f * a.c.hk / cuts) + 1);
+  uint32_t mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    if (each > 1)
+      units_of(a, group, rows_log2, b, units, steps);
+    mine += units * a.c.hk * ((steps + length - 1) / length);
+  }
+  uint32_t upto = mine;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, upto, x);
+    if (lane >= x)
+      upto += y;
+  }
+  const uint32_t owners = __ballot_sync(0xffffffffu, blockIdx.x < upto);
+  FewPiece p = {-1, 0, 0, 0, 1};
+  if (owners == 0)
+    return p;
+  const int owner = __ffs(owners) - 1;
+  uint32_t at = upto - mine, count = 1;
+  int found = b0;
+  if (lane == owner) {
+    for (;; ++found) {
+      units_of(a, group, rows_log2, found, units, steps);
+      count = (steps + length - 1) / length;
+      const uint32_t pieces = units * a.c.hk * count;
+      if (blockIdx.x < at + pieces || found + 1 >= b1)
+        break;
+      at += pieces;
+    }
+  }
+  p.b = __shfl_sync(0xffffffffu, found, owner);
+  p.count = int(__shfl_sync(0xffffffffu, count, owner));
+  units = __shfl_sync(0xffffffffu, units, owner);
+  const uint32_t rest = blockIdx.x - __shfl_sync(0xffffffffu, at, owner), unit = rest / uint32_t(p.count);
+  p.index = int(rest - unit * uint32_t(p.count));
+  p.kvh = int(unit / units);
+  p.tile = int(unit - uint32_t(p.kvh) * units);
+  return p;
+}
+
+// A lane's values of an output row, divided by the sum of the weights.
+template <int E>
+__device__ __forceinline__ void store_row(__nv_bfloat16 *out, const float (&sum)[E], float total) {
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  uint32_t w[E / 2];
+#pragma unroll
+  for (int e = 0; e < E; e += 2)
+    w[e / 2] = pack_bf16x2(sum[e] * inv, sum[e + 1] * inv);
+  if constexpr (E == 4)
+    *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
   else
-    return tile + r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+    *reinterpret_cast<uint32_t *>(out) = w[0];
 }
 
 template <int kFormat, int D, int kNT>
@@ -186,7 +279,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   extern __shared__ uint8_t few_raw[];
   uint8_t *few_sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(few_raw) + 1023) & ~uintptr_t(1023));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q4 = lane & 3;
-  const int kvh = blockIdx.y, split = blockIdx.z;
   const int group = a.hq / a.hk;
   uint8_t *ring = few_sm + warp * kStages * 2 * kTile;                                    // [kStages][K, V]
   float *scales = reinterpret_cast<float *>(few_sm + Shape::kRing) + warp * kStages * 32;   // [kStages][K, V][16]
@@ -199,8 +291,17 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   __syncwarp();
   pdl_wait();
   pdl_launch_dependents();
-  int tile;
-  const int b = unit_of(a, group, kRowsLog2, blockIdx.x, tile);
+  FewPiece piece;
+  if (a.cluster > 0) {                              // a unit's pieces are the CTAs of a cluster
+    const int unit = int(blockIdx.x) / a.cluster;
+    piece.kvh = unit % a.hk;
+    piece.b = unit_of(a, group, kRowsLog2, unit / a.hk, piece.tile);
+    piece.index = int(blockIdx.x) % a.cluster;
+    piece.count = a.cluster;
+  } else {
+    piece = piece_of_block(a, group, kRowsLog2);
+  }
+  const int b = piece.b, kvh = piece.kvh, tile = piece.tile;
   if (b < 0)
     return;
   const int64_t begin = max(__ldg(a.starts + b), 0);
@@ -212,13 +313,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   const int first_new = first_new_position(a.lengths, b, n);
   const int keys = max(0, min(length, first_new + (r1 - 1) / group + 1));
   const int all_see = min(length, first_new + r0 / group + 1);   // every row sees positions below this
-  // This split's 16-key steps.
+  // This piece's 16-key steps, as equal as the pieces of the unit can be.
   const int steps = (keys + 15) >> 4;
-  const int per = (((steps + a.splits - 1) / a.splits) + kFewWarps - 1) / kFewWarps * kFewWarps;
-  const int step_end = min(steps, (split + 1) * per);
+  const int step_begin = int(int64_t(steps) * piece.index / piece.count);
+  const int step_end = int(int64_t(steps) * (piece.index + 1) / piece.count);
 
   // The warp's steps: every kFewWarps-th from `step0` on.
-  const int step0 = split * per + warp;
+  const int step0 = step_begin + warp;
   const int count = step_end > step0 ? (step_end - step0 + kFewWarps - 1) / kFewWarps : 0;
   const int page_mask = (1 << a.c.shift) - 1;
   int pages_of_lane = 0;                            // the pages of the next 32 steps to copy
@@ -302,6 +403,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   // M row g of a step is its key `mine` (and g + 8 is 8 after it); K index 2 q4
   // is key 2 q4 and 2 q4 + 1 is key `odd` of its first eight.
   const int mine = g ^ ((g & 1) << 2), odd = (2 * q4 + 1) ^ 4;
+  // Their first pieces in a tile; the row 8 after has the same swizzle, the
+  // next four pieces of K lie 64 bytes across, those after 128 in the next box.
+  constexpr int kEight = kRowBytes >= 128 ? 1024 : 512;
+  const int k_off = offset_of<kRowBytes>(mine, q4);
+  const int v_even = VW == 2 ? offset_of<kRowBytes>(2 * q4, g >> 1) + (g & 1) * 8 : offset_of<kRowBytes>(2 * q4, g);
+  const int v_odd = VW == 2 ? offset_of<kRowBytes>(odd, g >> 1) + (g & 1) * 8 : offset_of<kRowBytes>(odd, g);
   int done = 0;
   for (; done < count; ++done) {
     const int step = step0 + done * kFewWarps, stage = done % kStages;
@@ -311,8 +418,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
     uint32_t kr[2][KW], vr[4][VW];                  // K rows mine, mine + 8; V rows 2 q4, odd, and 8 after them
 #pragma unroll
     for (int i = 0; i < KW / 4; ++i) {
-      *reinterpret_cast<uint4 *>(&kr[0][i * 4]) = *reinterpret_cast<const uint4 *>(piece_of<kRowBytes>(k_tile, mine, i * 4 + q4));
-      *reinterpret_cast<uint4 *>(&kr[1][i * 4]) = *reinterpret_cast<const uint4 *>(piece_of<kRowBytes>(k_tile, mine + 8, i * 4 + q4));
+      const uint8_t *at = k_tile + (i >> 1) * 2048 + (i & 1 ? k_off ^ 64 : k_off);
+      *reinterpret_cast<uint4 *>(&kr[0][i * 4]) = *reinterpret_cast<const uint4 *>(at);
+      *reinterpret_cast<uint4 *>(&kr[1][i * 4]) = *reinterpret_cast<const uint4 *>(at + kEight);
     }
     float ksc[2] = {1.f, 1.f}, vsc[2] = {1.f, 1.f};
     if constexpr (!kBf16) {
@@ -340,13 +448,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
     const float k_lo = ksc[0], k_hi = ksc[1];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const int r = (x & 1 ? odd : 2 * q4) + (x & 2) * 4;
+      const uint8_t *at = v_tile + (x & 1 ? v_odd : v_even) + (x >> 1) * kEight;
       if constexpr (VW == 2) {
-        *reinterpret_cast<uint2 *>(vr[x]) = *reinterpret_cast<const uint2 *>(piece_of<kRowBytes>(v_tile, r, g >> 1) + (g & 1) * 8);
+        *reinterpret_cast<uint2 *>(vr[x]) = *reinterpret_cast<const uint2 *>(at);
       } else {
 #pragma unroll
         for (int i = 0; i < VW / 4; ++i)
-          *reinterpret_cast<uint4 *>(&vr[x][i * 4]) = *reinterpret_cast<const uint4 *>(piece_of<kRowBytes>(v_tile, r, i * 8 + g));
+          *reinterpret_cast<uint4 *>(&vr[x][i * 4]) = *reinterpret_cast<const uint4 *>(at + i * 2048);
       }
     }
     __syncwarp();
@@ -503,6 +611,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   // The warps' partial sums, added in warp order.
   float *so = reinterpret_cast<float *>(few_sm);                // [warps][rows][D + 4]
   float *sm = so + kFewWarps * kRows * (D + 4), *sl = sm + kFewWarps * kRows;
+  float *joined = sl + kFewWarps * kRows;                       // [rows][D values, maximum, sum, -, -]
 #pragma unroll
   for (int t = 0; t < kNT; ++t) {
 #pragma unroll
@@ -545,17 +654,110 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
     }
     const int64_t row = begin + (r0 + r) / group;
     const int h = kvh * group + (r0 + r) % group;
-    if (a.splits == 1) {
+    if (piece.count == 1) {
       const float inv = total == 0.f ? 0.f : 1.f / total;
       *reinterpret_cast<uint2 *>(a.out + row * a.ldo + h * D + d) =
           make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+    } else if (a.cluster > 0) {
+      *reinterpret_cast<float4 *>(joined + r * (D + 4) + d) = sum;
+      if (d == 0)
+        joined[r * (D + 4) + D] = m, joined[r * (D + 4) + D + 1] = total;
     } else {
-      const int64_t at = (int64_t(split) * a.rows + row) * a.hq + h;
+      const int64_t at = int64_t(blockIdx.x) * kRows + r;
       *reinterpret_cast<float4 *>(a.part_o + at * D + d) = sum;
       if (d == 0)
         a.part_ml[at] = make_float2(m, total);
     }
   }
+  if (a.cluster > 1) {
+    // The cluster's CTAs each join a share of the unit's values, reading the
+    // others' shared memory, in rank order.
+    cluster_sync();
+    const uint32_t mine_sm = smem_u32(joined);
+    for (int i = piece.index * kFewWarps * 32 + threadIdx.x; i < kRows * (D / 4); i += a.cluster * kFewWarps * 32) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      if (r0 + r >= r1)
+        continue;
+      float m[8], l[8], top_of_all = -INFINITY;
+      int4 x[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        if (c >= a.cluster)
+          break;
+        const uint32_t row = map_peer(mine_sm + r * (D + 4) * 4, c);
+        m[c] = __int_as_float(ld_cluster_s32(row + D * 4));
+        l[c] = __int_as_float(ld_cluster_s32(row + D * 4 + 4));
+        x[c] = ld_cluster_v4(row + d * 4);
+        top_of_all = fmaxf(top_of_all, m[c]);
+      }
+      float total = 0.f;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        if (c >= a.cluster)
+          break;
+        const float f = m[c] == top_of_all ? 1.f : exp2_fast(m[c] - top_of_all);
+        total += f * l[c];
+        sum.x += f * __int_as_float(x[c].x), sum.y += f * __int_as_float(x[c].y);
+        sum.z += f * __int_as_float(x[c].z), sum.w += f * __int_as_float(x[c].w);
+      }
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      *reinterpret_cast<uint2 *>(a.out + (begin + (r0 + r) / group) * a.ldo + (kvh * group + (r0 + r) % group) * D + d) =
+          make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+    }
+    cluster_sync();                                 // no CTA ends while others read it
+  }
+  if (a.cluster > 0)
+    return;
+  // Where the unit's pieces are, for the join: its slot counts units as the
+  // sequences' first rows allow without a search.
+  if (piece.index == 0 && threadIdx.x == 0) {
+    const int64_t slot = ((begin * group) >> kRowsLog2) + b + tile;
+    a.part_units[slot * a.hk + kvh] = make_int2(int(blockIdx.x), piece.count);
+  }
+}
+
+// Joins the pieces of each (row, head) that has several, in order: a warp per
+// row and head, D / 32 values per lane.
+template <int D, int kNT>
+__global__ void __launch_bounds__(256) attention_join_pieces_kernel(const RaggedArgs a) {
+  constexpr int E = D / 32, kRowsLog2 = kNT == 1 ? 3 : 4;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t item = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const int64_t row = item / a.hq;
+  const int h = int(item % a.hq), group = a.hq / a.hk, kvh = h / group;
+  if (row >= a.rows)
+    return;
+  const int b = sequence_of_warp(a.starts, a.batch, row);
+  if (b < 0)
+    return;
+  const int64_t begin = max(__ldg(a.starts + b), 0), r = (row - begin) * group + h % group;
+  const int64_t slot = ((begin * group) >> kRowsLog2) + b + (r >> kRowsLog2);
+  const int2 unit = a.part_units[slot * a.hk + kvh];
+  if (unit.y < 2 || unit.x < 0 || unit.y > a.parts - unit.x)   // one piece (or starts that decrease)
+    return;
+  const int64_t first = (int64_t(unit.x) << kRowsLog2) + (r & ((1 << kRowsLog2) - 1));
+  float top = -INFINITY;
+  for (int s = lane; s < unit.y; s += 32)
+    top = fmaxf(top, a.part_ml[first + (int64_t(s) << kRowsLog2)].x);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1)
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  float total = 0.f, sum[E] = {};
+#pragma unroll 4
+  for (int s = 0; s < unit.y; ++s) {
+    const int64_t at = first + (int64_t(s) << kRowsLog2);
+    const float2 ml = a.part_ml[at];
+    const float f = ml.x == top ? 1.f : exp2_fast(ml.x - top);   // equal, -inf too: the sums as they are
+    total += f * ml.y;
+    const float *p = a.part_o + at * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      sum[e] += f * p[e];
+  }
+  store_row<E>(a.out + row * a.ldo + h * D + lane * E, sum, total);
 }
 
 // Joins the splits of each (row, head), in split order: a warp per row and
@@ -594,16 +796,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const RaggedArgs a)
     for (int e = 0; e < E; ++e)
       sum[e] += fs * p[e];
   }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  uint32_t w[E / 2];
-#pragma unroll
-  for (int e = 0; e < E; e += 2)
-    w[e / 2] = pack_bf16x2(sum[e] * inv, sum[e + 1] * inv);
-  __nv_bfloat16 *out = a.out + row * a.ldo + h * D + lane * E;
-  if constexpr (E == 4)
-    *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
-  else
-    *reinterpret_cast<uint32_t *>(out) = w[0];
+  store_row<E>(a.out + row * a.ldo + h * D + lane * E, sum, total);
 }
 
 } // namespace pir2b

@@ -81,21 +81,25 @@ static int make_pages(const char *what, const pir2b_kv_pages *p, const pir2b_seq
 
 // A launch that may start while its predecessor drains (every kernel here
 // begins with griddepcontrol.wait).
+// `cluster` consecutive CTAs form a thread-block cluster.
 template <typename... Args>
-static int launch_cache(const char *what, void (*kernel)(Args...), int64_t grid, int grid_y, int grid_z, int threads,
+static int launch_cache(const char *what, void (*kernel)(Args...), int64_t grid, int grid_y, int cluster, int threads,
                         size_t smem, void *stream, const std::remove_reference_t<Args> &...args) {
   if (grid > 0x7fffffff)
     return fail(PIR2B_EINVAL, "%s: too many rows", what);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(grid), unsigned(grid_y), unsigned(grid_z));
+  cfg.gridDim = dim3(unsigned(grid), unsigned(grid_y), 1);
   cfg.blockDim = dim3(unsigned(threads), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args...), what);
 }
 
@@ -128,24 +132,40 @@ static int launch_rows(bool write, int format, int d, const CacheRowsArgs &a, vo
   }
 }
 
-static const int kFewWaves = getenv("PIR2B_W") ? atoi(getenv("PIR2B_W")) : 2;
 constexpr int kFewRows = 32;   // rows a sequence has in a kv head, up to which the few-row kernel takes it
 
-// How the few-row kernel covers a call: rows per unit, grid slots and splits.
+// How the few-row kernel covers a call: a cluster of CTAs per unit of rows,
+// which joins its sums in shared memory, or, where eight CTAs a unit leave SMs
+// idle, a list of pieces that a second launch joins.
 struct FewPlan {
-  int nt;          // 8 nt rows per unit
-  int64_t slots;
-  int splits;
+  int nt;            // 8 nt rows per unit
+  int cluster;       // CTAs of a unit, 0: pieces
+  int64_t slots;     // of units
+  int64_t pieces;    // CTAs wanted
+  int64_t grid;
+  int64_t bytes(int hk, int d) const { return cluster ? 0 : grid * 8 * nt * (d * 4 + 8) + slots * hk * 8; }
 };
 
-static FewPlan plan_few(int64_t rows, int hq, int hk, int batch, int64_t positions, int sms) {
-  FewPlan p;
+static FewPlan plan_few(int64_t rows, int hq, int hk, int batch, int64_t positions, int format, int d, int sms) {
+  FewPlan p = {};
   const int group = hq / hk;
   p.nt = (rows + batch - 1) / batch * group <= 8 ? 1 : 2;
   p.slots = rows * group / (8 * p.nt) + batch;
-  // Two CTAs fit an SM; a split reads at least 128 keys.
-  const int64_t want = (int64_t(kFewWaves) * 2 * sms + p.slots * hk - 1) / (p.slots * hk);
-  p.splits = int(std::max<int64_t>(1, std::min<int64_t>({want, positions / (16 * kFewWarps), 32})));
+  const int resident = few_ctas(format, d, p.nt);
+  const int64_t units = batch * ((rows + batch - 1) / batch * group + 8 * p.nt - 1) / (8 * p.nt) * hk;
+  const int64_t longest = (positions + 16 * kFewWarps - 1) / (16 * kFewWarps);    // CTAs a unit can use
+  if (8 * units >= sms / 3 || longest <= 8) {
+    // As many CTAs as are resident at once: a second round costs more than it
+    // evens out (64 int8 sequences of 500-4000 tokens: 73 us in one round, 79
+    // in two, 104 in four).
+    p.cluster = 1;
+    while (p.cluster < 8 && p.cluster * units < resident * sms && 2 * p.cluster <= longest)
+      p.cluster *= 2;
+    p.grid = p.slots * hk * p.cluster;
+  } else {
+    p.pieces = int64_t(2) * resident * sms;
+    p.grid = p.pieces + p.slots * hk;              // each unit may have a piece more
+  }
   return p;
 }
 
@@ -179,8 +199,8 @@ static int launch_attention_few(const FewPlan &p, const RaggedArgs &a, void *str
     return r;
   if (int r = make_pages_map(&tm_v, a.c.v, a.c, D, a.c.v_page, kBytes, 16, true))
     return r;
-  return launch_cache("cache_attention launch", attention_few_kernel<kFormat, D, kNT>, p.slots, a.hk, p.splits,
-                      kFewWarps * 32, FewShape<kFormat, D, kNT>::kSmem, stream, a, tm_k, tm_v);
+  return launch_cache("cache_attention launch", attention_few_kernel<kFormat, D, kNT>, p.grid, 1, std::max(p.cluster, 1), kFewWarps * 32,
+                      FewShape<kFormat, D, kNT>::kSmem, stream, a, tm_k, tm_v);
 }
 
 template <int kFormat>
@@ -237,14 +257,14 @@ struct CachePlan {
   int tiles;
   FewPlan few;
   int splits;
+  bool joined() const { return tiles == 0 ? few.cluster == 0 : splits > 1; }
 };
 
-static CachePlan plan_cache(int64_t rows, int hq, int hk, int batch, int64_t positions, int format, int sms) {
+static CachePlan plan_cache(int64_t rows, int hq, int hk, int d, int batch, int64_t positions, int format, int sms) {
   CachePlan p = {};
   const int64_t per_sequence = (rows + batch - 1) / batch * (hq / hk);
   if (per_sequence <= kFewRows) {
-    p.few = plan_few(rows, hq, hk, batch, positions, sms);
-    p.splits = p.few.splits;
+    p.few = plan_few(rows, hq, hk, batch, positions, format, d, sms);
     return p;
   }
   p.tiles = format != kCacheBf16 || per_sequence > 128 ? 2 : 1;
@@ -277,7 +297,12 @@ static int launch_cache_attention(const CachePlan &p, int d, const RaggedArgs &a
   return d == 64 ? launch_cache_tile<kFormat, 64>(p, a, stream) : launch_cache_tile<kFormat, 128>(p, a, stream);
 }
 
-static int launch_join(int d, const RaggedArgs &a, void *stream) {
+static int launch_join(const CachePlan &p, int d, const RaggedArgs &a, void *stream) {
+  if (p.tiles == 0)
+    return launch_cache("cache_attention join launch",
+                        d == 64 ? (p.few.nt == 1 ? attention_join_pieces_kernel<64, 1> : attention_join_pieces_kernel<64, 2>)
+                                : (p.few.nt == 1 ? attention_join_pieces_kernel<128, 1> : attention_join_pieces_kernel<128, 2>),
+                        (a.rows * a.hq + 7) / 8, 1, 1, 256, 0, stream, a);
   return launch_cache("cache_attention join launch", d == 64 ? attention_join_kernel<64> : attention_join_kernel<128>,
                       (a.rows * a.hq + 7) / 8, 1, 1, 256, 0, stream, a);
 }
@@ -479,13 +504,18 @@ int pir2b_cache_attention(const void *q, int64_t q_row, int64_t q_head, int64_t 
   if (int r = cache_kernel_attributes(dev))
     return r;
   const CachePlan plan =
-      plan_cache(rows, hq, a.hk, a.batch, int64_t(a.c.width) << a.c.shift, pages->format, dev->sms);
+      plan_cache(rows, hq, a.hk, d, a.batch, int64_t(a.c.width) << a.c.shift, pages->format, dev->sms);
   a.splits = plan.splits;
-  if (plan.splits > 1) {
+  a.cluster = plan.few.cluster;
+  if (plan.joined()) {
     if (workspace == nullptr || !aligned(workspace, 16))
       return fail(PIR2B_EALIGN, "cache_attention: this shape needs a 16-byte aligned workspace");
+    const int64_t parts = plan.tiles == 0 ? plan.few.grid * 8 * plan.few.nt : plan.splits * rows * hq;
     a.part_o = static_cast<float *>(workspace);
-    a.part_ml = reinterpret_cast<float2 *>(a.part_o + int64_t(plan.splits) * rows * hq * d);
+    a.part_ml = reinterpret_cast<float2 *>(a.part_o + parts * d);
+    a.part_units = reinterpret_cast<int2 *>(a.part_ml + parts);
+    a.pieces = int(plan.few.pieces);
+    a.parts = int(plan.few.grid);
   }
   int status = PIR2B_OK;
   switch (pages->format) {
@@ -493,7 +523,7 @@ int pir2b_cache_attention(const void *q, int64_t q_row, int64_t q_head, int64_t 
   case kCacheE4m3: status = launch_cache_attention<kCacheE4m3>(plan, d, a, stream); break;
   default: status = launch_cache_attention<kCacheBf16>(plan, d, a, stream); break;
   }
-  return status != PIR2B_OK || plan.splits == 1 ? status : launch_join(d, a, stream);
+  return status != PIR2B_OK || !plan.joined() ? status : launch_join(plan, d, a, stream);
 }
 
 int64_t pir2b_cache_attention_workspace(int64_t rows, int hq, const pir2b_kv_pages *pages,
@@ -502,9 +532,12 @@ int64_t pir2b_cache_attention_workspace(int64_t rows, int hq, const pir2b_kv_pag
   if (pages == nullptr || sequences == nullptr || rows < 1 || pages->kv_heads < 1 || hq < pages->kv_heads ||
       sequences->batch < 1 || device_info(&dev) != PIR2B_OK)
     return 0;                                     // the call itself reports what is wrong
-  const CachePlan plan = plan_cache(rows, hq, pages->kv_heads, sequences->batch,
+  const CachePlan plan = plan_cache(rows, hq, pages->kv_heads, pages->head_dim, sequences->batch,
                                     int64_t(sequences->table_width) * pages->page_size, pages->format, dev->sms);
-  return plan.splits == 1 ? 0 : int64_t(plan.splits) * rows * hq * (pages->head_dim * 4 + 8);
+  if (!plan.joined())
+    return 0;
+  return plan.tiles == 0 ? plan.few.bytes(pages->kv_heads, pages->head_dim)
+                         : int64_t(plan.splits) * rows * hq * (pages->head_dim * 4 + 8);
 }
 
 } // extern "C"
