@@ -113,17 +113,24 @@ __device__ __forceinline__ int first_new_position(const int *lengths, int b, int
 // as their first slot, which leaves each of them ceil(rows * group / tile) at
 // least and takes floor(rows * group / tile) + batch in all, so the host can
 // size the grid without the lengths.  Returns the sequence, or -1.
-// All lanes of a warp search together, 128 candidates at a time.
-__device__ __forceinline__ int unit_of(const RaggedArgs &a, int group, int tile_log2, int slot, int &tile) {
+// All lanes of a warp search together, 128 candidates at a time; s0 and s1 are
+// the sequence's first row and the one after its last.
+__device__ __forceinline__ int unit_of(const RaggedArgs &a, int tile_log2, int slot, int &tile, int &s0, int &s1) {
   const int lane = threadIdx.x & 31;
-  int lo = 0, hi = a.batch;
+  int lo = 0, hi = a.batch, first[4], after[4], count = 0, step;
   do {
-    const int step = (hi - lo + 127) >> 7;
-    int count = 0;
+    step = (hi - lo + 127) >> 7;
+    count = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = min(lo + (i * 32 + lane) * step, a.batch);
+      first[i] = max(__ldg(a.starts + at), 0);
+      after[i] = __ldg(a.starts + min(at + 1, a.batch));
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int at = lo + (i * 32 + lane) * step;
-      const bool before = at < hi && ((int64_t(max(__ldg(a.starts + min(at, hi)), 0)) * group) >> tile_log2) + at <= slot;
+      const bool before = at < hi && ((int64_t(first[i]) * a.group) >> tile_log2) + at <= slot;
       count += __popc(__ballot_sync(0xffffffffu, before));
     }
     if (count == 0)
@@ -131,9 +138,12 @@ __device__ __forceinline__ int unit_of(const RaggedArgs &a, int group, int tile_
     lo += (count - 1) * step;
     hi = min(hi, lo + step);
   } while (hi - lo > 1);
-  const int64_t s0 = max(__ldg(a.starts + lo), 0), s1 = min(int64_t(__ldg(a.starts + lo + 1)), a.rows);
-  tile = slot - int((s0 * group) >> tile_log2) - lo;
-  return (tile >= 0 && (int64_t(tile) << tile_log2) < (s1 - s0) * group) ? lo : -1;
+  const int which = (count - 1) >> 5, of = (count - 1) & 31;
+  s0 = __shfl_sync(0xffffffffu, which & 2 ? (which & 1 ? first[3] : first[2]) : (which & 1 ? first[1] : first[0]), of);
+  s1 = __shfl_sync(0xffffffffu, which & 2 ? (which & 1 ? after[3] : after[2]) : (which & 1 ? after[1] : after[0]), of);
+  s1 = int(min(int64_t(s1), a.rows));
+  tile = slot - int((int64_t(s0) * a.group) >> tile_log2) - lo;
+  return (tile >= 0 && (int64_t(tile) << tile_log2) < int64_t(s1 - s0) * a.group) ? lo : -1;
 }
 
 // CTAs that the registers and shared memory of an SM take.
@@ -279,7 +289,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   extern __shared__ uint8_t few_raw[];
   uint8_t *few_sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(few_raw) + 1023) & ~uintptr_t(1023));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q4 = lane & 3;
-  const int group = a.hq / a.hk;
+  const int group = a.group;
   uint8_t *ring = few_sm + warp * kStages * 2 * kTile;                                    // [kStages][K, V]
   float *scales = reinterpret_cast<float *>(few_sm + Shape::kRing) + warp * kStages * 32;   // [kStages][K, V][16]
   uint64_t *full = reinterpret_cast<uint64_t *>(few_sm + Shape::kRing + Shape::kScales) + warp * kStages;
@@ -295,7 +305,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   if (a.cluster > 0) {                              // a unit's pieces are the CTAs of a cluster
     const int unit = int(blockIdx.x) / a.cluster;
     piece.kvh = unit % a.hk;
-    piece.b = unit_of(a, group, kRowsLog2, unit / a.hk, piece.tile);
+    int s0, s1;
+    piece.b = unit_of(a, kRowsLog2, unit / a.hk, piece.tile, s0, s1);
     piece.index = int(blockIdx.x) % a.cluster;
     piece.count = a.cluster;
   } else {

@@ -21,8 +21,10 @@ struct RaggedArgs {
   int64_t ldo;
   int64_t rows;
   int batch, hq, hk;
+  int group;                    // hq / hk
+  uint32_t inverse;             // floor(2^32 / group), 2^32 - 1 for 1
   float scale_log2;             // scale * log2(e)
-  int q_by_tma;                 // q tiles are whole boxes: the group divides 128
+  int q_by_tma, out_by_tma;     // q tiles (output rows of a warp) are whole boxes: the group divides 128 (32)
   int splits;                   // CTAs along the keys of a unit, at most 32
   float *part_o;                // [splits, rows, hq, D] sums, where splits > 1,
   float2 *part_ml;              // [splits, rows, hq] and their (maximum, sum of weights)
@@ -32,5 +34,11 @@ struct RaggedArgs {
   int pieces, parts;
   int2 *part_units;
 };
+
+// x / group, x >= 0: the product falls short of the quotient by one at most.
+__device__ __forceinline__ int over_group(const RaggedArgs &a, int x) {
+  const int q = int(__umulhi(uint32_t(x), a.inverse));
+  return q + (x - q * a.group >= a.group);
+}
 
 } // namespace pir2b

@@ -117,6 +117,12 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const void *tmap, uint64_
       : "memory");
 }
 
+__device__ __forceinline__ void tma_store_3d(const void *tmap, const void *src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(tmap),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+
 // What a CTA works on.  Positions count from `base`, the first of its split.
 struct TileWork {
   int b;              // sequence
@@ -138,7 +144,8 @@ struct TileWork {
 template <int kSource, int D, int kTiles>
 __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTiles == 2 ? 1 : 2)
     attention_tile_kernel(const RaggedArgs a, const __grid_constant__ CUtensorMap tm_q,
-                          const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+                          const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                          const __grid_constant__ CUtensorMap tm_o) {
   using Shape = TileShape<kSource, D, kTiles>;
   constexpr bool kScaled = Shape::kScaled, kPaged = kSource != kSourceRows;
   constexpr int kMmaWarp = kTiles * 4, kRows = kTiles * 128;
@@ -188,16 +195,17 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
   }
   pdl_wait();
   pdl_launch_dependents();
-  const int group = a.hq / a.hk;
+  const int group = a.group;
   // Later rows see more keys: they start first.
-  const int unit = int((gridDim.x - 1 - blockIdx.x) / a.splits), split = int(blockIdx.x % a.splits);
-  const int kvh = unit % a.hk, slot = unit / a.hk;
+  const int unit = int((gridDim.x - 1 - blockIdx.x) / uint32_t(a.splits)), split = int(blockIdx.x % uint32_t(a.splits));
+  const int kvh = int(uint32_t(unit) % uint32_t(a.hk)), slot = int(uint32_t(unit) / uint32_t(a.hk));
   TileWork w = {};
   int tile;
-  w.b = unit_of(a, group, kTiles == 2 ? 8 : 7, slot, tile);
+  int s0, s1;
+  w.b = unit_of(a, kTiles == 2 ? 8 : 7, slot, tile, s0, s1);
   if (w.b >= 0) {
-    w.begin = max(__ldg(a.starts + w.b), 0);
-    const int n = int(min(int64_t(__ldg(a.starts + w.b + 1)), a.rows) - w.begin);
+    w.begin = s0;
+    const int n = s1 - s0;
     w.r0 = tile * kRows;
     w.r1 = n * group;
     int length = n;
@@ -205,15 +213,16 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
       length = cache_length(a.c, a.lengths, w.b);
       w.first = first_new_position(a.lengths, w.b, n);
     }
-    w.all_see = max(0, min(length, w.first + w.r0 / group + 1));
+    w.all_see = max(0, min(length, w.first + over_group(a, w.r0) + 1));
 #pragma unroll
     for (int u = 0; u < kTiles; ++u) {
       const int last = min(w.r0 + 128 * (u + 1), w.r1) - 1;   // last row of the tile
-      const int keys = last < w.r0 + 128 * u ? 0 : max(0, min(length, w.first + last / group + 1));
+      const int keys = last < w.r0 + 128 * u ? 0 : max(0, min(length, w.first + over_group(a, last) + 1));
       (u ? w.keys1 : w.keys0) = keys;
       w.keys = max(w.keys, keys);
     }
-    const int per = ((w.keys + kTileKeys - 1) / kTileKeys + a.splits - 1) / a.splits * kTileKeys;   // of a split
+    const int all = (w.keys + kTileKeys - 1) / kTileKeys;
+    const int per = (a.splits == 1 ? all : (all + a.splits - 1) / a.splits) * kTileKeys;   // of a split
     w.base = split * per;
     w.keys0 = max(0, min(w.keys0 - w.base, per));
     w.keys1 = max(0, min(w.keys1 - w.base, per));
@@ -235,14 +244,11 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
     const uint32_t s_tm = tmem + lanes + u * 128, o_tm = tmem + lanes + kOCols + u * 128;
     const int r = w.r0 + u * 128 + t;                         // this thread's row
     const bool valid = w.b >= 0 && r < w.r1;
-    // Token and head of the CTA's i-th row, by a multiply: exact for i + rest
-    // below 2^21 / group (at most 256 + group, group at most 1024).
-    const int token0 = w.r0 / group;
-    const uint32_t rest = w.r0 - token0 * group, inverse = ((1u << 21) + group - 1) / group;
+    // Token and head of the CTA's i-th row.
     auto token_of = [&](int i, int &head) {
-      const int step = int(((rest + i) * inverse) >> 21);
-      head = kvh * group + int(rest) + i - step * group;
-      return token0 + step;
+      const int token = over_group(a, w.r0 + i);
+      head = kvh * group + w.r0 + i - token * group;
+      return token;
     };
     int my_head;
     const int my_token = token_of(u * 128 + t, my_head);
@@ -408,8 +414,9 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
       if (a.splits > 1 && valid)
         a.part_ml[part] = make_float2(top, l);
       const bool spoiled = *reinterpret_cast<volatile int *>(&bar.spoiled) != 0;
-      uint8_t *row_sm = q_sm + u * kBytes + t * (D * 2);
-#pragma unroll 1
+      // Into the tile that held Q (its products are done), in the same layout.
+      uint8_t *row_sm = q_sm + u * kBytes + t * 128;
+#pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         uint32_t o[32] = {};
         if (w.blocks(u) > 0) {
@@ -447,25 +454,38 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
           }
           continue;
         }
-        // The row's 16-byte pieces into the tile that held Q (its products are
-        // done), rotated by row so that a warp's writes spread over the banks.
 #pragma unroll
         for (int c = 0; c < 32; c += 8)
-          *reinterpret_cast<uint4 *>(row_sm + (((i * 4 + c / 8) ^ (t & 7)) << 4)) =
+          *reinterpret_cast<uint4 *>(row_sm + (i >> 1) * 16384 + ((((i & 1) * 4 + c / 8) ^ (t & 7)) << 4)) =
               make_uint4(pack_bf16x2(f[c], f[c + 1]), pack_bf16x2(f[c + 2], f[c + 3]), pack_bf16x2(f[c + 4], f[c + 5]),
                          pack_bf16x2(f[c + 6], f[c + 7]));
       }
-      // Whole rows at a time to memory, this warp's own 32.
-      __syncwarp();
-      constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces;
+      // This warp's 32 rows to memory: by TMA, or the last of a sequence row by
+      // row.
+      const int first_row = w.r0 + u * 128 + (warp & 3) * 32;
+      if (a.splits == 1 && a.out_by_tma && first_row + 32 <= w.r1) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h)
+            tma_store_3d(&tm_o, q_sm + u * kBytes + h * 16384 + (warp & 3) * 4096, h * 64, kvh * group,
+                         int(w.begin) + over_group(a, first_row));
+          tma_store_commit_and_wait();
+        }
+      } else if (a.splits == 1) {
+        __syncwarp();
+        constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces;
 #pragma unroll 4
-      for (int i = a.splits > 1 ? 32 : 0; i < 32; i += kAtOnce) {
-        const int rr = (warp & 3) * 32 + i + lane / kPieces, piece = lane % kPieces;
-        int head;
-        const int token = token_of(u * 128 + rr, head);
-        const uint4 x = *reinterpret_cast<const uint4 *>(q_sm + u * kBytes + rr * (D * 2) + ((piece ^ (rr & 7)) << 4));
-        if (w.r0 + u * 128 + rr < w.r1)
-          *reinterpret_cast<uint4 *>(a.out + (w.begin + token) * a.ldo + head * D + piece * 8) = x;
+        for (int i = 0; i < 32; i += kAtOnce) {
+          const int rr = (warp & 3) * 32 + i + lane / kPieces, piece = lane % kPieces;
+          int head;
+          const int token = token_of(u * 128 + rr, head);
+          const uint4 x = *reinterpret_cast<const uint4 *>(q_sm + u * kBytes + (piece >> 3) * 16384 + rr * 128 +
+                                                           (((piece & 7) ^ (rr & 7)) << 4));
+          if (w.r0 + u * 128 + rr < w.r1)
+            *reinterpret_cast<uint4 *>(a.out + (w.begin + token) * a.ldo + head * D + piece * 8) = x;
+        }
       }
     }
   } else {
@@ -549,7 +569,7 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
 #pragma unroll
         for (int h = 0; h < kHalves; ++h)
           tma_load_3d(q_sm + lane * kBytes + h * 16384, &tm_q, &bar.q_full[lane], h * 64, kvh * group,
-                      int(w.begin) + (w.r0 + lane * 128) / group);
+                      int(w.begin) + over_group(a, w.r0 + lane * 128));
       }
       // Item 2 j is block j's K, item 2 j + 1 its V.  From pages, a lane per
       // page copies it (a bad page reads page 0: any values do).  8-bit codes

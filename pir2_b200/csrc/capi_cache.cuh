@@ -26,6 +26,13 @@ static int check_heads(const char *what, int hq, int hk, int d) {
   return PIR2B_OK;
 }
 
+static void set_heads(RaggedArgs *a, int hq, int hk) {
+  a->hq = hq;
+  a->hk = hk;
+  a->group = hq / hk;
+  a->inverse = a->group == 1 ? 0xffffffffu : uint32_t((uint64_t(1) << 32) / a->group);
+}
+
 static int check_out(const char *what, const void *out, int64_t ldo, int64_t width) {
   if (out == nullptr || ldo < width)
     return fail(PIR2B_EINVAL, "%s: output missing or its row stride below its width", what);
@@ -232,17 +239,26 @@ static int make_rows_map(CUtensorMap *map, const void *base, int64_t rows, int h
 static int make_q_map(CUtensorMap *map, RaggedArgs *a, int d) {
   const int group = a->hq / a->hk;
   a->q_by_tma = 128 % group == 0;
+  a->out_by_tma = 32 % group == 0;
   return make_rows_map(map, a->q, a->rows, a->hq, d, a->q_row, a->q_head, a->q_by_tma ? group : 1,
                        a->q_by_tma ? 128 / group : 128);
+}
+
+// Output rows leave 32 at a time (a warp's) where the group divides 32.
+static int make_o_map(CUtensorMap *map, const RaggedArgs &a, int d) {
+  return make_rows_map(map, a.out, a.rows, a.hq, d, a.ldo, d, a.out_by_tma ? a.group : 1, a.out_by_tma ? 32 / a.group : 32);
 }
 
 template <int kSource, int D, int kTiles>
 static int launch_tile(const char *what, const RaggedArgs &a, const CUtensorMap &tm_q, const CUtensorMap &tm_k,
                        const CUtensorMap &tm_v, void *stream) {
+  CUtensorMap tm_o;
+  if (int r = make_o_map(&tm_o, a, D))
+    return r;
   using Shape = TileShape<kSource, D, kTiles>;
   const int64_t grid = (a.rows * (a.hq / a.hk) / (128 * kTiles) + a.batch) * a.hk * a.splits;
   return launch_cache(what, attention_tile_kernel<kSource, D, kTiles>, grid, 1, 1, Shape::kThreads, Shape::kSmem, stream, a,
-                      tm_q, tm_k, tm_v);
+                      tm_q, tm_k, tm_v, tm_o);
 }
 
 // Tiles per CTA of the tile kernel.  One tile and two CTAs on an SM cover the
@@ -392,8 +408,7 @@ int pir2b_prompt_attention(const void *q, int64_t q_row, int64_t q_head, const v
   a.ldo = ldo;
   a.rows = rows;
   a.batch = int(batch);
-  a.hq = hq;
-  a.hk = hk;
+  set_heads(&a, hq, hk);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.splits = 1;
   if (int r = cache_kernel_attributes(dev))
@@ -497,8 +512,7 @@ int pir2b_cache_attention(const void *q, int64_t q_row, int64_t q_head, int64_t 
   a.ldo = ldo;
   a.rows = rows;
   a.batch = sequences->batch;
-  a.hq = hq;
-  a.hk = pages->kv_heads;
+  set_heads(&a, hq, pages->kv_heads);
   a.scale_log2 = scale * 1.4426950408889634f;
   const int d = pages->head_dim;
   if (int r = cache_kernel_attributes(dev))
