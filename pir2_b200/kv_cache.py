@@ -62,6 +62,7 @@ class KVPages:
             pages, size, heads, dim, FORMATS[k.dtype],
         )
         self.address = ctypes.addressof(self.struct)
+        self.blank = torch.empty(0, dtype=torch.bfloat16, device=k.device)   # what reads allocate like
 
     @classmethod
     def allocate(cls, pages, kv_heads, head_dim, *, page_size=64, dtype=torch.int8, device="cuda"):

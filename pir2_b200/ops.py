@@ -630,21 +630,29 @@ def attention_rows(q, k, v, *, batch, heads, head_dim, scale=None, out=None):
     return out
 
 
+def _raw_stream(index):
+    """The current stream of device `index` as the library takes it."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _head_rows(x, what):
-    """(rows, heads, head_dim, row stride, head stride) of a packed bf16
-    [rows, heads, head_dim] view with unit stride along head_dim."""
-    if x.ndim != 3 or x.dtype != torch.bfloat16 or not x.is_cuda or x.stride(2) != 1:
+    """Shape and row and head strides of a packed bf16 [rows, heads, head_dim]
+    view with unit stride along head_dim."""
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or x.dtype != torch.bfloat16 or not x.is_cuda or stride[2] != 1:
         raise ValueError(f"{what} must be CUDA bf16 [rows, heads, head_dim] with unit stride along head_dim")
-    rows, heads, d = x.shape
-    return rows, heads, d, x.stride(0) if rows > 1 else heads * d, x.stride(1) if heads > 1 else d
+    rows, heads, d = shape
+    # The stride of a dimension of one entry says nothing.
+    return shape, stride[0] if rows > 1 else heads * d, stride[1] if heads > 1 else d
 
 
 def _attention_out(out, q, rows, width):
+    """(output, its row stride)"""
     if out is None:
-        return torch.empty((rows, width), device=q.device, dtype=torch.bfloat16)
+        return q.new_empty((rows, width)), width
     if out.shape != (rows, width) or out.dtype != torch.bfloat16 or out.device != q.device or out.stride(1) != 1:
         raise ValueError("out must be bf16 [rows, heads * head_dim] on q's device with unit column stride")
-    return out
+    return out, out.stride(0) if rows > 1 else width
 
 
 def prompt_attention(q, k, v, starts, *, scale=None, out=None):
@@ -658,23 +666,26 @@ def prompt_attention(q, k, v, starts, *, scale=None, out=None):
     [rows, hq * head_dim], the o_proj input; rows of no prompt are not
     written.
     """
-    rows, hq, d, q_row, q_head = _head_rows(q, "prompt_attention: q")
-    k_rows, hk, k_d, k_row, k_head = _head_rows(k, "prompt_attention: k")
-    *v_shape, v_row, v_head = _head_rows(v, "prompt_attention: v")
-    if v_shape != [rows, hk, d] or k_rows != rows or k_d != d:
+    (rows, hq, d), q_row, q_head = _head_rows(q, "prompt_attention: q")
+    k_shape, k_row, k_head = _head_rows(k, "prompt_attention: k")
+    v_shape, v_row, v_head = _head_rows(v, "prompt_attention: v")
+    hk = k_shape[1]
+    if k_shape != v_shape or k_shape[0] != rows or k_shape[2] != d:
         raise ValueError("prompt_attention: k and v must be [rows, hk, head_dim] with q's rows and head_dim")
     index = q.get_device()
     if k.get_device() != index or v.get_device() != index or starts.get_device() != index:
         raise ValueError("prompt_attention: all tensors must be on one device")
-    if starts.dtype != torch.int32 or starts.ndim != 1 or starts.numel() < 2 or not starts.is_contiguous():
+    count = starts.numel()
+    if starts.dtype != torch.int32 or starts.ndim != 1 or count < 2 or not starts.is_contiguous():
         raise ValueError("prompt_attention: starts must be contiguous int32 [prompts + 1]")
-    out = _attention_out(out, q, rows, hq * d)
+    out, out_row = _attention_out(out, q, rows, hq * d)
     status = _lib.lib().pir2b_prompt_attention(
         q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
-        starts.data_ptr(), starts.numel() - 1, rows, hq, hk, d, d**-0.5 if scale is None else scale, out.data_ptr(),
-        out.stride(0) if rows > 1 else hq * d, _stream(index),
+        starts.data_ptr(), count - 1, rows, hq, hk, d, d**-0.5 if scale is None else scale, out.data_ptr(), out_row,
+        _raw_stream(index),
     )
-    _lib.check(status, "pir2b_prompt_attention")
+    if status:
+        _lib.check(status, "pir2b_prompt_attention")
     return out
 
 
@@ -682,18 +693,20 @@ def cache_write(k, v, pages, sequences):
     """Quantises (in the pool's format) the new rows k, v: bf16 [rows,
     kv_heads, head_dim] views and writes them to the last positions of their
     sequences.  `pages`: kv_cache.KVPages, `sequences`: kv_cache.Sequences."""
-    rows, hk, d, k_row, k_head = _head_rows(k, "cache_write: k")
-    *v_shape, v_row, v_head = _head_rows(v, "cache_write: v")
-    if v_shape != [rows, hk, d] or hk != pages.kv_heads or d != pages.head_dim:
+    shape, k_row, k_head = _head_rows(k, "cache_write: k")
+    v_shape, v_row, v_head = _head_rows(v, "cache_write: v")
+    rows, hk, d = shape
+    if v_shape != shape or hk != pages.kv_heads or d != pages.head_dim:
         raise ValueError("cache_write: k and v must be [rows, kv_heads, head_dim] of the pool's heads")
     index = k.get_device()
     if v.get_device() != index or pages.index != index or sequences.index != index:
         raise ValueError("cache_write: rows, pages and sequences must be on one device")
     status = _lib.lib().pir2b_cache_write(
         k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, rows, pages.address, sequences.address,
-        _stream(index),
+        _raw_stream(index),
     )
-    _lib.check(status, "pir2b_cache_write")
+    if status:
+        _lib.check(status, "pir2b_cache_write")
 
 
 def cache_read(pages, sequences, rows):
@@ -705,11 +718,13 @@ def cache_read(pages, sequences, rows):
         raise ValueError("cache_read: pages and sequences must be on one device")
     if rows < 0:
         raise ValueError("cache_read: rows must not be negative")
-    k, v = torch.empty((2, rows, pages.kv_heads, pages.head_dim), device=pages.device, dtype=torch.bfloat16)
+    shape = (rows, pages.kv_heads, pages.head_dim)
+    k, v = pages.blank.new_empty(shape), pages.blank.new_empty(shape)
     status = _lib.lib().pir2b_cache_read(
-        pages.address, sequences.address, rows, k.data_ptr(), v.data_ptr(), _stream(index)
+        pages.address, sequences.address, rows, k.data_ptr(), v.data_ptr(), _raw_stream(index)
     )
-    _lib.check(status, "pir2b_cache_read")
+    if status:
+        _lib.check(status, "pir2b_cache_read")
     return k, v
 
 
@@ -722,19 +737,20 @@ def cache_attention(q, pages, sequences, *, scale=None, out=None):
     A row that sees no position gives zeros.  Returns bf16 [rows,
     hq * head_dim]; scale defaults to head_dim ** -0.5.
     """
-    rows, hq, d, q_row, q_head = _head_rows(q, "cache_attention: q")
+    (rows, hq, d), q_row, q_head = _head_rows(q, "cache_attention: q")
     if d != pages.head_dim or hq % pages.kv_heads:
         raise ValueError("cache_attention: q must be [rows, hq, head_dim], hq a multiple of the pool's kv_heads")
     index = q.get_device()
     if pages.index != index or sequences.index != index:
         raise ValueError("cache_attention: q, pages and sequences must be on one device")
-    out = _attention_out(out, q, rows, hq * d)
+    out, out_row = _attention_out(out, q, rows, hq * d)
     lib = _lib.lib()
     size = lib.pir2b_cache_attention_workspace(rows, hq, pages.address, sequences.address)
     workspace = torch.empty(size, device=q.device, dtype=torch.uint8) if size > 0 else None
     status = lib.pir2b_cache_attention(
         q.data_ptr(), q_row, q_head, rows, hq, pages.address, sequences.address, d**-0.5 if scale is None else scale,
-        out.data_ptr(), out.stride(0) if rows > 1 else hq * d, _ptr(workspace), _stream(index),
+        out.data_ptr(), out_row, None if workspace is None else workspace.data_ptr(), _raw_stream(index),
     )
-    _lib.check(status, "pir2b_cache_attention")
+    if status:
+        _lib.check(status, "pir2b_cache_attention")
     return out
