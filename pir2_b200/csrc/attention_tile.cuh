@@ -8,13 +8,13 @@
 //   P = exp2(scale S - m), rounded to bf16, written over half of S in TMEM,
 //   O += P V   (P from TMEM, V in shared memory as it lies: keys x D, the
 //               transposed B operand; O fp32 in TMEM).
-// Four warps per tile are its softmax, one thread per row, so row maxima and
-// sums need no shuffles; then one warp issues the MMAs, one loads K and V by
-// TMA into a ring, and two mend V blocks that hold positions some row must
-// not see.  While one tile's softmax runs, the tensor core works on the
-// other's products.  The running maximum moves only when a score
-// passes it by more than 8 (in log2): P stays below 2^8 and O is rescaled in
-// TMEM by the softmax warps only then.  Maxima, sums and O are fp32.
+// Eight warps per tile are its softmax, two threads per row with half of a
+// block's columns each; then one warp issues the MMAs, one loads K and V by TMA
+// into a ring, and one mends V blocks that hold positions some row must not
+// see.  While one tile's softmax runs, the tensor core works on the other's
+// products.  Weights are relative to a reference near the running maximum that
+// moves in few blocks: O is rescaled in TMEM by the softmax warps only then.
+// References, sums and O are fp32.
 //
 // TMEM columns: S/P of each tile (128 each), then O of each.
 // Every wait is bounded; on expiry all roles leave their loops, the loader
@@ -33,7 +33,7 @@ constexpr int kTileKeys = 128;
 template <int kSource, int D, int kTiles>
 struct TileShape {
   static constexpr bool kScaled = kSource == kCacheInt8 || kSource == kCacheE4m3;
-  static constexpr int kThreads = kTiles * 128 + 128 + (kScaled ? 128 : 0);
+  static constexpr int kThreads = kTiles * 256 + 96 + (kScaled ? 128 : 0);
   static constexpr int kBytes = 128 * D * 2;            // a Q, K or V tile
   static constexpr int kStages = kTiles == 2 ? (D == 128 ? (kScaled ? 3 : 5) : (kScaled ? 6 : 8)) : (D == 128 ? 2 : 5);
   // 8-bit caches: tiles of codes on their way to the converting warps, and
@@ -43,12 +43,12 @@ struct TileShape {
   static constexpr int kRaw = kScaled ? 3 : 0, kRawBytes = 128 * D;
   static constexpr int kDepth = (kStages + kRaw + 2) / 2;
   static constexpr int kScaleBytes = kScaled ? kDepth * 2 * kTileKeys * 4 : 0;
-  static constexpr int kSmem =
-      (kTiles + kStages) * kBytes + kRaw * kRawBytes + kScaleBytes + 1024 /* alignment */ + 512 /* barriers */;
+  static constexpr int kSumBytes = kTiles * 2 * 128 * 4;
+  static constexpr int kSmem = (kTiles + kStages) * kBytes + kRaw * kRawBytes + kScaleBytes + kSumBytes + 512 /* barriers */;
 };
 
 struct TileBarriers {   // at most 512 bytes
-  uint64_t full[8], empty[8], raw_full[3], raw_empty[3], q_full[2], s_full[2], p_full[2][2], o_full[2], to_mend[3], mended[3];
+  uint64_t full[8], empty[8], raw_full[3], raw_empty[3], q_full[2], s_full[2], p_full[2], o_full[2], to_mend[3], mended[3];
   uint32_t tmem;
   int spoiled;   // a V block held a value that is not finite at a position hidden from some row
 };
@@ -148,16 +148,16 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
                           const __grid_constant__ CUtensorMap tm_o) {
   using Shape = TileShape<kSource, D, kTiles>;
   constexpr bool kScaled = Shape::kScaled, kPaged = kSource != kSourceRows;
-  constexpr int kMmaWarp = kTiles * 4, kRows = kTiles * 128;
+  constexpr int kMmaWarp = kTiles * 8, kRows = kTiles * 128;
   constexpr uint32_t kOCols = kTiles * 128;       // TMEM: S/P of the tiles, then O
   constexpr int kStages = Shape::kStages, kBytes = Shape::kBytes;
   constexpr int kHalves = D / 64;                 // 64-column blocks of a tile, 16 KB each
-  extern __shared__ uint8_t tile_raw[];
-  uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tile_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *q_sm = sm, *ring = sm + kTiles * kBytes;
+  extern __shared__ __align__(1024) uint8_t tile_raw[];   // swizzled tiles need the alignment; nothing lies before
+  uint8_t *q_sm = tile_raw, *ring = q_sm + kTiles * kBytes;
   uint8_t *raw = ring + kStages * kBytes;                               // [kRaw][128][D] codes
   float *scales = reinterpret_cast<float *>(raw + Shape::kRaw * Shape::kRawBytes);   // [kDepth][K, V][128]
-  TileBarriers &bar = *reinterpret_cast<TileBarriers *>(reinterpret_cast<uint8_t *>(scales) + Shape::kScaleBytes);
+  float *sums = scales + Shape::kScaleBytes / 4;                        // [tile][half][row], between a row's two threads
+  TileBarriers &bar = *reinterpret_cast<TileBarriers *>(sums + Shape::kSumBytes / 4);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (warp == kMmaWarp) {
@@ -167,15 +167,14 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
         mbar_init(&bar.empty[i], 1);
       }
       for (int u = 0; u < kTiles; ++u) {
-        mbar_init(&bar.q_full[u], a.q_by_tma ? 1 : 128);
+        mbar_init(&bar.q_full[u], a.q_by_tma ? 1 : 256);
         mbar_init(&bar.s_full[u], 1);
-        mbar_init(&bar.p_full[u][0], 4);
-        mbar_init(&bar.p_full[u][1], 4);
+        mbar_init(&bar.p_full[u], 8);
         mbar_init(&bar.o_full[u], 1);
       }
       for (int i = 0; i < 3; ++i) {
         mbar_init(&bar.to_mend[i], 1);
-        mbar_init(&bar.mended[i], 2);
+        mbar_init(&bar.mended[i], 1);
       }
       for (int i = 0; i < Shape::kRaw; ++i) {
         mbar_init(&bar.raw_full[i], 1);
@@ -239,11 +238,13 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
   const int first_mend = w.all_see / kTileKeys;
 
   if (warp < kMmaWarp) {
-    const int u = warp >> 2, t = tid & 127;
+    // Two warps per 32 rows of a tile, each with half of a block's columns (and
+    // of O's): a row's two threads keep the same reference and sum.
+    const int u = warp >> 3, half = (warp >> 2) & 1, t = (warp & 3) * 32 + lane;
+    constexpr int kOwn = D / 2;                               // columns of O
     const uint32_t lanes = uint32_t(warp & 3) << 21;          // this warp's TMEM lanes
-    const uint32_t s_tm = tmem + lanes + u * 128, o_tm = tmem + lanes + kOCols + u * 128;
-    const int r = w.r0 + u * 128 + t;                         // this thread's row
-    const bool valid = w.b >= 0 && r < w.r1;
+    const uint32_t s_tm = tmem + lanes + u * 128 + half * 64, o_tm = tmem + lanes + kOCols + u * 128 + half * kOwn;
+    const bool valid = w.b >= 0 && w.r0 + u * 128 + t < w.r1;
     // Token and head of the CTA's i-th row.
     auto token_of = [&](int i, int &head) {
       const int token = over_group(a, w.r0 + i);
@@ -253,9 +254,11 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
     int my_head;
     const int my_token = token_of(u * 128 + t, my_head);
     const int limit = valid ? w.first + my_token - w.base : -1;   // it sees positions 0 .. limit
+    float *my_sum = sums + (u * 2 + half) * 128 + t, *other_sum = sums + (u * 2 + 1 - half) * 128 + t;
+    auto meet = [&]() { named_barrier(1 + u * 4 + (warp & 3), 64); };   // the two warps of these rows
     bool ok = true;
     if (w.blocks(u) > 0 && !a.q_by_tma) {
-      for (int i = t; i < 128 * (D / 8); i += 128) {
+      for (int i = half * 128 + t; i < 128 * (D / 8); i += 256) {
         const int qr = i / (D / 8), c = i % (D / 8);
         uint8_t *dst = q_sm + u * kBytes + (c >> 3) * 16384 + qr * 128 + (((c & 7) ^ (qr & 7)) << 4);
         int head;
@@ -269,10 +272,11 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
       fence_proxy_async_smem();
       mbar_arrive(&bar.q_full[u]);
     }
-    float top = -INFINITY, mu = 0.f;
-    float2 sum = make_float2(0.f, 0.f);
+    float mu = 0.f, sum = 0.f;    // weights are exp2(score - mu); their sum over the row
+    float last = 0.f;             // that of the block before
+    bool none = true;             // no score seen yet
     for (int j = 0; j < w.blocks(u); ++j) {
-      if (!mbar_wait(&bar.s_full[u], j & 1, kStatusTimeoutEpilogue)) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&bar.s_full[u], j & 1, kStatusTimeoutEpilogue))) {
         ok = false;
         break;
       }
@@ -280,144 +284,158 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
       // Columns above `seen` are hidden.  Only blocks past all_see have any,
       // and a warp's rows differ in few positions: a chunk of 32 columns is
       // mostly all seen or all hidden.
-      const int seen = limit - j * kTileKeys;
+      const int seen = limit - j * kTileKeys - half * 64;
       int seen_by_all = kTileKeys, seen_by_any = kTileKeys;
       if ((j + 1) * kTileKeys > w.all_see) {
         seen_by_all = __reduce_min_sync(0xffffffffu, seen);
         seen_by_any = __reduce_max_sync(0xffffffffu, seen);
       }
-      // The scores are read 64 columns at a time, 0 .. 63 twice: once for the
-      // maximum, once for the weights (a row does not fit the registers).
-      uint32_t s[2][32];
-      float most = -INFINITY;
-      const float *block_scales = scales + (j % Shape::kDepth) * 2 * kTileKeys;
-      auto load = [&](int half) {
-        tmem_ld_32(s_tm + half * 64, s[0]);
-        tmem_ld_32(s_tm + half * 64 + 32, s[1]);
+      // Only a row's first block is searched for its maximum: the weights are
+      // taken relative to mu, and their sum tells when that has become too
+      // small.  A block whose weights sum to more than 2^12 raises mu before the
+      // next one, by the power of two in that sum; one whose weights pass 2^64
+      // is done again under its own maximum.
+      const float *block_scales = scales + (j % Shape::kDepth) * 2 * kTileKeys + half * 64;
+      uint32_t s[32], p[2][16];
+      auto load = [&](int i) {
+        tmem_ld_32(s_tm + i * 32, s);
         tmem_ld_wait();
         if constexpr (kScaled) {
-          const float4 *k_scale = reinterpret_cast<const float4 *>(block_scales + half * 64);
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              const float4 x = k_scale[(i * 32 + c) / 4];
-              const float2 y = __fmul2_rn(make_float2(__uint_as_float(s[i][c]), __uint_as_float(s[i][c + 1])), make_float2(x.x, x.y));
-              const float2 z = __fmul2_rn(make_float2(__uint_as_float(s[i][c + 2]), __uint_as_float(s[i][c + 3])), make_float2(x.z, x.w));
-              s[i][c] = __float_as_uint(y.x), s[i][c + 1] = __float_as_uint(y.y);
-              s[i][c + 2] = __float_as_uint(z.x), s[i][c + 3] = __float_as_uint(z.y);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (seen_by_all < half * 64 + i * 32 + 31) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (half * 64 + i * 32 + c > seen)
-                s[i][c] = 0xff800000u;
-          }
-      };
-      auto maximum = [&]() {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float m0 = -INFINITY, m1 = -INFINITY;
+          const float4 *k_scale = reinterpret_cast<const float4 *>(block_scales + i * 32);
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
-            m0 = max3(m0, __uint_as_float(s[i][c]), __uint_as_float(s[i][c + 1]));
-            m1 = max3(m1, __uint_as_float(s[i][c + 2]), __uint_as_float(s[i][c + 3]));
+            const float4 x = k_scale[c / 4];
+            const float2 y = __fmul2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), make_float2(x.x, x.y));
+            const float2 z = __fmul2_rn(make_float2(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), make_float2(x.z, x.w));
+            s[c] = __float_as_uint(y.x), s[c + 1] = __float_as_uint(y.y);
+            s[c + 2] = __float_as_uint(z.x), s[c + 3] = __float_as_uint(z.y);
           }
-          most = max3(most, m0, m1);
+        }
+        if (seen_by_all < i * 32 + 31) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (i * 32 + c > seen)
+              s[c] = 0xff800000u;
         }
       };
-      load(0);
-      maximum();
-      if (seen_by_any >= 64) {
-        load(1);
-        maximum();
-      }
-      most *= a.scale_log2;
-      if (__any_sync(0xffffffffu, most > top + 8.f)) {
-        const float m = fmaxf(top, most);
-        const float keep = top == -INFINITY ? 1.f : exp2_fast(top - m);   // nothing summed yet: keep it
-        top = m;
-        mu = m == -INFINITY ? 0.f : m;
-        sum.x *= keep;
-        sum.y *= keep;
-        if (j > 0) {
+      // The maximum of the row's block, by both of its threads.
+      auto maximum = [&]() {
+        float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll 1
-          for (int i = 0; i < D / 16; ++i) {
-            uint32_t o[16];
-            tmem_ld_16(o_tm + i * 16, o);
-            tmem_ld_wait();
+        for (int i = 0; i < 2; ++i) {
+          if (seen_by_any < i * 32)
+            break;
+          load(i);
 #pragma unroll
-            for (int c = 0; c < 16; ++c)
-              o[c] = __float_as_uint(__uint_as_float(o[c]) * keep);
-            tmem_st_16(o_tm + i * 16, o);
+          for (int c = 0; c < 32; c += 4) {
+            m0 = max3(m0, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+            m1 = max3(m1, __uint_as_float(s[c + 2]), __uint_as_float(s[c + 3]));
           }
         }
-      }
-      const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), minus = make_float2(-mu, -mu);
-      // P goes over columns 64 .. 127 of S, which are in registers by then.
-      auto weights = [&](int half) {
+        *my_sum = fmaxf(m0, m1);
+        meet();
+        const float m = fmaxf(*my_sum, *other_sum) * a.scale_log2;
+        meet();
+        return m;
+      };
+      auto scale_o = [&](float keep) {
+#pragma unroll 1
+        for (int i = 0; i < kOwn / 16; ++i) {
+          uint32_t o[16];
+          tmem_ld_16(o_tm + i * 16, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 16; ++c)
+            o[c] = __float_as_uint(__uint_as_float(o[c]) * keep);
+          tmem_st_16(o_tm + i * 16, o);
+        }
+      };
+      // The weights of this thread's columns into p; returns the row's sum.
+      auto weights = [&]() {
+        const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), minus = make_float2(-mu, -mu);
+        float2 total = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint32_t p[16];
-          const float4 *v_scale = reinterpret_cast<const float4 *>(block_scales + kTileKeys + half * 64 + i * 32);
+          if (seen_by_any < i * 32) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+              p[i][c] = 0;
+            continue;
+          }
+          load(i);
+          const float4 *v_scale = reinterpret_cast<const float4 *>(block_scales + kTileKeys + i * 32);
           float4 v4;
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
-            const float2 x = __ffma2_rn(
-                make_float2(__uint_as_float(s[i][2 * c]), __uint_as_float(s[i][2 * c + 1])), scale2, minus);
+            const float2 x =
+                __ffma2_rn(make_float2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), scale2, minus);
             float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-            sum = __fadd2_rn(sum, e);
+            total = __fadd2_rn(total, e);
             if constexpr (kScaled) {
               if (!(c & 1))
                 v4 = v_scale[c / 2];
               const float2 v = (c & 1) ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
-              if (seen_by_all < half * 64 + i * 32 + 31)   // a hidden row's scale may be anything
+              if (seen_by_all < i * 32 + 31)   // a hidden row's scale may be anything
                 e = make_float2(e.x == 0.f ? 0.f : e.x * v.x, e.y == 0.f ? 0.f : e.y * v.y);
               else
                 e = __fmul2_rn(e, v);
             }
-            p[c] = pack_bf16x2(e.x, e.y);
+            p[i][c] = pack_bf16x2(e.x, e.y);
           }
-          tmem_st_16(s_tm + 64 + half * 32 + i * 16, p);
         }
+        *my_sum = total.x + total.y;
+        meet();
+        return *my_sum + *other_sum;
       };
-      auto ready = [&](int half) {
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0)
-          mbar_arrive(&bar.p_full[u][half]);
-      };
-      if (seen_by_any >= 64) {
-        weights(1);
-        ready(1);
-        load(0);
-      } else {
-        const uint32_t none[16] = {};
-        tmem_st_16(s_tm + 96, none);
-        tmem_st_16(s_tm + 112, none);
-        ready(1);
+      if (__any_sync(0xffffffffu, last > 4096.f)) {
+        const int up = last > 4096.f && last < INFINITY ? (__float_as_int(last) >> 23) - 127 : 0;
+        const float keep = __int_as_float((127 - up) << 23);
+        mu += up;
+        sum *= keep;
+        scale_o(keep);
       }
-      weights(0);
-      ready(0);
+      if (__any_sync(0xffffffffu, none && limit >= j * kTileKeys)) {
+        const float m = maximum();
+        if (none && m > -INFINITY) {
+          mu = m;
+          none = false;
+        }
+      }
+      last = weights();
+      if (__any_sync(0xffffffffu, !(last < 0x1p64f))) {
+        meet();                   // both have read the sums
+        const float m = fmaxf(mu, maximum()), keep = exp2_fast(mu - m);
+        mu = m;
+        sum *= keep;
+        scale_o(keep);
+        last = weights();
+      }
+      sum += last;
+      // P goes over the scores it came from.
+      tmem_st_16(s_tm, p[0]);
+      tmem_st_16(s_tm + 16, p[1]);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&bar.p_full[u]);
     }
     if (ok && w.blocks(u) > 0)
       ok = mbar_wait(&bar.o_full[u], 0, kStatusTimeoutEpilogue);
     tc_fence_after();
-    if (ok && w.b >= 0 && w.r0 + u * 128 < w.r1) {
-      const float l = sum.x + sum.y;
-      const float inv = l == 0.f ? 0.f : a.splits > 1 ? 1.f : 1.f / l;   // splits are divided when joined
+    if (__all_sync(0xffffffffu, ok) && w.b >= 0 && w.r0 + u * 128 < w.r1) {
+      const float inv = sum == 0.f ? 0.f : a.splits > 1 ? 1.f : 1.f / sum;   // splits are divided when joined
       const int64_t part = (int64_t(split) * a.rows + w.begin + my_token) * a.hq + my_head;
-      if (a.splits > 1 && valid)
-        a.part_ml[part] = make_float2(top, l);
+      if (a.splits > 1 && valid && half == 0)
+        a.part_ml[part] = make_float2(none ? -INFINITY : mu, sum);
       const bool spoiled = *reinterpret_cast<volatile int *>(&bar.spoiled) != 0;
       // Into the tile that held Q (its products are done), in the same layout.
-      uint8_t *row_sm = q_sm + u * kBytes + t * 128;
+      constexpr int kPieces = kOwn / 8;                       // 16-byte pieces of a row
+      uint8_t *own_sm = q_sm + u * kBytes + (D == 128 ? half * 16384 : 0);
+      const int piece0 = D == 128 ? 0 : half * kPieces;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
+      for (int i = 0; i < kOwn / 32; ++i) {
+        const int column = half * kOwn + i * 32;
         uint32_t o[32] = {};
         if (w.blocks(u) > 0) {
           tmem_ld_32(o_tm + i * 32, o);
@@ -435,9 +453,9 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
             if constexpr (kPaged) {
               const int64_t page = max(0, page_of(a.c, w.b, w.base + key));
               const int64_t slot = (int64_t(kvh) << a.c.shift) + (key & ((1 << a.c.shift) - 1));
-              v = static_cast<const __nv_bfloat16 *>(a.c.v) + page * a.c.v_page + slot * D + i * 32;
+              v = static_cast<const __nv_bfloat16 *>(a.c.v) + page * a.c.v_page + slot * D + column;
             } else {
-              v = a.v + (w.begin + w.base + key) * a.v_row + kvh * a.v_head + i * 32;
+              v = a.v + (w.begin + w.base + key) * a.v_row + kvh * a.v_head + column;
             }
             for (int c = 0; c < 32; ++c) {
               const float x = __bfloat162float(v[c]);
@@ -450,41 +468,39 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
           if (valid && w.blocks(u) > 0) {
 #pragma unroll
             for (int c = 0; c < 32; c += 4)
-              *reinterpret_cast<float4 *>(a.part_o + part * D + i * 32 + c) = make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]);
+              *reinterpret_cast<float4 *>(a.part_o + part * D + column + c) = make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]);
           }
           continue;
         }
 #pragma unroll
         for (int c = 0; c < 32; c += 8)
-          *reinterpret_cast<uint4 *>(row_sm + (i >> 1) * 16384 + ((((i & 1) * 4 + c / 8) ^ (t & 7)) << 4)) =
+          *reinterpret_cast<uint4 *>(own_sm + t * 128 + (((piece0 + i * 4 + c / 8) ^ (t & 7)) << 4)) =
               make_uint4(pack_bf16x2(f[c], f[c + 1]), pack_bf16x2(f[c + 2], f[c + 3]), pack_bf16x2(f[c + 4], f[c + 5]),
                          pack_bf16x2(f[c + 6], f[c + 7]));
       }
-      // This warp's 32 rows to memory: by TMA, or the last of a sequence row by
-      // row.
+      // 32 rows to memory: by TMA, or the last of a sequence row by row.
       const int first_row = w.r0 + u * 128 + (warp & 3) * 32;
       if (a.splits == 1 && a.out_by_tma && first_row + 32 <= w.r1) {
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
-#pragma unroll
-          for (int h = 0; h < kHalves; ++h)
-            tma_store_3d(&tm_o, q_sm + u * kBytes + h * 16384 + (warp & 3) * 4096, h * 64, kvh * group,
-                         int(w.begin) + over_group(a, first_row));
+        if (D == 64)
+          meet();                 // both halves are in one box
+        if (lane == 0 && (D == 128 || half == 0)) {
+          tma_store_3d(&tm_o, own_sm + (warp & 3) * 4096, D == 128 ? half * 64 : 0, kvh * group,
+                       int(w.begin) + over_group(a, first_row));
           tma_store_commit_and_wait();
         }
       } else if (a.splits == 1) {
         __syncwarp();
-        constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces;
+        constexpr int kAtOnce = 32 / kPieces;
 #pragma unroll 4
         for (int i = 0; i < 32; i += kAtOnce) {
           const int rr = (warp & 3) * 32 + i + lane / kPieces, piece = lane % kPieces;
           int head;
           const int token = token_of(u * 128 + rr, head);
-          const uint4 x = *reinterpret_cast<const uint4 *>(q_sm + u * kBytes + (piece >> 3) * 16384 + rr * 128 +
-                                                           (((piece & 7) ^ (rr & 7)) << 4));
+          const uint4 x = *reinterpret_cast<const uint4 *>(own_sm + rr * 128 + (((piece0 + piece) ^ (rr & 7)) << 4));
           if (w.r0 + u * 128 + rr < w.r1)
-            *reinterpret_cast<uint4 *>(a.out + (w.begin + token) * a.ldo + head * D + piece * 8) = x;
+            *reinterpret_cast<uint4 *>(a.out + (w.begin + token) * a.ldo + head * D + half * kOwn + piece * 8) = x;
         }
       }
     }
@@ -529,22 +545,14 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
             }
             const uint32_t v_addr = ring_addr + (v_item % kStages) * kBytes;
             const int steps = w.steps(u, j);
-            // Keys 64 .. 127 of the block first: their weights are ready first.
-            bool begun = j > 0;
-            for (int half = 1; half >= 0; --half) {
-              ok = ok && wait(&bar.p_full[u][half], j);
-              if (!ok)
-                break;
-              tc_fence_after();
-#pragma unroll 1
-              for (int s = half * 4; s < min(steps, half * 4 + 4); ++s) {
-                mma_bf16_ts(tmem + kOCols + u * 128, tmem + u * 128 + 64 + s * 8, smem_desc_rows(v_addr + s * 2048, 16384),
-                            kIdescO, begun);
-                begun = true;
-              }
-            }
+            ok = ok && wait(&bar.p_full[u], j);
             if (!ok)
               break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int s = 0; s < steps; ++s)
+              mma_bf16_ts(tmem + kOCols + u * 128, tmem + u * 128 + (s >> 2) * 64 + (s & 3) * 8,
+                          smem_desc_rows(v_addr + s * 2048, 16384), kIdescO, j > 0 || s > 0);
             if (j + 1 < w.blocks(u)) {
               if (!k_ready) {
                 ok = wait(&bar.full[k_item % kStages], k_item / kStages);
@@ -637,7 +645,7 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
         // Four warps turn tiles of codes into bf16 tiles, 16 bytes of a row at
         // a time.  Rows past the keys hold old codes, which are numbers.
         constexpr int kRuns = D / 16, kRowStep = 128 / kRuns;
-        const int t = tid - (kMmaWarp + 4) * 32, run = t % kRuns, row0 = t / kRuns;
+        const int t = tid - (kMmaWarp + 3) * 32, run = t % kRuns, row0 = t / kRuns;
         for (int item = 0; t >= 0 && item < 2 * blocks; ++item) {
           const int from = item % Shape::kRaw, stage = item % kStages;
           bool go = mbar_wait(&bar.raw_full[from], uint32_t((item / Shape::kRaw) & 1), kStatusTimeoutConvert);
@@ -687,12 +695,12 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
           const int c = i % (D / 8);
           return reinterpret_cast<uint4 *>(v + (c >> 3) * 16384 + key * 128 + (((c & 7) ^ (key & 7)) << 4));
         };
-        const int chunks = (used - from) * (D / 8), first_chunk = (warp - kMmaWarp - 2) * 32 + lane;
+        const int chunks = (used - from) * (D / 8), first_chunk = lane;
         // 0 times a value that is not finite is NaN, and stays in the sum.
         const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
         __nv_bfloat162 sum = zero;
 #pragma unroll 4
-        for (int i = first_chunk; i < chunks; i += 64) {
+        for (int i = first_chunk; i < chunks; i += 32) {
           int key;
           uint4 *at = chunk(i, key);
           if (key >= end) {
@@ -706,7 +714,7 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
           }
         }
         if (__any_sync(0xffffffffu, __hisnan2(sum).x != __nv_bfloat16(0.f) || __hisnan2(sum).y != __nv_bfloat16(0.f))) {
-          for (int i = first_chunk; i < chunks; i += 64) {
+          for (int i = first_chunk; i < chunks; i += 32) {
             int key;
             uint4 *at = chunk(i, key);
             uint4 x = *at;
