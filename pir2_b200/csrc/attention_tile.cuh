@@ -161,6 +161,10 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (warp == kMmaWarp) {
+    tmem_alloc(&bar.tmem, kTiles * 256);
+    tmem_relinquish();
+  }
+  if (warp == kMmaWarp + 1) {
     if (lane == 0) {
       for (int i = 0; i < kStages; ++i) {
         mbar_init(&bar.full[i], kScaled ? 4 : 1);
@@ -182,15 +186,11 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
       }
       bar.spoiled = 0;
       fence_barrier_init();
+      tma_prefetch_desc(&tm_q);
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
     }
     __syncwarp();
-    tmem_alloc(&bar.tmem, kTiles * 256);
-    tmem_relinquish();
-  }
-  if (warp == kMmaWarp + 1 && lane == 0) {
-    tma_prefetch_desc(&tm_q);
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_v);
   }
   pdl_wait();
   pdl_launch_dependents();
@@ -228,14 +228,81 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
     w.keys = max(w.keys0, w.keys1);
     w.all_see = max(0, w.all_see - w.base);
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = bar.tmem;
   const int blocks = max(w.blocks(0), w.blocks(1));
   // The rows' limits span at most 256 positions, so at most three blocks hold
   // positions hidden from some row; each has its barriers.
   const int first_mend = w.all_see / kTileKeys;
+  // Item 2 j is block j's K, item 2 j + 1 its V.  From pages, a lane per page
+  // copies it (a bad page reads page 0: any values do).  8-bit codes go to the
+  // converting warps' ring, with the block's scales.
+  constexpr int kRing = kScaled ? Shape::kRaw : kStages;
+  uint64_t *full = kScaled ? bar.raw_full : bar.full, *empty = kScaled ? bar.raw_empty : bar.empty;
+  int copied = 0, page = 0;     // the loader warp's
+  bool mine = lane == 0;
+  auto copy = [&](int item) {
+    const int stage = item % kRing, j = item >> 1;
+    if constexpr (kPaged) {
+      if (!(item & 1)) {
+        const int at = j * kTileKeys + (lane << a.c.shift);
+        mine = (lane << a.c.shift) < kTileKeys && at < w.keys;
+        if (mine)
+          page = max(0, page_of(a.c, w.b, w.base + at));
+      }
+    }
+    const int copies = __popc(__ballot_sync(0xffffffffu, mine));
+    bool free_stage = true;
+    if (item >= kRing)
+      free_stage = mbar_wait(&empty[stage], uint32_t((item / kRing - 1) & 1), kStatusTimeoutProducer);
+    if (!__all_sync(0xffffffffu, free_stage))
+      return false;
+    if (lane == 0) {
+      const int row_bytes = kScaled ? D + (item & 1 ? 0 : 8) : D * 2;
+      mbar_arrive_expect_tx(&full[stage], kPaged ? (copies << a.c.shift) * row_bytes : kBytes);
+    }
+    __syncwarp();
+    if (mine) {
+      const void *map = (item & 1) ? &tm_v : &tm_k;
+      if constexpr (kScaled) {
+        const int row = lane << a.c.shift;
+        tma_load_4d(raw + stage * Shape::kRawBytes + row * D, map, &full[stage], 0, 0, kvh, page);
+        if (!(item & 1)) {
+          float *block_scales = scales + (j % Shape::kDepth) * 2 * kTileKeys + row;
+          const int64_t slot = int64_t(kvh) << a.c.shift;
+          bulk_load(block_scales, a.c.ks + page * a.c.ks_page + slot, 4u << a.c.shift, &full[stage]);
+          bulk_load(block_scales + kTileKeys, a.c.vs + page * a.c.vs_page + slot, 4u << a.c.shift, &full[stage]);
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          uint8_t *dst = ring + stage * kBytes + h * 16384;
+          if constexpr (kPaged)
+            tma_load_4d(dst + (lane << a.c.shift) * 128, map, &full[stage], h * 64, 0, kvh, page);
+          else
+            tma_load_3d(dst, map, &full[stage], h * 64, kvh, int(w.begin) + w.base + j * kTileKeys);
+        }
+      }
+    }
+    if (!kScaled && lane == 0 && (item & 1) && (j + 1) * kTileKeys > w.all_see)
+      mbar_arrive(&bar.to_mend[j - first_mend]);
+    return true;
+  };
+  if (warp == kMmaWarp + 1) {
+    // What needs no free stage is on its way before the CTA is set up.
+    if (a.q_by_tma && lane < kTiles && w.blocks(lane) > 0) {
+      mbar_arrive_expect_tx(&bar.q_full[lane], kBytes);
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+        tma_load_3d(q_sm + lane * kBytes + h * 16384, &tm_q, &bar.q_full[lane], h * 64, kvh * group,
+                    int(w.begin) + over_group(a, w.r0 + lane * 128));
+    }
+    while (copied < min(kRing, 2 * blocks) && copy(copied))
+      ++copied;
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar.tmem;
 
   if (warp < kMmaWarp) {
     // Two warps per 32 rows of a tile, each with half of a block's columns (and
@@ -572,69 +639,11 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
         }
       }
     } else if (warp == kMmaWarp + 1) {
-      if (a.q_by_tma && lane < kTiles && w.blocks(lane) > 0) {
-        mbar_arrive_expect_tx(&bar.q_full[lane], kBytes);
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h)
-          tma_load_3d(q_sm + lane * kBytes + h * 16384, &tm_q, &bar.q_full[lane], h * 64, kvh * group,
-                      int(w.begin) + over_group(a, w.r0 + lane * 128));
-      }
-      // Item 2 j is block j's K, item 2 j + 1 its V.  From pages, a lane per
-      // page copies it (a bad page reads page 0: any values do).  8-bit codes
-      // go to the converting warps' ring, with the block's scales.
-      constexpr int kRing = kScaled ? Shape::kRaw : kStages;
-      uint64_t *full = kScaled ? bar.raw_full : bar.full, *empty = kScaled ? bar.raw_empty : bar.empty;
-      int item = 0, page = 0;
-      bool mine = lane == 0;
-      for (; item < 2 * blocks; ++item) {
-        const int stage = item % kRing, j = item >> 1;
-        if constexpr (kPaged) {
-          if (!(item & 1)) {
-            const int at = j * kTileKeys + (lane << a.c.shift);
-            mine = (lane << a.c.shift) < kTileKeys && at < w.keys;
-            if (mine)
-              page = max(0, page_of(a.c, w.b, w.base + at));
-          }
-        }
-        const int copies = __popc(__ballot_sync(0xffffffffu, mine));
-        bool free_stage = true;
-        if (item >= kRing)
-          free_stage = mbar_wait(&empty[stage], uint32_t((item / kRing - 1) & 1), kStatusTimeoutProducer);
-        if (!__all_sync(0xffffffffu, free_stage))
-          break;
-        if (lane == 0) {
-          const int row_bytes = kScaled ? D + (item & 1 ? 0 : 8) : D * 2;
-          mbar_arrive_expect_tx(&full[stage], kPaged ? (copies << a.c.shift) * row_bytes : kBytes);
-        }
-        __syncwarp();
-        if (mine) {
-          const void *map = (item & 1) ? &tm_v : &tm_k;
-          if constexpr (kScaled) {
-            const int row = lane << a.c.shift;
-            tma_load_4d(raw + stage * Shape::kRawBytes + row * D, map, &full[stage], 0, 0, kvh, page);
-            if (!(item & 1)) {
-              float *block_scales = scales + (j % Shape::kDepth) * 2 * kTileKeys + row;
-              const int64_t slot = int64_t(kvh) << a.c.shift;
-              bulk_load(block_scales, a.c.ks + page * a.c.ks_page + slot, 4u << a.c.shift, &full[stage]);
-              bulk_load(block_scales + kTileKeys, a.c.vs + page * a.c.vs_page + slot, 4u << a.c.shift, &full[stage]);
-            }
-          } else {
-#pragma unroll
-            for (int h = 0; h < kHalves; ++h) {
-              uint8_t *dst = ring + stage * kBytes + h * 16384;
-              if constexpr (kPaged)
-                tma_load_4d(dst + (lane << a.c.shift) * 128, map, &full[stage], h * 64, 0, kvh, page);
-              else
-                tma_load_3d(dst, map, &full[stage], h * 64, kvh, int(w.begin) + w.base + j * kTileKeys);
-            }
-          }
-        }
-        if (!kScaled && lane == 0 && (item & 1) && (j + 1) * kTileKeys > w.all_see)
-          mbar_arrive(&bar.to_mend[j - first_mend]);
-      }
+      while (copied < 2 * blocks && copy(copied))
+        ++copied;
       // No copy is in flight when the CTA ends (at once, unless a wait gave up).
       if (lane == 0) {
-        for (int i = max(0, item - kRing); i < item; ++i)
+        for (int i = max(0, copied - kRing); i < copied; ++i)
           mbar_wait(&full[i % kRing], uint32_t((i / kRing) & 1), kStatusTimeoutProducer);
         for (int u = 0; u < kTiles && a.q_by_tma; ++u)
           if (w.blocks(u) > 0)
