@@ -139,7 +139,12 @@ static int launch_rows(bool write, int format, int d, const CacheRowsArgs &a, vo
   }
 }
 
-constexpr int kFewRows = 32;   // rows a sequence has in a kv head, up to which the few-row kernel takes it
+// Rows a sequence has in a kv head up to which the few-row kernel takes it; it
+// reads the keys once per 16 rows, the tile kernel once per 128 or 256.  Over
+// 1000 tokens of 64 sequences: 16 rows 50 us against 55 (bf16) and 50 against
+// 110 (int8, whose tiles are converted first), 24 rows 80 against 56 and 84
+// against 111, 34 rows 115 against 55 and 125 against 110.
+constexpr int kFewRowsBf16 = 16, kFewRows8Bit = 32;
 
 // How the few-row kernel covers a call: a cluster of CTAs per unit of rows,
 // which joins its sums in shared memory, or, where eight CTAs a unit leave SMs
@@ -279,7 +284,7 @@ struct CachePlan {
 static CachePlan plan_cache(int64_t rows, int hq, int hk, int d, int batch, int64_t positions, int format, int sms) {
   CachePlan p = {};
   const int64_t per_sequence = (rows + batch - 1) / batch * (hq / hk);
-  if (per_sequence <= kFewRows) {
+  if (per_sequence <= (format == kCacheBf16 ? kFewRowsBf16 : kFewRows8Bit)) {
     p.few = plan_few(rows, hq, hk, batch, positions, format, d, sms);
     return p;
   }
