@@ -10,8 +10,7 @@
 //               transposed B operand; O fp32 in TMEM).
 // Eight warps per tile are its softmax, two threads per row with half of a
 // block's columns each; then one warp issues the MMAs, one loads K and V by TMA
-// into a ring, and one mends V blocks that hold positions some row must not
-// see.  While one tile's softmax runs, the tensor core works on the other's
+// into a ring, and one clears what a page holds past the keys.  While one tile's softmax runs, the tensor core works on the other's
 // products.  Weights are relative to a reference near the running maximum that
 // moves in few blocks: O is rescaled in TMEM by the softmax warps only then.
 // References, sums and O are fp32.
@@ -48,9 +47,8 @@ struct TileShape {
 };
 
 struct TileBarriers {   // at most 512 bytes
-  uint64_t full[8], empty[8], raw_full[3], raw_empty[3], q_full[2], s_full[2], p_full[2], o_full[2], to_mend[3], mended[3];
+  uint64_t full[8], empty[8], raw_full[3], raw_empty[3], q_full[2], s_full[2], p_full[2], o_full[2], to_mend, mended;
   uint32_t tmem;
-  int spoiled;   // a V block held a value that is not finite at a position hidden from some row
 };
 
 // bf16 x bf16 -> fp32, A and B in shared memory.
@@ -141,9 +139,51 @@ struct TileWork {
   }
 };
 
+// 32 columns of a row's output from its scores, if its hidden positions (those
+// of its last block past `limit`) hold values there that are not finite.
+template <int kSource, int D>
+__device__ __noinline__ void sum_again(const RaggedArgs &a, TileWork w, int kvh, int token, int head, int limit,
+                                       float mu, float inv, int column, float (&f)[32]) {
+  auto row_of = [&](const __nv_bfloat16 *rows, int64_t row, int64_t hd, const void *pages, int64_t page_stride, int key) {
+    if constexpr (kSource == kSourceRows) {
+      return rows + (w.begin + w.base + key) * row + kvh * hd;
+    } else {
+      const int64_t page = max(0, page_of(a.c, w.b, w.base + key));
+      const int64_t slot = (int64_t(kvh) << a.c.shift) + (key & ((1 << a.c.shift) - 1));
+      return static_cast<const __nv_bfloat16 *>(pages) + page * page_stride + slot * D;
+    }
+  };
+  auto v_of = [&](int key) { return row_of(a.v, a.v_row, a.v_head, a.c.v, a.c.v_page, key) + column; };
+  // Hidden positions that the products read: to the end of their 16 keys (of
+  // the rows there are, or the keys of the pages).
+  int end = (w.keys + 15) & ~15;
+  if constexpr (kSource == kSourceRows)
+    end = int(min(int64_t(end), a.rows - w.begin - w.base));
+  else
+    end = w.keys;
+  bool spoiled = false;
+  for (int key = limit + 1; key < end && !spoiled; ++key)
+    for (int c = 0; c < 32; ++c)
+      spoiled |= !(fabsf(__bfloat162float(v_of(key)[c])) < INFINITY);
+  if (!spoiled)
+    return;
+  const __nv_bfloat16 *q = a.q + (w.begin + token) * a.q_row + head * a.q_head;
+  for (int c = 0; c < 32; ++c)
+    f[c] = 0.f;
+  for (int key = 0; key <= min(limit, w.keys - 1); ++key) {
+    const __nv_bfloat16 *k = row_of(a.k, a.k_row, a.k_head, a.c.k, a.c.k_page, key);
+    float s = 0.f;
+    for (int d = 0; d < D; ++d)
+      s += __bfloat162float(q[d]) * __bfloat162float(k[d]);
+    const float p = __bfloat162float(__float2bfloat16(exp2_fast(s * a.scale_log2 - mu)));
+    for (int c = 0; c < 32; ++c)
+      f[c] += p * inv * __bfloat162float(v_of(key)[c]);
+  }
+}
+
 template <int kSource, int D, int kTiles>
 __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTiles == 2 ? 1 : 2)
-    attention_tile_kernel(const RaggedArgs a, const __grid_constant__ CUtensorMap tm_q,
+    attention_tile_kernel(const __grid_constant__ RaggedArgs a, const __grid_constant__ CUtensorMap tm_q,
                           const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                           const __grid_constant__ CUtensorMap tm_o) {
   using Shape = TileShape<kSource, D, kTiles>;
@@ -176,15 +216,12 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
         mbar_init(&bar.p_full[u], 8);
         mbar_init(&bar.o_full[u], 1);
       }
-      for (int i = 0; i < 3; ++i) {
-        mbar_init(&bar.to_mend[i], 1);
-        mbar_init(&bar.mended[i], 1);
-      }
+      mbar_init(&bar.to_mend, 1);
+      mbar_init(&bar.mended, 1);
       for (int i = 0; i < Shape::kRaw; ++i) {
         mbar_init(&bar.raw_full[i], 1);
         mbar_init(&bar.raw_empty[i], 4);
       }
-      bar.spoiled = 0;
       fence_barrier_init();
       tma_prefetch_desc(&tm_q);
       tma_prefetch_desc(&tm_k);
@@ -229,9 +266,10 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
     w.all_see = max(0, w.all_see - w.base);
   }
   const int blocks = max(w.blocks(0), w.blocks(1));
-  // The rows' limits span at most 256 positions, so at most three blocks hold
-  // positions hidden from some row; each has its barriers.
-  const int first_mend = w.all_see / kTileKeys;
+  // Products read keys in steps of 16: what a page holds past the keys in the
+  // last step is made 0 first.  (Past the rows of a prompt lie those of the
+  // next, or zeros.)
+  const bool mend = kPaged && !kScaled && w.keys % 16 != 0;
   // Item 2 j is block j's K, item 2 j + 1 its V.  From pages, a lane per page
   // copies it (a bad page reads page 0: any values do).  8-bit codes go to the
   // converting warps' ring, with the block's scales.
@@ -282,8 +320,8 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
         }
       }
     }
-    if (!kScaled && lane == 0 && (item & 1) && (j + 1) * kTileKeys > w.all_see)
-      mbar_arrive(&bar.to_mend[j - first_mend]);
+    if (mend && lane == 0 && item == 2 * blocks - 1)
+      mbar_arrive(&bar.to_mend);
     return true;
   };
   if (warp == kMmaWarp + 1) {
@@ -495,7 +533,6 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
       const int64_t part = (int64_t(split) * a.rows + w.begin + my_token) * a.hq + my_head;
       if (a.splits > 1 && valid && half == 0)
         a.part_ml[part] = make_float2(none ? -INFINITY : mu, sum);
-      const bool spoiled = *reinterpret_cast<volatile int *>(&bar.spoiled) != 0;
       // Into the tile that held Q (its products are done), in the same layout.
       constexpr int kPieces = kOwn / 8;                       // 16-byte pieces of a row
       uint8_t *own_sm = q_sm + u * kBytes + (D == 128 ? half * 16384 : 0);
@@ -512,24 +549,21 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
 #pragma unroll
         for (int c = 0; c < 32; ++c)
           f[c] = __uint_as_float(o[c]) * inv;
-        if (spoiled) {
-          // Values that are not finite were left out of the products from
-          // position all_see on: they go to the rows that see them.
-          for (int key = w.all_see; key <= min(limit, w.keys - 1); ++key) {
-            const __nv_bfloat16 *v;
-            if constexpr (kPaged) {
-              const int64_t page = max(0, page_of(a.c, w.b, w.base + key));
-              const int64_t slot = (int64_t(kvh) << a.c.shift) + (key & ((1 << a.c.shift) - 1));
-              v = static_cast<const __nv_bfloat16 *>(a.c.v) + page * a.c.v_page + slot * D + column;
-            } else {
-              v = a.v + (w.begin + w.base + key) * a.v_row + kvh * a.v_head + column;
-            }
-            for (int c = 0; c < 32; ++c) {
-              const float x = __bfloat162float(v[c]);
-              if (!(fabsf(x) < INFINITY))
-                f[c] += x;
-            }
-          }
+        // A weight of 0 times a value that is not finite is NaN: where a row's
+        // hidden positions hold one, its values are summed again without them.
+        float2 check = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < 32; c += 2)
+          check = __ffma2_rn(make_float2(f[c], f[c + 1]), make_float2(0.f, 0.f), check);
+        if (!kScaled && !(check.x + check.y == 0.f) && valid && w.blocks(u) > 0) {
+          float again[32];            // a copy: f stays in registers
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            again[c] = f[c];
+          sum_again<kSource, D>(a, w, kvh, my_token, my_head, limit, mu, inv, column, again);
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            f[c] = again[c];
         }
         if (a.splits > 1) {
           if (valid && w.blocks(u) > 0) {
@@ -604,8 +638,8 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
             if (j >= w.blocks(u))
               continue;
             if (!v_ready) {
-              if (!kScaled && (j + 1) * kTileKeys > w.all_see)
-                ok = wait(&bar.mended[j - first_mend], 0);
+              if (mend && j == blocks - 1)
+                ok = wait(&bar.mended, 0);
               else
                 ok = wait(&bar.full[v_item % kStages], v_item / kStages);
               v_ready = true;
@@ -686,63 +720,21 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
         }
       }
     } else {
-      // Positions some row of the tiles must not see: those past the keys
-      // become 0, and a value that is not finite is left out (0 times it
-      // would be NaN in the rows that do not see it).
-      // The loader says when such a block is on its way: only then is its
+      // The loader says when the last V block is on its way: only then is its
       // stage's barrier in the phase that is waited for.
-      for (int j = first_mend; j < blocks; ++j) {
-        const int item = 2 * j + 1;
-        if (!mbar_wait(&bar.to_mend[j - first_mend], 0, kStatusTimeoutConvert) ||
-            !mbar_wait(&bar.full[item % kStages], uint32_t((item / kStages) & 1), kStatusTimeoutConvert))
-          break;
-        uint8_t *v = ring + (item % kStages) * kBytes;
-        const int from = max(0, w.all_see - j * kTileKeys), end = w.keys - j * kTileKeys;
-        const int used = min(kTileKeys, (end + 15) & ~15);   // rows the products read
-        auto chunk = [&](int i, int &key) {          // 16-byte chunks of the rows from `from` on
-          key = from + i / (D / 8);
-          const int c = i % (D / 8);
-          return reinterpret_cast<uint4 *>(v + (c >> 3) * 16384 + key * 128 + (((c & 7) ^ (key & 7)) << 4));
-        };
-        const int chunks = (used - from) * (D / 8), first_chunk = lane;
-        // 0 times a value that is not finite is NaN, and stays in the sum.
-        const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
-        __nv_bfloat162 sum = zero;
-#pragma unroll 4
-        for (int i = first_chunk; i < chunks; i += 32) {
-          int key;
-          uint4 *at = chunk(i, key);
-          if (key >= end) {
-            *at = make_uint4(0, 0, 0, 0);
-          } else {
-            const uint4 x = *at;
-            const __nv_bfloat162 *pair = reinterpret_cast<const __nv_bfloat162 *>(&x);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              sum = __hfma2(pair[e], zero, sum);
-          }
-        }
-        if (__any_sync(0xffffffffu, __hisnan2(sum).x != __nv_bfloat16(0.f) || __hisnan2(sum).y != __nv_bfloat16(0.f))) {
-          for (int i = first_chunk; i < chunks; i += 32) {
-            int key;
-            uint4 *at = chunk(i, key);
-            uint4 x = *at;
-            uint32_t *word = reinterpret_cast<uint32_t *>(&x);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if ((word[e] & 0x7f80u) == 0x7f80u)
-                word[e] &= 0xffff0000u;
-              if ((word[e] & 0x7f800000u) == 0x7f800000u)
-                word[e] &= 0xffffu;
-            }
-            *at = x;
-          }
-          *reinterpret_cast<volatile int *>(&bar.spoiled) = 1;
+      const int item = 2 * blocks - 1, stage = item % kStages;
+      if (mend && mbar_wait(&bar.to_mend, 0, kStatusTimeoutConvert) &&
+          mbar_wait(&bar.full[stage], uint32_t((item / kStages) & 1), kStatusTimeoutConvert)) {
+        uint8_t *v = ring + stage * kBytes;
+        const int end = w.keys - (blocks - 1) * kTileKeys;
+        for (int i = lane; i < (16 - end % 16) * (D / 8); i += 32) {
+          const int key = end + i / (D / 8), c = i % (D / 8);
+          *reinterpret_cast<uint4 *>(v + (c >> 3) * 16384 + key * 128 + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0)
-          mbar_arrive(&bar.mended[j - first_mend]);
+          mbar_arrive(&bar.mended);
       }
     }
   }
