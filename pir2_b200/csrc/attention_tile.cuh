@@ -76,17 +76,16 @@ __host__ __device__ constexpr uint32_t idesc_bf16(uint32_t m, uint32_t n, bool b
   return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(b_rows) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
-// Descriptor of a B operand stored [K rows][64 columns] in 128-byte swizzled
-// rows, further 64-column blocks `block` bytes apart: 8 rows of K are 1024
-// bytes.
-__device__ __forceinline__ uint64_t smem_desc_rows(uint32_t saddr, uint32_t block) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>((block >> 4) & 0x3FFFu) << 16;
-  d |= static_cast<uint64_t>(1024u >> 4) << 32;
-  d |= static_cast<uint64_t>(1u) << 46;
-  d |= static_cast<uint64_t>(2u) << 61;
-  return d;
+// Shared-memory descriptors of operands in 128-byte swizzled rows (1024 bytes
+// per 8 rows).  One thread issues every product, so a descriptor is its low word,
+// made once per tile and moved by additions, and a constant high word.
+//   tile_lo: rows of M or N, 64 K elements each (K-major);
+//   rows_lo: rows of K, 64 columns of N each, further columns 16 KB apart.
+__device__ __forceinline__ uint32_t tile_lo(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t rows_lo(uint32_t saddr) { return (saddr >> 4) | ((16384u >> 4) << 16); }
+__device__ __forceinline__ uint64_t tile_desc(uint32_t lo) {
+  constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);   // stride, descriptor version, swizzle
+  return (uint64_t(kHi) << 32) | lo;
 }
 
 __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -612,13 +611,12 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
         const uint32_t q_addr = smem_u32(q_sm), ring_addr = smem_u32(ring);
         auto wait = [&](uint64_t *b, int parity) { return mbar_wait(b, uint32_t(parity & 1), kStatusTimeoutMma); };
         auto scores = [&](int u, int item) {
-          const uint32_t k_addr = ring_addr + (item % kStages) * kBytes;
+          const uint32_t k_lo = tile_lo(ring_addr + (item % kStages) * kBytes), q_lo = tile_lo(q_addr + u * kBytes);
           const uint32_t idesc = idesc_bf16(128, w.steps(u, item / 2) * 16, false);
 #pragma unroll
           for (int s = 0; s < D / 16; ++s) {
-            const uint32_t at = (s >> 2) * 16384 + (s & 3) * 32;
-            mma_bf16_ss(tmem + u * 128, smem_desc_sw128(q_addr + u * kBytes + at), smem_desc_sw128(k_addr + at), idesc,
-                        s > 0);
+            const uint32_t at = ((s >> 2) * 16384 + (s & 3) * 32) >> 4;
+            mma_bf16_ss(tmem + u * 128, tile_desc(q_lo + at), tile_desc(k_lo + at), idesc, s > 0);
           }
           mma_commit(&bar.s_full[u]);
         };
@@ -644,16 +642,25 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
                 ok = wait(&bar.full[v_item % kStages], v_item / kStages);
               v_ready = true;
             }
-            const uint32_t v_addr = ring_addr + (v_item % kStages) * kBytes;
+            const uint32_t v_lo = rows_lo(ring_addr + (v_item % kStages) * kBytes);
+            auto product = [&](int s) {
+              mma_bf16_ts(tmem + kOCols + u * 128, tmem + u * 128 + (s >> 2) * 64 + (s & 3) * 8, tile_desc(v_lo + s * 128),
+                          kIdescO, j > 0 || s > 0);
+            };
             const int steps = w.steps(u, j);
             ok = ok && wait(&bar.p_full[u], j);
             if (!ok)
               break;
             tc_fence_after();
+            if (steps == 8) {
+#pragma unroll
+              for (int s = 0; s < 8; ++s)
+                product(s);
+            } else {
 #pragma unroll 1
-            for (int s = 0; s < steps; ++s)
-              mma_bf16_ts(tmem + kOCols + u * 128, tmem + u * 128 + (s >> 2) * 64 + (s & 3) * 8,
-                          smem_desc_rows(v_addr + s * 2048, 16384), kIdescO, j > 0 || s > 0);
+              for (int s = 0; s < steps; ++s)
+                product(s);
+            }
             if (j + 1 < w.blocks(u)) {
               if (!k_ready) {
                 ok = wait(&bar.full[k_item % kStages], k_item / kStages);
