@@ -491,18 +491,20 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
         meet();
         return *my_sum + *other_sum;
       };
-      if (__any_sync(0xffffffffu, last > 4096.f)) {
+      // Both are rare: one vote for the two.
+      if (__any_sync(0xffffffffu, last > 4096.f || (none && limit >= j * kTileKeys))) {
         const int up = last > 4096.f && last < INFINITY ? (__float_as_int(last) >> 23) - 127 : 0;
         const float keep = __int_as_float((127 - up) << 23);
         mu += up;
         sum *= keep;
-        scale_o(keep);
-      }
-      if (__any_sync(0xffffffffu, none && limit >= j * kTileKeys)) {
-        const float m = maximum();
-        if (none && m > -INFINITY) {
-          mu = m;
-          none = false;
+        if (j > 0)
+          scale_o(keep);
+        if (__any_sync(0xffffffffu, none && limit >= j * kTileKeys)) {
+          const float m = maximum();
+          if (none && m > -INFINITY) {
+            mu = m;
+            none = false;
+          }
         }
       }
       last = weights();
