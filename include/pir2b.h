@@ -439,8 +439,9 @@ typedef struct pir2b_kv_pages {
  * (lengths, int32 [batch]; the rows are its last tokens) and the pages of its
  * positions (table int32 [batch, table_width]: position p is in page
  * table[b, p / page_size]).  All on the device; every index is checked there:
- * a position outside the table or a page outside the pool is neither read nor
- * written and sets the status word to PIR2B_STATUS_BAD_PAGE. */
+ * a position outside the table or a page outside the pool sets the status word
+ * to PIR2B_STATUS_BAD_PAGE, is not written, and reads as 0 in pir2b_cache_read;
+ * the output rows of pir2b_cache_attention that see it are unspecified. */
 typedef struct pir2b_sequences {
   const int32_t *starts, *lengths, *table;
   int64_t table_stride;

@@ -17,6 +17,12 @@
 // fp32.  P is transposed between the products by movmatrix.  The running maximum of a row
 // moves only when a score passes it by more than 8 (in log2), so that most
 // steps have one vote and no rescaling; sums and maxima are fp32.
+//
+// What bounds it, one new token per sequence, 16 query and 8 kv heads of 128:
+// bf16 over four histories of 29000-32700, 85 us, 6150 GB/s, 94 % of a copy's
+// rate.  int8 over 64 histories of 500-4000, 72 us, 4030 GB/s: instructions
+// (2.3 a cycle and SM), a third of them the conversion of codes, which no
+// warp-level MMA takes beside 16-bit weights.
 #pragma once
 #include <cuda.h>
 #include "attention_ragged.cuh"

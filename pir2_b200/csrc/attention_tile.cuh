@@ -9,11 +9,24 @@
 //   O += P V   (P from TMEM, V in shared memory as it lies: keys x D, the
 //               transposed B operand; O fp32 in TMEM).
 // Eight warps per tile are its softmax, two threads per row with half of a
-// block's columns each; then one warp issues the MMAs, one loads K and V by TMA
-// into a ring, and one clears what a page holds past the keys.  While one tile's softmax runs, the tensor core works on the other's
-// products.  Weights are relative to a reference near the running maximum that
-// moves in few blocks: O is rescaled in TMEM by the softmax warps only then.
-// References, sums and O are fp32.
+// block's columns each (one thread per row: 64 prompts of 280-816 tokens 192 us,
+// two: 179); then one warp issues the MMAs, one loads K and V by TMA into a
+// ring, and one clears what a page holds past the keys.  While one tile's
+// softmax runs, the tensor core works on the other's products.  Weights are
+// relative to a reference near the running maximum that moves in few blocks: O
+// is rescaled in TMEM by the softmax warps only then.  References, sums and O
+// are fp32; weights are rounded to bf16, the type of the values they multiply,
+// and a row's sum is that of the weights before that rounding.
+//
+// What bounds it, at 16 query and 8 kv heads of 128.  One prompt of 8192 tokens:
+// 231 us, 1190 TFLOP/s of the causal half; the tensor pipe is busy 56 % of the
+// time and the exponentials' unit as long, and neither hides the other in full.
+// The 64 prompts: 179 us against 67 for their bytes; a tile has three blocks on
+// average, and its start, end and each block's chain of scores, softmax and
+// product are overlapped only with those of the one other CTA on the SM that
+// TMEM has room for.  Chunks of 250-288 tokens over
+// 16 E4M3 histories of 544-2100: 133 us; reading each key's scales from shared
+// memory and turning codes into bf16 come on top.
 //
 // TMEM columns: S/P of each tile (128 each), then O of each.
 // Every wait is bounded; on expiry all roles leave their loops, the loader

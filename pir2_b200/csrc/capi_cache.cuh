@@ -268,8 +268,9 @@ static int launch_tile(const char *what, const RaggedArgs &a, const CUtensorMap 
 
 // Tiles per CTA of the tile kernel.  One tile and two CTAs on an SM cover the
 // latencies of a CTA's start and end with another's products (64 prompts of
-// 280-816 tokens: 197 us against 218); two tiles read K and V half as often,
-// which carries long prompts (8192 tokens: 241 us against 255).
+// 280-816 tokens: 179 us against 204, one of 544: 11.9 against 13.7); two tiles
+// read K and V half as often, which carries long prompts (8192 tokens: 231 us
+// against 245).
 static int tiles_per_cta(int64_t rows, int batch) { return rows / batch >= 2048 ? 2 : 1; }
 
 // How a call of cache_attention runs: the few-row kernel (tiles = 0) or
