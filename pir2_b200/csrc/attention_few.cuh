@@ -20,9 +20,9 @@
 //
 // What bounds it, one new token per sequence, 16 query and 8 kv heads of 128:
 // bf16 over four histories of 29000-32700, 85 us, 6150 GB/s, 94 % of a copy's
-// rate.  int8 over 64 histories of 500-4000, 72 us, 4030 GB/s: instructions
-// (2.3 a cycle and SM), a third of them the conversion of codes, which no
-// warp-level MMA takes beside 16-bit weights.
+// rate.  int8 over 64 histories of 500-4000, 62 us, 4710 GB/s: instructions,
+// a third of them the conversion of codes, which no warp-level MMA takes beside
+// 16-bit weights.
 #pragma once
 #include <cuda.h>
 #include "attention_ragged.cuh"
@@ -150,6 +150,74 @@ __device__ __forceinline__ int unit_of(const RaggedArgs &a, int tile_log2, int s
   s1 = int(min(int64_t(s1), a.rows));
   tile = slot - int((int64_t(s0) * a.group) >> tile_log2) - lo;
   return (tile >= 0 && (int64_t(tile) << tile_log2) < int64_t(s1 - s0) * a.group) ? lo : -1;
+}
+
+// Sequences that can be put in order of their length, four to a lane.
+constexpr int kOrdered = 128;
+
+// The same with the units of longer sequences first (batch <= kOrdered): where
+// CTAs wait for others to end, long ones started last would run alone.
+// Sequences are taken by sixteenths of the longest's length, and as they come
+// within a sixteenth.  `index` counts the units of one kv head without gaps.
+__device__ __forceinline__ int unit_by_length(const RaggedArgs &a, int tile_log2, int index, int &tile, int &s0, int &s1) {
+  const int lane = threadIdx.x & 31;
+  int first[4], rows[4], length[4], units[4], most = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int b = min(i * 32 + lane, a.batch - 1);
+    first[i] = max(__ldg(a.starts + b), 0);
+    rows[i] = i * 32 + lane < a.batch ? int(max(int64_t(0), min(int64_t(__ldg(a.starts + b + 1)), a.rows) - first[i])) : 0;
+    length[i] = max(__ldg(a.lengths + b), 0);
+    units[i] = int((int64_t(rows[i]) * a.group + (1 << tile_log2) - 1) >> tile_log2);
+    if (rows[i] > 0)
+      most = max(most, length[i]);
+  }
+  const float part = 15.99f / float(max(1, int(__reduce_max_sync(0xffffffffu, most))));
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    length[i] = int(float(length[i]) * part);
+  int before = 0, mine = 0, which = -1;
+#pragma unroll
+  for (int c = 15; c >= 0; --c) {
+    int here = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      here += length[i] == c ? units[i] : 0;
+    const int all = __reduce_add_sync(0xffffffffu, here);
+    if (which < 0) {
+      if (index - before < all) {
+        which = c;
+        mine = here;
+      } else {
+        before += all;
+      }
+    }
+  }
+  if (which < 0)
+    return -1;
+  int upto = mine;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, upto, x);
+    if (lane >= x)
+      upto += y;
+  }
+  const int owner = __ffs(__ballot_sync(0xffffffffu, upto > index - before)) - 1;
+  int at = index - before - (upto - mine), b = -1;
+  s0 = s1 = tile = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (length[i] == which && b < 0) {
+      if (at < units[i])
+        b = i * 32 + lane, tile = at, s0 = first[i], s1 = first[i] + rows[i];
+      at -= units[i];
+    }
+  }
+  b = __shfl_sync(0xffffffffu, b, owner);
+  tile = __shfl_sync(0xffffffffu, tile, owner);
+  s0 = __shfl_sync(0xffffffffu, s0, owner);
+  s1 = __shfl_sync(0xffffffffu, s1, owner);
+  return b;
 }
 
 // CTAs that the registers and shared memory of an SM take.
@@ -312,7 +380,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
     const int unit = int(blockIdx.x) / a.cluster;
     piece.kvh = unit % a.hk;
     int s0, s1;
-    piece.b = unit_of(a, kRowsLog2, unit / a.hk, piece.tile, s0, s1);
+    piece.b = a.ordered ? unit_by_length(a, kRowsLog2, unit / a.hk, piece.tile, s0, s1)
+                        : unit_of(a, kRowsLog2, unit / a.hk, piece.tile, s0, s1);
     piece.index = int(blockIdx.x) % a.cluster;
     piece.count = a.cluster;
   } else {

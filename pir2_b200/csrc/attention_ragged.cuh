@@ -28,6 +28,8 @@ struct RaggedArgs {
   int splits;                   // CTAs along the keys of a unit, at most 32
   float *part_o;                // [splits, rows, hq, D] sums, where splits > 1,
   float2 *part_ml;              // [splits, rows, hq] and their (maximum, sum of weights)
+  int sms;                      // of the device
+  int ordered;                  // longer sequences first
   int cluster;                  // few-row kernel: CTAs of a unit, as a cluster; 0: as pieces of a list
   // Few-row kernel: CTAs wanted and launched, and per unit of rows its first piece and how
   // many; part_o and part_ml are then [CTAs, unit rows].

@@ -25,7 +25,7 @@
 // average, and its start, end and each block's chain of scores, softmax and
 // product are overlapped only with those of the one other CTA on the SM that
 // TMEM has room for.  Chunks of 250-288 tokens over
-// 16 E4M3 histories of 544-2100: 133 us; reading each key's scales from shared
+// 16 E4M3 histories of 544-2100: 121 us; reading each key's scales from shared
 // memory and turning codes into bf16 come on top.
 //
 // TMEM columns: S/P of each tile (128 each), then O of each.
@@ -57,11 +57,6 @@ struct TileShape {
   static constexpr int kScaleBytes = kScaled ? kDepth * 2 * kTileKeys * 4 : 0;
   static constexpr int kSumBytes = kTiles * 2 * 128 * 4;
   static constexpr int kSmem = (kTiles + kStages) * kBytes + kRaw * kRawBytes + kScaleBytes + kSumBytes + 512 /* barriers */;
-};
-
-struct TileBarriers {   // at most 512 bytes
-  uint64_t full[8], empty[8], raw_full[3], raw_empty[3], q_full[2], s_full[2], p_full[2], o_full[2], to_mend, mended;
-  uint32_t tmem;
 };
 
 // bf16 x bf16 -> fp32, A and B in shared memory.
@@ -150,6 +145,13 @@ struct TileWork {
     return (min(kTileKeys, (u ? keys1 : keys0) - j * kTileKeys) + 15) >> 4;
   }
 };
+
+struct TileBarriers {
+  uint64_t full[8], empty[8], raw_full[3], raw_empty[3], q_full[2], s_full[2], p_full[2], o_full[2], to_mend, mended;
+  TileWork work;
+  uint32_t tmem;
+};
+static_assert(sizeof(TileBarriers) <= 512);
 
 // 32 columns of a row's output from its scores, if its hidden positions (those
 // of its last block past `limit`) hold values there that are not finite.
@@ -244,13 +246,19 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
   pdl_wait();
   pdl_launch_dependents();
   const int group = a.group;
-  // Later rows see more keys: they start first.
-  const int unit = int((gridDim.x - 1 - blockIdx.x) / uint32_t(a.splits)), split = int(blockIdx.x % uint32_t(a.splits));
+  const bool ordered = kPaged && a.ordered;
+  // Of a prompt, later rows see more keys: they start first.
+  const int unit = int((ordered ? blockIdx.x : gridDim.x - 1 - blockIdx.x) / uint32_t(a.splits));
+  const int split = int(blockIdx.x % uint32_t(a.splits));
   const int kvh = int(uint32_t(unit) % uint32_t(a.hk)), slot = int(uint32_t(unit) / uint32_t(a.hk));
+  // The loader warp finds out what the CTA works on; the others read it once
+  // the CTA is set up.
   TileWork w = {};
-  int tile;
-  int s0, s1;
-  w.b = unit_of(a, kTiles == 2 ? 8 : 7, slot, tile, s0, s1);
+  w.b = -1;
+  int tile = 0, s0 = 0, s1 = 0;
+  if (warp == kMmaWarp + 1)
+    w.b = ordered ? unit_by_length(a, kTiles == 2 ? 8 : 7, slot, tile, s0, s1)
+                  : unit_of(a, kTiles == 2 ? 8 : 7, slot, tile, s0, s1);
   if (w.b >= 0) {
     w.begin = s0;
     const int n = s1 - s0;
@@ -277,11 +285,11 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
     w.keys = max(w.keys0, w.keys1);
     w.all_see = max(0, w.all_see - w.base);
   }
-  const int blocks = max(w.blocks(0), w.blocks(1));
+  int blocks = max(w.blocks(0), w.blocks(1));
   // Products read keys in steps of 16: what a page holds past the keys in the
   // last step is made 0 first.  (Past the rows of a prompt lie those of the
   // next, or zeros.)
-  const bool mend = kPaged && !kScaled && w.keys % 16 != 0;
+  bool mend = kPaged && !kScaled && w.keys % 16 != 0;
   // Item 2 j is block j's K, item 2 j + 1 its V.  From pages, a lane per page
   // copies it (a bad page reads page 0: any values do).  8-bit codes go to the
   // converting warps' ring, with the block's scales.
@@ -337,6 +345,8 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
     return true;
   };
   if (warp == kMmaWarp + 1) {
+    if (lane == 0)
+      bar.work = w;
     // What needs no free stage is on its way before the CTA is set up.
     if (a.q_by_tma && lane < kTiles && w.blocks(lane) > 0) {
       mbar_arrive_expect_tx(&bar.q_full[lane], kBytes);
@@ -353,6 +363,11 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bar.tmem;
+  if (warp != kMmaWarp + 1) {
+    w = bar.work;
+    blocks = max(w.blocks(0), w.blocks(1));
+    mend = kPaged && !kScaled && w.keys % 16 != 0;
+  }
 
   if (warp < kMmaWarp) {
     // Two warps per 32 rows of a tile, each with half of a block's columns (and

@@ -167,9 +167,9 @@ static FewPlan plan_few(int64_t rows, int hq, int hk, int batch, int64_t positio
   const int64_t units = batch * ((rows + batch - 1) / batch * group + 8 * p.nt - 1) / (8 * p.nt) * hk;
   const int64_t longest = (positions + 16 * kFewWarps - 1) / (16 * kFewWarps);    // CTAs a unit can use
   if (8 * units >= sms / 3 || longest <= 8) {
-    // As many CTAs as are resident at once: a second round costs more than it
-    // evens out (64 int8 sequences of 500-4000 tokens: 73 us in one round, 79
-    // in two, 104 in four).
+    // CTAs for every place on the SMs, less than twice as many (64 int8
+    // sequences of 500-4000 tokens: 62 us with one or two to a unit, 74 with
+    // four).
     p.cluster = 1;
     while (p.cluster < 8 && p.cluster * units < resident * sms && 2 * p.cluster <= longest)
       p.cluster *= 2;
@@ -203,8 +203,20 @@ static int make_pages_map(CUtensorMap *map, const void *base, const CachePages &
   return r == CUDA_SUCCESS ? PIR2B_OK : fail(PIR2B_ECUDA, "cuTensorMapEncodeTiled (pages) failed (%d)", int(r));
 }
 
+// Whether CTAs start in the order of their sequences' lengths, longest first:
+// where there are more than run at once and a CTA may have 1024 keys or more
+// (64 sequences of 500-4000 tokens, one new token each: 62 us against 72; chunks
+// of 250-288 over 16 of 544-2100: 121 against 133).  Shorter ones lose more by
+// looking up the order (28 sequences of 660-1320 in eighths: 17.8 us against
+// 15.6), and so do the many short CTAs of prompts (64 prompts: 196 against 179).
+static bool by_length(const RaggedArgs &a, int64_t grid, int resident, int parts) {
+  return a.lengths != nullptr && a.batch > 1 && a.batch <= kOrdered && grid > int64_t(resident) * a.sms &&
+         (int64_t(a.c.width) << a.c.shift) >= int64_t(1024) * parts;
+}
+
 template <int kFormat, int D, int kNT>
-static int launch_attention_few(const FewPlan &p, const RaggedArgs &a, void *stream) {
+static int launch_attention_few(const FewPlan &p, RaggedArgs a, void *stream) {
+  a.ordered = by_length(a, p.grid, FewShape<kFormat, D, kNT>::kCtas, std::max(p.cluster, 1));
   constexpr int kBytes = kFormat == kCacheBf16 ? 2 : 1;
   CUtensorMap tm_k, tm_v;
   if (int r = make_pages_map(&tm_k, a.c.k, a.c, D, a.c.k_page, kBytes, 16, true))
@@ -255,13 +267,14 @@ static int make_o_map(CUtensorMap *map, const RaggedArgs &a, int d) {
 }
 
 template <int kSource, int D, int kTiles>
-static int launch_tile(const char *what, const RaggedArgs &a, const CUtensorMap &tm_q, const CUtensorMap &tm_k,
+static int launch_tile(const char *what, RaggedArgs a, const CUtensorMap &tm_q, const CUtensorMap &tm_k,
                        const CUtensorMap &tm_v, void *stream) {
   CUtensorMap tm_o;
   if (int r = make_o_map(&tm_o, a, D))
     return r;
   using Shape = TileShape<kSource, D, kTiles>;
   const int64_t grid = (a.rows * (a.hq / a.hk) / (128 * kTiles) + a.batch) * a.hk * a.splits;
+  a.ordered = by_length(a, grid, 3 - kTiles, a.splits);
   return launch_cache(what, attention_tile_kernel<kSource, D, kTiles>, grid, 1, 1, Shape::kThreads, Shape::kSmem, stream, a,
                       tm_q, tm_k, tm_v, tm_o);
 }
@@ -416,6 +429,7 @@ int pir2b_prompt_attention(const void *q, int64_t q_row, int64_t q_head, const v
   a.batch = int(batch);
   set_heads(&a, hq, hk);
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.sms = dev->sms;
   a.splits = 1;
   if (int r = cache_kernel_attributes(dev))
     return r;
@@ -520,6 +534,7 @@ int pir2b_cache_attention(const void *q, int64_t q_row, int64_t q_head, int64_t 
   a.batch = sequences->batch;
   set_heads(&a, hq, pages->kv_heads);
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.sms = dev->sms;
   const int d = pages->head_dim;
   if (int r = cache_kernel_attributes(dev))
     return r;

@@ -167,6 +167,22 @@ def test_attention_over_a_long_cache(dtype, new):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("batch", [41, 128, 129])
+@pytest.mark.parametrize("new", [1, 37, 70])
+def test_many_sequences_of_uneven_lengths(dtype, batch, new):
+    """More units of rows than run at once: they are taken by length."""
+    fresh = [0 if b % 11 == 5 else 1 + (b * 7) % new if new > 1 else 1 for b in range(batch)]
+    fresh[2] = 3 * new
+    total = [(n * 5 + b * 17) % 90 for b, n in enumerate(fresh)]
+    total[1], total[batch // 2], total[batch - 1] = 1500, 1101, 700
+    kc, vc, ks, vs, table, rows = make_pool(total, 16, 64, 64, dtype, seed=batch)
+    q, _ = new_rows(sum(fresh), 16, 64, seed=new)
+    q.div_(q.float().abs().amax(-1, keepdim=True)).mul_(3)
+    out = ops.cache_attention(q, KVPages(kc, vc, ks, vs), Sequences(starts_of(fresh), ints(total), table))
+    check(out, q, rows, fresh, total)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "int8", "e4m3"])
 def test_a_batch_of_many_kinds_of_rows(dtype):
     """Single tokens and whole prompts in one call, most sequences empty."""
     new = [1, 1, 0, 200, 1, 0, 7, 1, 40, 0, 1, 1]
