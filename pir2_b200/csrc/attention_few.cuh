@@ -260,8 +260,8 @@ __device__ __forceinline__ int offset_of(int r, int c) {
 // that fill the SMs: pieces of about equal length, however the
 // lengths of the sequences differ: with s_b 16-key steps for each of a
 // sequence's units, W steps in all and `pieces` CTAs wanted, T is a little over
-// W / pieces and each unit has ceil(s_b / T) pieces, W / T + units at most in
-// all.  They are numbered sequence, kv head, unit, piece.
+// W / (pieces - units), at least 16, and each unit has ceil(s_b / T) pieces, W /
+// T + units at most in all.  They are numbered sequence, kv head, unit, piece.
 struct FewPiece {
   int b, kvh, tile;      // sequence (-1: none), kv head, unit of its rows
   int index, count;      // piece of the unit
@@ -294,7 +294,7 @@ __device__ __forceinline__ FewPiece piece_of_block(const RaggedArgs &a, int grou
     whole += __shfl_xor_sync(0xffffffffu, whole, x);
   }
   const float cuts = fmaxf(a.pieces - whole * a.c.hk, 0.5f * a.pieces);
-  const uint32_t length = max(uint32_t(kFewWarps), uint32_t(work * 1.0001f * a.c.hk / cuts) + 1);
+  const uint32_t length = max(uint32_t(4 * kFewWarps), uint32_t(work * 1.0001f * a.c.hk / cuts) + 1);
   uint32_t mine = 0;
   for (int b = b0; b < b1; ++b) {
     if (each > 1)
@@ -803,19 +803,19 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   }
 }
 
-// Joins the pieces of each (row, head) that has several, in order: a warp per
-// row and head, D / 32 values per lane.
+// Joins the pieces of each (row, head): a CTA of eight warps for each, which
+// take the pieces in turn and are added in warp order (one warp for all pieces:
+// 170 us for one token over 30000 of one kv head, of which the join took nearly
+// all).
 template <int D, int kNT>
 __global__ void __launch_bounds__(256) attention_join_pieces_kernel(const RaggedArgs a) {
   constexpr int E = D / 32, kRowsLog2 = kNT == 1 ? 3 : 4;
+  __shared__ float so[8][D], sl[8], sm[8];
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t item = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const int64_t row = item / a.hq;
-  const int h = int(item % a.hq), group = a.hq / a.hk, kvh = h / group;
-  if (row >= a.rows)
-    return;
+  const int64_t row = blockIdx.x / a.hq;
+  const int h = int(blockIdx.x % a.hq), group = a.hq / a.hk, kvh = h / group;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = sequence_of_warp(a.starts, a.batch, row);
   if (b < 0)
     return;
@@ -826,14 +826,20 @@ __global__ void __launch_bounds__(256) attention_join_pieces_kernel(const Ragged
     return;
   const int64_t first = (int64_t(unit.x) << kRowsLog2) + (r & ((1 << kRowsLog2) - 1));
   float top = -INFINITY;
-  for (int s = lane; s < unit.y; s += 32)
+  for (int s = threadIdx.x; s < unit.y; s += 256)
     top = fmaxf(top, a.part_ml[first + (int64_t(s) << kRowsLog2)].x);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1)
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  if (lane == 0)
+    sm[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w)
+    top = fmaxf(top, sm[w]);
   float total = 0.f, sum[E] = {};
-#pragma unroll 4
-  for (int s = 0; s < unit.y; ++s) {
+#pragma unroll 8
+  for (int s = warp; s < unit.y; s += 8) {
     const int64_t at = first + (int64_t(s) << kRowsLog2);
     const float2 ml = a.part_ml[at];
     const float f = ml.x == top ? 1.f : exp2_fast(ml.x - top);   // equal, -inf too: the sums as they are
@@ -843,7 +849,21 @@ __global__ void __launch_bounds__(256) attention_join_pieces_kernel(const Ragged
     for (int e = 0; e < E; ++e)
       sum[e] += f * p[e];
   }
-  store_row<E>(a.out + row * a.ldo + h * D + lane * E, sum, total);
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    so[warp][lane * E + e] = sum[e];
+  if (lane == 0)
+    sl[warp] = total;
+  __syncthreads();
+  if (threadIdx.x < D) {
+    total = sum[0] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      total += sl[w];
+      sum[0] += so[w][threadIdx.x];
+    }
+    a.out[row * a.ldo + h * D + threadIdx.x] = __float2bfloat16(total == 0.f ? 0.f : sum[0] / total);
+  }
 }
 
 // Joins the splits of each (row, head), in split order: a warp per row and

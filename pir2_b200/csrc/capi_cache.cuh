@@ -147,8 +147,8 @@ static int launch_rows(bool write, int format, int d, const CacheRowsArgs &a, vo
 constexpr int kFewRowsBf16 = 16, kFewRows8Bit = 32;
 
 // How the few-row kernel covers a call: a cluster of CTAs per unit of rows,
-// which joins its sums in shared memory, or, where eight CTAs a unit leave SMs
-// idle, a list of pieces that a second launch joins.
+// which joins its sums in shared memory, or, where units are few and long, a
+// list of pieces that a second launch joins.
 struct FewPlan {
   int nt;            // 8 nt rows per unit
   int cluster;       // CTAs of a unit, 0: pieces
@@ -166,7 +166,13 @@ static FewPlan plan_few(int64_t rows, int hq, int hk, int batch, int64_t positio
   const int resident = few_ctas(format, d, p.nt);
   const int64_t units = batch * ((rows + batch - 1) / batch * group + 8 * p.nt - 1) / (8 * p.nt) * hk;
   const int64_t longest = (positions + 16 * kFewWarps - 1) / (16 * kFewWarps);    // CTAs a unit can use
-  if (8 * units >= sms / 3 || longest <= 8) {
+  // Pieces of equal length, in one round of CTAs, where a unit has four places
+  // or more on the SMs; but up to 2560 keys a cluster, which needs no second
+  // launch.  One token each, 8 kv heads, int8, cluster against pieces: one
+  // sequence of 2000 8.8 us against 10.2, of 8000 17.7 against 13.9, of 30000 50
+  // against 22; eight of 2000-4000 18.2 against 19.5; sixteen of 3500-7000 53
+  // against 47.
+  if (4 * units >= resident * sms || longest <= 40) {
     // CTAs for every place on the SMs, less than twice as many (64 int8
     // sequences of 500-4000 tokens: 62 us with one or two to a unit, 74 with
     // four).
@@ -175,7 +181,7 @@ static FewPlan plan_few(int64_t rows, int hq, int hk, int batch, int64_t positio
       p.cluster *= 2;
     p.grid = p.slots * hk * p.cluster;
   } else {
-    p.pieces = int64_t(2) * resident * sms;
+    p.pieces = int64_t(resident) * sms;
     p.grid = p.pieces + p.slots * hk;              // each unit may have a piece more
   }
   return p;
@@ -337,7 +343,7 @@ static int launch_join(const CachePlan &p, int d, const RaggedArgs &a, void *str
     return launch_cache("cache_attention join launch",
                         d == 64 ? (p.few.nt == 1 ? attention_join_pieces_kernel<64, 1> : attention_join_pieces_kernel<64, 2>)
                                 : (p.few.nt == 1 ? attention_join_pieces_kernel<128, 1> : attention_join_pieces_kernel<128, 2>),
-                        (a.rows * a.hq + 7) / 8, 1, 1, 256, 0, stream, a);
+                        a.rows * a.hq, 1, 1, 256, 0, stream, a);
   return launch_cache("cache_attention join launch", d == 64 ? attention_join_kernel<64> : attention_join_kernel<128>,
                       (a.rows * a.hq + 7) / 8, 1, 1, 256, 0, stream, a);
 }

@@ -167,6 +167,22 @@ def test_attention_over_a_long_cache(dtype, new):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("heads", [(2, 1, 128), (9, 3, 64)], ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("new", [[1, 1, 0, 1, 1], [1, 2, 0, 3, 4]], ids=["one", "few"])
+def test_few_sequences_one_of_them_long(dtype, heads, new):
+    """Units of rows of every length from none to many pieces."""
+    hq, hk, d = heads
+    total = [29990, 0, 5, 300, 4003]
+    kc, vc, ks, vs, table, rows = make_pool(total, hk, d, 32, dtype, seed=hq)
+    q, _ = new_rows(sum(new), hq, d, seed=31)
+    q.div_(q.float().abs().amax(-1, keepdim=True)).mul_(3)
+    sequences = Sequences(starts_of(new), ints(total), table)
+    out = ops.cache_attention(q, KVPages(kc, vc, ks, vs), sequences)
+    check(out, q, rows, new, total)
+    assert torch.equal(out, ops.cache_attention(q, KVPages(kc, vc, ks, vs), sequences))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "int8", "e4m3"])
 @pytest.mark.parametrize("batch", [41, 128, 129])
 @pytest.mark.parametrize("new", [1, 37, 70])
 def test_many_sequences_of_uneven_lengths(dtype, batch, new):
