@@ -893,14 +893,15 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const RaggedArgs a)
   for (int x = 16; x > 0; x >>= 1)
     total += __shfl_xor_sync(0xffffffffu, total, x);
   float sum[E] = {};
+#pragma unroll 8
   for (int s = 0; s < a.splits; ++s) {
     const float fs = __shfl_sync(0xffffffffu, f, s);
-    if (fs == 0.f)
-      continue;
     const float *p = a.part_o + (s * apart + item) * D + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      sum[e] += fs * p[e];
+    for (int e = 0; e < E; ++e) {
+      const float x = p[e];
+      sum[e] += fs == 0.f ? 0.f : fs * x;
+    }
   }
   store_row<E>(a.out + row * a.ldo + h * D + lane * E, sum, total);
 }
