@@ -425,8 +425,10 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
       // Only a row's first block is searched for its maximum: the weights are
       // taken relative to mu, and their sum tells when that has become too
       // small.  A block whose weights sum to more than 2^12 raises mu before the
-      // next one, by the power of two in that sum; one whose weights pass 2^64
-      // is done again under its own maximum.
+      // next one, by the power of two in that sum; one whose weights pass 2^16
+      // is done again under its own maximum: O must hold that many times the
+      // largest value, and with 2^16 it overflows only where the plain sum over
+      // 65536 keys would.
       const float *block_scales = scales + (j % Shape::kDepth) * 2 * kTileKeys + half * 64;
       uint32_t s[32], p[2][16];
       auto load = [&](int i) {
@@ -536,7 +538,7 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
         }
       }
       last = weights();
-      if (__any_sync(0xffffffffu, !(last < 0x1p64f))) {
+      if (__any_sync(0xffffffffu, !(last < 0x1p16f))) {
         meet();                   // both have read the sums
         const float m = fmaxf(mu, maximum()), keep = exp2_fast(mu - m);
         mu = m;
