@@ -105,6 +105,18 @@ __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[1
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld_8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_st_8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float m;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
@@ -405,8 +417,8 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
       mbar_arrive(&bar.q_full[u]);
     }
     float mu = 0.f, sum = 0.f;    // weights are exp2(score - mu); their sum over the row
-    float last = 0.f;             // that of the block before
     bool none = true;             // no score seen yet
+    constexpr float kAgain = kScaled ? 0x1p16f : 0x1p64f;
     for (int j = 0; j < w.blocks(u); ++j) {
       if (!__all_sync(0xffffffffu, mbar_wait(&bar.s_full[u], j & 1, kStatusTimeoutEpilogue))) {
         ok = false;
@@ -424,11 +436,11 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
       }
       // Only a row's first block is searched for its maximum: the weights are
       // taken relative to mu, and their sum tells when that has become too
-      // small.  A block whose weights sum to more than 2^12 raises mu before the
-      // next one, by the power of two in that sum; one whose weights pass 2^16
-      // is done again under its own maximum: O must hold that many times the
-      // largest value, and with 2^16 it overflows only where the plain sum over
-      // 65536 keys would.
+      // small.  A block whose weights sum to more than 2^12 raises mu by the
+      // power of two in that sum and scales its weights, exactly, before they
+      // meet V: products and O then overflow only where the plain sum would.
+      // One whose weights pass kAgain is done again under its own maximum: 2^64,
+      // or 2^16 where the weights are rounded to bf16 with V's scale in them.
       const float *block_scales = scales + (j % Shape::kDepth) * 2 * kTileKeys + half * 64;
       uint32_t s[32], p[2][16];
       auto load = [&](int i) {
@@ -474,14 +486,14 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
       };
       auto scale_o = [&](float keep) {
 #pragma unroll 1
-        for (int i = 0; i < kOwn / 16; ++i) {
-          uint32_t o[16];
-          tmem_ld_16(o_tm + i * 16, o);
+        for (int i = 0; i < kOwn / 8; ++i) {
+          uint32_t o[8];
+          tmem_ld_8(o_tm + i * 8, o);
           tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 16; ++c)
+          for (int c = 0; c < 8; ++c)
             o[c] = __float_as_uint(__uint_as_float(o[c]) * keep);
-          tmem_st_16(o_tm + i * 16, o);
+          tmem_st_8(o_tm + i * 8, o);
         }
       };
       // The weights of this thread's columns into p; returns the row's sum.
@@ -521,32 +533,41 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
         meet();
         return *my_sum + *other_sum;
       };
-      // Both are rare: one vote for the two.
-      if (__any_sync(0xffffffffu, last > 4096.f || (none && limit >= j * kTileKeys))) {
-        const int up = last > 4096.f && last < INFINITY ? (__float_as_int(last) >> 23) - 127 : 0;
-        const float keep = __int_as_float((127 - up) << 23);
-        mu += up;
-        sum *= keep;
-        if (j > 0)
-          scale_o(keep);
-        if (__any_sync(0xffffffffu, none && limit >= j * kTileKeys)) {
-          const float m = maximum();
-          if (none && m > -INFINITY) {
-            mu = m;
-            none = false;
-          }
+      if (__any_sync(0xffffffffu, none && limit >= j * kTileKeys)) {
+        const float m = maximum();
+        if (none && m > -INFINITY) {
+          mu = m;
+          none = false;
         }
       }
-      last = weights();
-      if (__any_sync(0xffffffffu, !(last < 0x1p16f))) {
-        meet();                   // both have read the sums
-        const float m = fmaxf(mu, maximum()), keep = exp2_fast(mu - m);
-        mu = m;
+      float total = weights();
+      // Of rows past the sequence nothing is kept.
+      if (__any_sync(0xffffffffu, valid && !(total <= 4096.f))) {
+        float keep;
+        if (__any_sync(0xffffffffu, valid && !(total < kAgain))) {
+          meet();                 // both have read the sums
+          const float m = fmaxf(mu, maximum());
+          keep = exp2_fast(mu - m);
+          mu = m;
+          total = weights();
+        } else {
+          const int up = valid && total > 4096.f ? (__float_as_int(total) >> 23) - 127 : 0;
+          keep = __int_as_float((127 - up) << 23);
+          mu += up;
+          total *= keep;
+          const __nv_bfloat162 keep2 = __float2bfloat162_rn(keep);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&p[i][c]), keep2);
+              p[i][c] = *reinterpret_cast<const uint32_t *>(&x);
+            }
+        }
         sum *= keep;
         scale_o(keep);
-        last = weights();
       }
-      sum += last;
+      sum += total;
       // P goes over the scores it came from.
       tmem_st_16(s_tm, p[0]);
       tmem_st_16(s_tm + 16, p[1]);
