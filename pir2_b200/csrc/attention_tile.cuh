@@ -188,7 +188,8 @@ __device__ __noinline__ void sum_again(const RaggedArgs &a, TileWork w, int kvh,
   else
     end = w.keys;
   bool spoiled = false;
-  for (int key = limit + 1; key < end && !spoiled; ++key)
+  // A row that sees nothing here has a limit below 0: no position lies there.
+  for (int key = max(0, limit + 1); key < end && !spoiled; ++key)
     for (int c = 0; c < 32; ++c)
       spoiled |= !(fabsf(__bfloat162float(v_of(key)[c])) < INFINITY);
   if (!spoiled)

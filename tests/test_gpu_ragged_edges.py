@@ -90,3 +90,22 @@ def test_large_values_in_the_cache_under_scores_that_grow(dtype, new, total, big
     scale = 0.6931471805599453
     out = ops.cache_attention(q, pages, Sequences(starts_of([new]), ints([total]), table), scale=scale)
     compare(out, q, hk, hv, scale)
+
+
+# ------------------------------------------- rows that see nothing, hidden infinities
+@pytest.mark.parametrize("heads", [(16, 8, 128), (4, 4, 64), (9, 3, 64)], ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize(
+    "new,total,bad,width",
+    [(40, 20, 10, None), (40, 20, 19, None), (150, 100, 3, None), (900, 30, 7, None), (60, 33, 5, 200)],
+)
+def test_rows_before_the_first_token_beside_a_hidden_infinity(heads, new, total, bad, width):
+    """More new rows than tokens: the first rows see nothing and give zeros,
+    and what is hidden from them leaves no status."""
+    hq, hk, d = heads
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = (torch.randn(total, hk, d, generator=g, device="cuda") for _ in range(2))
+    v[bad, :, 3] = float("inf")
+    q = torch.randn(new, hq, d, generator=g, device="cuda").to(torch.bfloat16)
+    pages, table, (kk, vv) = filled(k, v, 16, torch.bfloat16, width)
+    out = ops.cache_attention(q, pages, Sequences(starts_of([new]), ints([total]), table))
+    compare(out, q, kk, vv, d**-0.5)
