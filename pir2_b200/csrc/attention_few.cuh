@@ -553,7 +553,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
     for (int t = 0; t < kNT; ++t) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float v = kBf16 ? sc[t][e] * a.scale_log2 : sc[t][e] * (e < 2 ? k_lo : k_hi) * to_log2[t][e & 1];
+        // The factors first: a large key's scale alone could overflow the product.
+        float v = sc[t][e] * (kBf16 ? a.scale_log2 : (e < 2 ? k_lo : k_hi) * to_log2[t][e & 1]);
         if (masked && key0 + mine + (e & 2) * 4 > limit[t][e & 1])
           v = -INFINITY;
         sc[t][e] = v;

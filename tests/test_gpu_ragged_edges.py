@@ -109,3 +109,17 @@ def test_rows_before_the_first_token_beside_a_hidden_infinity(heads, new, total,
     pages, table, (kk, vv) = filled(k, v, 16, torch.bfloat16, width)
     out = ops.cache_attention(q, pages, Sequences(starts_of([new]), ints([total]), table))
     compare(out, q, kk, vv, d**-0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("new", [1, 6, 90])
+@pytest.mark.parametrize("tiny", [2.0**-121, 2.0**-100, 2.0**100])
+def test_keys_and_queries_of_opposite_magnitudes(dtype, new, tiny):
+    """Scores of ordinary size from queries and keys near the ends of bf16's
+    range."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    k, v = (torch.randn(100, 1, 128, generator=g, device="cuda") for _ in range(2))
+    q = (torch.randn(new, 2, 128, generator=g, device="cuda") * tiny).to(torch.bfloat16)
+    pages, table, (hk, hv) = filled(k / tiny, v, 32, dtype)
+    out = ops.cache_attention(q, pages, Sequences(starts_of([new]), ints([100]), table))
+    compare(out, q, hk, hv, 128**-0.5)
