@@ -70,11 +70,12 @@ int pir2b_device_status(int *status_out, void *stream);
 /* Status word value left by pir2b_wait_probe. */
 #define PIR2B_STATUS_TIMEOUT_PROBE 0x105
 
-/* Self-test of the bounded device waits: launches one thread that waits on
- * an mbarrier nothing arrives at.  The wait gives up after its budget
- * (about 1 s), sets the device status word to PIR2B_STATUS_TIMEOUT_PROBE
- * and writes 0 to the device int `result`.  Asynchronous on `stream`.
- * No counterpart in the reference. */
+/* Self-test of the bounded device waits: launches one warp that waits on an
+ * mbarrier nothing arrives at, and one that waits for the first at a barrier
+ * of the two.  The first gives up after its budget (about 1 s), sets the
+ * device status word to PIR2B_STATUS_TIMEOUT_PROBE and leaves, which lets the
+ * second go; 0 is then written to the device int `result` (else 1, 2 or 3).
+ * Asynchronous on `stream`.  No counterpart in the reference. */
 int pir2b_wait_probe(int *result, void *stream);
 
 /* Per-row symmetric quantization and packing of BF16 activations.

@@ -128,10 +128,11 @@ def check(status, what):
 
 
 def wait_probe(result, stream=None):
-    """Launches the bounded-wait self-test kernel: one thread waits on an
+    """Launches the bounded-wait self-test kernel: one warp waits on an
     mbarrier nothing arrives at, gives up after its ~1 s budget, sets the
-    device status word to STATUS_TIMEOUT_PROBE and writes 0 to `result`
-    (a CUDA int32 tensor of one element)."""
+    device status word to STATUS_TIMEOUT_PROBE and leaves; another, which waits
+    for it at a barrier of the two, is let go.  `result` (a CUDA int32 tensor
+    of one element) is then 0."""
     import torch
 
     if not result.is_cuda or result.dtype != torch.int32 or result.numel() != 1:

@@ -400,8 +400,7 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
     const int my_token = token_of(u * 128 + t, my_head);
     const int limit = valid ? w.first + my_token - w.base : -1;   // it sees positions 0 .. limit
     float *my_sum = sums + (u * 2 + half) * 128 + t, *other_sum = sums + (u * 2 + 1 - half) * 128 + t;
-    auto meet = [&]() { named_barrier(1 + u * 4 + (warp & 3), 64); };   // the two warps of these rows
-    bool ok = true;
+    PairMeeting pair{uint32_t(1 + u * 4 + (warp & 3))};   // the two warps of these rows
     if (w.blocks(u) > 0 && !a.q_by_tma) {
       for (int i = half * 128 + t; i < 128 * (D / 8); i += 256) {
         const int qr = i / (D / 8), c = i % (D / 8);
@@ -422,7 +421,7 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
     constexpr float kAgain = kScaled ? 0x1p16f : 0x1p64f;
     for (int j = 0; j < w.blocks(u); ++j) {
       if (!__all_sync(0xffffffffu, mbar_wait(&bar.s_full[u], j & 1, kStatusTimeoutEpilogue))) {
-        ok = false;
+        pair.leave();
         break;
       }
       tc_fence_after();
@@ -480,9 +479,10 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
           }
         }
         *my_sum = fmaxf(m0, m1);
-        meet();
+        if (!pair.meet())
+          return -INFINITY;
         const float m = fmaxf(*my_sum, *other_sum) * a.scale_log2;
-        meet();
+        pair.meet();
         return m;
       };
       auto scale_o = [&](float keep) {
@@ -531,11 +531,13 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
           }
         }
         *my_sum = total.x + total.y;
-        meet();
+        pair.meet();
         return *my_sum + *other_sum;
       };
       if (__any_sync(0xffffffffu, none && limit >= j * kTileKeys)) {
         const float m = maximum();
+        if (!pair.ok)             // the other warp has left
+          break;
         if (none && m > -INFINITY) {
           mu = m;
           none = false;
@@ -543,14 +545,21 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
       }
       float total = weights();
       // Of rows past the sequence nothing is kept.
-      if (__any_sync(0xffffffffu, valid && !(total <= 4096.f))) {
+      if (__any_sync(0xffffffffu, !pair.ok || (valid && !(total <= 4096.f)))) {
+        if (!pair.ok)
+          break;
         float keep;
         if (__any_sync(0xffffffffu, valid && !(total < kAgain))) {
-          meet();                 // both have read the sums
+          if (!pair.meet())       // both have read the sums
+            break;
           const float m = fmaxf(mu, maximum());
+          if (!pair.ok)
+            break;
           keep = exp2_fast(mu - m);
           mu = m;
           total = weights();
+          if (!pair.ok)
+            break;
         } else {
           const int up = valid && total > 4096.f ? (__float_as_int(total) >> 23) - 127 : 0;
           keep = __int_as_float((127 - up) << 23);
@@ -578,10 +587,16 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
       if (lane == 0)
         mbar_arrive(&bar.p_full[u]);
     }
-    if (ok && w.blocks(u) > 0)
-      ok = mbar_wait(&bar.o_full[u], 0, kStatusTimeoutEpilogue);
+    // 32 rows that leave by TMA; the two halves of heads of 64 in one box.
+    const int first_row = w.r0 + u * 128 + (warp & 3) * 32;
+    const bool whole = a.splits == 1 && a.out_by_tma && w.b >= 0 && first_row + 32 <= w.r1;
+    bool done = pair.ok;
+    if (done && w.blocks(u) > 0)
+      done = __all_sync(0xffffffffu, mbar_wait(&bar.o_full[u], 0, kStatusTimeoutEpilogue));
+    if (D == 64 && whole && pair.ok && !done)
+      pair.leave();
     tc_fence_after();
-    if (__all_sync(0xffffffffu, ok) && w.b >= 0 && w.r0 + u * 128 < w.r1) {
+    if (done && w.b >= 0 && w.r0 + u * 128 < w.r1) {
       const float inv = sum == 0.f ? 0.f : a.splits > 1 ? 1.f : 1.f / sum;   // splits are divided when joined
       const int64_t part = (int64_t(split) * a.rows + w.begin + my_token) * a.hq + my_head;
       if (a.splits > 1 && valid && half == 0)
@@ -633,13 +648,12 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
                          pack_bf16x2(f[c + 6], f[c + 7]));
       }
       // 32 rows to memory: by TMA, or the last of a sequence row by row.
-      const int first_row = w.r0 + u * 128 + (warp & 3) * 32;
-      if (a.splits == 1 && a.out_by_tma && first_row + 32 <= w.r1) {
+      if (whole) {
         fence_proxy_async_smem();
         __syncwarp();
         if (D == 64)
-          meet();                 // both halves are in one box
-        if (lane == 0 && (D == 128 || half == 0)) {
+          pair.meet();            // both halves are in one box
+        if (pair.ok && lane == 0 && (D == 128 || half == 0)) {
           tma_store_3d(&tm_o, own_sm + (warp & 3) * 4096, D == 128 ? half * 64 : 0, kvh * group,
                        int(w.begin) + over_group(a, first_row));
           tma_store_commit_and_wait();

@@ -780,15 +780,36 @@ static int launch_gemm(const GemmPlan &plan, const void *qa, const float *sa, co
   return cuda_status(e, "gemm launch");
 }
 
-// Self-test of the bounded wait: one thread waits on an mbarrier that
-// nothing arrives at.  After the wait budget (about 1 s of SM clock)
-// `mbar_wait` gives up and records kStatusTimeoutProbe in the status word;
-// the kernel then writes 0 to *result (1 would mean the wait completed).
+// Self-test of the bounded wait and of PairMeeting: warp 0 waits on an
+// mbarrier that nothing arrives at, warp 1 for warp 0 at their meeting.  After
+// the wait budget (about 1 s of SM clock) `mbar_wait` gives up and records
+// kStatusTimeoutProbe in the status word, warp 0 leaves and warp 1 is let go;
+// *result is then 0 (1 would mean that the wait completed, 2 that warp 1 met
+// warp 0 all the same).
 __global__ void wait_probe_kernel(int *result) {
   __shared__ uint64_t bar;
-  mbar_init(&bar, 1);
-  fence_barrier_init();
-  *result = mbar_wait(&bar, 0, kStatusTimeoutProbe) ? 1 : 0;
+  __shared__ int met;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar, 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  PairMeeting pair{1};
+  bool waited = false;
+  if (threadIdx.x < 32) {
+    waited = __all_sync(0xffffffffu, mbar_wait(&bar, 0, kStatusTimeoutProbe));
+    if (waited)
+      pair.meet();
+    else
+      pair.leave();
+  } else {
+    pair.meet();
+    if (threadIdx.x == 32)
+      met = pair.ok;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0)
+    *result = (waited ? 1 : 0) + (met ? 2 : 0);
 }
 
 } // namespace pir2b
@@ -807,7 +828,7 @@ int pir2b_wait_probe(int *result, void *stream) {
   DeviceInfo *dev = nullptr;
   if (int r = device_info(&dev))
     return r;
-  wait_probe_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(result);
+  wait_probe_kernel<<<1, 64, 0, static_cast<cudaStream_t>(stream)>>>(result);
   return cuda_status(cudaGetLastError(), "wait probe launch");
 }
 

@@ -343,6 +343,36 @@ __device__ __forceinline__ void named_barrier(uint32_t id, uint32_t count) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
 }
 
+// The same, and whether any of the threads came with `flag`.
+__device__ __forceinline__ bool named_barrier_any(uint32_t id, uint32_t count, bool flag) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "bar.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(id), "r"(count), "r"(uint32_t(flag))
+      : "memory");
+  return any != 0;
+}
+
+// Two warps that exchange values through shared memory and meet equally often
+// at hardware barrier `id`.  Such a barrier knows no time limit, so a warp that
+// gives up a wait of its own comes to the next meeting to say so: both learn
+// there that one has left, and meet no more.  A wait between meetings being
+// bounded, so is each meeting.
+struct PairMeeting {
+  uint32_t id;
+  bool ok = true;     // neither has left (the same in all threads of both)
+
+  __device__ __forceinline__ bool meet() { return ok = !named_barrier_any(id, 64, false); }
+  __device__ __forceinline__ void leave() {
+    named_barrier_any(id, 64, true);
+    ok = false;
+  }
+};
+
 // ---------------------------------------------------------------- cluster
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;
