@@ -17,6 +17,7 @@ import torch
 
 from . import ops
 from .kv_cache import KVPages, Sequences
+from .transformer import _MODE_BITS
 
 
 class TextCache:
@@ -76,28 +77,32 @@ class TextCache:
 
 class PackedTextDecoder:
     """Runs a text backbone's layers (Qwen3-VL attention: q/k norm, RoPE,
-    grouped heads of 128) on packed rows over a TextCache."""
+    grouped heads of 128) on packed rows over a TextCache.  With a TransformerINT
+    `controller`, q, k and v are one grouped GEMM of the precision that it has
+    installed at the time of a call (only of `bits`, if given)."""
 
-    def __init__(self, backbone, cache, *, controller=None, bits=8):
-        self.backbone, self.cache = backbone, cache
+    def __init__(self, backbone, cache, *, controller=None, bits=None):
+        self.backbone, self.cache, self.controller = backbone, cache, controller
         self.attentions = [layer.self_attn for layer in backbone.layers]
         if len(self.attentions) != len(cache.layers):
             raise ValueError("the cache must have one pool per layer")
         if any(attn.head_dim != 128 for attn in self.attentions):
             raise ValueError("PackedTextDecoder needs heads of 128")
-        self.groups = {}
+        self.groups = {}          # (bits, attention) -> its q|k|v group
         if controller is not None:
             names = {id(site[0]): name for name, site in controller.sites.items()}
-            grouped = {names_of[0]: group for names_of, group in controller.grouped[bits] if len(names_of) == 3}
-            for attn in self.attentions:
-                group = grouped.get(names.get(id(attn.q_proj)))
-                if group is not None:
-                    self.groups[id(attn)] = group
+            for precision in (8, 4) if bits is None else (bits,):
+                grouped = {members[0]: group for members, group in controller.grouped[precision] if len(members) == 3}
+                for attn in self.attentions:
+                    group = grouped.get(names.get(id(attn.q_proj)))
+                    if group is not None:
+                        self.groups[precision, id(attn)] = group
         self.rope = None
         self.prompts = False      # every sequence of the batch starts with this call
 
     def _project(self, attn, x):
-        group = self.groups.get(id(attn))
+        mode = None if self.controller is None else self.controller.mode
+        group = self.groups.get((_MODE_BITS.get(mode), id(attn)))
         if group is not None:
             return group.linear(x)
         return torch.cat((attn.q_proj(x), attn.k_proj(x), attn.v_proj(x)), dim=-1)
