@@ -69,6 +69,16 @@ class TextCache:
         self.lengths.copy_(torch.tensor(self.tokens, dtype=torch.int32))
         return self.sequences
 
+    def rewind(self, tokens):
+        """Back to `tokens` of each sequence, at most those it has: the later
+        ones are forgotten and their pages free."""
+        if len(tokens) != self.batch or any(not 0 <= n <= t for n, t in zip(tokens, self.tokens)):
+            raise ValueError("rewind: one count per sequence, at most its tokens")
+        for b in range(self.batch - 1, -1, -1):
+            while len(self.held[b]) > -(-tokens[b] // self.page_size):
+                self.free.append(self.held[b].pop())
+            self.tokens[b] = tokens[b]
+
     def release(self, b):
         """Sequence b ends: its pages are free again."""
         self.free.extend(reversed(self.held[b]))
@@ -140,13 +150,19 @@ class PackedTextDecoder:
     def run(self, hidden, new):
         """hidden: [rows, hidden] embeddings of the sequences' next tokens, one
         sequence after the other, new[b] of them for sequence b.  Returns the
-        last layer's [rows, hidden]."""
+        last layer's [rows, hidden].  Where a layer raises, the cache is as it
+        was before the call."""
         if hidden.ndim != 2 or hidden.shape[0] != sum(new):
             raise ValueError("run: hidden must hold the new tokens' rows")
         past = list(self.cache.tokens)
-        self.cache.extend(new)
-        if not hidden.shape[0]:
-            return hidden
+        try:
+            self.cache.extend(new)
+            return self._layers(hidden, past, new) if hidden.shape[0] else hidden
+        except BaseException:
+            self.cache.rewind(past)      # rows that no layer may have written
+            raise
+
+    def _layers(self, hidden, past, new):
         self.prompts = all(p == 0 for p, n in zip(past, new) if n)
         positions = [p + i for p, n in zip(past, new) for i in range(n)]
         cos, sin = self._rope(positions, hidden.device, hidden.dtype)
