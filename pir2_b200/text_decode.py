@@ -13,6 +13,10 @@ their grouped q|k|v GEMM when a TransformerINT controller is passed.
 host; a batch's index tensors are rewritten in place by every `extend`.
 """
 
+import threading
+from contextlib import contextmanager
+from functools import partial
+
 import torch
 
 from . import ops
@@ -85,6 +89,51 @@ class TextCache:
         self.held[b], self.tokens[b] = [], 0
 
 
+class _Routes:
+    """Which forward of an attention module a thread calls.  The layers call
+    their attention themselves, so a run puts its own forward in the place of the
+    module's; a backbone may be shared by decoders and plain calls of several
+    threads, each of which must get its own."""
+
+    def __init__(self):
+        self.lock = threading.Lock()
+        self.modules = {}       # id -> (its own instance attribute or None, {thread: forward})
+
+    @staticmethod
+    def _by_thread(mine, plain):
+        return lambda *args, **kwargs: mine.get(threading.get_ident(), plain)(*args, **kwargs)
+
+    @contextmanager
+    def routed(self, modules, forwards):
+        """In this thread, and within the block, module i's forward is
+        forwards[i]."""
+        thread = threading.get_ident()
+        with self.lock:
+            for module, forward in zip(modules, forwards):
+                if id(module) not in self.modules:
+                    own, mine = module.__dict__.get("forward"), {}
+                    module.forward = self._by_thread(mine, module.forward)
+                    self.modules[id(module)] = own, mine
+                self.modules[id(module)][1][thread] = forward
+        try:
+            yield
+        finally:
+            with self.lock:
+                for module in modules:
+                    own, mine = self.modules[id(module)]
+                    del mine[thread]
+                    if mine:
+                        continue
+                    del self.modules[id(module)]
+                    if own is None:
+                        module.__dict__.pop("forward", None)
+                    else:
+                        module.forward = own
+
+
+_ROUTES = _Routes()
+
+
 class PackedTextDecoder:
     """Runs a text backbone's layers (Qwen3-VL attention: q/k norm, RoPE,
     grouped heads of 128) on packed rows over a TextCache.  With a TransformerINT
@@ -108,7 +157,6 @@ class PackedTextDecoder:
                     if group is not None:
                         self.groups[precision, id(attn)] = group
         self.rope = None
-        self.prompts = False      # every sequence of the batch starts with this call
 
     def _project(self, attn, x):
         mode = None if self.controller is None else self.controller.mode
@@ -117,7 +165,7 @@ class PackedTextDecoder:
             return group.linear(x)
         return torch.cat((attn.q_proj(x), attn.k_proj(x), attn.v_proj(x)), dim=-1)
 
-    def _attend(self, index, x, cos, sin):
+    def _attend(self, index, prompts, x, cos, sin):
         attn, pages, sequences = self.attentions[index], self.cache.layers[index], self.cache.sequences
         rows = x.shape[1]
         qkv = self._project(attn, x)
@@ -127,7 +175,7 @@ class PackedTextDecoder:
         )
         q, k, v = (z[0].transpose(0, 1) for z in (q, k, v))        # [rows, heads, 128] views
         ops.cache_write(k, v, pages, sequences)
-        if self.prompts:
+        if prompts:
             y = ops.prompt_attention(q, k, v, sequences.starts)
         else:
             y = ops.cache_attention(q, pages, sequences)
@@ -163,21 +211,14 @@ class PackedTextDecoder:
             raise
 
     def _layers(self, hidden, past, new):
-        self.prompts = all(p == 0 for p, n in zip(past, new) if n)
+        prompts = all(p == 0 for p, n in zip(past, new) if n)   # every sequence of the batch starts with this call
         positions = [p + i for p, n in zip(past, new) for i in range(n)]
         cos, sin = self._rope(positions, hidden.device, hidden.dtype)
-        saved = [attn.__dict__.get("forward") for attn in self.attentions]
+        forwards = [partial(self._attend, index, prompts) for index in range(len(self.attentions))]
         h = hidden[None]
-        try:
-            for index, (layer, attn) in enumerate(zip(self.backbone.layers, self.attentions)):
-                attn.forward = lambda x, cos, sin, index=index: self._attend(index, x, cos, sin)
+        with _ROUTES.routed(self.attentions, forwards):
+            for layer in self.backbone.layers:
                 h = layer(h, cos, sin)
-        finally:
-            for attn, forward in zip(self.attentions, saved):
-                if forward is None:
-                    attn.__dict__.pop("forward", None)
-                else:
-                    attn.forward = forward
         return h[0]
 
     @torch.inference_mode()
