@@ -123,3 +123,124 @@ def test_keys_and_queries_of_opposite_magnitudes(dtype, new, tiny):
     pages, table, (hk, hv) = filled(k / tiny, v, 32, dtype)
     out = ops.cache_attention(q, pages, Sequences(starts_of([new]), ints([100]), table))
     compare(out, q, hk, hv, 128**-0.5)
+
+
+# ------------------------------------------------ hidden values that are not finite
+# Row i of the last new rows sees `bad` or does not; (new, total, table width in
+# pages of 16): few rows of one and of two groups of 8, in one CTA, a cluster and
+# pieces; one tile, two tiles, and both with the keys split.
+HIDDEN = [
+    (3, 40, None),
+    (7, 40, None),
+    (4, 1500, None),
+    (7, 9001, None),
+    (8, 30000, None),
+    (40, 90, None),
+    (40, 3001, None),
+    (200, 411, None),
+    (200, 5003, None),
+    (300, 1000, 4000),
+]
+
+
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("heads", [(4, 2, 128), (4, 2, 64), (3, 1, 128)], ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("new,total,width", HIDDEN)
+def test_values_hidden_from_some_rows_of_a_cache(new, total, width, heads, what):
+    """A value or key in the cache that is not finite spoils the rows that see
+    it, a value only in its own column, and no others."""
+    hq, hk, d = heads
+    g = torch.Generator(device="cuda").manual_seed(total)
+    q = torch.randn(new, hq, d, generator=g, device="cuda").to(torch.bfloat16)
+    k, v = (torch.randn(total, hk, d, generator=g, device="cuda") for _ in range(2))
+    first = total - new
+    for back in sorted({1, 2, new // 2, new - 1}):        # hidden from the first rows, seen by `back` of them
+        spoiled = v.clone()
+        spoiled[total - back, hk - 1, 5] = what
+        pages, table, (kk, vv) = filled(k, spoiled, 16, torch.bfloat16, width)
+        sequences = Sequences(starts_of([new]), ints([total]), table)
+        out = ops.cache_attention(q, pages, sequences)
+        compare(out, q, kk, vv, d**-0.5)
+        hit = ~torch.isfinite(out.view(new, hq, d))
+        seen = torch.arange(first, total, device="cuda") >= total - back
+        want = torch.zeros_like(hit)
+        want[:, hq - hq // hk :, 5] = seen[:, None]
+        assert torch.equal(hit, want)
+    # A key: every row that sees it, whole, in the heads that read it.
+    spoiled = k.clone()
+    spoiled[total - 2, hk - 1, 5] = what
+    pages, table, (kk, vv) = filled(spoiled, v, 16, torch.bfloat16, width)
+    out = ops.cache_attention(q, pages, Sequences(starts_of([new]), ints([total]), table)).view(new, hq, d)
+    other = hq - hq // hk
+    finite = torch.isfinite(out)
+    assert finite[: new - 2].all() and finite[:, :other].all()
+    if what != what:
+        assert not finite[new - 2 :, other:].any()
+    compare(out[: new - 2], q[: new - 2], k[: total - 2].to(torch.bfloat16), v[: total - 2].to(torch.bfloat16), d**-0.5)
+
+
+@pytest.mark.parametrize("n", [420, 2300])
+@pytest.mark.parametrize("heads", [(4, 2, 128), (4, 2, 64), (6, 2, 64)], ids=lambda h: "x".join(map(str, h)))
+def test_a_key_that_is_nan_spoils_the_rows_that_see_it(n, heads):
+    hq, hk, d = heads
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v = (torch.randn(n, h, d, generator=g, device="cuda").to(torch.bfloat16) for h in (hq, hk, hk))
+    k[n // 2, 1] = float("nan")
+    out = ops.prompt_attention(q, k, v, starts_of([n])).view(n, hq, d)
+    finite = torch.isfinite(out)
+    assert finite[: n // 2].all() and finite[:, : hq // hk].all() and not finite[n // 2 :, hq // hk :].any()
+    compare(out[: n // 2], q[: n // 2], k[: n // 2], v[: n // 2], d**-0.5)
+
+
+# ------------------------------------------------------------- heads and lengths
+@pytest.mark.parametrize("heads", [(64, 1, 64), (128, 1, 128), (128, 2, 64), (160, 1, 64), (256, 1, 128)],
+                         ids=lambda h: "x".join(map(str, h)))
+def test_many_heads_for_one_key_head(heads):
+    """Groups of 64 to 256: a query tile is one box of two tokens, of one, or
+    gathered, and its rows leave one by one."""
+    hq, hk, d = heads
+    g = torch.Generator(device="cuda").manual_seed(6)
+    lengths = [1, 37, 0, 150]
+    rows = sum(lengths)
+    q = torch.randn(rows, hq, d, generator=g, device="cuda").to(torch.bfloat16)
+    k, v = (torch.randn(rows, hk, d, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    out = ops.prompt_attention(q, k, v, starts_of(lengths))
+    at = 0
+    for n in lengths:
+        mine = slice(at, at + n)
+        if n:
+            compare(out[mine], q[mine], k[mine], v[mine], d**-0.5)
+        at += n
+    for dtype in DTYPES:
+        pages, table, (kk, vv) = filled(k.float(), v.float(), 32, dtype)
+        for new in (1, 9):
+            out = ops.cache_attention(q[:new], pages, Sequences(starts_of([new]), ints([rows]), table))
+            compare(out, q[:new], kk, vv, d**-0.5)
+
+
+@pytest.mark.parametrize("lengths", [[2048], [2500], [2050, 2047], [4099]], ids=lambda x: "-".join(map(str, x)))
+@pytest.mark.parametrize("heads", [(2, 1, 64), (3, 1, 64), (6, 2, 128)], ids=lambda h: "x".join(map(str, h)))
+def test_long_prompts_of_narrow_and_odd_heads(lengths, heads):
+    hq, hk, d = heads
+    g = torch.Generator(device="cuda").manual_seed(7)
+    rows = sum(lengths)
+    q, k, v = (torch.randn(rows, h, d, generator=g, device="cuda").to(torch.bfloat16) for h in (hq, hk, hk))
+    out = ops.prompt_attention(q, k, v, starts_of(lengths))
+    at = 0
+    for n in lengths:
+        mine = slice(at, at + n)
+        compare(out[mine], q[mine], k[mine], v[mine], d**-0.5)
+        at += n
+
+
+@pytest.mark.parametrize("what", ["heads", "rows", "all"])
+def test_broadcast_keys_and_values(what):
+    """Strides of 0: one key head for all, or one row for all."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    q = torch.randn(200, 4, 128, generator=g, device="cuda").to(torch.bfloat16)
+    k, v = (torch.randn(200, 2, 128, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    if what in ("heads", "all"):
+        k, v = (x[:, :1].expand(200, 2, 128) for x in (k, v))
+    if what in ("rows", "all"):
+        k, v = (x[:1].expand(200, 2, 128) for x in (k, v))
+    compare(ops.prompt_attention(q, k, v, starts_of([200])), q, k, v, 128**-0.5)
