@@ -161,27 +161,32 @@ struct FewPlan {
 static FewPlan plan_few(int64_t rows, int hq, int hk, int batch, int64_t positions, int format, int d, int sms) {
   FewPlan p = {};
   const int group = hq / hk;
-  p.nt = (rows + batch - 1) / batch * group <= 8 ? 1 : 2;
+  const int64_t per_sequence = (rows + batch - 1) / batch * group;
+  p.nt = per_sequence <= 8 ? 1 : 2;
   p.slots = rows * group / (8 * p.nt) + batch;
   const int resident = few_ctas(format, d, p.nt);
-  const int64_t units = batch * ((rows + batch - 1) / batch * group + 8 * p.nt - 1) / (8 * p.nt) * hk;
+  const int64_t units = batch * ((per_sequence + 8 * p.nt - 1) / (8 * p.nt)) * hk;
   const int64_t longest = (positions + 16 * kFewWarps - 1) / (16 * kFewWarps);    // CTAs a unit can use
+  const int64_t places = int64_t(resident) * sms;
   // Pieces of equal length, in one round of CTAs, where a unit has four places
   // or more on the SMs; but up to 2560 keys a cluster, which needs no second
-  // launch.  One token each, 8 kv heads, int8, cluster against pieces: one
-  // sequence of 2000 8.8 us against 10.2, of 8000 17.7 against 13.9, of 30000 50
-  // against 22; eight of 2000-4000 18.2 against 19.5; sixteen of 3500-7000 53
-  // against 47.
-  if (4 * units >= resident * sms || longest <= 40) {
-    // CTAs for every place on the SMs, less than twice as many (64 int8
-    // sequences of 500-4000 tokens: 62 us with one or two to a unit, 74 with
-    // four).
+  // launch, and up to 6144 where clusters of four fill the SMs.  8 kv heads,
+  // cluster against pieces, one token: one int8 sequence of 2000 8.8 us against
+  // 10.2, of 8000 17.7 against 13.9, of 30000 50 against 22; two tokens in a group
+  // of four, eight bf16 sequences: of 2000-4000 20.5 against 22.9, of 3000-6000
+  // 32.3 against 34.9.
+  if (4 * units >= places || longest <= (8 * units > places ? 96 : 40)) {
+    // One round of CTAs; a second only where each has 1280 keys or more (eight
+    // bf16 sequences of 1000-2000 12.1 us with four to a unit, 18.2 with eight;
+    // 64 int8 ones of 500-4000 62 with two, 74 with four; 64 of 2000-4000, group
+    // of four, 80 with two, 102 with one).
     p.cluster = 1;
-    while (p.cluster < 8 && p.cluster * units < resident * sms && 2 * p.cluster <= longest)
+    while (p.cluster < 8 && 2 * p.cluster <= longest && p.cluster * units < places &&
+           (2 * p.cluster * units <= places || positions >= 1280 * 2 * p.cluster))
       p.cluster *= 2;
     p.grid = p.slots * hk * p.cluster;
   } else {
-    p.pieces = int64_t(resident) * sms;
+    p.pieces = places;
     p.grid = p.pieces + p.slots * hk;              // each unit may have a piece more
   }
   return p;

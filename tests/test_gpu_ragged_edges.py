@@ -244,3 +244,18 @@ def test_broadcast_keys_and_values(what):
     if what in ("rows", "all"):
         k, v = (x[:1].expand(200, 2, 128) for x in (k, v))
     compare(ops.prompt_attention(q, k, v, starts_of([200])), q, k, v, 128**-0.5)
+
+
+@pytest.mark.parametrize("batch,new,group,pieces", [(8, 8, 2, True), (9, 8, 2, True), (10, 8, 2, False), (18, 4, 2, True),
+                                                    (9, 2, 8, True), (10, 2, 8, False), (18, 1, 4, True), (19, 1, 4, False)])
+def test_units_of_rows_are_counted_whole(batch, new, group, pieces):
+    """A call is cut into pieces (which need a workspace) where its units of 8
+    or 16 rows have four places or more each on 148 SMs of two (four, 8-row)
+    int8 CTAs: 8 kv heads of `batch` sequences, each one unit."""
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("counted for 148 SMs")
+    pages = KVPages.allocate(2, 8, 128, page_size=128, dtype=torch.int8)
+    table = torch.zeros(batch, 200, dtype=torch.int32, device="cuda")
+    sequences = Sequences(starts_of([new] * batch), ints([200] * batch), table)
+    size = _lib.lib().pir2b_cache_attention_workspace(batch * new, 8 * group, pages.address, sequences.address)
+    assert (size > 0) == pieces
