@@ -290,12 +290,14 @@ static int launch_tile(const char *what, RaggedArgs a, const CUtensorMap &tm_q, 
                       tm_q, tm_k, tm_v, tm_o);
 }
 
-// Tiles per CTA of the tile kernel.  One tile and two CTAs on an SM cover the
-// latencies of a CTA's start and end with another's products (64 prompts of
-// 280-816 tokens: 179 us against 204, one of 544: 11.9 against 13.7); two tiles
-// read K and V half as often, which carries long prompts (8192 tokens: 231 us
-// against 245).
-static int tiles_per_cta(int64_t rows, int batch) { return rows / batch >= 2048 ? 2 : 1; }
+// Tiles per CTA of the tile kernel over prompts.  One tile and two CTAs on an SM
+// cover the latencies of a CTA's start and end with another's products (64 prompts
+// of 280-816 tokens: 178 us against 203, one of 544: 12.5 against 13.9, one of
+// 2048: 35.1 against 36.8); two tiles read K and V half as often, which carries
+// long prompts of heads of 128 (16 and 8 heads, one of 8192: 235 against 236, two:
+// 460 against 472, one of 16384: 880 against 912) but not of 64 (12 and 4 heads,
+// one of 8192: 180 against 165, of 16384: 640 against 605).
+static int tiles_per_cta(int64_t rows, int batch, int d) { return d == 128 && rows / batch >= 8192 ? 2 : 1; }
 
 // How a call of cache_attention runs: the few-row kernel (tiles = 0) or
 // 128-row tiles, and its splits along the keys.
@@ -377,7 +379,6 @@ static int cache_kernel_attributes(DeviceInfo *dev) {
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 128, 1>), FewShape<kCacheE4m3, 128, 1>::kSmem},
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 128, 2>), FewShape<kCacheE4m3, 128, 2>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 64, 1>), TileShape<kSourceRows, 64, 1>::kSmem},
-      {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 64, 2>), TileShape<kSourceRows, 64, 2>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 128, 1>), TileShape<kSourceRows, 128, 1>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 128, 2>), TileShape<kSourceRows, 128, 2>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kCacheBf16, 64, 1>), TileShape<kCacheBf16, 64, 1>::kSmem},
@@ -456,9 +457,9 @@ int pir2b_prompt_attention(const void *q, int64_t q_row, int64_t q_head, const v
     return r;
   if (int r = make_q_map(&tm_q, &a, head_dim))
     return r;
-  const bool two = tiles_per_cta(rows, int(batch)) == 2;
-  return head_dim == 64 ? (two ? launch_tile<kSourceRows, 64, 2> : launch_tile<kSourceRows, 64, 1>)(what, a, tm_q, tm_k, tm_v, stream)
-                        : (two ? launch_tile<kSourceRows, 128, 2> : launch_tile<kSourceRows, 128, 1>)(what, a, tm_q, tm_k, tm_v, stream);
+  const bool two = tiles_per_cta(rows, int(batch), head_dim) == 2;
+  return (head_dim == 64 ? launch_tile<kSourceRows, 64, 1> : two ? launch_tile<kSourceRows, 128, 2> : launch_tile<kSourceRows, 128, 1>)(
+      what, a, tm_q, tm_k, tm_v, stream);
 }
 
 int pir2b_cache_write(const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row,

@@ -259,3 +259,12 @@ def test_units_of_rows_are_counted_whole(batch, new, group, pieces):
     sequences = Sequences(starts_of([new] * batch), ints([200] * batch), table)
     size = _lib.lib().pir2b_cache_attention_workspace(batch * new, 8 * group, pages.address, sequences.address)
     assert (size > 0) == pieces
+
+
+def test_one_prompt_of_8200_in_two_tiles():
+    g = torch.Generator(device="cuda").manual_seed(9)
+    q, k, v = (torch.randn(8200, h, 128, generator=g, device="cuda").to(torch.bfloat16) for h in (2, 1, 1))
+    k[5000, 0, 3] = 40.0                  # the reference moves
+    compare(ops.prompt_attention(q, k, v, starts_of([8200])), q, k, v, 128**-0.5)
+    v[8190, 0, 7] = float("inf")          # hidden from the last tile's first rows
+    compare(ops.prompt_attention(q, k, v, starts_of([8200])), q, k, v, 128**-0.5)
