@@ -1,7 +1,7 @@
 // Attention of a few new rows per sequence over the paged K/V cache.
 //
 // A unit is up to 8 kNT rows (query token x head of one kv head's group) of
-// one sequence; a CTA streams a range of the unit's keys once, eight warps
+// one sequence; a CTA streams a range of the unit's keys once, four warps
 // taking 16-key steps in turn.  Few rows cannot fill a 128-row tensor tile
 // and the work is reading the cache, so the products run on warp-level MMAs
 // (m16n8k16, fp32 sums) with the keys as the M rows:
@@ -18,11 +18,11 @@
 // moves only when a score passes it by more than 8 (in log2), so that most
 // steps have one vote and no rescaling; sums and maxima are fp32.
 //
-// What bounds it, one new token per sequence, 16 query and 8 kv heads of 128:
-// bf16 over four histories of 29000-32700, 85 us, 6150 GB/s, 94 % of a copy's
-// rate.  int8 over 64 histories of 500-4000, 62 us, 4710 GB/s: instructions,
-// a third of them the conversion of codes, which no warp-level MMA takes beside
-// 16-bit weights.
+// What bounds it, one new token per sequence, 16 query and 8 kv heads of 128,
+// replayed from a graph (called in a loop): bf16 over four histories of
+// 29000-32700, 85 us (87), 6150 GB/s, 94 % of a copy's rate.  int8 over 64
+// histories of 500-4000, 62 us (65), 4710 GB/s: instructions, a third of them the
+// conversion of codes, which no warp-level MMA takes beside 16-bit weights.
 #pragma once
 #include <cuda.h>
 #include "attention_ragged.cuh"

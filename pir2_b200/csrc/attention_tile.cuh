@@ -14,23 +14,29 @@
 // ring, and one clears what a page holds past the keys.  While one tile's
 // softmax runs, the tensor core works on the other's products.  Weights are
 // relative to a reference near the running maximum that moves in few blocks: O
-// is rescaled in TMEM by the softmax warps only then.  References, sums and O
-// are fp32; weights are rounded to bf16, the type of the values they multiply,
-// and a row's sum is that of the weights before that rounding.
+// is rescaled in TMEM by the softmax warps only then (scores of deviation 6, 10
+// and 30, which move it often: the 8192 tokens below 266, 277-293 and 299 us).
+// References, sums and O are fp32; weights are rounded to bf16, the type of the
+// values they multiply, and a row's sum is that of the weights before that
+// rounding.
 //
-// What bounds it, at 16 query and 8 kv heads of 128.  One prompt of 8192 tokens:
-// 231 us, 1190 TFLOP/s of the causal half; the tensor pipe is busy 56 % of the
-// time and the exponentials' unit as long, and neither hides the other in full.
-// The 64 prompts: 179 us against 67 for their bytes; a tile has three blocks on
-// average, and its start, end and each block's chain of scores, softmax and
-// product are overlapped only with those of the one other CTA on the SM that
-// TMEM has room for.  Chunks of 250-288 tokens over
-// 16 E4M3 histories of 544-2100: 121 us; reading each key's scales from shared
-// memory and turning codes into bf16 come on top.
+// What bounds it, at 16 query and 8 kv heads of 128 (replayed from a graph; called
+// in a loop in brackets).  One prompt of 8192 tokens: 236 us (271, at the board's
+// power limit), 1165 TFLOP/s of the causal half; the tensor pipe is busy 55 % of
+// the time and the exponentials' unit as long, and neither hides the other in
+// full.  The 64 prompts: 179 us (197) against 67 for their bytes; a tile has three
+// blocks on average, and its start, end and each block's chain of scores, softmax
+// and product are overlapped only with those of the one other CTA on the SM that
+// TMEM has room for.  Chunks of 250-288 tokens over 16 E4M3 histories of 544-2100:
+// 120 us (121); reading each key's scales from shared memory and turning codes
+// into bf16 come on top.
 //
 // TMEM columns: S/P of each tile (128 each), then O of each.
 // Every wait is bounded; on expiry all roles leave their loops, the loader
-// waits for its copies in flight and TMEM is freed.
+// waits for its copies in flight and TMEM is freed.  The two softmax warps of 32
+// rows meet at a hardware barrier, to which one that leaves still comes
+// (PairMeeting; that costs 1 to 2 % against a plain barrier, and half of what an
+// mbarrier with its time limit does).
 #pragma once
 #include <cuda.h>
 #include "attention_few.cuh"
