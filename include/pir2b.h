@@ -419,21 +419,34 @@ int pir2b_attention_causal(const void *q, const void *k, const void *v, int64_t 
  * row of zeros, L = 127 / 448, code = v / s rounded to nearest even and
  * clamped.  The maximum is over the finite values and an infinity becomes the
  * largest code; a row with a NaN gets codes of 0 and a NaN scale, so the codes
- * are always numbers (attention takes no E4M3 NaN codes). */
+ * are always numbers (attention takes no E4M3 NaN codes).
+ * int4: codes of -7..7 in two's complement, two to a byte with the even channel
+ * in the low bits, an E4M3 factor for every 32 channels of a row and one fp32
+ * scale per token and head; value = code * factor * scale.  With m the row's
+ * largest finite magnitude: s = 2^(floor(log2 m) - 10), at least 2^-126, 1 for a
+ * row of zeros; factor = E4M3(m_group / s / 7); code = v / s / factor rounded to
+ * nearest even and clamped, 0 where the factor is 0.  An infinity counts as m; a
+ * row with a NaN gets codes and factors of 0 and a NaN scale. */
 #define PIR2B_CACHE_BF16 16
 #define PIR2B_CACHE_INT8 8
 #define PIR2B_CACHE_E4M3 9
+#define PIR2B_CACHE_INT4 24
 
 /* A pool of pages, each holding `page_size` (16, 32, 64 or 128) consecutive
- * tokens of one sequence: k, v [pages, kv_heads, page_size, head_dim], 16-byte
- * aligned; scales fp32 [pages, kv_heads, page_size] (null with bf16).  The
- * page strides are in elements (multiples of 16 for k and v). */
+ * tokens of one sequence: k, v [pages, kv_heads, page_size, head_dim] (int4:
+ * head_dim / 2 bytes), 16-byte aligned; scales fp32 [pages, kv_heads, page_size]
+ * (null with bf16); factors E4M3 [pages, kv_heads, page_size, head_dim / 32]
+ * (int4 alone; the last four fields are read with no other format).  The page
+ * strides are in elements, of int4 codes in bytes (multiples of 16 for k, v and
+ * the factors). */
 typedef struct pir2b_kv_pages {
   void *k, *v;
   float *k_scale, *v_scale;
   int64_t k_page_stride, v_page_stride;
   int64_t k_scale_page_stride, v_scale_page_stride;
   int32_t pages, page_size, kv_heads, head_dim, format;
+  uint8_t *k_factor, *v_factor;
+  int64_t k_factor_page_stride, v_factor_page_stride;
 } pir2b_kv_pages;
 
 /* The sequences of a batch: packed rows (starts), tokens each has after them
@@ -465,7 +478,8 @@ int pir2b_cache_write(const void *k, int64_t k_row, int64_t k_head, const void *
                       int64_t v_head, int64_t rows, const pir2b_kv_pages *pages,
                       const pir2b_sequences *sequences, void *stream);
 
-/* Reads positions 0, 1, ... of each sequence back as bf16(code * scale), into
+/* Reads positions 0, 1, ... of each sequence back as bf16(code * scale) (int4:
+ * bf16(code * factor * scale), rounded once), into
  * contiguous k_out, v_out [rows, kv_heads, head_dim]: starts gives the packed
  * rows (lengths is not used). */
 int pir2b_cache_read(const pir2b_kv_pages *pages, const pir2b_sequences *sequences, int64_t rows,

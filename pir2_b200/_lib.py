@@ -23,7 +23,7 @@ OUT_FP8_VALUES = 32   # FP8 producers' first pass: bf16 values + fp32 row maxima
 STATUS_TIMEOUT_PROBE = 0x105   # device status word left by pir2b_wait_probe
 
 STATUS_BAD_PAGE = 0x201        # device status word left by an index outside a K/V pool or table
-CACHE_BF16, CACHE_INT8, CACHE_E4M3 = 16, 8, 9
+CACHE_BF16, CACHE_INT8, CACHE_E4M3, CACHE_INT4 = 16, 8, 9, 24
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -39,6 +39,7 @@ class KVPagesStruct(ctypes.Structure):
         ("k_page_stride", _I64), ("v_page_stride", _I64),
         ("k_scale_page_stride", _I64), ("v_scale_page_stride", _I64),
         ("pages", _I), ("page_size", _I), ("kv_heads", _I), ("head_dim", _I), ("format", _I),
+        ("k_factor", _P), ("v_factor", _P), ("k_factor_page_stride", _I64), ("v_factor_page_stride", _I64),
     ]
 
 

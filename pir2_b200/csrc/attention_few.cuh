@@ -73,6 +73,61 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t
   }
 }
 
+// int4: a nibble t (two's complement, t = u ^ 8 with u = code + 8) moved to the
+// mantissa of a constant makes a small number of u there, and one FMA takes u's
+// offset away and applies the factor, exactly: (c + u / n) f - (c + 8 / n) f.
+// K's fp16 pairs come a quarter as large (66 times the largest factor must not
+// overflow): from bits 2-5 64 + u / 4, from bits 6-9 4 + u / 4.
+struct Int4Factors {
+  uint32_t f, minus_66f, minus_6f;    // fp16 pairs of one factor
+};
+
+__device__ __forceinline__ uint32_t half2_mul(uint32_t x, uint32_t y) {
+  uint32_t z;
+  asm("mul.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
+  return z;
+}
+
+__device__ __forceinline__ uint32_t half2_fma(uint32_t x, uint32_t y, uint32_t z) {
+  uint32_t w;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(w) : "r"(x), "r"(y), "r"(z));
+  return w;
+}
+
+__device__ __forceinline__ uint32_t bf162_fma(uint32_t x, uint32_t y, uint32_t z) {
+  uint32_t w;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(w) : "r"(x), "r"(y), "r"(z));
+  return w;
+}
+
+__device__ __forceinline__ Int4Factors int4_factors(uint32_t pair) {   // of an fp16 pair of one factor
+  return {pair, half2_mul(pair, 0xd420d420u), half2_mul(pair, 0xc600c600u)};
+}
+
+// A word's codes 2 kHalf, 2 kHalf + 1 with those four places on, as fp16 pairs times f / 4.
+template <int kHalf>
+__device__ __forceinline__ void int4_to_half(uint32_t w, const Int4Factors &f, uint32_t &even, uint32_t &odd) {
+  const uint32_t t = kHalf ? w >> 6 : w << 2;
+  even = half2_fma((t & 0x003c003cu) ^ 0x54205420u, f.f, f.minus_66f);
+  odd = half2_fma((t & 0x03c003c0u) ^ 0x46004600u, f.f, f.minus_6f);
+}
+
+// Code kAt of each half of a word as a bf16 pair times the halves' factors:
+// bits 3-6 of 16 + u.
+template <int kAt>
+__device__ __forceinline__ uint32_t int4_to_bf16(uint32_t w, uint32_t f, uint32_t minus_24f) {
+  const uint32_t t = kAt == 0 ? w << 3 : w >> (kAt == 0 ? 0 : 4 * kAt - 3);
+  return bf162_fma((t & 0x00780078u) ^ 0x41c041c0u, f, minus_24f);
+}
+
+// Two factors as a bf16 pair, and -24 times it.  Any byte gives a number.
+__device__ __forceinline__ uint32_t factor_pair_bf16(uint32_t lo, uint32_t hi, uint32_t &minus_24f) {
+  const uint32_t zero = 0x80008000u, x = ((lo | (hi << 16)) & 0x007f007fu) << 4;
+  const uint32_t f = bf162_fma(x, 0x7b807b80u, zero);            // 2^120, as for E4M3 codes
+  minus_24f = bf162_fma(f, 0xc1c0c1c0u, zero);
+  return f;
+}
+
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&h);
@@ -224,20 +279,24 @@ __device__ __forceinline__ int unit_by_length(const RaggedArgs &a, int tile_log2
 constexpr int few_ctas(int format, int d, int nt) { return nt == 2 || (format == kCacheBf16 && d == 128) ? 2 : 4; }
 
 // Shared memory of the few-row kernel: each warp's ring of K and V tiles of 16
-// rows, their scales and barriers; at the end the warps' partial sums.
+// rows, their scales, factors and barriers; at the end the warps' partial sums.
 template <int kFormat, int D, int kNT>
 struct FewShape {
-  static constexpr bool kBf16 = kFormat == kCacheBf16;
-  static constexpr int kRowBytes = D * (kBf16 ? 2 : 1);
+  static constexpr int kRowBytes = code_bytes(kFormat, D);
   static constexpr int kBoxes = kRowBytes > 128 ? 2 : 1;          // a swizzled row has at most 128 bytes
   static constexpr int kTile = 16 * kRowBytes;
   static constexpr int kStages = 3;
   static constexpr int kCtas = few_ctas(kFormat, D, kNT);   // on an SM
   static constexpr int kRing = kFewWarps * kStages * 2 * kTile;
   static constexpr int kScales = kFewWarps * kStages * 2 * 16 * 4;
+  static constexpr int kFactorTile = kFormat == kCacheInt4 ? 16 * (D / kFactorGroup) : 0;
+  static constexpr int kFactors = kFewWarps * kStages * 2 * kFactorTile;
+  static constexpr int kCopied = kRing + kScales + kFactors;
   static constexpr int kSums = kFewWarps * kNT * 8 * (D + 4 + 2) * 4 + kNT * 8 * (D + 4) * 4;
-  static constexpr int kSmem =
-      1024 /* alignment */ + (kRing + kScales + kFewWarps * kStages * 8 > kSums ? kRing + kScales + kFewWarps * kStages * 8 : kSums);
+  // The barriers lie behind both: their memory may hold nothing else (sums
+  // written over them were seen to turn back into barriers).
+  static constexpr int kBarriers = kCopied > kSums ? kCopied : kSums;
+  static constexpr int kSmem = 1024 /* alignment */ + kBarriers + kFewWarps * kStages * 8;
 };
 
 // 4-D tiled load into this CTA's shared memory.
@@ -253,7 +312,8 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const void *tmap, uint64_
 // kRowBytes rows (of 256 bytes: in the first of two boxes of 128-byte halves).
 template <int kRowBytes>
 __device__ __forceinline__ int offset_of(int r, int c) {
-  return kRowBytes >= 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+  return kRowBytes >= 128 ? r * 128 + ((c ^ (r & 7)) << 4)
+         : kRowBytes == 64 ? r * 64 + ((c ^ ((r >> 1) & 3)) << 4) : r * 32 + (c << 4);   // rows of 32 lie plain
 }
 
 // Where sequences and kv heads are few, the work of a call is cut into pieces
@@ -354,11 +414,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
     attention_few_kernel(const RaggedArgs a, const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v) {
   using Shape = FewShape<kFormat, D, kNT>;
-  constexpr bool kBf16 = kFormat == kCacheBf16;
+  constexpr bool kBf16 = kFormat == kCacheBf16, kInt4 = kFormat == kCacheInt4;
   constexpr int kRows = 8 * kNT, kRowsLog2 = kNT == 1 ? 3 : 4;
   constexpr int KS = D / 16;                       // K steps of S, and M tiles of O
-  constexpr int KW = kBf16 ? D / 8 : D / 16;       // words of a lane's quarter of a K row
-  constexpr int VW = kBf16 ? D / 16 : D / 32;      // words of a lane's eighth of a V row
+  constexpr int KW = Shape::kRowBytes / 16;        // words of a lane's quarter of a K row
+  constexpr int VW = Shape::kRowBytes / 32;        // words of a lane's eighth of a V row
   constexpr int kRowBytes = Shape::kRowBytes, kStages = Shape::kStages, kTile = Shape::kTile;
   extern __shared__ uint8_t few_raw[];
   uint8_t *few_sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(few_raw) + 1023) & ~uintptr_t(1023));
@@ -366,7 +426,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   const int group = a.group;
   uint8_t *ring = few_sm + warp * kStages * 2 * kTile;                                    // [kStages][K, V]
   float *scales = reinterpret_cast<float *>(few_sm + Shape::kRing) + warp * kStages * 32;   // [kStages][K, V][16]
-  uint64_t *full = reinterpret_cast<uint64_t *>(few_sm + Shape::kRing + Shape::kScales) + warp * kStages;
+  uint8_t *factors = few_sm + Shape::kRing + Shape::kScales + warp * kStages * 2 * Shape::kFactorTile;   // [kStages][K, V][16][D / 32]
+  uint64_t *full = reinterpret_cast<uint64_t *>(few_sm + Shape::kBarriers) + warp * kStages;
   if (lane == 0) {
     for (int i = 0; i < kStages; ++i)
       mbar_init(&full[i], 1);
@@ -417,7 +478,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
     if (lane == 0) {
       uint8_t *to = ring + stage * 2 * kTile;
       const int in_page = (step << 4) & page_mask;
-      mbar_arrive_expect_tx(&full[stage], 2 * kTile + (kBf16 ? 0 : 128));
+      mbar_arrive_expect_tx(&full[stage], 2 * (kTile + Shape::kFactorTile) + (kBf16 ? 0 : 128));
 #pragma unroll
       for (int h = 0; h < Shape::kBoxes; ++h) {
         tma_load_4d(to + h * 2048, &tm_k, &full[stage], h * 64, in_page, kvh, page);
@@ -427,6 +488,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
         const int64_t slot = (int64_t(kvh) << a.c.shift) + in_page;
         bulk_load(scales + stage * 32, a.c.ks + page * a.c.ks_page + slot, 64, &full[stage]);
         bulk_load(scales + stage * 32 + 16, a.c.vs + page * a.c.vs_page + slot, 64, &full[stage]);
+        if constexpr (kInt4) {
+          uint8_t *f = factors + stage * 2 * Shape::kFactorTile;
+          const int64_t at = slot * (D / kFactorGroup);
+          bulk_load(f, a.c.kf + page * a.c.kf_page + at, Shape::kFactorTile, &full[stage]);
+          bulk_load(f + Shape::kFactorTile, a.c.vf + page * a.c.vf_page + at, Shape::kFactorTile, &full[stage]);
+        }
       }
     }
   };
@@ -441,8 +508,16 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
     const int r = r0 + t * 8 + g;
     // The four elements of each product step that this lane holds of a K row.
     const __nv_bfloat16 *src = a.q + (begin + r / group) * a.q_row + (kvh * group + r % group) * a.q_head;
+    if constexpr (kInt4) {                         // pairs four apart, as a word's codes come
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
+      for (int s = 0; s < KS; s += 2) {
+        const uint4 w = r < r1 ? __ldg(reinterpret_cast<const uint4 *>(src + q4 * (D / 4) + s * 4)) : make_uint4(0, 0, 0, 0);
+        qf[t][s][0] = __byte_perm(w.x, w.z, 0x5410), qf[t][s][1] = __byte_perm(w.x, w.z, 0x7632);
+        qf[t][s + 1][0] = __byte_perm(w.y, w.w, 0x5410), qf[t][s + 1][1] = __byte_perm(w.y, w.w, 0x7632);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < (kInt4 ? 0 : KS); ++s) {
       const int at = kBf16 ? (s / 2 * 4 + q4) * 8 + s % 2 * 4 : (s / 4 * 4 + q4) * 16 + s % 4 * 4;
       const uint2 w = r < r1 ? __ldg(reinterpret_cast<const uint2 *>(src + at)) : make_uint2(0, 0);
       qf[t][s][0] = w.x;
@@ -461,7 +536,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
       most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
       const int up = most == 0 ? 127 : min(264 - int(most >> 7), 253);   // exponent field of the power
       const float factor = __int_as_float(up << 23);
-      undo = __int_as_float((254 - up) << 23);
+      undo = __int_as_float((254 - up) << 23) * (kInt4 ? 4.f : 1.f);   // its K is a quarter of what it is
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -491,10 +566,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   const int mine = g ^ ((g & 1) << 2), odd = (2 * q4 + 1) ^ 4;
   // Their first pieces in a tile; the row 8 after has the same swizzle, the
   // next four pieces of K lie 64 bytes across, those after 128 in the next box.
-  constexpr int kEight = kRowBytes >= 128 ? 1024 : 512;
-  const int k_off = offset_of<kRowBytes>(mine, q4);
-  const int v_even = VW == 2 ? offset_of<kRowBytes>(2 * q4, g >> 1) + (g & 1) * 8 : offset_of<kRowBytes>(2 * q4, g);
-  const int v_odd = VW == 2 ? offset_of<kRowBytes>(odd, g >> 1) + (g & 1) * 8 : offset_of<kRowBytes>(odd, g);
+  constexpr int kEight = kRowBytes >= 128 ? 1024 : 8 * kRowBytes;
+  constexpr int kPart = VW < 4 ? 4 / VW : 1;       // lanes that share a piece of a V row
+  const int k_off = KW == 2 ? offset_of<kRowBytes>(mine, q4 >> 1) + (q4 & 1) * 8 : offset_of<kRowBytes>(mine, q4);
+  const int v_even = offset_of<kRowBytes>(2 * q4, g / kPart) + g % kPart * (VW * 4);
+  const int v_odd = offset_of<kRowBytes>(odd, g / kPart) + g % kPart * (VW * 4);
   int done = 0;
   for (; done < count; ++done) {
     const int step = step0 + done * kFewWarps, stage = done % kStages;
@@ -502,6 +578,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
       break;
     const uint8_t *k_tile = ring + stage * 2 * kTile, *v_tile = k_tile + kTile;
     uint32_t kr[2][KW], vr[4][VW];                  // K rows mine, mine + 8; V rows 2 q4, odd, and 8 after them
+    if constexpr (KW == 2) {
+      *reinterpret_cast<uint2 *>(kr[0]) = *reinterpret_cast<const uint2 *>(k_tile + k_off);
+      *reinterpret_cast<uint2 *>(kr[1]) = *reinterpret_cast<const uint2 *>(k_tile + k_off + kEight);
+    }
 #pragma unroll
     for (int i = 0; i < KW / 4; ++i) {
       const uint8_t *at = k_tile + (i >> 1) * 2048 + (i & 1 ? k_off ^ 64 : k_off);
@@ -513,12 +593,34 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
       const float *s = scales + stage * 32 + mine;
       ksc[0] = s[0], ksc[1] = s[8], vsc[0] = s[16], vsc[1] = s[24];
     }
+    Int4Factors k_lo4, k_hi4;
+    uint32_t vf[2], minus_24vf[2];                  // of keys 2 q4 and odd, and 8 after them
+    if constexpr (kInt4) {
+      constexpr int kGroups = D / kFactorGroup;
+      const uint8_t *f = factors + stage * 2 * Shape::kFactorTile + q4 * (D / 4) / kFactorGroup;
+      uint32_t two;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(two) : "h"(uint16_t(f[mine * kGroups] | (f[(mine + 8) * kGroups] << 8))));
+      k_lo4 = int4_factors(__byte_perm(two, two, 0x1010));
+      k_hi4 = int4_factors(__byte_perm(two, two, 0x3232));
+      f = factors + (stage * 2 + 1) * Shape::kFactorTile + g * (D / 8) / kFactorGroup;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        vf[h] = factor_pair_bf16(f[(2 * q4 + 8 * h) * kGroups], f[(odd + 8 * h) * kGroups], minus_24vf[h]);
+    }
     float sc[kNT][4] = {};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       uint32_t af[4];
       if constexpr (kBf16) {
         af[0] = kr[0][2 * s], af[1] = kr[1][2 * s], af[2] = kr[0][2 * s + 1], af[3] = kr[1][2 * s + 1];
+      } else if constexpr (kInt4) {
+        if (s & 1) {
+          int4_to_half<1>(kr[0][s / 2], k_lo4, af[0], af[2]);
+          int4_to_half<1>(kr[1][s / 2], k_hi4, af[1], af[3]);
+        } else {
+          int4_to_half<0>(kr[0][s / 2], k_lo4, af[0], af[2]);
+          int4_to_half<0>(kr[1][s / 2], k_hi4, af[1], af[3]);
+        }
       } else {
         codes_to_half<kFormat>(kr[0][s], af[0], af[2]);
         codes_to_half<kFormat>(kr[1][s], af[1], af[3]);
@@ -535,7 +637,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const uint8_t *at = v_tile + (x & 1 ? v_odd : v_even) + (x >> 1) * kEight;
-      if constexpr (VW == 2) {
+      if constexpr (VW == 1) {
+        vr[x][0] = *reinterpret_cast<const uint32_t *>(at);
+      } else if constexpr (VW == 2) {
         *reinterpret_cast<uint2 *>(vr[x]) = *reinterpret_cast<const uint2 *>(at);
       } else {
 #pragma unroll
@@ -605,6 +709,24 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
 #pragma unroll
           for (int t = 0; t < kNT; ++t)
             mma_bf16_16816(o[t][j], af, pp[t][0], pp[t][1]);
+        } else if constexpr (kInt4) {
+          // Channels 0-3 of the two keys in one word, 4-7 in the next.
+          uint32_t af[4][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)      // keys 2 q4 .. and 2 q4 + 8 ..
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t x = __byte_perm(vr[2 * h][j], vr[2 * h + 1][j], c ? 0x7632 : 0x5410);
+              af[2 * c][2 * h] = int4_to_bf16<0>(x, vf[h], minus_24vf[h]);
+              af[2 * c][2 * h + 1] = int4_to_bf16<1>(x, vf[h], minus_24vf[h]);
+              af[2 * c + 1][2 * h] = int4_to_bf16<2>(x, vf[h], minus_24vf[h]);
+              af[2 * c + 1][2 * h + 1] = int4_to_bf16<3>(x, vf[h], minus_24vf[h]);
+            }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < kNT; ++t)
+              mma_bf16_16816(o[t][4 * j + i], af[i], pp[t][0], pp[t][1]);
         } else {
           uint32_t af[2][4];
 #pragma unroll

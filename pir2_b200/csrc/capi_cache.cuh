@@ -57,10 +57,12 @@ static int make_pages(const char *what, const pir2b_kv_pages *p, const pir2b_seq
     return fail(PIR2B_EINVAL, "%s: page_size must be 16, 32, 64 or 128", what);
   if (p->head_dim != 64 && p->head_dim != 128)
     return fail(PIR2B_EINVAL, "%s: head_dim must be 64 or 128", what);
-  if (p->format != PIR2B_CACHE_BF16 && p->format != PIR2B_CACHE_INT8 && p->format != PIR2B_CACHE_E4M3)
+  if (p->format != PIR2B_CACHE_BF16 && p->format != PIR2B_CACHE_INT8 && p->format != PIR2B_CACHE_E4M3 &&
+      p->format != PIR2B_CACHE_INT4)
     return fail(PIR2B_EINVAL, "%s: unknown cache format %d", what, p->format);
   const int64_t tokens = int64_t(p->kv_heads) * p->page_size;
-  if (p->k_page_stride < tokens * p->head_dim || p->v_page_stride < tokens * p->head_dim)
+  const int64_t row = p->format == PIR2B_CACHE_INT4 ? p->head_dim / 2 : p->head_dim;   // elements of a row
+  if (p->k_page_stride < tokens * row || p->v_page_stride < tokens * row)
     return fail(PIR2B_EINVAL, "%s: page strides below a page's size", what);
   if (!aligned(p->k, 16) || !aligned(p->v, 16) || p->k_page_stride % 16 != 0 || p->v_page_stride % 16 != 0)
     return fail(PIR2B_EALIGN, "%s: pages must be 16-byte aligned", what);
@@ -68,7 +70,18 @@ static int make_pages(const char *what, const pir2b_kv_pages *p, const pir2b_seq
       (p->k_scale == nullptr || p->v_scale == nullptr || !aligned(p->k_scale, 16) || !aligned(p->v_scale, 16) ||
        p->k_scale_page_stride < tokens || p->v_scale_page_stride < tokens || p->k_scale_page_stride % 4 != 0 ||
        p->v_scale_page_stride % 4 != 0))
-    return fail(PIR2B_EINVAL, "%s: 8-bit pages need 16-byte aligned fp32 scales", what);
+    return fail(PIR2B_EINVAL, "%s: quantised pages need 16-byte aligned fp32 scales", what);
+  if (p->format == PIR2B_CACHE_INT4) {
+    const int64_t factors = tokens * (p->head_dim / kFactorGroup);
+    if (p->k_factor == nullptr || p->v_factor == nullptr || !aligned(p->k_factor, 16) || !aligned(p->v_factor, 16) ||
+        p->k_factor_page_stride < factors || p->v_factor_page_stride < factors || p->k_factor_page_stride % 16 != 0 ||
+        p->v_factor_page_stride % 16 != 0)
+      return fail(PIR2B_EINVAL, "%s: int4 pages need 16-byte aligned factors", what);
+    out->kf = p->k_factor;
+    out->vf = p->v_factor;
+    out->kf_page = p->k_factor_page_stride;
+    out->vf_page = p->v_factor_page_stride;
+  }
   out->k = p->k;
   out->v = p->v;
   out->ks = p->k_scale;
@@ -135,6 +148,7 @@ static int launch_rows(bool write, int format, int d, const CacheRowsArgs &a, vo
   switch (format) {
   case kCacheInt8: return launch_rows<kCacheInt8>(write, d, a, stream);
   case kCacheE4m3: return launch_rows<kCacheE4m3>(write, d, a, stream);
+  case kCacheInt4: return launch_rows<kCacheInt4>(write, d, a, stream);
   default: return launch_rows<kCacheBf16>(write, d, a, stream);
   }
 }
@@ -193,8 +207,8 @@ static FewPlan plan_few(int64_t rows, int hq, int hk, int batch, int64_t positio
 }
 
 // 4-D map over pages [pages, hk, page, d], box of `rows` rows of one head: 64
-// columns of bf16 or whole rows of codes, swizzled over the row's 128 or 64
-// bytes or as they lie.
+// columns of bf16 or whole rows of codes (d: elements of a row in memory),
+// swizzled over the row's 128 or 64 bytes or as they lie.
 static int make_pages_map(CUtensorMap *map, const void *base, const CachePages &c, int d, int64_t page_stride, int bytes,
                           int rows, bool swizzled) {
   EncodeTiledFn fn = encode_fn();
@@ -228,11 +242,11 @@ static bool by_length(const RaggedArgs &a, int64_t grid, int resident, int parts
 template <int kFormat, int D, int kNT>
 static int launch_attention_few(const FewPlan &p, RaggedArgs a, void *stream) {
   a.ordered = by_length(a, p.grid, FewShape<kFormat, D, kNT>::kCtas, std::max(p.cluster, 1));
-  constexpr int kBytes = kFormat == kCacheBf16 ? 2 : 1;
+  constexpr int kBytes = kFormat == kCacheBf16 ? 2 : 1, kWide = code_bytes(kFormat, D) / kBytes;
   CUtensorMap tm_k, tm_v;
-  if (int r = make_pages_map(&tm_k, a.c.k, a.c, D, a.c.k_page, kBytes, 16, true))
+  if (int r = make_pages_map(&tm_k, a.c.k, a.c, kWide, a.c.k_page, kBytes, 16, kWide > 32))
     return r;
-  if (int r = make_pages_map(&tm_v, a.c.v, a.c, D, a.c.v_page, kBytes, 16, true))
+  if (int r = make_pages_map(&tm_v, a.c.v, a.c, kWide, a.c.v_page, kBytes, 16, kWide > 32))
     return r;
   return launch_cache("cache_attention launch", attention_few_kernel<kFormat, D, kNT>, p.grid, 1, std::max(p.cluster, 1), kFewWarps * 32,
                       FewShape<kFormat, D, kNT>::kSmem, stream, a, tm_k, tm_v);
@@ -311,7 +325,7 @@ struct CachePlan {
 static CachePlan plan_cache(int64_t rows, int hq, int hk, int d, int batch, int64_t positions, int format, int sms) {
   CachePlan p = {};
   const int64_t per_sequence = (rows + batch - 1) / batch * (hq / hk);
-  if (per_sequence <= (format == kCacheBf16 ? kFewRowsBf16 : kFewRows8Bit)) {
+  if (format == kCacheInt4 || per_sequence <= (format == kCacheBf16 ? kFewRowsBf16 : kFewRows8Bit)) {
     p.few = plan_few(rows, hq, hk, batch, positions, format, d, sms);
     return p;
   }
@@ -345,9 +359,11 @@ static int launch_cache_tile(const CachePlan &p, RaggedArgs a, void *stream) {
 
 template <int kFormat>
 static int launch_cache_attention(const CachePlan &p, int d, const RaggedArgs &a, void *stream) {
-  if (p.tiles == 0)
+  if (p.tiles == 0 || kFormat == kCacheInt4)
     return launch_attention_few<kFormat>(p.few, d, a, stream);
-  return d == 64 ? launch_cache_tile<kFormat, 64>(p, a, stream) : launch_cache_tile<kFormat, 128>(p, a, stream);
+  if constexpr (kFormat != kCacheInt4)
+    return d == 64 ? launch_cache_tile<kFormat, 64>(p, a, stream) : launch_cache_tile<kFormat, 128>(p, a, stream);
+  return PIR2B_OK;
 }
 
 static int launch_join(const CachePlan &p, int d, const RaggedArgs &a, void *stream) {
@@ -378,6 +394,10 @@ static int cache_kernel_attributes(DeviceInfo *dev) {
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 64, 2>), FewShape<kCacheE4m3, 64, 2>::kSmem},
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 128, 1>), FewShape<kCacheE4m3, 128, 1>::kSmem},
       {reinterpret_cast<const void *>(attention_few_kernel<kCacheE4m3, 128, 2>), FewShape<kCacheE4m3, 128, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheInt4, 64, 1>), FewShape<kCacheInt4, 64, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheInt4, 64, 2>), FewShape<kCacheInt4, 64, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheInt4, 128, 1>), FewShape<kCacheInt4, 128, 1>::kSmem},
+      {reinterpret_cast<const void *>(attention_few_kernel<kCacheInt4, 128, 2>), FewShape<kCacheInt4, 128, 2>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 64, 1>), TileShape<kSourceRows, 64, 1>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 128, 1>), TileShape<kSourceRows, 128, 1>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kSourceRows, 128, 2>), TileShape<kSourceRows, 128, 2>::kSmem},
@@ -573,6 +593,7 @@ int pir2b_cache_attention(const void *q, int64_t q_row, int64_t q_head, int64_t 
   switch (pages->format) {
   case kCacheInt8: status = launch_cache_attention<kCacheInt8>(plan, d, a, stream); break;
   case kCacheE4m3: status = launch_cache_attention<kCacheE4m3>(plan, d, a, stream); break;
+  case kCacheInt4: status = launch_cache_attention<kCacheInt4>(plan, d, a, stream); break;
   default: status = launch_cache_attention<kCacheBf16>(plan, d, a, stream); break;
   }
   return status != PIR2B_OK || !plan.joined() ? status : launch_join(plan, d, a, stream);

@@ -11,16 +11,34 @@
 // nearest E4M3 number.  An infinity becomes the largest code.  A row with a
 // NaN gets codes of 0 and the NaN as its scale, so every reader of the row
 // sees it and the codes themselves are always numbers.
+//
+// int4 rows are codes of -7..7, two to a byte (the even channel in the low
+// bits, two's complement), an E4M3 factor for every 32 channels and the row's
+// fp32 scale: value = code * factor * scale, the first product exact in bf16.
+// With m the row's largest finite magnitude, s = 2^(floor(log2 m) - 10), at
+// least 2^-126, 1 for a row of zeros; f = E4M3(m_group / s / 7); code = v / s /
+// f rounded to nearest even and clamped, 0 where f is 0.  s is a power of two
+// so that the quotients are those of numbers of 8 and of 4 bits, which lie on a
+// border of the rounding or far from it: any exact division gives these codes.
+// m / s is below 2048, so f is below 304.  An infinity counts as m; a row with
+// a NaN gets codes and factors of 0 and the NaN as its scale.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cstdint>
 #include "args.cuh"
+#include "attention.cuh"
 #include "ptx.cuh"
 
 namespace pir2b {
 
-constexpr int kCacheBf16 = 16, kCacheInt8 = 8, kCacheE4m3 = 9;
+constexpr int kCacheBf16 = 16, kCacheInt8 = 8, kCacheE4m3 = 9, kCacheInt4 = 24;
+constexpr int kFactorGroup = 32;   // channels of an int4 row that share a factor
+
+// Bytes of d channels' codes.
+__host__ __device__ constexpr int code_bytes(int format, int d) {
+  return format == kCacheBf16 ? 2 * d : format == kCacheInt4 ? d / 2 : d;
+}
 
 // Codes of bad device-side indices (a page outside the pool, a position
 // outside the table): the access is skipped and the status word records it.
@@ -30,9 +48,10 @@ __device__ __forceinline__ void record_status(int code) { atomicCAS(&g_device_st
 
 struct CachePages {
   void *k, *v;             // [pages, hk, page, D] codes
-  float *ks, *vs;          // [pages, hk, page] scales (8-bit formats)
-  int64_t k_page, v_page;  // elements from one page to the next
-  int64_t ks_page, vs_page;
+  float *ks, *vs;          // [pages, hk, page] scales (quantised formats)
+  uint8_t *kf, *vf;        // [pages, hk, page, D / 32] factors (int4)
+  int64_t k_page, v_page;  // elements (int4: bytes) from one page to the next
+  int64_t ks_page, vs_page, kf_page, vf_page;
   const int *table;        // [batch, width] page of each block of positions
   int64_t ldt;             // table row stride
   int width;               // table columns
@@ -162,6 +181,62 @@ __device__ __noinline__ uint2 quantise8_any(uint4 x, float s) {
   return make_uint2(out[0], out[1]);
 }
 
+// Scale of an int4 row whose largest finite magnitude has the bits m (a bf16's;
+// a NaN's give a NaN).
+__device__ __forceinline__ float int4_scale(uint32_t m) {
+  if (m > 0x7f80u)
+    return __uint_as_float(m << 16);
+  return m == 0 ? 1.f : __uint_as_float(uint32_t(max(int(m >> 7) - 10, 1)) << 23);
+}
+
+// E4M3 factor of a group whose largest magnitude has the bits m, in the low byte.
+__device__ __forceinline__ uint32_t int4_factor(uint32_t m, float inverse) {
+  return e4m3_pair(__fdiv_rn(__uint_as_float(m << 16) * inverse, 7.f), 0.f) & 0xffu;
+}
+
+__device__ __forceinline__ float e4m3_value(uint32_t code) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(code)));
+  return __half2float(__ushort_as_half(uint16_t(h)));
+}
+
+// Eight finite bf16 -> eight 4-bit codes.  quotients() is exact here: all 2^10
+// pairs of significands give the integer of the true quotient (a test compares
+// them).  A pair of codes, 8 added to each, is one small number's low byte.
+__device__ __forceinline__ uint32_t quantise8_int4(const uint4 &x, float inverse, float f) {
+  const float rf = f == 0.f ? 0.f : __frcp_rn(f);
+  const float2 inv = make_float2(inverse, inverse), minus_f = make_float2(-f, -f), rr = make_float2(rf, rf);
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t pair[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 q = quotients(__fmul2_rn(bf16_pair(w[i]), inv), minus_f, rr);
+    q.x = fminf(fmaxf(q.x, -7.f), 7.f), q.y = fminf(fmaxf(q.y, -7.f), 7.f);
+    // 1.5 * 2^23 + 8: rounds to an integer, to even as it is even itself.
+    q = __fadd2_rn(__fadd2_rn(q, make_float2(12582920.f, 12582920.f)), make_float2(-12582912.f, -12582912.f));
+    pair[i] = __float_as_uint(__fmaf_rn(q.y, 16.f, q.x) + 12582912.f);
+  }
+  return __byte_perm(__byte_perm(pair[0], pair[1], 0x0040), __byte_perm(pair[2], pair[3], 0x0040), 0x5410) ^ 0x88888888u;
+}
+
+// Infinities of a piece as the magnitude m with their sign.
+__device__ __noinline__ uint4 bounded8(uint4 x, uint32_t m) {
+  uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  for (int i = 0; i < 8; ++i) {
+    const int at = (i & 1) * 16;
+    if (((w[i >> 1] >> at) & 0x7fffu) == 0x7f80u)
+      w[i >> 1] = (w[i >> 1] & ~(0x7fffu << at)) | (m << at);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Eight 4-bit codes times their factor as fp32 values.
+__device__ __forceinline__ void int4_values(uint32_t w, float f, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    v[i] = float(int32_t(w << (28 - 4 * i)) >> 28) * f;
+}
+
 // Two 8-bit codes (the low 16 bits of `pair`) as fp32 values.
 template <int kFormat>
 __device__ __forceinline__ float2 code_values(uint32_t pair) {
@@ -247,6 +322,43 @@ __global__ void __launch_bounds__(kCacheWarps * 32) cache_write_kernel(const Cac
         *reinterpret_cast<uint4 *>(to) = x[i][0];
         *reinterpret_cast<uint4 *>(to + kLanes * 8) = x[i][1];
       }
+    } else if constexpr (kFormat == kCacheInt4) {
+      // Four lanes' pieces are a group; a row's scale is that of all its groups.
+      uint32_t mg[2] = {magnitude8(x[i][0]), magnitude8(x[i][1])};
+      const bool odd = __any_sync(0xffffffffu, max(mg[0], mg[1]) >= 0x7f80u);   // an infinity or a NaN in some row
+      if (odd) {
+        mg[0] = magnitude8_finite(x[i][0]), mg[1] = magnitude8_finite(x[i][1]);
+      }
+      uint32_t m = max(mg[0], mg[1]);
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1)
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float s = int4_scale(m);
+      if (odd) {
+        if (m > 0x7f80u)
+          x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
+        x[i][0] = bounded8(x[i][0], m), x[i][1] = bounded8(x[i][1], m);
+        mg[0] = magnitude8(x[i][0]), mg[1] = magnitude8(x[i][1]);
+      }
+#pragma unroll
+      for (int o = 2; o > 0; o >>= 1) {
+        mg[0] = max(mg[0], __shfl_xor_sync(0xffffffffu, mg[0], o));
+        mg[1] = max(mg[1], __shfl_xor_sync(0xffffffffu, mg[1], o));
+      }
+      const float inverse = m > 0x7f80u ? 1.f : __uint_as_float(0x7f000000u - __float_as_uint(s));   // 1 / s
+      const uint32_t f0 = int4_factor(mg[0], inverse), f1 = int4_factor(mg[1], inverse);
+      const uint32_t q0 = quantise8_int4(x[i][0], inverse, e4m3_value(f0)), q1 = quantise8_int4(x[i][1], inverse, e4m3_value(f1));
+      if (r < 2 * hk) {
+        uint8_t *to = static_cast<uint8_t *>(r < hk ? a.c.k : a.c.v) + (r < hk ? k_at : v_at) + (slot * (D / 2) + l * 4);
+        *reinterpret_cast<uint32_t *>(to) = q0;
+        *reinterpret_cast<uint32_t *>(to + kLanes * 4) = q1;
+        if (l % 4 == 0) {
+          uint8_t *factor = (r < hk ? a.c.kf + page * a.c.kf_page : a.c.vf + page * a.c.vf_page) + slot * (D / kFactorGroup) + l / 4;
+          factor[0] = uint8_t(f0), factor[kLanes / 4] = uint8_t(f1);
+        }
+        if (l == 0)
+          (r < hk ? k_scale : v_scale)[slot] = s;
+      }
     } else {
       uint32_t m = max(magnitude8(x[i][0]), magnitude8(x[i][1]));
 #pragma unroll
@@ -302,17 +414,25 @@ __global__ void __launch_bounds__(kCacheWarps * 32) cache_read_kernel(const Cach
   for (int r0 = 0; r0 < 2 * hk; r0 += kRows * kFlight) {
     uint4 x[kFlight];
     float s[kFlight];
+    uint32_t factor[kFlight];
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
       const int r = r0 + i * kRows + lane / kLanes, head = r < hk ? r : r - hk;
       const int64_t slot = (int64_t(head) << a.c.shift) + in_page;
-      const int64_t at = page * (r < hk ? a.c.k_page : a.c.v_page) + slot * D + l * 8;
+      const int64_t at = page * (r < hk ? a.c.k_page : a.c.v_page) +
+                         (kFormat == kCacheInt4 ? slot * (D / 2) + l * 4 : slot * D + l * 8);
       x[i] = make_uint4(0, 0, 0, 0);
       s[i] = 0.f;
+      factor[i] = 0;
       if (r < 2 * hk && page >= 0) {
         const void *codes = r < hk ? a.c.k : a.c.v;
         if constexpr (kFormat == kCacheBf16) {
           x[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(codes) + at));
+        } else if constexpr (kFormat == kCacheInt4) {
+          x[i].x = __ldg(reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(codes) + at));
+          factor[i] = __ldg((r < hk ? a.c.kf + page * a.c.kf_page : a.c.vf + page * a.c.vf_page) +
+                            slot * (D / kFactorGroup) + l / 4);
+          s[i] = __ldg((r < hk ? a.c.ks + page * a.c.ks_page : a.c.vs + page * a.c.vs_page) + slot);
         } else {
           const uint2 q = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(codes) + at));
           x[i].x = q.x, x[i].y = q.y;
@@ -324,7 +444,12 @@ __global__ void __launch_bounds__(kCacheWarps * 32) cache_read_kernel(const Cach
     for (int i = 0; i < kFlight; ++i) {
       const int r = r0 + i * kRows + lane / kLanes, head = r < hk ? r : r - hk;
       uint4 y = x[i];
-      if constexpr (kFormat != kCacheBf16) {
+      if constexpr (kFormat == kCacheInt4) {
+        float f[8];
+        int4_values(x[i].x, e4m3_value(factor[i]), f);
+        y = make_uint4(pack_bf16x2(f[0] * s[i], f[1] * s[i]), pack_bf16x2(f[2] * s[i], f[3] * s[i]),
+                       pack_bf16x2(f[4] * s[i], f[5] * s[i]), pack_bf16x2(f[6] * s[i], f[7] * s[i]));
+      } else if constexpr (kFormat != kCacheBf16) {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

@@ -7,7 +7,8 @@ transformers' "sdpa" attention without one, coexecution/optimization/groot/
 vlm.py:312-313).  These serve several robots whose prompts differ in length
 and grow afterwards: each sequence owns pages of a shared pool, in bf16, or
 as int8 / E4M3 codes with one fp32 scale per token and head (the arithmetic
-of the symmetric-row-v1 activation pack).
+of the symmetric-row-v1 activation pack), or in 4 bits: codes of -7..7, an E4M3
+factor for every 32 channels and one power of two per token and head.
 """
 
 import ctypes
@@ -18,60 +19,83 @@ from . import _lib
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
-FORMATS = {torch.bfloat16: _lib.CACHE_BF16, torch.int8: _lib.CACHE_INT8, torch.float8_e4m3fn: _lib.CACHE_E4M3}
+FORMATS = {
+    torch.bfloat16: _lib.CACHE_BF16, torch.int8: _lib.CACHE_INT8, torch.float8_e4m3fn: _lib.CACHE_E4M3,
+    torch.uint8: _lib.CACHE_INT4,
+}
+FACTOR_GROUP = 32   # channels of a 4-bit row that share a factor
 
 
 class KVPages:
     """One layer's pool: k, v [pages, kv_heads, page_size, head_dim] of one
-    dtype (bfloat16, int8 or float8_e4m3fn) and, for the 8-bit ones, fp32
-    scales [pages, kv_heads, page_size].  Pages may lie apart (any stride of
-    the first dimension, so that all layers share one allocation); inside a
-    page everything is contiguous."""
+    dtype (bfloat16, int8 or float8_e4m3fn; uint8 [..., head_dim / 2] holds 4-bit
+    codes, the even channel in the low bits) and, for the quantised ones, fp32
+    scales [pages, kv_heads, page_size]; 4-bit pages also have factors,
+    float8_e4m3fn [pages, kv_heads, page_size, head_dim / 32].  Pages may lie
+    apart (any stride of the first dimension, so that all layers share one
+    allocation); inside a page everything is contiguous."""
 
-    def __init__(self, k, v, k_scale=None, v_scale=None):
+    def __init__(self, k, v, k_scale=None, v_scale=None, k_factor=None, v_factor=None):
         if k.ndim != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in FORMATS:
-            raise ValueError("KVPages: k and v must be [pages, kv_heads, page_size, head_dim] bf16, int8 or float8_e4m3fn")
-        pages, heads, size, dim = k.shape
+            raise ValueError("KVPages: k and v must be [pages, kv_heads, page_size, head_dim] bf16, int8 or float8_e4m3fn, or uint8 of 4-bit codes")
+        pages, heads, size, wide = k.shape
+        packed = k.dtype == torch.uint8
+        dim = 2 * wide if packed else wide
         if pages < 1 or heads < 1 or size not in PAGE_SIZES or dim not in HEAD_DIMS:
             raise ValueError(f"KVPages: page_size must be one of {PAGE_SIZES} and head_dim one of {HEAD_DIMS}")
         quantised = k.dtype != torch.bfloat16
         if quantised != (k_scale is not None) or quantised != (v_scale is not None):
-            raise ValueError("KVPages: 8-bit pages need k_scale and v_scale, bf16 pages take none")
-        tensors = [k, v] + ([k_scale, v_scale] if quantised else [])
+            raise ValueError("KVPages: 8-bit and 4-bit pages need k_scale and v_scale, bf16 pages take none")
+        if packed != (k_factor is not None) or packed != (v_factor is not None):
+            raise ValueError("KVPages: 4-bit pages need k_factor and v_factor, others take none")
+        tensors = [k, v] + ([k_scale, v_scale] if quantised else []) + ([k_factor, v_factor] if packed else [])
         if any(not t.is_cuda or t.device != k.device for t in tensors):
             raise ValueError("KVPages: all tensors must be on one CUDA device")
         for t in (k, v):
-            if t.stride()[1:] != (size * dim, dim, 1) or (pages > 1 and t.stride(0) < heads * size * dim):
+            if t.stride()[1:] != (size * wide, wide, 1) or (pages > 1 and t.stride(0) < heads * size * wide):
                 raise ValueError("KVPages: pages must be contiguous and apart")
-        for t in tensors[2:]:
+        for t in tensors[2:4]:
             if t.shape != (pages, heads, size) or t.dtype != torch.float32:
                 raise ValueError("KVPages: scales must be fp32 [pages, kv_heads, page_size]")
             if t.stride()[1:] != (size, 1) or (pages > 1 and t.stride(0) < heads * size):
                 raise ValueError("KVPages: scales of a page must be contiguous and apart")
+        groups = dim // FACTOR_GROUP
+        for t in tensors[4:]:
+            if t.shape != (pages, heads, size, groups) or t.dtype != torch.float8_e4m3fn:
+                raise ValueError("KVPages: factors must be float8_e4m3fn [pages, kv_heads, page_size, head_dim / 32]")
+            if t.stride()[1:] != (size * groups, groups, 1) or (pages > 1 and t.stride(0) < heads * size * groups):
+                raise ValueError("KVPages: factors of a page must be contiguous and apart")
 
         def apart(t, size_of_page):
             return t.stride(0) if pages > 1 else size_of_page
 
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.k_factor, self.v_factor = k_factor, v_factor
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, dim
         self.dtype, self.device, self.index = k.dtype, k.device, k.get_device()
         self.struct = _lib.KVPagesStruct(
             k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if quantised else None,
-            v_scale.data_ptr() if quantised else None, apart(k, heads * size * dim), apart(v, heads * size * dim),
+            v_scale.data_ptr() if quantised else None, apart(k, heads * size * wide), apart(v, heads * size * wide),
             apart(k_scale, heads * size) if quantised else 0, apart(v_scale, heads * size) if quantised else 0,
             pages, size, heads, dim, FORMATS[k.dtype],
+            k_factor.data_ptr() if packed else None, v_factor.data_ptr() if packed else None,
+            apart(k_factor, heads * size * groups) if packed else 0, apart(v_factor, heads * size * groups) if packed else 0,
         )
         self.address = ctypes.addressof(self.struct)
         self.blank = torch.empty(0, dtype=torch.bfloat16, device=k.device)   # what reads allocate like
 
     @classmethod
     def allocate(cls, pages, kv_heads, head_dim, *, page_size=64, dtype=torch.int8, device="cuda"):
-        """A pool of its own allocation, zeroed."""
-        shape = (pages, kv_heads, page_size, head_dim)
+        """A pool of its own allocation, zeroed; dtype uint8: of 4-bit codes."""
+        packed = dtype == torch.uint8
+        shape = (pages, kv_heads, page_size, head_dim // 2 if packed else head_dim)
         k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
         if dtype == torch.bfloat16:
             return cls(k, v)
-        return cls(k, v, *(torch.ones(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
+        scales = [torch.ones(shape[:3], dtype=torch.float32, device=device) for _ in range(2)]
+        groups = (*shape[:3], head_dim // FACTOR_GROUP)
+        factors = [torch.zeros(groups, dtype=torch.float8_e4m3fn, device=device) for _ in range(2 if packed else 0)]
+        return cls(k, v, *scales, *factors)
 
 
 class Sequences:

@@ -20,24 +20,24 @@ from functools import partial
 import torch
 
 from . import ops
-from .kv_cache import KVPages, Sequences
+from .kv_cache import FACTOR_GROUP, KVPages, Sequences
 from .transformer import _MODE_BITS
 
 
 class TextCache:
     """Pools of `layers` layers in one allocation ([pages, layers, 2, kv_heads,
-    page_size, head_dim]) and the pages of up to `batch` sequences of at most
+    page_size, head_dim]; dtype uint8: two 4-bit codes to a byte) and the pages of up to `batch` sequences of at most
     `max_tokens` tokens."""
 
     def __init__(self, layers, pages, kv_heads, head_dim, *, batch, max_tokens, page_size=64, dtype=torch.int8, device="cuda"):
-        shape = (pages, layers, 2, kv_heads, page_size, head_dim)
+        packed = dtype == torch.uint8
+        shape = (pages, layers, 2, kv_heads, page_size, head_dim // 2 if packed else head_dim)
         self.codes = torch.zeros(shape, dtype=dtype, device=device)
         self.scales = None if dtype == torch.bfloat16 else torch.ones(shape[:-1], dtype=torch.float32, device=device)
+        groups = (*shape[:-1], head_dim // FACTOR_GROUP)
+        self.factors = torch.zeros(groups, dtype=torch.float8_e4m3fn, device=device) if packed else None
         self.layers = [
-            KVPages(
-                self.codes[:, i, 0], self.codes[:, i, 1],
-                *(() if self.scales is None else (self.scales[:, i, 0], self.scales[:, i, 1])),
-            )
+            KVPages(*(t[:, i, which] for t in (self.codes, self.scales, self.factors) if t is not None for which in (0, 1)))
             for i in range(layers)
         ]
         self.page_size, self.batch = page_size, batch
