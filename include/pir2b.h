@@ -478,6 +478,26 @@ int pir2b_cache_write(const void *k, int64_t k_row, int64_t k_head, const void *
                       int64_t v_head, int64_t rows, const pir2b_kv_pages *pages,
                       const pir2b_sequences *sequences, void *stream);
 
+/* Norm, rotation and cache write of new tokens in one pass.  qkv: bf16 [rows, hq
+ * + 2 kv_heads, head_dim] view, the heads of q, k and v (a merged projection).
+ * Each q and k head row x becomes x / sqrt(mean x^2 + eps) * weight (bf16
+ * [head_dim]; without a norm where the weight is null) and is turned by its
+ * position: channel pairs (i, i + head_dim / 2) by the angles whose fp32 cosines
+ * and sines are rows of cos, sin [turns, head_dim / 2].  The position is that in
+ * the cache, or positions[row] (int32 [rows] on the device; null: none).  All in
+ * fp32 and rounded to bf16 once; k (in that rounding) and v go to the pages as
+ * pir2b_cache_write would put them, q to q_out [rows, hq, head_dim] and k, if
+ * k_out is not null, to k_out [rows, kv_heads, head_dim] (bf16, heads contiguous,
+ * row strides q_row, k_row; they may be those parts of qkv itself).  A position
+ * outside the table sets the status word to PIR2B_STATUS_BAD_POSITION; that row
+ * is not cached and its q and k are unspecified. */
+#define PIR2B_STATUS_BAD_POSITION 0x202
+int pir2b_cache_append(const void *qkv, int64_t row, int64_t head, int64_t rows, int hq,
+                       const void *q_weight, const void *k_weight, float eps, const float *cos,
+                       const float *sin, int64_t turns, const int32_t *positions,
+                       const pir2b_kv_pages *pages, const pir2b_sequences *sequences, void *q_out,
+                       int64_t q_row, void *k_out, int64_t k_row, void *stream);
+
 /* Reads positions 0, 1, ... of each sequence back as bf16(code * scale) (int4:
  * bf16(code * factor * scale), rounded once), into
  * contiguous k_out, v_out [rows, kv_heads, head_dim]: starts gives the packed

@@ -23,6 +23,7 @@ OUT_FP8_VALUES = 32   # FP8 producers' first pass: bf16 values + fp32 row maxima
 STATUS_TIMEOUT_PROBE = 0x105   # device status word left by pir2b_wait_probe
 
 STATUS_BAD_PAGE = 0x201        # device status word left by an index outside a K/V pool or table
+STATUS_BAD_POSITION = 0x202    # ... by a position outside a rotation table
 CACHE_BF16, CACHE_INT8, CACHE_E4M3, CACHE_INT4 = 16, 8, 9, 24
 
 _P = ctypes.c_void_p
@@ -86,6 +87,9 @@ SIGNATURES = {
         _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _I, _I, _F, _P, _I64, _P,
     ],
     "pir2b_cache_write": [_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P],
+    "pir2b_cache_append": [
+        _P, _I64, _I64, _I64, _I, _P, _P, _F, _P, _P, _I64, _P, _P, _P, _P, _I64, _P, _I64, _P,
+    ],
     "pir2b_cache_read": [_P, _P, _I64, _P, _P, _P],
     "pir2b_cache_attention": [_P, _I64, _I64, _I64, _I, _P, _P, _F, _P, _I64, _P, _P],
     "pir2b_cache_attention_workspace": [_I64, _I, _P, _P],

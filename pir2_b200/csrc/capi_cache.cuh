@@ -153,6 +153,22 @@ static int launch_rows(bool write, int format, int d, const CacheRowsArgs &a, vo
   }
 }
 
+// Few tokens are spread over more warps, as in launch_rows.
+template <int kFormat, int D>
+static int launch_append(const CacheAppendArgs &a, void *stream) {
+  constexpr int kRows = 32 / (D / 8);
+  const int64_t grid = (a.rows + kCacheWarps - 1) / kCacheWarps;
+  const int loads = (a.hq + 2 * a.c.hk + kRows - 1) / kRows;
+  if (a.rows * loads <= 4096)
+    return launch_cache("cache_append launch", cache_append_kernel<kFormat, D, 1>, grid, loads, 1, kCacheWarps * 32, 0, stream, a);
+  return launch_cache("cache_append launch", cache_append_kernel<kFormat, D, 4>, grid, 1, 1, kCacheWarps * 32, 0, stream, a);
+}
+
+template <int kFormat>
+static int launch_append(int d, const CacheAppendArgs &a, void *stream) {
+  return d == 64 ? launch_append<kFormat, 64>(a, stream) : launch_append<kFormat, 128>(a, stream);
+}
+
 // Rows a sequence has in a kv head up to which the few-row kernel takes it; it
 // reads the keys once per 16 rows, the tile kernel once per 128 or 256.  Over
 // 1000 tokens of 64 sequences: 16 rows 50 us against 55 (bf16) and 50 against
@@ -511,6 +527,64 @@ int pir2b_cache_write(const void *k, int64_t k_row, int64_t k_head, const void *
   a.batch = sequences->batch;
   a.rows = rows;
   return launch_rows(true, pages->format, pages->head_dim, a, stream);
+}
+
+int pir2b_cache_append(const void *qkv, int64_t row, int64_t head, int64_t rows, int hq,
+                       const void *q_weight, const void *k_weight, float eps, const float *cos,
+                       const float *sin, int64_t turns, const int32_t *positions,
+                       const pir2b_kv_pages *pages, const pir2b_sequences *sequences, void *q_out,
+                       int64_t q_row, void *k_out, int64_t k_row, void *stream) {
+  const char *what = "cache_append";
+  CacheAppendArgs a = {};
+  if (int r = check_sequences(what, sequences, rows, true))
+    return r;
+  if (int r = make_pages(what, pages, sequences, &a.c))
+    return r;
+  if (hq < 1 || hq > 1024)
+    return fail(PIR2B_EINVAL, "cache_append: 1 to 1024 query heads");
+  if (!(eps >= 0.f) || !(eps < 3.0e38f))
+    return fail(PIR2B_EINVAL, "cache_append: eps must be finite and not negative");
+  if (cos == nullptr || sin == nullptr || turns < 1)
+    return fail(PIR2B_EINVAL, "cache_append needs cos and sin of at least one position");
+  if (!aligned(cos, 16) || !aligned(sin, 16) || !aligned(q_weight, 8) || !aligned(k_weight, 8))
+    return fail(PIR2B_EALIGN, "cache_append: cos and sin must be 16-byte, norm weights 8-byte aligned");
+  if (rows == 0)
+    return PIR2B_OK;
+  if (int r = check_view("cache_append qkv", qkv, row, head))
+    return r;
+  if (int r = check_out("cache_append q", q_out, q_row, int64_t(hq) * pages->head_dim))
+    return r;
+  if (k_out != nullptr)
+    if (int r = check_out("cache_append k", k_out, k_row, int64_t(pages->kv_heads) * pages->head_dim))
+      return r;
+  DeviceInfo *dev = nullptr;
+  if (int r = device_info(&dev))
+    return r;
+  a.qkv = static_cast<const __nv_bfloat16 *>(qkv);
+  a.row = row;
+  a.head = head;
+  a.q_weight = static_cast<const __nv_bfloat16 *>(q_weight);
+  a.k_weight = static_cast<const __nv_bfloat16 *>(k_weight);
+  a.eps = eps;
+  a.cos = cos;
+  a.sin = sin;
+  a.turns = turns;
+  a.positions = positions;
+  a.q_out = static_cast<__nv_bfloat16 *>(q_out);
+  a.k_out = static_cast<__nv_bfloat16 *>(k_out);
+  a.q_row = q_row;
+  a.k_row = k_row;
+  a.starts = sequences->starts;
+  a.lengths = sequences->lengths;
+  a.batch = sequences->batch;
+  a.hq = hq;
+  a.rows = rows;
+  switch (pages->format) {
+  case kCacheInt8: return launch_append<kCacheInt8>(pages->head_dim, a, stream);
+  case kCacheE4m3: return launch_append<kCacheE4m3>(pages->head_dim, a, stream);
+  case kCacheInt4: return launch_append<kCacheInt4>(pages->head_dim, a, stream);
+  default: return launch_append<kCacheBf16>(pages->head_dim, a, stream);
+  }
 }
 
 int pir2b_cache_read(const pir2b_kv_pages *pages, const pir2b_sequences *sequences, int64_t rows,

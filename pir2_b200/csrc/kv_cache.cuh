@@ -200,23 +200,26 @@ __device__ __forceinline__ float e4m3_value(uint32_t code) {
   return __half2float(__ushort_as_half(uint16_t(h)));
 }
 
-// Eight finite bf16 -> eight 4-bit codes.  quotients() is exact here: all 2^10
+// Four finite bf16 -> four 4-bit codes.  quotients() is exact here: all 2^10
 // pairs of significands give the integer of the true quotient (a test compares
 // them).  A pair of codes, 8 added to each, is one small number's low byte.
-__device__ __forceinline__ uint32_t quantise8_int4(const uint4 &x, float inverse, float f) {
+__device__ __forceinline__ uint32_t quantise4_int4(uint32_t x, uint32_t y, float inverse, float f) {
   const float rf = f == 0.f ? 0.f : __frcp_rn(f);
   const float2 inv = make_float2(inverse, inverse), minus_f = make_float2(-f, -f), rr = make_float2(rf, rf);
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint32_t pair[4];
+  uint32_t pair[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float2 q = quotients(__fmul2_rn(bf16_pair(w[i]), inv), minus_f, rr);
+  for (int i = 0; i < 2; ++i) {
+    float2 q = quotients(__fmul2_rn(bf16_pair(i ? y : x), inv), minus_f, rr);
     q.x = fminf(fmaxf(q.x, -7.f), 7.f), q.y = fminf(fmaxf(q.y, -7.f), 7.f);
     // 1.5 * 2^23 + 8: rounds to an integer, to even as it is even itself.
     q = __fadd2_rn(__fadd2_rn(q, make_float2(12582920.f, 12582920.f)), make_float2(-12582912.f, -12582912.f));
     pair[i] = __float_as_uint(__fmaf_rn(q.y, 16.f, q.x) + 12582912.f);
   }
-  return __byte_perm(__byte_perm(pair[0], pair[1], 0x0040), __byte_perm(pair[2], pair[3], 0x0040), 0x5410) ^ 0x88888888u;
+  return (__byte_perm(pair[0], pair[1], 0x0040) & 0xffffu) ^ 0x8888u;
+}
+
+__device__ __forceinline__ uint32_t quantise8_int4(const uint4 &x, float inverse, float f) {
+  return quantise4_int4(x.x, x.y, inverse, f) | (quantise4_int4(x.z, x.w, inverse, f) << 16);
 }
 
 // Infinities of a piece as the magnitude m with their sign.
@@ -390,6 +393,197 @@ __global__ void __launch_bounds__(kCacheWarps * 32) cache_write_kernel(const Cac
           (r < hk ? k_scale : v_scale)[slot] = s;
       }
     }
+  }
+}
+
+// Position of a new token outside the rotation's table.
+constexpr int kStatusBadPosition = 0x202;
+
+struct CacheAppendArgs {
+  CachePages c;
+  const __nv_bfloat16 *qkv;      // [rows, hq + 2 hk, D] view
+  int64_t row, head;
+  const __nv_bfloat16 *q_weight, *k_weight;   // [D] of the heads' norms, or null
+  float eps;
+  const float *cos, *sin;        // [turns, D / 2]
+  int64_t turns;
+  const int *positions;          // [rows] rows of the table, or null: positions in the cache
+  __nv_bfloat16 *q_out, *k_out;  // [rows, hq, D], [rows, hk, D] or null
+  int64_t q_row, k_row;
+  const int *starts, *lengths;
+  int batch, hq;
+  int64_t rows;
+};
+
+// Norm, rotation and cache write of new tokens in one pass: for each head row x
+// of q and k
+//   y = x / sqrt(mean x^2 + eps) w            (where there is a weight)
+//   z = (y_a cos - y_b sin, y_b cos + y_a sin), a and b the halves of the head,
+// in fp32, each operation rounded by itself (no contraction: the values next to
+// borders of codes are then those of the same operations anywhere else), the
+// squares added within a lane, then by halves of the lanes.  z is rounded to
+// bf16; q leaves in it, and k and v are quantised from it as cache_write does.
+//
+// D / 8 lanes per head row, each with four channels of either half, so that a
+// rotation's pairs meet in a lane; a warp per token and 32 kFlight / (D / 8) of
+// its head rows at a time, all loaded before the token's place is known.
+template <int kFormat, int D, int kFlight>
+__global__ void __launch_bounds__(kCacheWarps * 32) cache_append_kernel(const CacheAppendArgs a) {
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t row = int64_t(blockIdx.x) * kCacheWarps + (threadIdx.x >> 5);
+  if (row >= a.rows)
+    return;
+  const int lane = threadIdx.x & 31, l = lane % kLanes, hk = a.c.hk, heads = a.hq + 2 * hk;
+  auto fetch = [&](int first, uint2 (&x)[kFlight][2]) {
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      const int r = first + i * kRows + lane / kLanes;
+      x[i][0] = x[i][1] = make_uint2(0, 0);
+      if (r < heads) {
+        const uint2 *src = reinterpret_cast<const uint2 *>(a.qkv + row * a.row + r * a.head) + l;
+        x[i][0] = *src;
+        x[i][1] = src[D / 8];
+      }
+    }
+  };
+  const int step = gridDim.y * kRows * kFlight;
+  int first = blockIdx.y * kRows * kFlight;
+  uint2 x[kFlight][2];
+  fetch(first, x);
+  const int b = sequence_of_warp(a.starts, a.batch, row);
+  if (b < 0)
+    return;
+  const int64_t pos = int64_t(__ldg(a.lengths + b)) - __ldg(a.starts + b + 1) + row;
+  int64_t turn = a.positions ? int64_t(__ldg(a.positions + row)) : pos;
+  const bool turned = turn >= 0 && turn < a.turns;
+  if (!turned) {
+    record_status(kStatusBadPosition);
+    turn = 0;
+  }
+  float2 cos[2], sin[2];
+  {
+    const float4 c = __ldg(reinterpret_cast<const float4 *>(a.cos + turn * (D / 2)) + l);
+    const float4 s = __ldg(reinterpret_cast<const float4 *>(a.sin + turn * (D / 2)) + l);
+    cos[0] = make_float2(c.x, c.y), cos[1] = make_float2(c.z, c.w);
+    sin[0] = make_float2(s.x, s.y), sin[1] = make_float2(s.z, s.w);
+  }
+  const int page = turned ? page_of(a.c, b, pos) : -1;
+  const int in_page = int(pos & ((1 << a.c.shift) - 1));
+  for (;;) {
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      const int r0 = first + i * kRows, r = r0 + lane / kLanes;
+      if (r0 >= heads)
+        break;
+      const bool is_q = r < a.hq, is_v = r >= a.hq + hk;
+      uint2 &lo = x[i][0], &hi = x[i][1];
+      if (r0 < a.hq + hk) {                       // some row of the warp is turned
+        float2 u[2] = {bf16_pair(lo.x), bf16_pair(lo.y)}, v[2] = {bf16_pair(hi.x), bf16_pair(hi.y)};
+        const __nv_bfloat16 *weight = is_q ? a.q_weight : a.k_weight;
+        const float2 p = __fadd2_rn(__fmul2_rn(u[0], u[0]), __fmul2_rn(v[0], v[0]));
+        const float2 q = __fadd2_rn(__fmul2_rn(u[1], u[1]), __fmul2_rn(v[1], v[1]));
+        const float2 pq = __fadd2_rn(p, q);
+        float sum = __fadd_rn(pq.x, pq.y);
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1)
+          sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
+        if (weight != nullptr) {
+          const float inv = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(sum * (1.f / D), a.eps)));
+          const float2 inv2 = make_float2(inv, inv);
+          const uint2 wl = __ldg(reinterpret_cast<const uint2 *>(weight) + l), wh = __ldg(reinterpret_cast<const uint2 *>(weight) + l + D / 8);
+          u[0] = __fmul2_rn(__fmul2_rn(u[0], inv2), bf16_pair(wl.x)), u[1] = __fmul2_rn(__fmul2_rn(u[1], inv2), bf16_pair(wl.y));
+          v[0] = __fmul2_rn(__fmul2_rn(v[0], inv2), bf16_pair(wh.x)), v[1] = __fmul2_rn(__fmul2_rn(v[1], inv2), bf16_pair(wh.y));
+        }
+        if (!is_v) {
+          uint32_t ww[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            // Single sums: a pair's would be joined with the products into FMAs.
+            const float2 uc = __fmul2_rn(u[j], cos[j]), vs = __fmul2_rn(v[j], sin[j]);
+            const float2 vc = __fmul2_rn(v[j], cos[j]), us = __fmul2_rn(u[j], sin[j]);
+            ww[j] = pack_bf16x2(__fsub_rn(uc.x, vs.x), __fsub_rn(uc.y, vs.y));
+            ww[2 + j] = pack_bf16x2(__fadd_rn(vc.x, us.x), __fadd_rn(vc.y, us.y));
+          }
+          lo = make_uint2(ww[0], ww[1]), hi = make_uint2(ww[2], ww[3]);
+          __nv_bfloat16 *to = is_q ? a.q_out + row * a.q_row + r * D : a.k_out + row * a.k_row + (r - a.hq) * D;
+          if (is_q || a.k_out != nullptr) {
+            *reinterpret_cast<uint2 *>(to + l * 4) = lo;
+            *reinterpret_cast<uint2 *>(to + D / 2 + l * 4) = hi;
+          }
+        }
+      }
+      if (r0 + kRows <= a.hq)                     // rows of q alone
+        continue;
+      const bool kept = !is_q && r < heads && page >= 0;
+      const int head = is_v ? r - a.hq - hk : r - a.hq;
+      const int slot = (max(head, 0) << a.c.shift) + in_page;
+      const int64_t page_at = int64_t(page) * (is_v ? a.c.v_page : a.c.k_page);
+      void *codes = is_v ? a.c.v : a.c.k;
+      if constexpr (kFormat == kCacheBf16) {
+        if (kept) {
+          __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(codes) + page_at + slot * D + l * 4;
+          *reinterpret_cast<uint2 *>(to) = lo;
+          *reinterpret_cast<uint2 *>(to + D / 2) = hi;
+        }
+      } else {
+        uint4 y = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        uint32_t m = magnitude8(y);
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1)
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const bool odd = __any_sync(0xffffffffu, m >= 0x7f80u);   // an infinity or a NaN in some row
+        if (odd) {
+          m = magnitude8_finite(y);
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1)
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        }
+        float *scales = (is_v ? a.c.vs + int64_t(page) * a.c.vs_page : a.c.ks + int64_t(page) * a.c.ks_page);
+        if constexpr (kFormat == kCacheInt4) {
+          const float s = int4_scale(m);
+          if (odd)
+            y = m > 0x7f80u ? make_uint4(0, 0, 0, 0) : bounded8(y, m);
+          const float inverse = m > 0x7f80u ? 1.f : __uint_as_float(0x7f000000u - __float_as_uint(s));
+          // Eight lanes' channels of either half are a group.
+          uint32_t most = __vmaxu2(y.x & 0x7fff7fffu, y.y & 0x7fff7fffu), next = __vmaxu2(y.z & 0x7fff7fffu, y.w & 0x7fff7fffu);
+          most = max(most & 0xffffu, most >> 16) | (max(next & 0xffffu, next >> 16) << 16);
+#pragma unroll
+          for (int o = 4; o > 0; o >>= 1)
+            most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
+          const uint32_t f0 = int4_factor(most & 0xffffu, inverse), f1 = int4_factor(most >> 16, inverse);
+          const uint32_t q0 = quantise4_int4(y.x, y.y, inverse, e4m3_value(f0)), q1 = quantise4_int4(y.z, y.w, inverse, e4m3_value(f1));
+          if (kept) {
+            uint8_t *to = static_cast<uint8_t *>(codes) + page_at + slot * (D / 2) + l * 2;
+            *reinterpret_cast<uint16_t *>(to) = uint16_t(q0);
+            *reinterpret_cast<uint16_t *>(to + D / 4) = uint16_t(q1);
+            if (l % 8 == 0) {
+              uint8_t *factor = (is_v ? a.c.vf + int64_t(page) * a.c.vf_page : a.c.kf + int64_t(page) * a.c.kf_page) +
+                                slot * (D / kFactorGroup) + l / 8;
+              factor[0] = uint8_t(f0), factor[D / 2 / kFactorGroup] = uint8_t(f1);
+            }
+            if (l == 0)
+              scales[slot] = s;
+          }
+        } else {
+          const float most = __uint_as_float(m << 16);
+          const float s = m == 0 ? 1.f : __fmul_rn(most, kFormat == kCacheInt8 ? 1.0f / 127.0f : 1.0f / 448.0f);
+          const uint2 q = !odd && s > 0x1p-80f && s < 0x1p100f ? quantise8<kFormat>(y, s, __frcp_rn(s)) : quantise8_any<kFormat>(y, s);
+          if (kept) {
+            uint8_t *to = static_cast<uint8_t *>(codes) + page_at + slot * D + l * 4;
+            *reinterpret_cast<uint32_t *>(to) = q.x;
+            *reinterpret_cast<uint32_t *>(to + D / 2) = q.y;
+            if (l == 0)
+              scales[slot] = s;
+          }
+        }
+      }
+    }
+    first += step;
+    if (first >= heads)
+      break;
+    fetch(first, x);
   }
 }
 

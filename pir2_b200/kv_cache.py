@@ -26,6 +26,17 @@ FORMATS = {
 FACTOR_GROUP = 32   # channels of a 4-bit row that share a factor
 
 
+def rotary_table(positions, head_dim, theta=1e4, *, device="cuda"):
+    """(cos, sin) fp32 [positions, head_dim / 2] of the angles p theta^(-2 i /
+    head_dim), as `ops.cache_append` takes them; the angles are computed in 64
+    bits (in 32, those of far positions are off by 2^-24 of many turns)."""
+    if positions < 1 or head_dim not in HEAD_DIMS:
+        raise ValueError(f"rotary_table: positions must be at least 1, head_dim one of {HEAD_DIMS}")
+    inverse = theta ** (-torch.arange(0, head_dim, 2, dtype=torch.float64, device=device) / head_dim)
+    angles = torch.outer(torch.arange(positions, dtype=torch.float64, device=device), inverse)
+    return angles.cos().float(), angles.sin().float()
+
+
 class KVPages:
     """One layer's pool: k, v [pages, kv_heads, page_size, head_dim] of one
     dtype (bfloat16, int8 or float8_e4m3fn; uint8 [..., head_dim / 2] holds 4-bit

@@ -709,6 +709,53 @@ def cache_write(k, v, pages, sequences):
         _lib.check(status, "pir2b_cache_write")
 
 
+def cache_append(qkv, pages, sequences, cos, sin, *, q_weight=None, k_weight=None, eps=1e-6, positions=None, out=None,
+                 k_out=None):
+    """Per-head norm and rotation of new rows' q and k, and their k and v into
+    the last positions of their sequences, in one pass.
+
+    qkv: bf16 [rows, hq + 2 kv_heads, head_dim] view of a merged projection; cos,
+    sin: fp32 [positions, head_dim / 2] (`kv_cache.rotary_table`), looked up by
+    a row's position in the cache, or by `positions` (int32 [rows] on the device);
+    q_weight, k_weight: bf16 [head_dim] of the heads' RMS norms, or None for
+    none.  Computed in fp32 and rounded to bf16 once; the cache holds that
+    rounding of k, and v, as `cache_write` would write them.  Returns q: bf16
+    [rows, hq, head_dim] (`out`, which may be qkv's own heads); `k_out` [rows,
+    kv_heads, head_dim] receives k as well, e.g. for `prompt_attention`.
+    """
+    (rows, heads, d), row, head = _head_rows(qkv, "cache_append: qkv")
+    hk = pages.kv_heads
+    hq = heads - 2 * hk
+    if hq < 1 or d != pages.head_dim:
+        raise ValueError("cache_append: qkv must be [rows, hq + 2 kv_heads, head_dim] with the pool's kv_heads and head_dim")
+    index = qkv.get_device()
+    if pages.index != index or sequences.index != index:
+        raise ValueError("cache_append: rows, pages and sequences must be on one device")
+    for t in (cos, sin):
+        if t.dtype != torch.float32 or t.ndim != 2 or t.shape != cos.shape or t.shape[1] != d // 2 or not t.is_contiguous() or t.get_device() != index:
+            raise ValueError("cache_append: cos and sin must be contiguous fp32 [positions, head_dim / 2] on the rows' device")
+    for t in (q_weight, k_weight):
+        if t is not None and (t.dtype != torch.bfloat16 or t.shape != (d,) or not t.is_contiguous() or t.get_device() != index):
+            raise ValueError("cache_append: norm weights must be contiguous bf16 [head_dim] on the rows' device")
+    if positions is not None and (positions.dtype != torch.int32 or positions.shape != (rows,) or not positions.is_contiguous()
+                                  or positions.get_device() != index):
+        raise ValueError("cache_append: positions must be contiguous int32 [rows] on the rows' device")
+    if out is None:
+        out = qkv.new_empty((rows, hq, d))
+    for t, count in ((out, hq), (k_out, hk)):
+        if t is not None and (t.shape != (rows, count, d) or t.dtype != torch.bfloat16 or t.get_device() != index or t.stride(2) != 1
+                              or (count > 1 and t.stride(1) != d)):
+            raise ValueError("cache_append: outputs must be bf16 [rows, heads, head_dim] with contiguous heads on the rows' device")
+    status = _lib.lib().pir2b_cache_append(
+        qkv.data_ptr(), row, head, rows, hq, _ptr(q_weight), _ptr(k_weight), eps, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+        _ptr(positions), pages.address, sequences.address, out.data_ptr(), out.stride(0) if rows > 1 else hq * d, _ptr(k_out),
+        0 if k_out is None else k_out.stride(0) if rows > 1 else hk * d, _raw_stream(index),
+    )
+    if status:
+        _lib.check(status, "pir2b_cache_append")
+    return out
+
+
 def cache_read(pages, sequences, rows):
     """Positions 0, 1, ... of each sequence as packed bf16 rows: (k, v), each
     [rows, kv_heads, head_dim]; sequence b is rows starts[b] ..
