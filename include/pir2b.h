@@ -398,6 +398,18 @@ int pir2b_attention_causal(const void *q, const void *k, const void *v, int64_t 
                            int64_t tokens, int hq, int hk, int head_dim, float scale, void *out,
                            int64_t ldo, void *stream);
 
+/* Products of a few bf16 rows with 4-bit weights (no counterpart in the
+ * reference, whose int4 weights carry one scale per channel and meet int4
+ * activations): out[m, n] = bf16(sum_k x[m, k] * code[n, k] * scale[n, k / group]
+ * + bias[n]), sums in fp32.  packed: [n, k / 2], two's complement codes of -8..7,
+ * two to a byte with the even k in the low bits; scales: bf16 [n, k / group],
+ * group 32, 64 or 128; bias: bf16 [n] or null; k a multiple of group.  x is
+ * 16-byte aligned with a row stride that is a multiple of 8.  Meant for decoding:
+ * the weights are read once for every 64 rows. */
+int pir2b_gemm_w4a16(const void *x, int64_t ldx, const void *packed, const void *scales, int group,
+                     const void *bias, int64_t m, int64_t n, int64_t k, void *out, int64_t ldo,
+                     void *stream);
+
 /* ---- ragged batches and the paged K/V cache of the text layers ----------
  *
  * The reference prefills one observation per robot and keeps no K/V cache

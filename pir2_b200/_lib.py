@@ -83,6 +83,7 @@ SIGNATURES = {
     "pir2b_attention_rows": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I, _I, _F, _P],
     "pir2b_unpack_int4": [_P, _I64, _I64, _P, _P],
     "pir2b_attention_causal": [_P, _P, _P, _I64, _I64, _I, _I, _I, _F, _P, _I64, _P],
+    "pir2b_gemm_w4a16": [_P, _I64, _P, _P, _I, _P, _I64, _I64, _I64, _P, _I64, _P],
     "pir2b_prompt_attention": [
         _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _I, _I, _F, _P, _I64, _P,
     ],

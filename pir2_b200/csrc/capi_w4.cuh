@@ -1,0 +1,69 @@
+// C ABI of the products with 4-bit weights: argument checks and launches.
+#pragma once
+#include "capi_cache.cuh"
+#include "gemm_w4.cuh"
+
+namespace pir2b {
+
+constexpr int kW4Rows = 64;   // rows of a launch
+
+template <int kGroup, int kTiles>
+static int launch_w4(const W4Args &a, void *stream) {
+  return launch_cache("gemm_w4a16 launch", gemm_w4_kernel<kGroup, kTiles>, (a.n + kW4Channels - 1) / kW4Channels, 1, 1,
+                      kW4Warps * 32, 0, stream, a);
+}
+
+template <int kGroup>
+static int launch_w4(const W4Args &a, void *stream) {
+  if (a.m <= 8)
+    return launch_w4<kGroup, 1>(a, stream);
+  if (a.m <= 16)
+    return launch_w4<kGroup, 2>(a, stream);
+  if (a.m <= 32)
+    return launch_w4<kGroup, 4>(a, stream);
+  return launch_w4<kGroup, 8>(a, stream);
+}
+
+} // namespace pir2b
+
+using namespace pir2b;
+
+extern "C" {
+
+int pir2b_gemm_w4a16(const void *x, int64_t ldx, const void *packed, const void *scales, int group,
+                     const void *bias, int64_t m, int64_t n, int64_t k, void *out, int64_t ldo,
+                     void *stream) {
+  if (group != 32 && group != 64 && group != 128)
+    return fail(PIR2B_EINVAL, "gemm_w4a16: a group is 32, 64 or 128 weights");
+  if (m < 0 || m > 0x7fffffff || n < 1 || n > 0x7ffffff0 || k < group || k > (1 << 20) || k % group != 0)
+    return fail(PIR2B_EINVAL, "gemm_w4a16: needs rows >= 0, n >= 1 and k a multiple of the group, at most 2^20");
+  if (m == 0)
+    return PIR2B_OK;
+  if (x == nullptr || packed == nullptr || scales == nullptr || out == nullptr)
+    return fail(PIR2B_EINVAL, "gemm_w4a16: x, packed, scales and out must be non-null");
+  if (ldx < k || ldo < n)
+    return fail(PIR2B_EINVAL, "gemm_w4a16: a row stride is below its row's width");
+  if (!aligned(x, 16) || ldx % 8 != 0 || !aligned(packed, 16) || !aligned(scales, 2) || !aligned(bias, 2) || !aligned(out, 2))
+    return fail(PIR2B_EALIGN, "gemm_w4a16: x and packed must be 16-byte aligned, x with a row stride that is a multiple of 8");
+  DeviceInfo *dev = nullptr;
+  if (int r = device_info(&dev))
+    return r;
+  W4Args a = {};
+  a.w = static_cast<const uint8_t *>(packed);
+  a.scales = static_cast<const __nv_bfloat16 *>(scales);
+  a.bias = static_cast<const __nv_bfloat16 *>(bias);
+  a.ldx = ldx;
+  a.ldo = ldo;
+  a.n = int(n);
+  a.k = int(k);
+  for (int64_t first = 0; first < m; first += kW4Rows) {   // more rows read the weights again
+    a.x = static_cast<const __nv_bfloat16 *>(x) + first * ldx;
+    a.out = static_cast<__nv_bfloat16 *>(out) + first * ldo;
+    a.m = int(std::min<int64_t>(kW4Rows, m - first));
+    if (int r = group == 32 ? launch_w4<32>(a, stream) : group == 64 ? launch_w4<64>(a, stream) : launch_w4<128>(a, stream))
+      return r;
+  }
+  return PIR2B_OK;
+}
+
+} // extern "C"

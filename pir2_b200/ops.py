@@ -604,6 +604,43 @@ def gemm_nvfp4(a_packed, a_sf, w_packed, w_sf, bias=None, *, n, alpha=1.0, out=N
     return out
 
 
+def gemm_w4a16(x, packed, scales, bias=None, *, out=None):
+    """Products of a few bf16 rows with 4-bit weights -> bf16 [rows, n].
+
+    x: bf16 [rows, k] with unit column stride and a row stride that is a multiple
+    of 8; packed: uint8 [n, k / 2] codes of -8..7 (two's complement, the even k in
+    the low bits); scales: bf16 [n, k / group], group 32, 64 or 128; bias: bf16
+    [n].  Sums in fp32, rounded once.  The weights are read once for every 64
+    rows (`weight_only.WeightOnlyLinear` makes them from a Linear).
+    """
+    if x.dtype != torch.bfloat16 or not x.is_cuda or x.ndim != 2 or x.stride(1) != 1:
+        raise ValueError("gemm_w4a16: x must be CUDA bf16 [rows, k] with unit column stride")
+    m, k = x.shape
+    index = x.get_device()
+    if packed.dtype != torch.uint8 or packed.ndim != 2 or packed.shape[1] * 2 != k or not packed.is_contiguous():
+        raise ValueError("gemm_w4a16: packed must be contiguous uint8 [n, k / 2]")
+    n = packed.shape[0]
+    if scales.dtype != torch.bfloat16 or scales.ndim != 2 or scales.shape[0] != n or scales.shape[1] < 1 or not scales.is_contiguous():
+        raise ValueError("gemm_w4a16: scales must be contiguous bf16 [n, k / group]")
+    if k % scales.shape[1]:
+        raise ValueError("gemm_w4a16: k must be a multiple of the group")
+    if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (n,) or not bias.is_contiguous()):
+        raise ValueError("gemm_w4a16: bias must be contiguous bf16 [n]")
+    if out is None:
+        out = x.new_empty((m, n))
+    elif out.shape != (m, n) or out.dtype != torch.bfloat16 or out.stride(1) != 1:
+        raise ValueError("gemm_w4a16: out must be bf16 [rows, n] with unit column stride")
+    if any(t is not None and t.get_device() != index for t in (packed, scales, bias, out)):
+        raise ValueError("gemm_w4a16: all tensors must be on one device")
+    status = _lib.lib().pir2b_gemm_w4a16(
+        x.data_ptr(), x.stride(0) if m > 1 else k, packed.data_ptr(), scales.data_ptr(), k // scales.shape[1], _ptr(bias), m, n, k,
+        out.data_ptr(), out.stride(0) if m > 1 else n, _raw_stream(index),
+    )
+    if status:
+        _lib.check(status, "pir2b_gemm_w4a16")
+    return out
+
+
 def attention_rows(q, k, v, *, batch, heads, head_dim, scale=None, out=None):
     """Unmasked attention over projection rows.
 

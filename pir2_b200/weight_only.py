@@ -1,0 +1,65 @@
+"""Linears whose weights are held in 4 bits and whose activations stay bf16, for
+decoding a few rows at a time.
+
+The reference's int4 format (coexecution/kernels/ampere_ada/integer.py:222-238)
+has one scale per output channel and quantises activations to 4 bits as well,
+which suits many rows; a decoded token's Linears are bound by reading weights,
+so here the weights alone are narrow, with a bf16 scale for every group of 32, 64
+or 128 of a channel's weights.
+"""
+
+import torch
+
+from . import ops
+
+GROUPS = (32, 64, 128)
+
+
+def quantize_groups(weight, group):
+    """(packed uint8 [n, k / 2], scales bf16 [n, k / group]) of weights [n, k]:
+    scale = bf16(max|w| / 7) of a group (1 for zeros), code = w / scale rounded
+    to nearest even and clamped to -7..7, the even k in the low bits."""
+    if group not in GROUPS or weight.ndim != 2 or weight.shape[1] % group or not weight.shape[1]:
+        raise ValueError(f"quantize_groups: group must be one of {GROUPS} and divide the weights' columns")
+    w = weight.detach().float()
+    if not torch.isfinite(w).all():
+        raise ValueError("Weights must be finite")
+    w = w.unflatten(1, (-1, group))
+    most = w.abs().amax(-1)
+    scales = (most / 7).to(torch.bfloat16)
+    scales = torch.where(scales == 0, torch.ones_like(scales), scales)
+    codes = torch.round(w / scales.float()[..., None]).clamp(-7, 7).flatten(1).to(torch.int8)
+    u = codes.view(torch.uint8) & 15
+    return u[:, 0::2] | (u[:, 1::2] << 4), scales
+
+
+class WeightOnlyLinear(torch.nn.Module):
+    """y = x W^T + b with W in 4 bits and groups of `group` weights per scale."""
+
+    def __init__(self, packed, scales, bias=None):
+        super().__init__()
+        self.register_buffer("packed_weight", packed)
+        self.register_buffer("weight_scale", scales)
+        self.register_buffer("bias", bias)
+        self.out_features, self.in_features = packed.shape[0], 2 * packed.shape[1]
+        self.group = self.in_features // scales.shape[1]
+
+    @classmethod
+    def from_linear(cls, *linears, group=128):
+        """Of one Linear, or of several with the same input side by side (their
+        outputs concatenated)."""
+        weights = [linear.weight for linear in linears]
+        if not weights or any(not w.is_cuda or w.dtype != torch.bfloat16 or w.shape[1] != weights[0].shape[1] for w in weights):
+            raise ValueError("WeightOnlyLinear requires CUDA BF16 weights of one input width")
+        packed, scales = zip(*(quantize_groups(w, group) for w in weights))
+        biases = [linear.bias for linear in linears]
+        bias = None
+        if any(b is not None for b in biases):
+            bias = torch.cat([w.new_zeros(w.shape[0]) if b is None else b.detach().to(torch.bfloat16) for w, b in zip(weights, biases)])
+        return cls(torch.cat(packed), torch.cat(scales), bias)
+
+    def forward(self, x):
+        if x.shape[-1] != self.in_features:
+            raise ValueError("Wrong input feature count")
+        rows = x.reshape(-1, self.in_features)
+        return ops.gemm_w4a16(rows, self.packed_weight, self.weight_scale, self.bias).view(*x.shape[:-1], self.out_features)
