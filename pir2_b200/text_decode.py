@@ -20,7 +20,7 @@ from functools import partial
 import torch
 
 from . import ops
-from .kv_cache import FACTOR_GROUP, KVPages, Sequences
+from .kv_cache import FACTOR_GROUP, KVPages, Sequences, rotary_table
 from .transformer import _MODE_BITS
 
 
@@ -138,10 +138,19 @@ class PackedTextDecoder:
     """Runs a text backbone's layers (Qwen3-VL attention: q/k norm, RoPE,
     grouped heads of 128) on packed rows over a TextCache.  With a TransformerINT
     `controller`, q, k and v are one grouped GEMM of the precision that it has
-    installed at the time of a call (only of `bits`, if given)."""
+    installed at the time of a call (only of `bits`, if given).
 
-    def __init__(self, backbone, cache, *, controller=None, bits=None):
+    `append`: norm, rotation and cache write of a layer are one launch
+    (`ops.cache_append`), in fp32 with one rounding, where the layers' own
+    arithmetic rounds each step to bf16: results differ in the last bits.
+    `weight_only` (weight_only.TextProjections): the projections, SwiGLU and
+    output layer of calls with few rows, in 4-bit weights.  While anything is
+    installed in a layer's projections, norms or the layer itself (quantised
+    projections, fusions), its layers run as installed."""
+
+    def __init__(self, backbone, cache, *, controller=None, bits=None, append=False, weight_only=None):
         self.backbone, self.cache, self.controller = backbone, cache, controller
+        self.append, self.weight_only = append, weight_only
         self.attentions = [layer.self_attn for layer in backbone.layers]
         if len(self.attentions) != len(cache.layers):
             raise ValueError("the cache must have one pool per layer")
@@ -156,7 +165,18 @@ class PackedTextDecoder:
                     group = grouped.get(names.get(id(attn.q_proj)))
                     if group is not None:
                         self.groups[precision, id(attn)] = group
-        self.rope = None
+        if weight_only is not None and len(weight_only.qkv) != len(self.attentions):
+            raise ValueError("weight_only must have the backbone's layers")
+        self.rope = self.turns = None
+
+    def _narrow(self, rows):
+        """Whether the 4-bit projections take a call of so many rows."""
+        if self.weight_only is None or rows > self.weight_only.rows:
+            return False
+        return not any("forward" in module.__dict__ for layer in self.backbone.layers for module in (
+            layer, layer.input_layernorm, layer.post_attention_layernorm, layer.self_attn.q_proj, layer.self_attn.k_proj,
+            layer.self_attn.v_proj, layer.self_attn.o_proj, layer.mlp.gate_proj, layer.mlp.up_proj, layer.mlp.down_proj,
+        ))
 
     def _project(self, attn, x):
         mode = None if self.controller is None else self.controller.mode
@@ -165,21 +185,29 @@ class PackedTextDecoder:
             return group.linear(x)
         return torch.cat((attn.q_proj(x), attn.k_proj(x), attn.v_proj(x)), dim=-1)
 
-    def _attend(self, index, prompts, x, cos, sin):
+    def _attend(self, index, prompts, narrow, x, cos, sin):
         attn, pages, sequences = self.attentions[index], self.cache.layers[index], self.cache.sequences
         rows = x.shape[1]
-        qkv = self._project(attn, x)
-        q, k, v = ops.qk_norm_rope(
-            qkv.reshape(rows, qkv.shape[-1]), attn.q_norm.weight, attn.k_norm.weight, cos, sin, tokens=rows,
-            hq=attn.heads, hk=attn.kv_heads, eps=attn.q_norm.variance_epsilon,
-        )
-        q, k, v = (z[0].transpose(0, 1) for z in (q, k, v))        # [rows, heads, 128] views
-        ops.cache_write(k, v, pages, sequences)
+        qkv = self.weight_only.qkv[index](x) if narrow else self._project(attn, x)
+        if self.append:
+            qkv = qkv.reshape(rows, -1, attn.head_dim)
+            v = qkv[:, attn.heads + attn.kv_heads :]
+            k = v.new_empty((rows, attn.kv_heads, attn.head_dim)) if prompts else None
+            q = ops.cache_append(qkv, pages, sequences, *self.turns, q_weight=attn.q_norm.weight, k_weight=attn.k_norm.weight,
+                                 eps=attn.q_norm.variance_epsilon, k_out=k)
+        else:
+            q, k, v = ops.qk_norm_rope(
+                qkv.reshape(rows, qkv.shape[-1]), attn.q_norm.weight, attn.k_norm.weight, cos, sin, tokens=rows,
+                hq=attn.heads, hk=attn.kv_heads, eps=attn.q_norm.variance_epsilon,
+            )
+            q, k, v = (z[0].transpose(0, 1) for z in (q, k, v))        # [rows, heads, 128] views
+            ops.cache_write(k, v, pages, sequences)
         if prompts:
             y = ops.prompt_attention(q, k, v, sequences.starts)
         else:
             y = ops.cache_attention(q, pages, sequences)
-        return attn.o_proj(y.view(1, rows, y.shape[1]))
+        y = y.view(1, rows, y.shape[1])
+        return self.weight_only.o[index](y) if narrow else attn.o_proj(y)
 
     def _rope(self, positions, device, dtype):
         longest = max(positions) + 1
@@ -193,6 +221,12 @@ class PackedTextDecoder:
             self.rope = angles.cos().to(dtype), angles.sin().to(dtype)
         at = torch.tensor(positions, dtype=torch.int64).to(device)
         return self.rope[0][at], self.rope[1][at]
+
+    def _turns(self, longest, device):
+        if self.turns is None or self.turns[0].shape[0] < longest:
+            size = max(longest, 2 * (0 if self.turns is None else self.turns[0].shape[0]))
+            c = self.backbone.config
+            self.turns = rotary_table(size, c.head_dim, c.rope_theta, device=device)
 
     @torch.inference_mode()
     def run(self, hidden, new):
@@ -212,11 +246,20 @@ class PackedTextDecoder:
 
     def _layers(self, hidden, past, new):
         prompts = all(p == 0 for p, n in zip(past, new) if n)   # every sequence of the batch starts with this call
-        positions = [p + i for p, n in zip(past, new) for i in range(n)]
-        cos, sin = self._rope(positions, hidden.device, hidden.dtype)
-        forwards = [partial(self._attend, index, prompts) for index in range(len(self.attentions))]
+        if self.append:
+            cos = sin = None                                     # positions are looked up on the device
+            self._turns(max(p + n for p, n in zip(past, new)), hidden.device)
+        else:
+            positions = [p + i for p, n in zip(past, new) for i in range(n)]
+            cos, sin = self._rope(positions, hidden.device, hidden.dtype)
+        narrow = self._narrow(hidden.shape[0])
+        modules = list(self.attentions)
+        forwards = [partial(self._attend, index, prompts, narrow) for index in range(len(self.attentions))]
+        if narrow:
+            modules += [layer.mlp for layer in self.backbone.layers]
+            forwards += [partial(self.weight_only.feed, index) for index in range(len(self.attentions))]
         h = hidden[None]
-        with _ROUTES.routed(self.attentions, forwards):
+        with _ROUTES.routed(modules, forwards):
             for layer in self.backbone.layers:
                 h = layer(h, cos, sin)
         return h[0]
@@ -229,7 +272,9 @@ class PackedTextDecoder:
         embed = self.backbone.embed_tokens.weight
         tokens = []
         for _ in range(steps):
-            ids = (last_hidden @ embed.T).argmax(-1)
+            narrow = self.weight_only is not None and last_hidden.shape[0] <= self.weight_only.rows
+            logits = self.weight_only.vocabulary(last_hidden) if narrow else last_hidden @ embed.T
+            ids = logits.argmax(-1)
             tokens.append(ids)
             last_hidden = self.run(embed[ids], [1] * self.cache.batch)
         return torch.stack(tokens, dim=1)

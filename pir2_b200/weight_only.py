@@ -9,6 +9,7 @@ or 128 of a channel's weights.
 """
 
 import torch
+import torch.nn.functional as F
 
 from . import ops
 
@@ -63,3 +64,31 @@ class WeightOnlyLinear(torch.nn.Module):
             raise ValueError("Wrong input feature count")
         rows = x.reshape(-1, self.in_features)
         return ops.gemm_w4a16(rows, self.packed_weight, self.weight_scale, self.bias).view(*x.shape[:-1], self.out_features)
+
+
+class TextProjections:
+    """A text backbone's projections in 4 bits, beside its own, for decoding:
+    q|k|v and gate|up of a layer merged, o and down, and the output layer over the
+    input embeddings.  `PackedTextDecoder` takes them where a call has at most
+    `rows` new rows; longer ones (prompts, camera views) keep the layers' own."""
+
+    def __init__(self, backbone, *, group=128, rows=64):
+        def of(*linears):
+            return WeightOnlyLinear.from_linear(*linears, group=group)
+
+        self.rows = rows
+        self.qkv, self.o, self.gate_up, self.down = [], [], [], []
+        for layer in backbone.layers:
+            attn, mlp = layer.self_attn, layer.mlp
+            if mlp.config.hidden_act != "silu":
+                raise ValueError("TextProjections needs SiLU text layers")
+            self.qkv.append(of(attn.q_proj, attn.k_proj, attn.v_proj))
+            self.o.append(of(attn.o_proj))
+            self.gate_up.append(of(mlp.gate_proj, mlp.up_proj))
+            self.down.append(of(mlp.down_proj))
+        self.vocabulary = WeightOnlyLinear(*quantize_groups(backbone.embed_tokens.weight, group))
+
+    def feed(self, index, x):
+        """Layer `index`'s SwiGLU."""
+        gate, up = self.gate_up[index](x).chunk(2, dim=-1)
+        return self.down[index](F.silu(gate) * up)
