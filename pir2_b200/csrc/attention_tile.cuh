@@ -50,15 +50,16 @@ constexpr int kTileKeys = 128;
 // beside the other's products.
 template <int kSource, int D, int kTiles>
 struct TileShape {
-  static constexpr bool kScaled = kSource == kCacheInt8 || kSource == kCacheE4m3;
+  static constexpr bool kScaled = kSource == kCacheInt8 || kSource == kCacheE4m3 || kSource == kCacheInt4;
   static constexpr int kThreads = kTiles * 256 + 96 + (kScaled ? 128 : 0);
   static constexpr int kBytes = 128 * D * 2;            // a Q, K or V tile
   static constexpr int kStages = kTiles == 2 ? (D == 128 ? (kScaled ? 3 : 5) : (kScaled ? 6 : 8)) : (D == 128 ? 2 : 5);
-  // 8-bit caches: tiles of codes on their way to the converting warps, and
-  // blocks whose scales are kept.  The loader writes block j's scales when
+  // Quantised caches: tiles of codes (int4: and their factors) on their way to the
+  // converting warps, and blocks whose scales are kept.  The loader writes block j's scales when
   // item 2 j - kRaw has been converted, so item 2 j - kRaw - kStages has been
   // used; V item 2 (j - kDepth) + 1 must not come after that.
-  static constexpr int kRaw = kScaled ? 3 : 0, kRawBytes = 128 * D;
+  static constexpr int kRowCodes = code_bytes(kSource, D), kRowFactors = kSource == kCacheInt4 ? D / kFactorGroup : 0;
+  static constexpr int kRaw = kScaled ? 3 : 0, kRawBytes = 128 * (kRowCodes + kRowFactors);
   static constexpr int kDepth = (kStages + kRaw + 2) / 2;
   static constexpr int kScaleBytes = kScaled ? kDepth * 2 * kTileKeys * 4 : 0;
   static constexpr int kSumBytes = kTiles * 2 * 128 * 4;
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
   constexpr int kHalves = D / 64;                 // 64-column blocks of a tile, 16 KB each
   extern __shared__ __align__(1024) uint8_t tile_raw[];   // swizzled tiles need the alignment; nothing lies before
   uint8_t *q_sm = tile_raw, *ring = q_sm + kTiles * kBytes;
-  uint8_t *raw = ring + kStages * kBytes;                               // [kRaw][128][D] codes
+  uint8_t *raw = ring + kStages * kBytes;                               // [kRaw]: [128][D] codes, [128][D / 32] factors
   float *scales = reinterpret_cast<float *>(raw + Shape::kRaw * Shape::kRawBytes);   // [kDepth][K, V][128]
   float *sums = scales + Shape::kScaleBytes / 4;                        // [tile][half][row], between a row's two threads
   TileBarriers &bar = *reinterpret_cast<TileBarriers *>(sums + Shape::kSumBytes / 4);
@@ -333,7 +334,7 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
     if (!__all_sync(0xffffffffu, free_stage))
       return false;
     if (lane == 0) {
-      const int row_bytes = kScaled ? D + (item & 1 ? 0 : 8) : D * 2;
+      const int row_bytes = kScaled ? Shape::kRowCodes + Shape::kRowFactors + (item & 1 ? 0 : 8) : D * 2;
       mbar_arrive_expect_tx(&full[stage], kPaged ? (copies << a.c.shift) * row_bytes : kBytes);
     }
     __syncwarp();
@@ -341,7 +342,13 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
       const void *map = (item & 1) ? &tm_v : &tm_k;
       if constexpr (kScaled) {
         const int row = lane << a.c.shift;
-        tma_load_4d(raw + stage * Shape::kRawBytes + row * D, map, &full[stage], 0, 0, kvh, page);
+        tma_load_4d(raw + stage * Shape::kRawBytes + row * Shape::kRowCodes, map, &full[stage], 0, 0, kvh, page);
+        if constexpr (kSource == kCacheInt4) {
+          const uint8_t *factors = (item & 1) ? a.c.vf + page * a.c.vf_page : a.c.kf + page * a.c.kf_page;
+          bulk_load(raw + stage * Shape::kRawBytes + 128 * Shape::kRowCodes + row * Shape::kRowFactors,
+                    factors + (int64_t(kvh) << a.c.shift) * Shape::kRowFactors, uint32_t(Shape::kRowFactors) << a.c.shift,
+                    &full[stage]);
+        }
         if (!(item & 1)) {
           float *block_scales = scales + (j % Shape::kDepth) * 2 * kTileKeys + row;
           const int64_t slot = int64_t(kvh) << a.c.shift;
@@ -767,8 +774,9 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
     } else if (kScaled) {
       if constexpr (kScaled) {
         // Four warps turn tiles of codes into bf16 tiles, 16 bytes of a row at
-        // a time.  Rows past the keys hold old codes, which are numbers.
-        constexpr int kRuns = D / 16, kRowStep = 128 / kRuns;
+        // a time (of int4 the channels of one factor).  Rows past the keys hold
+        // old codes, which are numbers.
+        constexpr int kRuns = Shape::kRowCodes / 16, kRowStep = 128 / kRuns;
         const int t = tid - (kMmaWarp + 3) * 32, run = t % kRuns, row0 = t / kRuns;
         for (int item = 0; t >= 0 && item < 2 * blocks; ++item) {
           const int from = item % Shape::kRaw, stage = item % kStages;
@@ -777,13 +785,28 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
             go = mbar_wait(&bar.empty[stage], uint32_t((item / kStages - 1) & 1), kStatusTimeoutConvert);
           if (!__all_sync(0xffffffffu, go))
             break;
-          const uint8_t *src = raw + from * Shape::kRawBytes + row0 * D + run * 16;
-          uint8_t *dst = ring + stage * kBytes + (run >> 2) * 16384;
-          const int piece = (run & 3) * 2;
+          const uint8_t *src = raw + from * Shape::kRawBytes + row0 * Shape::kRowCodes + run * 16;
+          constexpr int kPieces = 2 * D / kRuns / 16;         // 16-byte pieces of bf16 that a run becomes
+          uint8_t *dst = ring + stage * kBytes + run * kPieces / 8 * 16384;
+          const int piece = run * kPieces % 8;
 #pragma unroll
           for (int i = 0; i < kTileKeys / kRowStep; ++i) {
             const int row = row0 + i * kRowStep;
-            const uint4 x = *reinterpret_cast<const uint4 *>(src + i * kRowStep * D);
+            const uint4 x = *reinterpret_cast<const uint4 *>(src + i * kRowStep * Shape::kRowCodes);
+            if constexpr (kSource == kCacheInt4) {
+              const uint32_t byte = raw[from * Shape::kRawBytes + 128 * Shape::kRowCodes + row * Shape::kRowFactors + run];
+              uint32_t minus_24f;
+              const uint32_t f = factor_pair_bf16(byte, byte, minus_24f), w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const uint32_t p0 = int4_to_bf16<0>(w[c], f, minus_24f), p1 = int4_to_bf16<1>(w[c], f, minus_24f);
+                const uint32_t p2 = int4_to_bf16<2>(w[c], f, minus_24f), p3 = int4_to_bf16<3>(w[c], f, minus_24f);
+                *reinterpret_cast<uint4 *>(dst + row * 128 + (((piece + c) ^ (row & 7)) << 4)) =
+                    make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632),
+                               __byte_perm(p2, p3, 0x7632));
+              }
+              continue;
+            }
             uint4 lo, hi;
             codes_to_bf16<kSource>(x.x, lo.x, lo.y);
             codes_to_bf16<kSource>(x.y, lo.z, lo.w);

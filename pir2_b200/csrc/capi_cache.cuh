@@ -341,7 +341,7 @@ struct CachePlan {
 static CachePlan plan_cache(int64_t rows, int hq, int hk, int d, int batch, int64_t positions, int format, int sms) {
   CachePlan p = {};
   const int64_t per_sequence = (rows + batch - 1) / batch * (hq / hk);
-  if (format == kCacheInt4 || per_sequence <= (format == kCacheBf16 ? kFewRowsBf16 : kFewRows8Bit)) {
+  if (per_sequence <= (format == kCacheBf16 ? kFewRowsBf16 : kFewRows8Bit)) {
     p.few = plan_few(rows, hq, hk, batch, positions, format, d, sms);
     return p;
   }
@@ -358,13 +358,13 @@ static CachePlan plan_cache(int64_t rows, int hq, int hk, int d, int batch, int6
 
 template <int kSource, int D>
 static int launch_cache_tile(const CachePlan &p, RaggedArgs a, void *stream) {
-  constexpr int kBytes = kSource == kCacheBf16 ? 2 : 1;
+  constexpr int kBytes = kSource == kCacheBf16 ? 2 : 1, kWide = code_bytes(kSource, D) / kBytes;
   CUtensorMap tm_q, tm_k, tm_v;
   if (int r = make_q_map(&tm_q, &a, D))
     return r;
-  if (int r = make_pages_map(&tm_k, a.c.k, a.c, D, a.c.k_page, kBytes, 1 << a.c.shift, kBytes == 2))
+  if (int r = make_pages_map(&tm_k, a.c.k, a.c, kWide, a.c.k_page, kBytes, 1 << a.c.shift, kBytes == 2))
     return r;
-  if (int r = make_pages_map(&tm_v, a.c.v, a.c, D, a.c.v_page, kBytes, 1 << a.c.shift, kBytes == 2))
+  if (int r = make_pages_map(&tm_v, a.c.v, a.c, kWide, a.c.v_page, kBytes, 1 << a.c.shift, kBytes == 2))
     return r;
   if constexpr (kSource == kCacheBf16) {
     if (p.tiles == 1)
@@ -375,11 +375,9 @@ static int launch_cache_tile(const CachePlan &p, RaggedArgs a, void *stream) {
 
 template <int kFormat>
 static int launch_cache_attention(const CachePlan &p, int d, const RaggedArgs &a, void *stream) {
-  if (p.tiles == 0 || kFormat == kCacheInt4)
+  if (p.tiles == 0)
     return launch_attention_few<kFormat>(p.few, d, a, stream);
-  if constexpr (kFormat != kCacheInt4)
-    return d == 64 ? launch_cache_tile<kFormat, 64>(p, a, stream) : launch_cache_tile<kFormat, 128>(p, a, stream);
-  return PIR2B_OK;
+  return d == 64 ? launch_cache_tile<kFormat, 64>(p, a, stream) : launch_cache_tile<kFormat, 128>(p, a, stream);
 }
 
 static int launch_join(const CachePlan &p, int d, const RaggedArgs &a, void *stream) {
@@ -423,6 +421,8 @@ static int cache_kernel_attributes(DeviceInfo *dev) {
       {reinterpret_cast<const void *>(attention_tile_kernel<kCacheBf16, 128, 2>), TileShape<kCacheBf16, 128, 2>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kCacheInt8, 64, 2>), TileShape<kCacheInt8, 64, 2>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kCacheInt8, 128, 2>), TileShape<kCacheInt8, 128, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kCacheInt4, 64, 2>), TileShape<kCacheInt4, 64, 2>::kSmem},
+      {reinterpret_cast<const void *>(attention_tile_kernel<kCacheInt4, 128, 2>), TileShape<kCacheInt4, 128, 2>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kCacheE4m3, 64, 2>), TileShape<kCacheE4m3, 64, 2>::kSmem},
       {reinterpret_cast<const void *>(attention_tile_kernel<kCacheE4m3, 128, 2>), TileShape<kCacheE4m3, 128, 2>::kSmem},
   };
