@@ -104,20 +104,41 @@ __device__ __forceinline__ Int4Factors int4_factors(uint32_t pair) {   // of an 
   return {pair, half2_mul(pair, 0xd420d420u), half2_mul(pair, 0xc600c600u)};
 }
 
+// (x & mask) ^ kBits in one instruction: of its operands one may be a constant, so
+// the mask has to be in a register that the compiler does not see through.
+template <uint32_t kBits>
+__device__ __forceinline__ uint32_t masked_xor(uint32_t x, uint32_t mask) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(y) : "r"(x), "r"(mask), "n"(kBits));
+  return y;
+}
+
+struct Int4Masks {
+  uint32_t low, high, mantissa;     // bits 2-5, 6-9 and 3-6 of each half
+};
+
+__device__ __forceinline__ Int4Masks int4_masks() {
+  Int4Masks m;
+  asm volatile("mov.b32 %0, 0x003c003c;" : "=r"(m.low));
+  asm volatile("mov.b32 %0, 0x03c003c0;" : "=r"(m.high));
+  asm volatile("mov.b32 %0, 0x00780078;" : "=r"(m.mantissa));
+  return m;
+}
+
 // A word's codes 2 kHalf, 2 kHalf + 1 with those four places on, as fp16 pairs times f / 4.
 template <int kHalf>
-__device__ __forceinline__ void int4_to_half(uint32_t w, const Int4Factors &f, uint32_t &even, uint32_t &odd) {
+__device__ __forceinline__ void int4_to_half(uint32_t w, const Int4Factors &f, const Int4Masks &m, uint32_t &even, uint32_t &odd) {
   const uint32_t t = kHalf ? w >> 6 : w << 2;
-  even = half2_fma((t & 0x003c003cu) ^ 0x54205420u, f.f, f.minus_66f);
-  odd = half2_fma((t & 0x03c003c0u) ^ 0x46004600u, f.f, f.minus_6f);
+  even = half2_fma(masked_xor<0x54205420u>(t, m.low), f.f, f.minus_66f);
+  odd = half2_fma(masked_xor<0x46004600u>(t, m.high), f.f, f.minus_6f);
 }
 
 // Code kAt of each half of a word as a bf16 pair times the halves' factors:
 // bits 3-6 of 16 + u.
 template <int kAt>
-__device__ __forceinline__ uint32_t int4_to_bf16(uint32_t w, uint32_t f, uint32_t minus_24f) {
+__device__ __forceinline__ uint32_t int4_to_bf16(uint32_t w, uint32_t f, uint32_t minus_24f, const Int4Masks &m) {
   const uint32_t t = kAt == 0 ? w << 3 : w >> (kAt == 0 ? 0 : 4 * kAt - 3);
-  return bf162_fma((t & 0x00780078u) ^ 0x41c041c0u, f, minus_24f);
+  return bf162_fma(masked_xor<0x41c041c0u>(t, m.mantissa), f, minus_24f);
 }
 
 // Two factors as a bf16 pair, and -24 times it.  Any byte gives a number.
@@ -285,18 +306,20 @@ struct FewShape {
   static constexpr int kRowBytes = code_bytes(kFormat, D);
   static constexpr int kBoxes = kRowBytes > 128 ? 2 : 1;          // a swizzled row has at most 128 bytes
   static constexpr int kTile = 16 * kRowBytes;
+  static constexpr bool kInt4 = kFormat == kCacheInt4;
+  static constexpr int kSub = kInt4 ? 2 : 1;                      // tiles of 16 keys in a step
   static constexpr int kStages = 3;
   static constexpr int kCtas = few_ctas(kFormat, D, kNT);   // on an SM
-  static constexpr int kRing = kFewWarps * kStages * 2 * kTile;
-  static constexpr int kScales = kFewWarps * kStages * 2 * 16 * 4;
-  static constexpr int kFactorTile = kFormat == kCacheInt4 ? 16 * (D / kFactorGroup) : 0;
-  static constexpr int kFactors = kFewWarps * kStages * 2 * kFactorTile;
-  static constexpr int kCopied = kRing + kScales + kFactors;
+  static constexpr int kRing = kFewWarps * kStages * 2 * kSub * kTile;
+  // int4: of 16 keys, K's factors, V's factors, K's scales, V's scales, 64 bytes for each.
+  static constexpr int kBeside = 256;
+  static constexpr int kScales = kFewWarps * kStages * (kInt4 ? kSub * kBeside : 2 * 16 * 4);
+  static constexpr int kCopied = kRing + kScales;
   static constexpr int kSums = kFewWarps * kNT * 8 * (D + 4 + 2) * 4 + kNT * 8 * (D + 4) * 4;
   // The barriers lie behind both: their memory may hold nothing else (sums
   // written over them were seen to turn back into barriers).
   static constexpr int kBarriers = kCopied > kSums ? kCopied : kSums;
-  static constexpr int kSmem = 1024 /* alignment */ + kBarriers + kFewWarps * kStages * 8;
+  static constexpr int kSmem = kInt4 ? kBarriers : 1024 /* alignment */ + kBarriers + kFewWarps * kStages * 8;
 };
 
 // 4-D tiled load into this CTA's shared memory.
@@ -420,15 +443,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   constexpr int KW = Shape::kRowBytes / 16;        // words of a lane's quarter of a K row
   constexpr int VW = Shape::kRowBytes / 32;        // words of a lane's eighth of a V row
   constexpr int kRowBytes = Shape::kRowBytes, kStages = Shape::kStages, kTile = Shape::kTile;
-  extern __shared__ uint8_t few_raw[];
-  uint8_t *few_sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(few_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(16) uint8_t few_raw[];
+  uint8_t *few_sm =
+      kInt4 ? few_raw : reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(few_raw) + 1023) & ~uintptr_t(1023));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q4 = lane & 3;
   const int group = a.group;
-  uint8_t *ring = few_sm + warp * kStages * 2 * kTile;                                    // [kStages][K, V]
+  uint8_t *ring = few_sm + warp * kStages * 2 * Shape::kSub * kTile;                      // [kStages][K, V][kSub]
   float *scales = reinterpret_cast<float *>(few_sm + Shape::kRing) + warp * kStages * 32;   // [kStages][K, V][16]
-  uint8_t *factors = few_sm + Shape::kRing + Shape::kScales + warp * kStages * 2 * Shape::kFactorTile;   // [kStages][K, V][16][D / 32]
   uint64_t *full = reinterpret_cast<uint64_t *>(few_sm + Shape::kBarriers) + warp * kStages;
-  if (lane == 0) {
+  if (!kInt4 && lane == 0) {
     for (int i = 0; i < kStages; ++i)
       mbar_init(&full[i], 1);
     fence_barrier_init();
@@ -460,8 +483,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   const int first_new = first_new_position(a.lengths, b, n);
   const int keys = max(0, min(length, first_new + (r1 - 1) / group + 1));
   const int all_see = min(length, first_new + r0 / group + 1);   // every row sees positions below this
-  // This piece's 16-key steps, as equal as the pieces of the unit can be.
-  const int steps = (keys + 15) >> 4;
+  // This piece's steps of 16 (int4: 32) keys, as equal as the pieces of the unit can be.
+  constexpr int kStepLog2 = kInt4 ? 5 : 4;
+  const int steps = (keys + (1 << kStepLog2) - 1) >> kStepLog2;
   const int step_begin = int(int64_t(steps) * piece.index / piece.count);
   const int step_end = int(int64_t(steps) * (piece.index + 1) / piece.count);
 
@@ -478,7 +502,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
     if (lane == 0) {
       uint8_t *to = ring + stage * 2 * kTile;
       const int in_page = (step << 4) & page_mask;
-      mbar_arrive_expect_tx(&full[stage], 2 * (kTile + Shape::kFactorTile) + (kBf16 ? 0 : 128));
+      mbar_arrive_expect_tx(&full[stage], 2 * kTile + (kBf16 ? 0 : 128));
 #pragma unroll
       for (int h = 0; h < Shape::kBoxes; ++h) {
         tma_load_4d(to + h * 2048, &tm_k, &full[stage], h * 64, in_page, kvh, page);
@@ -488,17 +512,77 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
         const int64_t slot = (int64_t(kvh) << a.c.shift) + in_page;
         bulk_load(scales + stage * 32, a.c.ks + page * a.c.ks_page + slot, 64, &full[stage]);
         bulk_load(scales + stage * 32 + 16, a.c.vs + page * a.c.vs_page + slot, 64, &full[stage]);
-        if constexpr (kInt4) {
-          uint8_t *f = factors + stage * 2 * Shape::kFactorTile;
-          const int64_t at = slot * (D / kFactorGroup);
-          bulk_load(f, a.c.kf + page * a.c.kf_page + at, Shape::kFactorTile, &full[stage]);
-          bulk_load(f + Shape::kFactorTile, a.c.vf + page * a.c.vf_page + at, Shape::kFactorTile, &full[stage]);
-        }
       }
     }
   };
-  for (int i = 0; i < min(kStages, count); ++i)
-    copy(i);
+  // int4: small pieces of six arrays, copied by all lanes, 16 bytes each (a lane
+  // that issues six bulk copies per 16 keys spends more instructions on them than
+  // the warp on the products).  Lane i of 16 keys' codes has piece i of 32; of
+  // what lies beside them, 16 lanes for each half of the step.
+  uint8_t *beside = few_sm + Shape::kRing + warp * kStages * Shape::kSub * Shape::kBeside;   // [kStages][kSub][kBeside]
+  constexpr int kHeadUnit = D / kFactorGroup;           // bytes of a row's factors
+  const int which = (lane >> 2) & 3, unit = which < 2 ? kHeadUnit : 4;
+  const int64_t of_head = int64_t(kvh) << a.c.shift;
+  const uint8_t *k_src = static_cast<const uint8_t *>(a.c.k) + of_head * kRowBytes + lane * 16;
+  const uint8_t *v_src = static_cast<const uint8_t *>(a.c.v) + of_head * kRowBytes + lane * 16;
+  const Int4Masks masks = int4_masks();
+  const uint8_t *beside_src = (which == 0   ? a.c.kf
+                               : which == 1 ? a.c.vf
+                               : which == 2 ? reinterpret_cast<const uint8_t *>(a.c.ks)
+                                            : reinterpret_cast<const uint8_t *>(a.c.vs)) + of_head * unit + (lane & 3) * 16;
+  // From page to page in units of 16 bytes, below 2^32: one product of 32 bits each.
+  const uint32_t beside_page = uint32_t((which == 0   ? a.c.kf_page
+                                         : which == 1 ? a.c.vf_page
+                                         : which == 2 ? a.c.ks_page * 4
+                                                      : a.c.vs_page * 4) >> 4);
+  const uint32_t k_page = uint32_t(a.c.k_page >> 4), v_page = uint32_t(a.c.v_page >> 4);
+  auto at_page = [](const uint8_t *p, int page, uint32_t stride, int beyond) { return p + (uint64_t(uint32_t(page)) * stride << 4) + beyond; };
+  const bool beside_mine = (lane & 3) * 16 < 16 * unit;
+  const int piece_at = kRowBytes == 64 ? (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4) : lane * 16;
+  auto copy4 = [&](int i, int stage) {
+    if (i < count) {
+      const int key0 = (step0 + i * kFewWarps) << 5, in_page = key0 & page_mask;
+      uint8_t *to = ring + stage * 4 * kTile + piece_at, *beside_to = beside + stage * 512 + lane * 16;
+      if (a.c.shift > 4) {                          // 32 keys of a page
+        if ((i & 31) == 0)                          // the pages of the next 32 steps
+          pages_of_lane = i + lane < count ? max(0, page_of(a.c, b, key0 + lane * (32 * kFewWarps))) : 0;
+        const int page = __shfl_sync(0xffffffffu, pages_of_lane, i & 31);
+        const uint8_t *k_at = at_page(k_src, page, k_page, in_page * kRowBytes), *v_at = at_page(v_src, page, v_page, in_page * kRowBytes);
+#pragma unroll
+        for (int j = 0; j < 2 * kTile / 512; ++j) {
+          cp_async_16(to + j * 512, k_at + j * 512);
+          cp_async_16(to + 2 * kTile + j * 512, v_at + j * 512);
+        }
+        if (beside_mine)
+          cp_async_16(beside_to, at_page(beside_src, page, beside_page, (in_page + (lane & 16)) * unit));
+      } else {                                      // 16 keys each of two pages
+        if ((i & 15) == 0) {
+          const int key = key0 + (lane >> 1) * (32 * kFewWarps) + (lane & 1) * 16;
+          pages_of_lane = i + (lane >> 1) < count && key < keys ? max(0, page_of(a.c, b, key)) : 0;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int page = __shfl_sync(0xffffffffu, pages_of_lane, (2 * i + h) & 31);
+          const uint8_t *k_at = at_page(k_src, page, k_page, 0), *v_at = at_page(v_src, page, v_page, 0);
+#pragma unroll
+          for (int j = 0; j < kTile / 512; ++j) {
+            cp_async_16(to + h * kTile + j * 512, k_at + j * 512);
+            cp_async_16(to + (2 + h) * kTile + j * 512, v_at + j * 512);
+          }
+          if (lane >> 4 == h && beside_mine)
+            cp_async_16(beside_to, at_page(beside_src, page, beside_page, 0));
+        }
+      }
+    }
+    cp_async_commit();
+  };
+  if constexpr (kInt4) {
+    for (int i = 0; i < kStages - 1; ++i)
+      copy4(i, i);
+  } else {
+    for (int i = 0; i < min(kStages, count); ++i)
+      copy(i);
+  }
 
   uint32_t qf[kNT][KS][2];
   int limit[kNT][2];
@@ -572,16 +656,147 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   const int v_even = offset_of<kRowBytes>(2 * q4, g / kPart) + g % kPart * (VW * 4);
   const int v_odd = offset_of<kRowBytes>(odd, g / kPart) + g % kPart * (VW * 4);
   int done = 0;
+  if constexpr (kInt4) {
+    constexpr int kGroups = D / kFactorGroup;
+    int stage = 0, next = kStages - 1;
+    for (; done < count; ++done, stage = stage == kStages - 1 ? 0 : stage + 1, next = next == kStages - 1 ? 0 : next + 1) {
+      const int key0 = (step0 + done * kFewWarps) << 5;
+      cp_async_wait_group<kStages - 2>();
+      __syncwarp();                                 // all lanes' copies of this stage; all have read the last one
+      copy4(done + kStages - 1, next);
+      const uint8_t *k_tile = ring + stage * 4 * kTile, *v_tile = k_tile + 2 * kTile;
+      const uint8_t *side = beside + stage * 2 * Shape::kBeside;
+      float sc[2][kNT][4] = {};
+      bool raise = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t kr[2][KW];                         // K rows mine, mine + 8
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint8_t *at = k_tile + h * kTile + k_off + x * kEight;
+          if constexpr (KW == 4)
+            *reinterpret_cast<uint4 *>(kr[x]) = *reinterpret_cast<const uint4 *>(at);
+          else
+            *reinterpret_cast<uint2 *>(kr[x]) = *reinterpret_cast<const uint2 *>(at);
+        }
+        const uint8_t *f = side + h * Shape::kBeside + q4 * (D / 4) / kFactorGroup;
+        uint32_t two;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(two) : "h"(uint16_t(f[mine * kGroups] | (f[(mine + 8) * kGroups] << 8))));
+        const Int4Factors lo = int4_factors(__byte_perm(two, two, 0x1010)), hi = int4_factors(__byte_perm(two, two, 0x3232));
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          uint32_t af[4];
+          if (s & 1) {
+            int4_to_half<1>(kr[0][s / 2], lo, masks, af[0], af[2]);
+            int4_to_half<1>(kr[1][s / 2], hi, masks, af[1], af[3]);
+          } else {
+            int4_to_half<0>(kr[0][s / 2], lo, masks, af[0], af[2]);
+            int4_to_half<0>(kr[1][s / 2], hi, masks, af[1], af[3]);
+          }
+#pragma unroll
+          for (int t = 0; t < kNT; ++t)
+            mma_half_16816(sc[h][t], af, qf[t][s][0], qf[t][s][1]);
+        }
+        const float *k_scale = reinterpret_cast<const float *>(side + h * Shape::kBeside + 128) + mine;
+        const float k_lo = k_scale[0], k_hi = k_scale[8];
+        const bool masked = key0 + h * 16 + 16 > all_see;
+#pragma unroll
+        for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // The factors first: a large key's scale alone could overflow the product.
+            float v = sc[h][t][e] * ((e < 2 ? k_lo : k_hi) * to_log2[t][e & 1]);
+            if (masked && key0 + h * 16 + mine + (e & 2) * 4 > limit[t][e & 1])
+              v = -INFINITY;
+            sc[h][t][e] = v;
+            raise |= v > top[t][e & 1] + 8.f;
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float m = fmaxf(fmaxf(top[t][e], fmaxf(sc[0][t][e], sc[0][t][e + 2])), fmaxf(sc[1][t][e], sc[1][t][e + 2]));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            const float keep = top[t][e] == -INFINITY ? 1.f : exp2_fast(top[t][e] - m);   // nothing summed yet: keep it
+            top[t][e] = m;
+            mu[t][e] = m == -INFINITY ? 0.f : m;
+            l[t][e] *= keep;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              o[t][s][e] *= keep;
+              o[t][s][e + 2] *= keep;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t vr[4][VW];                         // V rows 2 q4, odd, and 8 after them
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint8_t *at = v_tile + h * kTile + (x & 1 ? v_odd : v_even) + (x >> 1) * kEight;
+          if constexpr (VW == 2)
+            *reinterpret_cast<uint2 *>(vr[x]) = *reinterpret_cast<const uint2 *>(at);
+          else
+            vr[x][0] = *reinterpret_cast<const uint32_t *>(at);
+        }
+        const uint8_t *f = side + h * Shape::kBeside + 64 + g * (D / 8) / kFactorGroup;
+        uint32_t vf[2], minus_24vf[2];              // of keys 2 q4 and odd, and 8 after them
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          vf[x] = factor_pair_bf16(f[(2 * q4 + 8 * x) * kGroups], f[(odd + 8 * x) * kGroups], minus_24vf[x]);
+        const float *v_scale = reinterpret_cast<const float *>(side + h * Shape::kBeside + 192) + mine;
+        const float vsc[2] = {v_scale[0], v_scale[8]};
+        const bool masked = key0 + h * 16 + 16 > all_see;
+        uint32_t pf[kNT][2];
+#pragma unroll
+        for (int t = 0; t < kNT; ++t) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = exp2_fast(sc[h][t][e] - mu[t][e & 1]);
+            l[t][e & 1] += x;
+            // A hidden key's scale may be anything.
+            w[e] = masked && sc[h][t][e] == -INFINITY ? 0.f : x * vsc[e >> 1];
+          }
+          pf[t][0] = transpose_8x8(pack_bf16x2(w[0], w[1]));
+          pf[t][1] = transpose_8x8(pack_bf16x2(w[2], w[3]));
+        }
+#pragma unroll
+        for (int j = 0; j < VW; ++j) {
+          // Channels 0-3 of the two keys in one word, 4-7 in the next.
+          uint32_t af[4][4];
+#pragma unroll
+          for (int x = 0; x < 2; ++x)      // keys 2 q4 .. and 2 q4 + 8 ..
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t y = __byte_perm(vr[2 * x][j], vr[2 * x + 1][j], c ? 0x7632 : 0x5410);
+              af[2 * c][2 * x] = int4_to_bf16<0>(y, vf[x], minus_24vf[x], masks);
+              af[2 * c][2 * x + 1] = int4_to_bf16<1>(y, vf[x], minus_24vf[x], masks);
+              af[2 * c + 1][2 * x] = int4_to_bf16<2>(y, vf[x], minus_24vf[x], masks);
+              af[2 * c + 1][2 * x + 1] = int4_to_bf16<3>(y, vf[x], minus_24vf[x], masks);
+            }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < kNT; ++t)
+              mma_bf16_16816(o[t][4 * j + i], af[i], pf[t][0], pf[t][1]);
+        }
+      }
+    }
+  }
+  if constexpr (!kInt4)
   for (; done < count; ++done) {
     const int step = step0 + done * kFewWarps, stage = done % kStages;
     if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], uint32_t((done / kStages) & 1), kStatusTimeoutProducer)))
       break;
     const uint8_t *k_tile = ring + stage * 2 * kTile, *v_tile = k_tile + kTile;
     uint32_t kr[2][KW], vr[4][VW];                  // K rows mine, mine + 8; V rows 2 q4, odd, and 8 after them
-    if constexpr (KW == 2) {
-      *reinterpret_cast<uint2 *>(kr[0]) = *reinterpret_cast<const uint2 *>(k_tile + k_off);
-      *reinterpret_cast<uint2 *>(kr[1]) = *reinterpret_cast<const uint2 *>(k_tile + k_off + kEight);
-    }
 #pragma unroll
     for (int i = 0; i < KW / 4; ++i) {
       const uint8_t *at = k_tile + (i >> 1) * 2048 + (i & 1 ? k_off ^ 64 : k_off);
@@ -593,34 +808,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
       const float *s = scales + stage * 32 + mine;
       ksc[0] = s[0], ksc[1] = s[8], vsc[0] = s[16], vsc[1] = s[24];
     }
-    Int4Factors k_lo4, k_hi4;
-    uint32_t vf[2], minus_24vf[2];                  // of keys 2 q4 and odd, and 8 after them
-    if constexpr (kInt4) {
-      constexpr int kGroups = D / kFactorGroup;
-      const uint8_t *f = factors + stage * 2 * Shape::kFactorTile + q4 * (D / 4) / kFactorGroup;
-      uint32_t two;
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(two) : "h"(uint16_t(f[mine * kGroups] | (f[(mine + 8) * kGroups] << 8))));
-      k_lo4 = int4_factors(__byte_perm(two, two, 0x1010));
-      k_hi4 = int4_factors(__byte_perm(two, two, 0x3232));
-      f = factors + (stage * 2 + 1) * Shape::kFactorTile + g * (D / 8) / kFactorGroup;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        vf[h] = factor_pair_bf16(f[(2 * q4 + 8 * h) * kGroups], f[(odd + 8 * h) * kGroups], minus_24vf[h]);
-    }
     float sc[kNT][4] = {};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       uint32_t af[4];
       if constexpr (kBf16) {
         af[0] = kr[0][2 * s], af[1] = kr[1][2 * s], af[2] = kr[0][2 * s + 1], af[3] = kr[1][2 * s + 1];
-      } else if constexpr (kInt4) {
-        if (s & 1) {
-          int4_to_half<1>(kr[0][s / 2], k_lo4, af[0], af[2]);
-          int4_to_half<1>(kr[1][s / 2], k_hi4, af[1], af[3]);
-        } else {
-          int4_to_half<0>(kr[0][s / 2], k_lo4, af[0], af[2]);
-          int4_to_half<0>(kr[1][s / 2], k_hi4, af[1], af[3]);
-        }
       } else {
         codes_to_half<kFormat>(kr[0][s], af[0], af[2]);
         codes_to_half<kFormat>(kr[1][s], af[1], af[3]);
@@ -637,9 +830,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const uint8_t *at = v_tile + (x & 1 ? v_odd : v_even) + (x >> 1) * kEight;
-      if constexpr (VW == 1) {
-        vr[x][0] = *reinterpret_cast<const uint32_t *>(at);
-      } else if constexpr (VW == 2) {
+      if constexpr (VW == 2) {
         *reinterpret_cast<uint2 *>(vr[x]) = *reinterpret_cast<const uint2 *>(at);
       } else {
 #pragma unroll
@@ -709,24 +900,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
 #pragma unroll
           for (int t = 0; t < kNT; ++t)
             mma_bf16_16816(o[t][j], af, pp[t][0], pp[t][1]);
-        } else if constexpr (kInt4) {
-          // Channels 0-3 of the two keys in one word, 4-7 in the next.
-          uint32_t af[4][4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h)      // keys 2 q4 .. and 2 q4 + 8 ..
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const uint32_t x = __byte_perm(vr[2 * h][j], vr[2 * h + 1][j], c ? 0x7632 : 0x5410);
-              af[2 * c][2 * h] = int4_to_bf16<0>(x, vf[h], minus_24vf[h]);
-              af[2 * c][2 * h + 1] = int4_to_bf16<1>(x, vf[h], minus_24vf[h]);
-              af[2 * c + 1][2 * h] = int4_to_bf16<2>(x, vf[h], minus_24vf[h]);
-              af[2 * c + 1][2 * h + 1] = int4_to_bf16<3>(x, vf[h], minus_24vf[h]);
-            }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int t = 0; t < kNT; ++t)
-              mma_bf16_16816(o[t][4 * j + i], af[i], pp[t][0], pp[t][1]);
         } else {
           uint32_t af[2][4];
 #pragma unroll
@@ -814,6 +987,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   }
 
   // No copy is in flight past this point (at once, unless a wait gave up).
+  if constexpr (kInt4)
+    cp_async_wait_group<0>();
+  else
   for (int i = done; i < min(done + kStages, count); ++i)
     mbar_wait(&full[i % kStages], uint32_t((i / kStages) & 1), kStatusTimeoutProducer);
   __syncthreads();

@@ -777,6 +777,7 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
         // a time (of int4 the channels of one factor).  Rows past the keys hold
         // old codes, which are numbers.
         constexpr int kRuns = Shape::kRowCodes / 16, kRowStep = 128 / kRuns;
+        const Int4Masks masks = int4_masks();
         const int t = tid - (kMmaWarp + 3) * 32, run = t % kRuns, row0 = t / kRuns;
         for (int item = 0; t >= 0 && item < 2 * blocks; ++item) {
           const int from = item % Shape::kRaw, stage = item % kStages;
@@ -799,8 +800,8 @@ __global__ void __launch_bounds__(TileShape<kSource, D, kTiles>::kThreads, kTile
               const uint32_t f = factor_pair_bf16(byte, byte, minus_24f), w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
-                const uint32_t p0 = int4_to_bf16<0>(w[c], f, minus_24f), p1 = int4_to_bf16<1>(w[c], f, minus_24f);
-                const uint32_t p2 = int4_to_bf16<2>(w[c], f, minus_24f), p3 = int4_to_bf16<3>(w[c], f, minus_24f);
+                const uint32_t p0 = int4_to_bf16<0>(w[c], f, minus_24f, masks), p1 = int4_to_bf16<1>(w[c], f, minus_24f, masks);
+                const uint32_t p2 = int4_to_bf16<2>(w[c], f, minus_24f, masks), p3 = int4_to_bf16<3>(w[c], f, minus_24f, masks);
                 *reinterpret_cast<uint4 *>(dst + row * 128 + (((piece + c) ^ (row & 7)) << 4)) =
                     make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632),
                                __byte_perm(p2, p3, 0x7632));

@@ -77,6 +77,10 @@ static int make_pages(const char *what, const pir2b_kv_pages *p, const pir2b_seq
         p->k_factor_page_stride < factors || p->v_factor_page_stride < factors || p->k_factor_page_stride % 16 != 0 ||
         p->v_factor_page_stride % 16 != 0)
       return fail(PIR2B_EINVAL, "%s: int4 pages need 16-byte aligned factors", what);
+    const int64_t most = int64_t(1) << 36;   // the kernels count strides in 32 bits of 16 bytes
+    if (p->k_page_stride >= most || p->v_page_stride >= most || p->k_scale_page_stride >= most / 4 ||
+        p->v_scale_page_stride >= most / 4 || p->k_factor_page_stride >= most || p->v_factor_page_stride >= most)
+      return fail(PIR2B_EINVAL, "%s: page strides of int4 pages must be below 2^36 bytes", what);
     out->kf = p->k_factor;
     out->vf = p->v_factor;
     out->kf_page = p->k_factor_page_stride;
