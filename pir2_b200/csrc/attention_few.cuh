@@ -25,6 +25,7 @@
 // conversion of codes, which no warp-level MMA takes beside 16-bit weights.
 #pragma once
 #include <cuda.h>
+#include <type_traits>
 #include "attention_ragged.cuh"
 
 namespace pir2b {
@@ -109,7 +110,7 @@ __device__ __forceinline__ Int4Factors int4_factors(uint32_t pair) {   // of an 
 template <uint32_t kBits>
 __device__ __forceinline__ uint32_t masked_xor(uint32_t x, uint32_t mask) {
   uint32_t y;
-  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(y) : "r"(x), "r"(mask), "n"(kBits));
+  asm("lop3.b32 %0, %1, %2, %3, 0x6c;" : "=r"(y) : "r"(x), "n"(kBits), "r"(mask));
   return y;
 }
 
@@ -308,13 +309,15 @@ struct FewShape {
   static constexpr int kTile = 16 * kRowBytes;
   static constexpr bool kInt4 = kFormat == kCacheInt4;
   static constexpr int kSub = kInt4 ? 2 : 1;                      // tiles of 16 keys in a step
-  static constexpr int kStages = 3;
+  static constexpr int kStages = kInt4 ? 2 : 3;
   static constexpr int kCtas = few_ctas(kFormat, D, kNT);   // on an SM
   static constexpr int kRing = kFewWarps * kStages * 2 * kSub * kTile;
   // int4: of 16 keys, K's factors, V's factors, K's scales, V's scales, 64 bytes for each.
   static constexpr int kBeside = 256;
   static constexpr int kScales = kFewWarps * kStages * (kInt4 ? kSub * kBeside : 2 * 16 * 4);
-  static constexpr int kCopied = kRing + kScales;
+  // int4: q's fragments, which its longer conversions leave no registers for.
+  static constexpr int kQuery = kInt4 ? kFewWarps * kNT * (D / 16) * 2 * 32 * 4 : 0;
+  static constexpr int kCopied = kRing + kScales + kQuery;
   static constexpr int kSums = kFewWarps * kNT * 8 * (D + 4 + 2) * 4 + kNT * 8 * (D + 4) * 4;
   // The barriers lie behind both: their memory may hold nothing else (sums
   // written over them were seen to turn back into barriers).
@@ -637,6 +640,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
     }
   }
 
+  uint4 *query = reinterpret_cast<uint4 *>(few_sm + Shape::kRing + Shape::kScales) + warp * kNT * (KS / 2) * 32 + lane;
+  if constexpr (kInt4) {
+#pragma unroll
+    for (int t = 0; t < kNT; ++t)
+#pragma unroll
+      for (int s = 0; s < KS; s += 2)
+        query[(t * KS + s) / 2 * 32] = make_uint4(qf[t][s][0], qf[t][s][1], qf[t][s + 1][0], qf[t][s + 1][1]);
+    __syncwarp();
+  }
   float o[kNT][KS][4] = {};
   float l[kNT][2] = {}, mu[kNT][2] = {};           // mu: the maximum subtracted (0 while none)
   float top[kNT][2];                               // the running maximum
@@ -666,8 +678,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
       copy4(done + kStages - 1, next);
       const uint8_t *k_tile = ring + stage * 4 * kTile, *v_tile = k_tile + 2 * kTile;
       const uint8_t *side = beside + stage * 2 * Shape::kBeside;
+      auto work = [&](auto some_hidden) {
+      constexpr bool kMasked = some_hidden.value;
       float sc[2][kNT][4] = {};
-      bool raise = false;
+      uint4 qs[kNT][KS / 2];
+#pragma unroll
+      for (int t = 0; t < kNT; ++t)
+#pragma unroll
+        for (int s = 0; s < KS / 2; ++s)
+          qs[t][s] = query[(t * (KS / 2) + s) * 32];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t kr[2][KW];                         // K rows mine, mine + 8
@@ -695,24 +714,28 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
           }
 #pragma unroll
           for (int t = 0; t < kNT; ++t)
-            mma_half_16816(sc[h][t], af, qf[t][s][0], qf[t][s][1]);
+            mma_half_16816(sc[h][t], af, s & 1 ? qs[t][s / 2].z : qs[t][s / 2].x, s & 1 ? qs[t][s / 2].w : qs[t][s / 2].y);
         }
         const float *k_scale = reinterpret_cast<const float *>(side + h * Shape::kBeside + 128) + mine;
         const float k_lo = k_scale[0], k_hi = k_scale[8];
-        const bool masked = key0 + h * 16 + 16 > all_see;
 #pragma unroll
         for (int t = 0; t < kNT; ++t) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             // The factors first: a large key's scale alone could overflow the product.
             float v = sc[h][t][e] * ((e < 2 ? k_lo : k_hi) * to_log2[t][e & 1]);
-            if (masked && key0 + h * 16 + mine + (e & 2) * 4 > limit[t][e & 1])
+            if (kMasked && key0 + h * 16 + mine + (e & 2) * 4 > limit[t][e & 1])
               v = -INFINITY;
             sc[h][t][e] = v;
-            raise |= v > top[t][e & 1] + 8.f;
           }
         }
       }
+      bool raise = false;
+#pragma unroll
+      for (int t = 0; t < kNT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          raise |= fmaxf(fmaxf(sc[0][t][e], sc[0][t][e + 2]), fmaxf(sc[1][t][e], sc[1][t][e + 2])) > top[t][e] + 8.f;
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
         for (int t = 0; t < kNT; ++t) {
@@ -752,7 +775,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
           vf[x] = factor_pair_bf16(f[(2 * q4 + 8 * x) * kGroups], f[(odd + 8 * x) * kGroups], minus_24vf[x]);
         const float *v_scale = reinterpret_cast<const float *>(side + h * Shape::kBeside + 192) + mine;
         const float vsc[2] = {v_scale[0], v_scale[8]};
-        const bool masked = key0 + h * 16 + 16 > all_see;
         uint32_t pf[kNT][2];
 #pragma unroll
         for (int t = 0; t < kNT; ++t) {
@@ -762,7 +784,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
             const float x = exp2_fast(sc[h][t][e] - mu[t][e & 1]);
             l[t][e & 1] += x;
             // A hidden key's scale may be anything.
-            w[e] = masked && sc[h][t][e] == -INFINITY ? 0.f : x * vsc[e >> 1];
+            w[e] = kMasked && sc[h][t][e] == -INFINITY ? 0.f : x * vsc[e >> 1];
           }
           pf[t][0] = transpose_8x8(pack_bf16x2(w[0], w[1]));
           pf[t][1] = transpose_8x8(pack_bf16x2(w[2], w[3]));
@@ -788,6 +810,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
               mma_bf16_16816(o[t][4 * j + i], af[i], pf[t][0], pf[t][1]);
         }
       }
+      };
+      // Few steps have positions that some row does not see.
+      if (key0 + 32 > all_see)
+        work(std::true_type{});
+      else
+        work(std::false_type{});
     }
   }
   if constexpr (!kInt4)
