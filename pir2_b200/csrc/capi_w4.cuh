@@ -7,21 +7,50 @@ namespace pir2b {
 
 constexpr int kW4Rows = 64;   // rows of a launch
 
+// How many warps split K in the staged kernel: the fewest rounds of chunks of
+// 128, a round's meeting counted as one more.
+static int w4_split(const W4Args &a, int warps, int ctas) {
+  const int64_t blocks = (a.n + 15) / 16, units = a.k / 256;
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int wk = 1; wk <= warps; wk *= 2) {
+    const int64_t wc = warps / wk, rounds = ((blocks + wc - 1) / wc + ctas - 1) / ctas;
+    const int64_t cost = rounds * (2 * ((units + wk - 1) / wk) + (wk > 1));
+    if (cost < least)
+      least = cost, best = wk;
+  }
+  return best;
+}
+
+static std::atomic<int> g_w4_mode{0};   // probe
+
 template <int kGroup, int kTiles>
-static int launch_w4(const W4Args &a, void *stream) {
+static int launch_w4(W4Args a, const DeviceInfo *dev, void *stream) {
+  using Shape = W4Shape<kTiles>;
+  const int smem = Shape::bytes(a.k, kGroup), limit = 227 * 1024;
+  const int mode = g_w4_mode.load();
+  const bool fits = a.k % 256 == 0 && smem <= limit && aligned(a.scales, 16);
+  if (fits && (mode == 2 || (mode == 0 && a.n >= 8192))) {
+    const int resident = kTiles > 1 ? 1 : std::min(3, 228 * 1024 / (smem + 1024));
+    const int64_t ctas = int64_t(dev->sms) * resident;
+    a.wk = w4_split(a, Shape::kWarps, int(ctas));
+    const int64_t wc = Shape::kWarps / a.wk, grid = std::min<int64_t>(ctas, ((a.n + 15) / 16 + wc - 1) / wc);
+    cudaFuncSetAttribute(gemm_w4_staged_kernel<kGroup, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
+    return launch_cache("gemm_w4a16 launch", gemm_w4_staged_kernel<kGroup, kTiles>, grid, 1, 1, Shape::kWarps * 32, smem, stream, a);
+  }
   return launch_cache("gemm_w4a16 launch", gemm_w4_kernel<kGroup, kTiles>, (a.n + kW4Channels - 1) / kW4Channels, 1, 1,
                       kW4Warps * 32, 0, stream, a);
 }
 
 template <int kGroup>
-static int launch_w4(const W4Args &a, void *stream) {
+static int launch_w4(const W4Args &a, const DeviceInfo *dev, void *stream) {
   if (a.m <= 8)
-    return launch_w4<kGroup, 1>(a, stream);
+    return launch_w4<kGroup, 1>(a, dev, stream);
   if (a.m <= 16)
-    return launch_w4<kGroup, 2>(a, stream);
+    return launch_w4<kGroup, 2>(a, dev, stream);
   if (a.m <= 32)
-    return launch_w4<kGroup, 4>(a, stream);
-  return launch_w4<kGroup, 8>(a, stream);
+    return launch_w4<kGroup, 4>(a, dev, stream);
+  return launch_w4<kGroup, 8>(a, dev, stream);
 }
 
 } // namespace pir2b
@@ -29,6 +58,8 @@ static int launch_w4(const W4Args &a, void *stream) {
 using namespace pir2b;
 
 extern "C" {
+
+int pir2b_set_w4_mode(int mode) { return g_w4_mode.exchange(mode); }
 
 int pir2b_gemm_w4a16(const void *x, int64_t ldx, const void *packed, const void *scales, int group,
                      const void *bias, int64_t m, int64_t n, int64_t k, void *out, int64_t ldo,
@@ -56,11 +87,12 @@ int pir2b_gemm_w4a16(const void *x, int64_t ldx, const void *packed, const void 
   a.ldo = ldo;
   a.n = int(n);
   a.k = int(k);
+  a.pairs = ldo % 2 == 0 && aligned(out, 4);
   for (int64_t first = 0; first < m; first += kW4Rows) {   // more rows read the weights again
     a.x = static_cast<const __nv_bfloat16 *>(x) + first * ldx;
     a.out = static_cast<__nv_bfloat16 *>(out) + first * ldo;
     a.m = int(std::min<int64_t>(kW4Rows, m - first));
-    if (int r = group == 32 ? launch_w4<32>(a, stream) : group == 64 ? launch_w4<64>(a, stream) : launch_w4<128>(a, stream))
+    if (int r = group == 32 ? launch_w4<32>(a, dev, stream) : group == 64 ? launch_w4<64>(a, dev, stream) : launch_w4<128>(a, dev, stream))
       return r;
   }
   return PIR2B_OK;

@@ -26,13 +26,15 @@ struct W4Args {
   __nv_bfloat16 *out;            // [m, n], row stride ldo
   int64_t ldo;
   int m, n, k;
+  int wk;                        // staged: warps that split K
+  int pairs;                     // output channels may be stored two at a time
 };
 
 // Code kAt of each half of a word as a bf16 pair.
 template <int kAt>
-__device__ __forceinline__ uint32_t w4_pair(uint32_t w) {
+__device__ __forceinline__ uint32_t w4_pair(uint32_t w, const Int4Masks &m) {
   const uint32_t t = kAt == 0 ? w << 3 : w >> (kAt == 0 ? 0 : 4 * kAt - 3);
-  return bf162_fma((t & 0x00780078u) ^ 0x41c041c0u, 0x3f803f80u, 0xc1c0c1c0u);
+  return bf162_fma(masked_xor<0x41c041c0u>(t, m.mantissa), 0x3f803f80u, 0xc1c0c1c0u);
 }
 
 // kPieces pieces of 4 / kPieces words.
@@ -65,6 +67,7 @@ __global__ void __launch_bounds__(kW4Warps * 32) gemm_w4_kernel(const W4Args a) 
   const int begin = warp * chunks / kW4Warps, end = (warp + 1) * chunks / kW4Warps;
   const int row[2] = {min(c0 + g, a.n - 1), min(c0 + g + 8, a.n - 1)};   // rows past the last are not stored
   float acc[kTiles][4] = {};
+  const Int4Masks masks = int4_masks();
   pdl_wait();
   pdl_launch_dependents();
 #pragma unroll 1
@@ -85,8 +88,8 @@ __global__ void __launch_bounds__(kW4Warps * 32) gemm_w4_kernel(const W4Args a) 
 #pragma unroll
       for (int i = 0; i < kWords; ++i) {
         const uint32_t u = w[0][p * kWords + i], v = w[1][p * kWords + i];
-        const uint32_t even[4] = {w4_pair<0>(u), w4_pair<0>(v), w4_pair<1>(u), w4_pair<1>(v)};
-        const uint32_t odd[4] = {w4_pair<2>(u), w4_pair<2>(v), w4_pair<3>(u), w4_pair<3>(v)};
+        const uint32_t even[4] = {w4_pair<0>(u, masks), w4_pair<0>(v, masks), w4_pair<1>(u, masks), w4_pair<1>(v, masks)};
+        const uint32_t odd[4] = {w4_pair<2>(u, masks), w4_pair<2>(v, masks), w4_pair<3>(u, masks), w4_pair<3>(v, masks)};
         const int k = ch * 128 + p * kGroup + q4 * (kGroup / 4) + i * 8;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
@@ -123,6 +126,291 @@ __global__ void __launch_bounds__(kW4Warps * 32) gemm_w4_kernel(const W4Args a) 
       sum += __bfloat162float(a.bias[c0 + c]);
     a.out[token * a.ldo + c0 + c] = __float2bfloat16_rn(sum);
   }
+}
+
+// Many channels: a persistent CTA keeps all rows in shared memory, as the lanes
+// take them, and streams the weights of its blocks of 16 channels through a ring
+// per warp; `wk` warps split K, and their sums meet in shared memory.
+//
+// x enters as fp16: a power of two brings a row's largest value to 2^10, below
+// which fp16 holds the row to 2^-35 of that value.  fp16 has room for a code in
+// two places: with u = code + 8, bits 2-5 make 64 + u / 4 (even k) and bits 6-9 4 +
+// u / 4 (odd k), so a word of eight needs two shifts, and none of the eight a
+// subtraction: a group's sums start at -66 (-6) times the sum of its even (odd) x,
+// which is made once per CTA.  The fp32 sums then pass through values some 100
+// times a typical result, which costs 2^-14 of it.  Where a row holds a value that
+// is not finite the codes themselves are taken instead.
+template <int kTiles>
+struct W4Shape {
+  static constexpr int kWarps = kTiles == 1 ? 8 : 16;
+  static constexpr int kStages = 2;
+  static constexpr int kCols = 8 * kTiles;
+  static constexpr int kStage = 2 * (1024 + 128);        // of two chunks: codes of 16 channels, 16 bytes for each one's scales
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kRedRow = 20;                     // words of a token's 16 sums, apart by banks
+  static constexpr int kRed = kWarps * kCols * kRedRow * 4;
+  static constexpr int bytes(int64_t k, int group) {
+    return int(k * kCols * 2 + k / group * kCols * 4) + kRing + kRed + kCols * 4;
+  }
+};
+
+// Place of 16-byte piece c of row r: pieces of eight rows read in any width lie
+// in different banks.
+__device__ __forceinline__ int w4_place(int r, int c) { return r * 64 + ((c ^ ((r & 2) | ((r >> 2) & 1))) << 4); }
+
+template <int kBytes>
+__device__ __forceinline__ void cp_async_ca(uint32_t dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
+}
+
+template <int kGroup, int kTiles>
+__global__ void __launch_bounds__(W4Shape<kTiles>::kWarps * 32, kTiles == 1 ? 3 : 1) gemm_w4_staged_kernel(const W4Args a) {
+  using Shape = W4Shape<kTiles>;
+  constexpr int kPieces = 128 / kGroup, kWords = 4 / kPieces, kCols = Shape::kCols, kWarps = Shape::kWarps;
+  constexpr int kStages = Shape::kStages;
+  extern __shared__ __align__(1024) uint8_t tile_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  const int units = a.k >> 8, groups = a.k / kGroup;      // units of two chunks
+  uint4 *xs = reinterpret_cast<uint4 *>(tile_raw);                           // [chunk][word][tile][lane]
+  float *offsets = reinterpret_cast<float *>(tile_raw + int64_t(a.k) * kCols * 2);   // [group][token]
+  uint8_t *ring = reinterpret_cast<uint8_t *>(offsets + groups * kCols) + warp * kStages * Shape::kStage;
+  float *red = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(offsets + groups * kCols) + Shape::kRing);
+  uint32_t *most = reinterpret_cast<uint32_t *>(red + Shape::kRed / 4);      // [token] largest magnitude
+  const int wk = a.wk, wc = kWarps / wk, part = warp % wk, which = warp / wk;
+  const int begin = part * units / wk, end = (part + 1) * units / wk;
+  const int blocks = (a.n + 15) >> 4, stride = gridDim.x * wc;
+  const Int4Masks masks = int4_masks();
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // The next two chunks to copy: a row for every two lanes, which have alternate
+  // 16-byte pieces of it.  Rows past the last are left as they are.
+  int next_block = int(blockIdx.x) * wc + which, next = begin;
+  bool mine = false;
+  const uint8_t *src = nullptr;
+  const __nv_bfloat16 *scale_src = nullptr;
+  const uint32_t ring_at = smem_u32(ring);
+  int turn = Shape::kStage;
+  uint32_t to = ring_at + w4_place(lane >> 1, lane & 1), scale_to = ring_at + 2048 + (lane >> 1) * 16;
+  auto at_block = [&]() {
+    const int row = next_block * 16 + (lane >> 1);
+    mine = row < a.n;
+    src = a.w + int64_t(row) * (a.k >> 1) + begin * 128 + (lane & 1) * 16;
+    scale_src = a.scales + int64_t(row) * groups + begin * 2 * kPieces;
+  };
+  auto copy = [&]() {
+    if (next_block < blocks && begin < end) {
+      if (mine) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          cp_async_16_at((i & 1 ? to ^ 32 : to) + (i >> 1) * 1024, src + i * 32);
+        if ((lane & 1) == 0) {
+          if constexpr (kPieces == 4)
+            cp_async_16_at(scale_to, scale_src);
+          else
+            cp_async_ca<4 * kPieces>(scale_to, scale_src);
+        }
+      }
+      src += 128;
+      scale_src += 2 * kPieces;
+      if (++next == end) {
+        next = begin;
+        next_block += stride;
+        at_block();
+      }
+    }
+    to += turn, scale_to += turn, turn = -turn;     // the other stage
+    cp_async_commit();
+  };
+  at_block();
+  copy();
+
+  // The rows' largest finite magnitudes, 256 values of a row at a time.
+  for (int i = threadIdx.x; i < kCols; i += kWarps * 32)
+    most[i] = 0;
+  __syncthreads();
+  bool odd_values = false;
+  const int segments = units;
+  for (int i = warp; i < a.m * segments; i += kWarps) {
+    const int token = i / segments, at = (i % segments) * 256 + lane * 8;
+    const uint4 x = *reinterpret_cast<const uint4 *>(a.x + token * a.ldx + at);
+    uint32_t m = magnitude8(x);
+    if (m >= 0x7f80u) {
+      odd_values = true;
+      m = magnitude8_finite(x);
+      m = m > 0x7f80u ? 0 : m;                      // a NaN
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0)
+      atomicMax(&most[token], m);
+  }
+  const bool alone = __syncthreads_or(odd_values);
+  // Exponent field of a row's power of two.
+  auto power_of = [&](int token) { return most[token] == 0 ? 127 : min(264 - int(most[token] >> 7), 253); };
+  // The rows as the lanes take them: a warp makes a group at a time.
+  for (int i = warp; i < groups * kTiles; i += kWarps) {
+    const int group = i / kTiles, t = i % kTiles, token = t * 8 + g;
+    const float factor = __int_as_float(power_of(token) << 23);
+    float even = 0.f, odd = 0.f;
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (token < a.m)
+        x = *reinterpret_cast<const uint4 *>(a.x + token * a.ldx + group * kGroup + q4 * (kGroup / 4) + j * 8);
+      uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float2 v = bf16_pair(y[c]);
+        y[c] = pack_half2(v.x * factor, v.y * factor);
+        const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&y[c]));
+        even += r.x, odd += r.y;
+      }
+      xs[((group * kWords + j) * kTiles + t) * 32 + lane] =
+          make_uint4(__byte_perm(y[0], y[2], 0x5410), __byte_perm(y[0], y[2], 0x7632), __byte_perm(y[1], y[3], 0x5410),
+                     __byte_perm(y[1], y[3], 0x7632));
+    }
+    float sum = -66.f * even - 6.f * odd;
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    if (q4 == 0)
+      offsets[group * kCols + token] = alone ? 0.f : sum;
+  }
+  __syncthreads();
+
+  auto undo = [&](int token) { return 4.f * __int_as_float((254 - power_of(token)) << 23); };
+  int stage = 0;
+  for (int base = int(blockIdx.x) * wc; base < blocks; base += stride) {
+    const int block = base + which, c0 = block * 16;
+    float acc[kTiles][4] = {};
+    auto chunk = [&](int unit, auto second, auto codes_alone) {
+      constexpr bool kAlone = codes_alone.value;
+      constexpr int kSecond = second.value;
+      const int ch = 2 * unit + kSecond;
+      const uint8_t *at = ring + stage * Shape::kStage + kSecond * 1024;
+      uint32_t w[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+          const uint8_t *row = at + h * 512;
+          if constexpr (kPieces == 1)
+            *reinterpret_cast<uint4 *>(w[h]) = *reinterpret_cast<const uint4 *>(row + w4_place(g, q4));
+          else if constexpr (kPieces == 2)
+            *reinterpret_cast<uint2 *>(w[h] + 2 * p) = *reinterpret_cast<const uint2 *>(row + w4_place(g, 2 * p + (q4 >> 1)) + (q4 & 1) * 8);
+          else
+            w[h][p] = *reinterpret_cast<const uint32_t *>(row + w4_place(g, p) + q4 * 4);
+        }
+      }
+      float s[2][kPieces];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t *words = reinterpret_cast<const uint32_t *>(ring + stage * Shape::kStage + 2048 + (g + h * 8) * 16);
+        if constexpr (kPieces == 1) {
+          s[h][0] = __uint_as_float(kSecond ? words[0] & 0xffff0000u : words[0] << 16);
+        } else {
+#pragma unroll
+          for (int p = 0; p < kPieces; p += 2) {
+            const float2 two = bf16_pair(words[kSecond * kPieces / 2 + p / 2]);
+            s[h][p] = two.x, s[h][p + 1] = two.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+        float sums[kTiles][4];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          const float2 o = *reinterpret_cast<const float2 *>(offsets + (ch * kPieces + p) * kCols + t * 8 + 2 * q4);
+          sums[t][0] = sums[t][2] = o.x, sums[t][1] = sums[t][3] = o.y;
+        }
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+          const uint32_t u = w[0][p * kWords + i], v = w[1][p * kWords + i];
+          auto low = [&](uint32_t x) {              // places 0 and 4 of a word, or 2 and 6
+            const uint32_t y = masked_xor<0x54205420u>(x, masks.low);
+            return kAlone ? half2_fma(y, 0x3c003c00u, 0xd420d420u) : y;
+          };
+          auto high = [&](uint32_t x) {             // 1 and 5, or 3 and 7
+            const uint32_t y = masked_xor<0x46004600u>(x, masks.high);
+            return kAlone ? half2_fma(y, 0x3c003c00u, 0xc600c600u) : y;
+          };
+          const uint32_t first[4] = {low(u << 2), low(v << 2), high(u << 2), high(v << 2)};
+          const uint32_t last[4] = {low(u >> 6), low(v >> 6), high(u >> 6), high(v >> 6)};
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) {
+            const uint4 x = xs[((ch * 4 + p * kWords + i) * kTiles + t) * 32 + lane];
+            mma_half_16816(sums[t], first, x.x, x.y);
+            mma_half_16816(sums[t], last, x.z, x.w);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[t][e] = fmaf(sums[t][e], s[e >> 1][p], acc[t][e]);
+      }
+    };
+    if (block < blocks) {
+#pragma unroll 1
+      for (int unit = begin; unit < end; ++unit) {
+        cp_async_wait_group<0>();
+        __syncwarp();                               // all lanes' copies of this stage; all have read the last one
+        copy();
+        if (!alone) {
+          chunk(unit, std::integral_constant<int, 0>{}, std::false_type{});
+          chunk(unit, std::integral_constant<int, 1>{}, std::false_type{});
+        } else {
+          chunk(unit, std::integral_constant<int, 0>{}, std::true_type{});
+          chunk(unit, std::integral_constant<int, 1>{}, std::true_type{});
+        }
+        stage ^= 1;
+      }
+    }
+    if (wk == 1) {
+      if (block < blocks) {
+        const float b0 = a.bias && c0 + g < a.n ? __bfloat162float(a.bias[c0 + g]) : 0.f;
+        const float b1 = a.bias && c0 + g + 8 < a.n ? __bfloat162float(a.bias[c0 + g + 8]) : 0.f;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float b = h ? b1 : b0;            // token g, channels 2 q4 and 2 q4 + 1 of the half
+            const uint32_t y = transpose_8x8(pack_bf16x2(fmaf(acc[t][2 * h], undo(t * 8 + 2 * q4), b),
+                                                         fmaf(acc[t][2 * h + 1], undo(t * 8 + 2 * q4 + 1), b)));
+            const int token = t * 8 + g, c = c0 + h * 8 + 2 * q4;
+            uint16_t *out = reinterpret_cast<uint16_t *>(a.out + token * a.ldo + c);
+            const bool first = token < a.m && c < a.n, second = token < a.m && c + 1 < a.n;
+            if (second && a.pairs) {
+              *reinterpret_cast<uint32_t *>(out) = y;
+            } else {
+              if (first)
+                out[0] = uint16_t(y);
+              if (second)
+                out[1] = uint16_t(y >> 16);
+            }
+          }
+      }
+      continue;
+    }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        red[(warp * kCols + t * 8 + 2 * q4 + (e & 1)) * Shape::kRedRow + g + (e >> 1) * 8] = acc[t][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < wc * kCols * 16; i += kWarps * 32) {
+      const int c = i % 16, token = i / 16 % kCols, of = i / (16 * kCols), channel = (base + of) * 16 + c;
+      if (token >= a.m || channel >= a.n)
+        continue;
+      float sum = 0.f;
+      for (int x = 0; x < wk; ++x)                  // in order of K
+        sum += red[((of * wk + x) * kCols + token) * Shape::kRedRow + c];
+      const float b = a.bias != nullptr ? __bfloat162float(a.bias[channel]) : 0.f;
+      a.out[token * a.ldo + channel] = __float2bfloat16_rn(fmaf(sum, undo(token), b));
+    }
+    __syncthreads();
+  }
+  cp_async_wait_group<0>();
 }
 
 } // namespace pir2b

@@ -324,6 +324,11 @@ __device__ __forceinline__ void cp_async_16(void *dst, const void *src) {
                : "memory");
 }
 
+// The same to a shared-memory address.
+__device__ __forceinline__ void cp_async_16_at(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 __device__ __forceinline__ void cp_async_wait_all() {
   asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
 }
