@@ -13,8 +13,8 @@ static int w4_split(const W4Args &a, int warps, int ctas) {
   const int64_t blocks = (a.n + 15) / 16, units = a.k / 256;
   int best = 1;
   int64_t least = INT64_MAX;
-  for (int wk = 1; wk <= warps; wk *= 2) {
-    const int64_t wc = warps / wk, rounds = ((blocks + wc - 1) / wc + ctas - 1) / ctas;
+  for (int wk = 1; wk <= warps && warps % wk == 0; wk *= 2) {
+    const int64_t wc = warps / wk, rounds = ((blocks + ctas - 1) / ctas + wc - 1) / wc;
     const int64_t cost = rounds * (2 * ((units + wk - 1) / wk) + (wk > 1));
     if (cost < least)
       least = cost, best = wk;
@@ -27,14 +27,17 @@ static std::atomic<int> g_w4_mode{0};   // probe
 template <int kGroup, int kTiles>
 static int launch_w4(W4Args a, const DeviceInfo *dev, void *stream) {
   using Shape = W4Shape<kTiles>;
-  const int smem = Shape::bytes(a.k, kGroup), limit = 227 * 1024;
+  const int limit = 227 * 1024;
+  a.stages = Shape::kMostStages;
+  while (a.stages > 2 && Shape::bytes(a.k, kGroup, a.stages) > limit)
+    --a.stages;
+  const int smem = Shape::bytes(a.k, kGroup, a.stages);
   const int mode = g_w4_mode.load();
   const bool fits = a.k % 256 == 0 && smem <= limit && aligned(a.scales, 16);
   if (fits && (mode == 2 || (mode == 0 && a.n >= 8192))) {
-    const int resident = kTiles > 1 ? 1 : std::min(3, 228 * 1024 / (smem + 1024));
-    const int64_t ctas = int64_t(dev->sms) * resident;
+    const int64_t ctas = dev->sms;
     a.wk = w4_split(a, Shape::kWarps, int(ctas));
-    const int64_t wc = Shape::kWarps / a.wk, grid = std::min<int64_t>(ctas, ((a.n + 15) / 16 + wc - 1) / wc);
+    const int64_t grid = std::min<int64_t>(ctas, (a.n + 15) / 16);
     cudaFuncSetAttribute(gemm_w4_staged_kernel<kGroup, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
     return launch_cache("gemm_w4a16 launch", gemm_w4_staged_kernel<kGroup, kTiles>, grid, 1, 1, Shape::kWarps * 32, smem, stream, a);
   }

@@ -26,7 +26,7 @@ struct W4Args {
   __nv_bfloat16 *out;            // [m, n], row stride ldo
   int64_t ldo;
   int m, n, k;
-  int wk;                        // staged: warps that split K
+  int wk, stages;                // staged: warps that split K, of their rings
   int pairs;                     // output channels may be stored two at a time
 };
 
@@ -142,15 +142,14 @@ __global__ void __launch_bounds__(kW4Warps * 32) gemm_w4_kernel(const W4Args a) 
 // is not finite the codes themselves are taken instead.
 template <int kTiles>
 struct W4Shape {
-  static constexpr int kWarps = kTiles == 1 ? 8 : 16;
-  static constexpr int kStages = 2;
+  static constexpr int kWarps = kTiles == 1 ? 24 : 16;
+  static constexpr int kMostStages = 2;
   static constexpr int kCols = 8 * kTiles;
   static constexpr int kStage = 2 * (1024 + 128);        // of two chunks: codes of 16 channels, 16 bytes for each one's scales
-  static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kRedRow = 20;                     // words of a token's 16 sums, apart by banks
   static constexpr int kRed = kWarps * kCols * kRedRow * 4;
-  static constexpr int bytes(int64_t k, int group) {
-    return int(k * kCols * 2 + k / group * kCols * 4) + kRing + kRed + kCols * 4;
+  static constexpr int bytes(int64_t k, int group, int stages) {
+    return int(k * kCols * 2 + k / group * kCols * 4) + kWarps * stages * kStage + kRed + kCols * 4;
   }
 };
 
@@ -164,20 +163,20 @@ __device__ __forceinline__ void cp_async_ca(uint32_t dst, const void *src) {
 }
 
 template <int kGroup, int kTiles>
-__global__ void __launch_bounds__(W4Shape<kTiles>::kWarps * 32, kTiles == 1 ? 3 : 1) gemm_w4_staged_kernel(const W4Args a) {
+__global__ void __launch_bounds__(W4Shape<kTiles>::kWarps * 32, 1) gemm_w4_staged_kernel(const W4Args a) {
   using Shape = W4Shape<kTiles>;
   constexpr int kPieces = 128 / kGroup, kWords = 4 / kPieces, kCols = Shape::kCols, kWarps = Shape::kWarps;
-  constexpr int kStages = Shape::kStages;
   extern __shared__ __align__(1024) uint8_t tile_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   const int units = a.k >> 8, groups = a.k / kGroup;      // units of two chunks
   uint4 *xs = reinterpret_cast<uint4 *>(tile_raw);                           // [chunk][word][tile][lane]
   float *offsets = reinterpret_cast<float *>(tile_raw + int64_t(a.k) * kCols * 2);   // [group][token]
-  uint8_t *ring = reinterpret_cast<uint8_t *>(offsets + groups * kCols) + warp * kStages * Shape::kStage;
-  float *red = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(offsets + groups * kCols) + Shape::kRing);
+  uint8_t *ring = reinterpret_cast<uint8_t *>(offsets + groups * kCols) + warp * a.stages * Shape::kStage;
+  float *red = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(offsets + groups * kCols) + kWarps * a.stages * Shape::kStage);
   uint32_t *most = reinterpret_cast<uint32_t *>(red + Shape::kRed / 4);      // [token] largest magnitude
   const int wk = a.wk, wc = kWarps / wk, part = warp % wk, which = warp / wk;
   const int begin = part * units / wk, end = (part + 1) * units / wk;
+  // Block blockIdx + gridDim i of 16 channels is the CTA's i-th.
   const int blocks = (a.n + 15) >> 4, stride = gridDim.x * wc;
   const Int4Masks masks = int4_masks();
   pdl_wait();
@@ -185,12 +184,12 @@ __global__ void __launch_bounds__(W4Shape<kTiles>::kWarps * 32, kTiles == 1 ? 3 
 
   // The next two chunks to copy: a row for every two lanes, which have alternate
   // 16-byte pieces of it.  Rows past the last are left as they are.
-  int next_block = int(blockIdx.x) * wc + which, next = begin;
+  int next_block = int(blockIdx.x + gridDim.x * which), next = begin;
   bool mine = false;
   const uint8_t *src = nullptr;
   const __nv_bfloat16 *scale_src = nullptr;
   const uint32_t ring_at = smem_u32(ring);
-  int turn = Shape::kStage;
+  int stage_in = 0;
   uint32_t to = ring_at + w4_place(lane >> 1, lane & 1), scale_to = ring_at + 2048 + (lane >> 1) * 16;
   auto at_block = [&]() {
     const int row = next_block * 16 + (lane >> 1);
@@ -219,11 +218,14 @@ __global__ void __launch_bounds__(W4Shape<kTiles>::kWarps * 32, kTiles == 1 ? 3 
         at_block();
       }
     }
-    to += turn, scale_to += turn, turn = -turn;     // the other stage
+    const int step = ++stage_in == a.stages ? Shape::kStage - a.stages * Shape::kStage : Shape::kStage;
+    stage_in = stage_in == a.stages ? 0 : stage_in;
+    to += step, scale_to += step;
     cp_async_commit();
   };
   at_block();
-  copy();
+  for (int i = 0; i < a.stages - 1; ++i)
+    copy();
 
   // The rows' largest finite magnitudes, 256 values of a row at a time.
   for (int i = threadIdx.x; i < kCols; i += kWarps * 32)
@@ -279,8 +281,8 @@ __global__ void __launch_bounds__(W4Shape<kTiles>::kWarps * 32, kTiles == 1 ? 3 
 
   auto undo = [&](int token) { return 4.f * __int_as_float((254 - power_of(token)) << 23); };
   int stage = 0;
-  for (int base = int(blockIdx.x) * wc; base < blocks; base += stride) {
-    const int block = base + which, c0 = block * 16;
+  for (int base = int(blockIdx.x); base < blocks; base += stride) {
+    const int block = base + int(gridDim.x) * which, c0 = block * 16;
     float acc[kTiles][4] = {};
     auto chunk = [&](int unit, auto second, auto codes_alone) {
       constexpr bool kAlone = codes_alone.value;
@@ -353,7 +355,12 @@ __global__ void __launch_bounds__(W4Shape<kTiles>::kWarps * 32, kTiles == 1 ? 3 
     if (block < blocks) {
 #pragma unroll 1
       for (int unit = begin; unit < end; ++unit) {
-        cp_async_wait_group<0>();
+        if (a.stages == 2)
+          cp_async_wait_group<0>();
+        else if (a.stages == 3)
+          cp_async_wait_group<1>();
+        else
+          cp_async_wait_group<2>();
         __syncwarp();                               // all lanes' copies of this stage; all have read the last one
         copy();
         if (!alone) {
@@ -363,7 +370,7 @@ __global__ void __launch_bounds__(W4Shape<kTiles>::kWarps * 32, kTiles == 1 ? 3 
           chunk(unit, std::integral_constant<int, 0>{}, std::true_type{});
           chunk(unit, std::integral_constant<int, 1>{}, std::true_type{});
         }
-        stage ^= 1;
+        stage = stage == a.stages - 1 ? 0 : stage + 1;
       }
     }
     if (wk == 1) {
@@ -399,7 +406,7 @@ __global__ void __launch_bounds__(W4Shape<kTiles>::kWarps * 32, kTiles == 1 ? 3 
         red[(warp * kCols + t * 8 + 2 * q4 + (e & 1)) * Shape::kRedRow + g + (e >> 1) * 8] = acc[t][e];
     __syncthreads();
     for (int i = threadIdx.x; i < wc * kCols * 16; i += kWarps * 32) {
-      const int c = i % 16, token = i / 16 % kCols, of = i / (16 * kCols), channel = (base + of) * 16 + c;
+      const int c = i % 16, token = i / 16 % kCols, of = i / (16 * kCols), channel = (base + int(gridDim.x) * of) * 16 + c;
       if (token >= a.m || channel >= a.n)
         continue;
       float sum = 0.f;
