@@ -41,8 +41,16 @@ static int launch_w4(W4Args a, const DeviceInfo *dev, void *stream) {
     cudaFuncSetAttribute(gemm_w4_staged_kernel<kGroup, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
     return launch_cache("gemm_w4a16 launch", gemm_w4_staged_kernel<kGroup, kTiles>, grid, 1, 1, Shape::kWarps * 32, smem, stream, a);
   }
-  return launch_cache("gemm_w4a16 launch", gemm_w4_kernel<kGroup, kTiles>, (a.n + kW4Channels - 1) / kW4Channels, 1, 1,
-                      kW4Warps * 32, 0, stream, a);
+  // Long K is split over twice the warps; a CTA takes several blocks of channels
+  // only where more CTAs would not fit at once, and reads its rows through L1.
+  const int warps = a.k >= 4096 ? 16 : 8, smem2 = warps * 8 * kTiles * 20 * 4;
+  const int64_t grid = std::min<int64_t>((a.n + 15) / 16, int64_t(dev->sms) * (kTiles == 1 ? 5 * 8 : 2 * 8) / warps);
+  if (warps == 16) {
+    cudaFuncSetAttribute(gemm_w4_kernel<kGroup, kTiles, 16>, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
+    return launch_cache("gemm_w4a16 launch", gemm_w4_kernel<kGroup, kTiles, 16>, grid, 1, 1, warps * 32, smem2, stream, a);
+  }
+  cudaFuncSetAttribute(gemm_w4_kernel<kGroup, kTiles, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
+  return launch_cache("gemm_w4a16 launch", gemm_w4_kernel<kGroup, kTiles, 8>, grid, 1, 1, warps * 32, smem2, stream, a);
 }
 
 template <int kGroup>

@@ -15,8 +15,6 @@
 
 namespace pir2b {
 
-constexpr int kW4Channels = 16, kW4Warps = 8;
-
 struct W4Args {
   const __nv_bfloat16 *x;        // [m, k], row stride ldx
   int64_t ldx;
@@ -56,75 +54,125 @@ __device__ __forceinline__ void w4_load(uint32_t (&w)[4], const uint8_t *row, in
   }
 }
 
+// What a lane holds of a chunk of 128 k: codes and scales of two channels, and x
+// of one token where that is all.
 template <int kGroup, int kTiles>
-__global__ void __launch_bounds__(kW4Warps * 32) gemm_w4_kernel(const W4Args a) {
+struct W4Chunk {
+  uint32_t w[2][4];
+  __nv_bfloat16 s[2][128 / kGroup];
+  uint4 x[kTiles == 1 ? 4 : 1];
+};
+
+template <int kGroup, int kTiles, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32) gemm_w4_kernel(const W4Args a) {
   constexpr int kPieces = 128 / kGroup, kWords = 4 / kPieces;   // of a lane and chunk; words of a piece
-  constexpr int kCols = 8 * kTiles;
-  __shared__ float red[kW4Warps][kCols][kW4Channels];
+  constexpr int kCols = 8 * kTiles, kRow = 20;                  // words of a token's 16 sums, apart by banks
+  extern __shared__ __align__(1024) uint8_t tile_raw[];
+  float *red = reinterpret_cast<float *>(tile_raw);             // [warp][token][channel]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
-  const int c0 = blockIdx.x * kW4Channels, groups = a.k / kGroup;
-  const int chunks = (a.k + 127) >> 7;
-  const int begin = warp * chunks / kW4Warps, end = (warp + 1) * chunks / kW4Warps;
-  const int row[2] = {min(c0 + g, a.n - 1), min(c0 + g + 8, a.n - 1)};   // rows past the last are not stored
-  float acc[kTiles][4] = {};
+  const int groups = a.k / kGroup, chunks = (a.k + 127) >> 7, blocks = (a.n + 15) >> 4;
+  const int begin = warp * chunks / kWarps, end = (warp + 1) * chunks / kWarps;
   const Int4Masks masks = int4_masks();
-  pdl_wait();
-  pdl_launch_dependents();
-#pragma unroll 1
-  for (int ch = begin; ch < end; ++ch) {
+  auto row_of = [&](int block, int h) { return int64_t(min(block * 16 + g + h * 8, a.n - 1)); };   // past the last: not stored
+  auto codes_of = [&](int block, int h) { return a.w + row_of(block, h) * (a.k >> 1) + q4 * (16 / kPieces); };
+  auto load = [&](W4Chunk<kGroup, kTiles> &c, int block, int ch) {
     const int left = groups - ch * kPieces;
-    uint32_t w[2][4];
-    float s[2][kPieces];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      w4_load<kPieces>(w[h], a.w + int64_t(row[h]) * (a.k >> 1) + ch * 64 + q4 * (16 / kPieces), left);
+      w4_load<kPieces>(c.w[h], codes_of(block, h) + ch * 64, left);
+      const __nv_bfloat16 *s = a.scales + row_of(block, h) * groups + ch * kPieces;
 #pragma unroll
       for (int p = 0; p < kPieces; ++p)
-        s[h][p] = p < left ? __bfloat162float(a.scales[int64_t(row[h]) * groups + ch * kPieces + p]) : 0.f;
+        c.s[h][p] = p < left ? s[p] : __float2bfloat16(0.f);
     }
+    if constexpr (kTiles == 1) {
 #pragma unroll
-    for (int p = 0; p < kPieces; ++p) {
-      float part[kTiles][4] = {};
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) {
-        const uint32_t u = w[0][p * kWords + i], v = w[1][p * kWords + i];
-        const uint32_t even[4] = {w4_pair<0>(u, masks), w4_pair<0>(v, masks), w4_pair<1>(u, masks), w4_pair<1>(v, masks)};
-        const uint32_t odd[4] = {w4_pair<2>(u, masks), w4_pair<2>(v, masks), w4_pair<3>(u, masks), w4_pair<3>(v, masks)};
-        const int k = ch * 128 + p * kGroup + q4 * (kGroup / 4) + i * 8;
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          const int token = t * 8 + g;
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (token < a.m && p < left)
-            x = *reinterpret_cast<const uint4 *>(a.x + token * a.ldx + k);
-          mma_bf16_16816(part[t], even, __byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632));
-          mma_bf16_16816(part[t], odd, __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int p = i / kWords;
+        c.x[i] = make_uint4(0, 0, 0, 0);
+        if (g < a.m && p < left)
+          c.x[i] = *reinterpret_cast<const uint4 *>(a.x + g * a.ldx + ch * 128 + p * kGroup + q4 * (kGroup / 4) + i % kWords * 8);
       }
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          acc[t][e] = fmaf(part[t][e], s[e >> 1][p], acc[t][e]);
     }
+  };
+  // The first weights start for L2 while the launch before this one ends; nothing
+  // is read of them yet.
+  if (begin < end) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(codes_of(blockIdx.x, h) + begin * 64));
   }
+  pdl_wait();
+  pdl_launch_dependents();
+  W4Chunk<kGroup, kTiles> one, two;
+  if (begin < end)
+    load(one, blockIdx.x, begin);
+  for (int block = blockIdx.x; block < blocks; block += gridDim.x) {
+    float acc[kTiles][4] = {};
+    auto multiply = [&](const W4Chunk<kGroup, kTiles> &c, int ch) {
+      const int left = groups - ch * kPieces;
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t)
+      for (int p = 0; p < kPieces; ++p) {
+        float part[kTiles][4] = {};
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      red[warp][t * 8 + 2 * q4 + (e & 1)][g + (e >> 1) * 8] = acc[t][e];
-  __syncthreads();
-  for (int i = threadIdx.x; i < kCols * kW4Channels; i += kW4Warps * 32) {
-    const int token = i / kW4Channels, c = i % kW4Channels;
-    if (token >= a.m || c0 + c >= a.n)
-      continue;
-    float sum = 0.f;
+        for (int i = 0; i < kWords; ++i) {
+          const uint32_t u = c.w[0][p * kWords + i], v = c.w[1][p * kWords + i];
+          const uint32_t even[4] = {w4_pair<0>(u, masks), w4_pair<0>(v, masks), w4_pair<1>(u, masks), w4_pair<1>(v, masks)};
+          const uint32_t odd[4] = {w4_pair<2>(u, masks), w4_pair<2>(v, masks), w4_pair<3>(u, masks), w4_pair<3>(v, masks)};
+          const int k = ch * 128 + p * kGroup + q4 * (kGroup / 4) + i * 8;
 #pragma unroll
-    for (int x = 0; x < kW4Warps; ++x)
-      sum += red[x][token][c];
-    if (a.bias != nullptr)
-      sum += __bfloat162float(a.bias[c0 + c]);
-    a.out[token * a.ldo + c0 + c] = __float2bfloat16_rn(sum);
+          for (int t = 0; t < kTiles; ++t) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if constexpr (kTiles == 1) {
+              x = c.x[p * kWords + i];
+            } else {
+              const int token = t * 8 + g;
+              if (token < a.m && p < left)
+                x = *reinterpret_cast<const uint4 *>(a.x + token * a.ldx + k);
+            }
+            mma_bf16_16816(part[t], even, __byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632));
+            mma_bf16_16816(part[t], odd, __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[t][e] = fmaf(part[t][e], __bfloat162float(c.s[e >> 1][p]), acc[t][e]);
+      }
+    };
+#pragma unroll 1
+    for (int ch = begin; ch < end; ch += 2) {
+      if (ch + 1 < end)
+        load(two, block, ch + 1);
+      multiply(one, ch);
+      if (ch + 2 < end)
+        load(one, block, ch + 2);
+      if (ch + 1 < end)
+        multiply(two, ch + 1);
+    }
+    if (begin < end && block + gridDim.x < blocks)
+      load(one, block + gridDim.x, begin);
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        red[(warp * kCols + t * 8 + 2 * q4 + (e & 1)) * kRow + g + (e >> 1) * 8] = acc[t][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < kCols * 16; i += kWarps * 32) {
+      const int token = i / 16, c = i % 16, channel = block * 16 + c;
+      if (token >= a.m || channel >= a.n)
+        continue;
+      float sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x)              // in order of K
+        sum += red[(x * kCols + token) * kRow + c];
+      if (a.bias != nullptr)
+        sum += __bfloat162float(a.bias[channel]);
+      a.out[token * a.ldo + channel] = __float2bfloat16_rn(sum);
+    }
+    if (block + gridDim.x < blocks)
+      __syncthreads();
   }
 }
 
