@@ -95,12 +95,6 @@ __device__ __forceinline__ uint32_t half2_fma(uint32_t x, uint32_t y, uint32_t z
   return w;
 }
 
-__device__ __forceinline__ uint32_t bf162_fma(uint32_t x, uint32_t y, uint32_t z) {
-  uint32_t w;
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(w) : "r"(x), "r"(y), "r"(z));
-  return w;
-}
-
 __device__ __forceinline__ Int4Factors int4_factors(uint32_t pair) {   // of an fp16 pair of one factor
   return {pair, half2_mul(pair, 0xd420d420u), half2_mul(pair, 0xc600c600u)};
 }

@@ -160,12 +160,12 @@ static int launch_rows(bool write, int format, int d, const CacheRowsArgs &a, vo
 // Few tokens are spread over more warps, as in launch_rows.
 template <int kFormat, int D>
 static int launch_append(const CacheAppendArgs &a, void *stream) {
-  constexpr int kRows = 32 / (D / 8);
+  constexpr int kRows = 32 / (D / 16);
   const int64_t grid = (a.rows + kCacheWarps - 1) / kCacheWarps;
-  const int loads = (a.hq + 2 * a.c.hk + kRows - 1) / kRows;
+  const int loads = (a.hq + kRows - 1) / kRows + 2 * ((a.c.hk + kRows - 1) / kRows);
   if (a.rows * loads <= 4096)
     return launch_cache("cache_append launch", cache_append_kernel<kFormat, D, 1>, grid, loads, 1, kCacheWarps * 32, 0, stream, a);
-  return launch_cache("cache_append launch", cache_append_kernel<kFormat, D, 4>, grid, 1, 1, kCacheWarps * 32, 0, stream, a);
+  return launch_cache("cache_append launch", cache_append_kernel<kFormat, D, 2>, grid, 1, 1, kCacheWarps * 32, 0, stream, a);
 }
 
 template <int kFormat>
@@ -550,8 +550,8 @@ int pir2b_cache_append(const void *qkv, int64_t row, int64_t head, int64_t rows,
     return fail(PIR2B_EINVAL, "cache_append: eps must be finite and not negative");
   if (cos == nullptr || sin == nullptr || turns < 1)
     return fail(PIR2B_EINVAL, "cache_append needs cos and sin of at least one position");
-  if (!aligned(cos, 16) || !aligned(sin, 16) || !aligned(q_weight, 8) || !aligned(k_weight, 8))
-    return fail(PIR2B_EALIGN, "cache_append: cos and sin must be 16-byte, norm weights 8-byte aligned");
+  if (!aligned(cos, 16) || !aligned(sin, 16) || !aligned(q_weight, 16) || !aligned(k_weight, 16))
+    return fail(PIR2B_EALIGN, "cache_append: cos, sin and norm weights must be 16-byte aligned");
   if (rows == 0)
     return PIR2B_OK;
   if (int r = check_view("cache_append qkv", qkv, row, head))

@@ -41,6 +41,35 @@ static int launch_w4(W4Args a, const DeviceInfo *dev, void *stream) {
     cudaFuncSetAttribute(gemm_w4_staged_kernel<kGroup, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
     return launch_cache("gemm_w4a16 launch", gemm_w4_staged_kernel<kGroup, kTiles>, grid, 1, 1, Shape::kWarps * 32, smem, stream, a);
   }
+  if constexpr (kTiles > 1) {
+    if (mode == 3 && a.k % 256 == 0) {
+      static uint8_t *ws = nullptr;
+      if (!ws) cudaMalloc(&ws, 64 << 20);
+      W4Rows r;
+      r.x = reinterpret_cast<uint4 *>(ws);
+      r.offsets = reinterpret_cast<float *>(ws + (32 << 20));
+      r.odd = reinterpret_cast<uint32_t *>(ws + (48 << 20));
+      const int64_t items = a.k / kGroup * kTiles;
+      if (int x = launch_cache("w4 rows launch", w4_rows_kernel<kGroup, kTiles>, (items + 3) / 4, 1, 1, 128, 0, stream, a, r))
+        return x;
+      using Wide = W4Wide<kTiles>;
+      a.slab = a.k;
+      while (Wide::bytes(a.slab, kGroup) > limit)
+        a.slab = (a.slab / 2 + 255) / 256 * 256;
+      cudaFuncSetAttribute(gemm_w4_wide_kernel<kGroup, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
+      const int64_t blocks = (a.n + 15) / 16, grid = std::min<int64_t>(blocks, dev->sms);
+      int64_t least = INT64_MAX;
+      const int slabs = (a.k + a.slab - 1) / a.slab;
+      for (int wk = 1; wk <= Wide::kWarps; wk *= 2) {
+        const int64_t wc = Wide::kWarps / wk, rounds = ((blocks + grid - 1) / grid + wc - 1) / wc;
+        const int64_t cost = rounds * (slabs * 2 * ((a.slab / 256 + wk - 1) / wk) + 2);
+        if (cost < least)
+          least = cost, a.wk = wk;
+      }
+      return launch_cache("gemm_w4a16 launch", gemm_w4_wide_kernel<kGroup, kTiles>, grid, 1, 1, Wide::kWarps * 32,
+                          Wide::bytes(a.slab, kGroup), stream, a, r);
+    }
+  }
   // Long K is split over twice the warps; a CTA takes several blocks of channels
   // only where more CTAs would not fit at once, and reads its rows through L1.
   const int warps = a.k >= 4096 ? 16 : 8, smem2 = warps * 8 * kTiles * 20 * 4;

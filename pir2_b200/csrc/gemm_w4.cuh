@@ -24,6 +24,7 @@ struct W4Args {
   __nv_bfloat16 *out;            // [m, n], row stride ldo
   int64_t ldo;
   int m, n, k;
+  int slab;                      // wide: k whose rows are in shared memory at once
   int wk, stages;                // staged: warps that split K, of their rings
   int pairs;                     // output channels may be stored two at a time
 };
@@ -466,6 +467,242 @@ __global__ void __launch_bounds__(W4Shape<kTiles>::kWarps * 32, 1) gemm_w4_stage
     __syncthreads();
   }
   cp_async_wait_group<0>();
+}
+
+// More than eight rows.  What a product takes of x is then made once for all CTAs,
+// by a launch of its own: the rows as the lanes take them, [K / 8 words of a lane][tile]
+// [lane], and -24 times each group's sum (24 + code needs no subtraction, as above),
+// with a word that says whether a value of the group is past 2^100 or not finite.
+struct W4Rows {
+  uint4 *x;            // [4 chunks][tiles][32]
+  float *offsets;      // [groups][8 tiles]
+  uint32_t *odd;       // [groups][tiles]
+};
+
+template <int kGroup, int kTiles>
+__global__ void __launch_bounds__(128) w4_rows_kernel(const W4Args a, const W4Rows r) {
+  constexpr int kWords = kGroup / 32;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  const int item = blockIdx.x * 4 + (threadIdx.x >> 5), group = item / kTiles, t = item % kTiles, token = t * 8 + g;
+  if (group >= a.k / kGroup)
+    return;
+  float sum = 0.f;
+  bool odd = false;
+  uint4 x[kWords];
+#pragma unroll
+  for (int j = 0; j < kWords; ++j) {
+    x[j] = make_uint4(0, 0, 0, 0);
+    if (token < a.m)
+      x[j] = *reinterpret_cast<const uint4 *>(a.x + token * a.ldx + group * kGroup + q4 * (kGroup / 4) + j * 8);
+  }
+#pragma unroll
+  for (int j = 0; j < kWords; ++j) {
+    odd |= magnitude8(x[j]) >= (227u << 7);
+    const float2 p = bf16_pair(x[j].x), q = bf16_pair(x[j].y), u = bf16_pair(x[j].z), v = bf16_pair(x[j].w);
+    sum += ((p.x + p.y) + (q.x + q.y)) + ((u.x + u.y) + (v.x + v.y));
+    r.x[(int64_t(group * kWords + j) * kTiles + t) * 32 + lane] =
+        make_uint4(__byte_perm(x[j].x, x[j].z, 0x5410), __byte_perm(x[j].x, x[j].z, 0x7632),
+                   __byte_perm(x[j].y, x[j].w, 0x5410), __byte_perm(x[j].y, x[j].w, 0x7632));
+  }
+  sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+  odd = __any_sync(0xffffffffu, odd);
+  if (q4 == 0)
+    r.offsets[group * 8 * kTiles + token] = -24.f * sum;
+  if (lane == 0)
+    r.odd[group * kTiles + t] = odd;
+}
+
+// A persistent CTA keeps those of a slab of K (all of it, where it fits) in shared
+// memory and streams weights past them, 16 channels to a warp; `wk` warps split the
+// slab.  The sums of a round meet where the rings were.
+template <int kTiles>
+struct W4Wide {
+  static constexpr int kWarps = 16, kCols = 8 * kTiles;
+  static constexpr int kStage = 16 * (128 + 16);                 // of 256 k: codes of 16 channels, their scales
+  static constexpr int kRedRow = 20;                             // words of a token's 16 sums, apart by banks
+  static constexpr int kRing = kWarps * 2 * kStage, kRed = kWarps * kCols * kRedRow * 4;
+  static constexpr int kMeet = kRing > kRed ? kRing : kRed;
+  static constexpr int bytes(int slab, int group) { return slab * kCols * 2 + slab / group * kCols * 4 + kMeet + 16; }
+};
+
+template <int kGroup, int kTiles>
+__global__ void __launch_bounds__(W4Wide<kTiles>::kWarps * 32, 1) gemm_w4_wide_kernel(const W4Args a, const W4Rows r) {
+  using Shape = W4Wide<kTiles>;
+  constexpr int kPieces = 128 / kGroup, kWords = 4 / kPieces, kCols = Shape::kCols, kWarps = Shape::kWarps;
+  extern __shared__ __align__(1024) uint8_t tile_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  const int groups = a.k / kGroup, slab_groups = a.slab / kGroup;
+  uint4 *xs = reinterpret_cast<uint4 *>(tile_raw);                                    // [chunk][word][tile][lane]
+  float *offsets = reinterpret_cast<float *>(tile_raw + int64_t(a.slab) * kCols * 2);  // [group][token]
+  uint8_t *meet = reinterpret_cast<uint8_t *>(offsets + slab_groups * kCols);
+  uint8_t *ring = meet + warp * 2 * Shape::kStage;
+  float *red = reinterpret_cast<float *>(meet);                                       // [warp][token][channel]
+  uint64_t *full = reinterpret_cast<uint64_t *>(meet + Shape::kMeet);
+  const int wk = a.wk, wc = kWarps / wk, part = warp % wk, which = warp / wk;
+  const int blocks = (a.n + 15) >> 4, slabs = (a.k + a.slab - 1) / a.slab;
+  const Int4Masks masks = int4_masks();
+  if (threadIdx.x == 0) {
+    mbar_init(full, 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+  bool odd = false;
+  for (int i = threadIdx.x; i < groups * kTiles; i += kWarps * 32)
+    odd |= r.odd[i] != 0;
+  const bool alone = __syncthreads_or(odd);
+
+  // A row for every two lanes, which have alternate 16-byte pieces of it.
+  const uint32_t ring_at = smem_u32(ring);
+  int loaded = 0;                                   // slabs so far
+  bool ok = true;
+  for (int base = int(blockIdx.x); base < blocks && ok; base += int(gridDim.x) * wc) {
+    const int block = base + int(gridDim.x) * which;
+    const int row = block * 16 + (lane >> 1);
+    const bool live = block < blocks, mine = row < a.n;
+    const uint8_t *src = a.w + int64_t(row) * (a.k >> 1) + (lane & 1) * 16;
+    const __nv_bfloat16 *scale_src = a.scales + int64_t(row) * groups;
+    float acc[kTiles][4] = {};
+    for (int slab = 0; slab < slabs && ok; ++slab) {
+      const int first = slab * a.slab, units = min(a.slab, a.k - first) >> 8;
+      const int begin = part * units / wk, end = (part + 1) * units / wk;
+      auto copy = [&](int unit) {
+        if (live && mine && unit < end) {
+          const uint32_t at = ring_at + (unit & 1) * Shape::kStage;
+          const int k = first + unit * 256;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)               // chunk i / 2, piece 2 (i % 2) + (lane & 1)
+            cp_async_16_at(at + (i >> 1) * 1024 + w4_place(lane >> 1, 2 * (i & 1) + (lane & 1)), src + (k >> 1) + i * 32);
+          if ((lane & 1) == 0) {
+            const __nv_bfloat16 *s = scale_src + k / kGroup;
+            if constexpr (kPieces == 4)
+              cp_async_16_at(at + 2048 + lane * 8, s);
+            else
+              cp_async_ca<4 * kPieces>(at + 2048 + lane * 8, s);
+          }
+        }
+        cp_async_commit();
+      };
+      copy(begin);
+      if (loaded == 0 || slabs > 1) {
+        if (loaded > 0)
+          __syncthreads();                          // all have read the slab before
+        if (threadIdx.x == 0) {
+          const int g0 = first / kGroup, bytes_x = units * 256 * kCols * 2, bytes_o = units * 256 / kGroup * kCols * 4;
+          fence_proxy_async_smem();
+          mbar_arrive_expect_tx(full, bytes_x + bytes_o);
+          bulk_load(xs, r.x + int64_t(first >> 5) * kTiles * 32, bytes_x, full);
+          bulk_load(offsets, r.offsets + g0 * kCols, bytes_o, full);
+        }
+        ok = __syncthreads_and(mbar_wait(full, uint32_t(loaded & 1), kStatusTimeoutProducer));
+        ++loaded;
+      }
+      auto chunk = [&](int unit, auto second, auto codes_alone) {
+        constexpr bool kAlone = codes_alone.value;
+        constexpr int kSecond = second.value;
+        const int ch = 2 * unit + kSecond;          // of the slab
+        const uint8_t *at = ring + (unit & 1) * Shape::kStage;
+        uint32_t w[2][4];
+        float s[2][kPieces];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint8_t *rows = at + kSecond * 1024 + h * 512;
+#pragma unroll
+          for (int p = 0; p < kPieces; ++p) {
+            if constexpr (kPieces == 1)
+              *reinterpret_cast<uint4 *>(w[h]) = *reinterpret_cast<const uint4 *>(rows + w4_place(g, q4));
+            else if constexpr (kPieces == 2)
+              *reinterpret_cast<uint2 *>(w[h] + 2 * p) = *reinterpret_cast<const uint2 *>(rows + w4_place(g, 2 * p + (q4 >> 1)) + (q4 & 1) * 8);
+            else
+              w[h][p] = *reinterpret_cast<const uint32_t *>(rows + w4_place(g, p) + q4 * 4);
+          }
+          const uint32_t *words = reinterpret_cast<const uint32_t *>(at + 2048 + (g + h * 8) * 16);
+          if constexpr (kPieces == 1) {
+            s[h][0] = __uint_as_float(kSecond ? words[0] & 0xffff0000u : words[0] << 16);
+          } else {
+#pragma unroll
+            for (int p = 0; p < kPieces; p += 2) {
+              const float2 two = bf16_pair(words[kSecond * kPieces / 2 + p / 2]);
+              s[h][p] = two.x, s[h][p + 1] = two.y;
+            }
+          }
+        }
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+          float sums[kTiles][4];
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) {
+            const float2 o = kAlone ? make_float2(0.f, 0.f)
+                                    : *reinterpret_cast<const float2 *>(offsets + (ch * kPieces + p) * kCols + t * 8 + 2 * q4);
+            sums[t][0] = sums[t][2] = o.x, sums[t][1] = sums[t][3] = o.y;
+          }
+#pragma unroll
+          for (int i = 0; i < kWords; ++i) {
+            uint32_t even[4], last[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t u = w[h][p * kWords + i];
+              auto pair = [&](uint32_t t) {
+                const uint32_t y = masked_xor<0x41c041c0u>(t, masks.mantissa);
+                return kAlone ? bf162_fma(y, 0x3f803f80u, 0xc1c0c1c0u) : y;
+              };
+              even[h] = pair(u << 3), even[h + 2] = pair(u >> 1);
+              last[h] = pair(u >> 5), last[h + 2] = pair(u >> 9);
+            }
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+              const uint4 x = xs[((ch * 4 + p * kWords + i) * kTiles + t) * 32 + lane];
+              mma_bf16_16816(sums[t], even, x.x, x.y);
+              mma_bf16_16816(sums[t], last, x.z, x.w);
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[t][e] = fmaf(sums[t][e], s[e >> 1][p], acc[t][e]);
+        }
+      };
+#pragma unroll 1
+      for (int unit = begin; unit < end && live; ++unit) {
+        cp_async_wait_group<0>();
+        __syncwarp();                               // all lanes' copies of this unit; all have read the last one
+        copy(unit + 1);
+        if (alone) {
+          chunk(unit, std::integral_constant<int, 0>{}, std::true_type{});
+          chunk(unit, std::integral_constant<int, 1>{}, std::true_type{});
+        } else {
+          chunk(unit, std::integral_constant<int, 0>{}, std::false_type{});
+          chunk(unit, std::integral_constant<int, 1>{}, std::false_type{});
+        }
+      }
+      __syncwarp();
+    }
+    cp_async_wait_group<0>();
+    __syncthreads();                                // the rings are read
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        red[(warp * kCols + t * 8 + 2 * q4 + (e & 1)) * Shape::kRedRow + g + (e >> 1) * 8] = acc[t][e];
+    __syncthreads();
+    for (int i = threadIdx.x >> 4; i < wc * a.m && ok; i += kWarps * 2) {
+      const int of = i / a.m, token = i % a.m, c = lane & 15, channel = (base + int(gridDim.x) * of) * 16 + c;
+      if (channel >= a.n)
+        continue;
+      float sum = 0.f;
+      for (int x = 0; x < wk; ++x)                  // in order of K
+        sum += red[((of * wk + x) * kCols + token) * Shape::kRedRow + c];
+      if (a.bias != nullptr)
+        sum += __bfloat162float(a.bias[channel]);
+      a.out[token * a.ldo + channel] = __float2bfloat16_rn(sum);
+    }
+    __syncthreads();
+  }
 }
 
 } // namespace pir2b

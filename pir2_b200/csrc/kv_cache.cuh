@@ -26,6 +26,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cstdint>
+#include <type_traits>
 #include "args.cuh"
 #include "attention.cuh"
 #include "ptx.cuh"
@@ -190,8 +191,10 @@ __device__ __forceinline__ float int4_scale(uint32_t m) {
 }
 
 // E4M3 factor of a group whose largest magnitude has the bits m, in the low byte.
+// (The division as in quotients(): of a bf16 by 7 it is the correctly rounded one.)
 __device__ __forceinline__ uint32_t int4_factor(uint32_t m, float inverse) {
-  return e4m3_pair(__fdiv_rn(__uint_as_float(m << 16) * inverse, 7.f), 0.f) & 0xffu;
+  const float x = __uint_as_float(m << 16) * inverse, q = __fmul_rn(x, 1.0f / 7.0f);
+  return e4m3_pair(__fmaf_rn(__fmaf_rn(q, -7.f, x), 1.0f / 7.0f, q), 0.f) & 0xffu;
 }
 
 __device__ __forceinline__ float e4m3_value(uint32_t code) {
@@ -218,8 +221,28 @@ __device__ __forceinline__ uint32_t quantise4_int4(uint32_t x, uint32_t y, float
   return (__byte_perm(pair[0], pair[1], 0x0040) & 0xffffu) ^ 0x8888u;
 }
 
-__device__ __forceinline__ uint32_t quantise8_int4(const uint4 &x, float inverse, float f) {
-  return quantise4_int4(x.x, x.y, inverse, f) | (quantise4_int4(x.z, x.w, inverse, f) << 16);
+// The same for a row of ordinary scale and a group of ordinary factor (or none but
+// zeros), where no code passes 7 before it is rounded: straight by the product fs
+// of the two, with an approximate reciprocal, which quotients() makes up for (a
+// test takes reciprocals off by three places).
+__device__ __forceinline__ bool int4_ordinary(uint32_t factor) { return factor == 0 || factor >= 8; }   // E4M3's subnormal ones are below 8
+
+__device__ __forceinline__ float reciprocal_of_factor(float fs) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fs));
+  return fs == 0.f ? 0.f : y;
+}
+
+__device__ __forceinline__ uint32_t ordinary8_int4(const uint4 &x, float fs, float r) {
+  const float2 minus = make_float2(-fs, -fs), rr = make_float2(r, r), up = make_float2(12582920.f, 12582920.f);
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t pair[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 q = __fadd2_rn(quotients(bf16_pair(w[i]), minus, rr), up);
+    pair[i] = (__float_as_uint(q.y) << 4) + __float_as_uint(q.x);
+  }
+  return __byte_perm(__byte_perm(pair[0], pair[1], 0x0040), __byte_perm(pair[2], pair[3], 0x0040), 0x5410) ^ 0x88888888u;
 }
 
 // Infinities of a piece as the magnitude m with their sign.
@@ -238,6 +261,30 @@ __device__ __forceinline__ void int4_values(uint32_t w, float f, float (&v)[8]) 
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     v[i] = float(int32_t(w << (28 - 4 * i)) >> 28) * f;
+}
+
+__device__ __forceinline__ uint32_t bf162_fma(uint32_t x, uint32_t y, uint32_t z) {
+  uint32_t w;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(w) : "r"(x), "r"(y), "r"(z));
+  return w;
+}
+
+// Places kAt and kAt + 4 of a word's codes times f: a nibble t (two's complement, t
+// = u ^ 8 with u = code + 8) in bits 3-6 of a bf16 16 makes 16 + u, and an FMA takes
+// 24 f away.
+template <int kAt>
+__device__ __forceinline__ uint32_t int4_pair_bf16(uint32_t w, uint32_t f, uint32_t minus_24f) {
+  const uint32_t t = kAt == 0 ? w << 3 : w >> (kAt == 0 ? 0 : 4 * kAt - 3);
+  return bf162_fma((t & 0x00780078u) ^ 0x41c041c0u, f, minus_24f);
+}
+
+// Eight codes times f in order, exact where f is a number of four bits far from
+// bf16's limits.
+__device__ __forceinline__ uint4 int4_to_bf16x8(uint32_t w, float f) {
+  const uint32_t ff = pack_bf16x2(f, f), m = pack_bf16x2(-24.f * f, -24.f * f);
+  const uint32_t p0 = int4_pair_bf16<0>(w, ff, m), p1 = int4_pair_bf16<1>(w, ff, m);
+  const uint32_t p2 = int4_pair_bf16<2>(w, ff, m), p3 = int4_pair_bf16<3>(w, ff, m);
+  return make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
 }
 
 // Two 8-bit codes (the low 16 bits of `pair`) as fp32 values.
@@ -270,6 +317,95 @@ __device__ __forceinline__ int sequence_of_warp(const int *starts, int batch, in
     hi = min(hi, lo + step);
   } while (hi - lo > 1);
   return r < __ldg(starts + lo + 1) ? lo : -1;
+}
+
+// A row to its slot: D / 16 lanes of it with 16 bytes of either half each (x0 from
+// l * 8 on, x1 from D / 2 + l * 8 on); `codes`, `factors` and `scale` are the lane's
+// places.  All lanes of the warp come here.
+template <int kFormat, int D>
+__device__ __forceinline__ void keep_row(uint4 x0, uint4 x1, int l, bool kept, uint8_t *codes, uint8_t *factors, float *scale) {
+  constexpr int kLanes = D / 16;
+  if constexpr (kFormat == kCacheBf16) {
+    if (kept) {
+      *reinterpret_cast<uint4 *>(codes) = x0;
+      *reinterpret_cast<uint4 *>(codes + D) = x1;
+    }
+    return;
+  }
+  const uint32_t m0 = magnitude8(x0), m1 = magnitude8(x1);
+  if constexpr (kFormat == kCacheInt4) {
+    // Four lanes' pieces are a group; the halves of a word are the two groups'.
+    uint32_t mg = m0 | (m1 << 16);
+    mg = __vmaxu2(mg, __shfl_xor_sync(0xffffffffu, mg, 1));
+    mg = __vmaxu2(mg, __shfl_xor_sync(0xffffffffu, mg, 2));
+    uint32_t m = max(mg & 0xffffu, mg >> 16);
+    if (kLanes == 8)
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
+    if (__any_sync(0xffffffffu, m >= 0x7f80u)) {      // an infinity or a NaN in some row
+      m = max(magnitude8_finite(x0), magnitude8_finite(x1));
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1)
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (m > 0x7f80u)
+        x0 = x1 = make_uint4(0, 0, 0, 0);
+      x0 = bounded8(x0, m), x1 = bounded8(x1, m);
+      mg = magnitude8(x0) | (magnitude8(x1) << 16);
+      mg = __vmaxu2(mg, __shfl_xor_sync(0xffffffffu, mg, 1));
+      mg = __vmaxu2(mg, __shfl_xor_sync(0xffffffffu, mg, 2));
+    }
+    const float s = int4_scale(m), inverse = m > 0x7f80u ? 1.f : __uint_as_float(0x7f000000u - __float_as_uint(s));   // 1 / s
+    // Two lanes of a group make its first factor, two its second.
+    const uint32_t mine = int4_factor(l & 2 ? mg >> 16 : mg & 0xffffu, inverse);
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 2);
+    const uint32_t f0 = l & 2 ? other : mine, f1 = l & 2 ? mine : other;
+    const float a = e4m3_value(f0), b = e4m3_value(f1);
+    uint32_t q0, q1;
+    if (__all_sync(0xffffffffu, s >= 0x1p-100f && int4_ordinary(f0) && int4_ordinary(f1))) {
+      const float as = a * s, bs = b * s, ra = reciprocal_of_factor(as), rb = reciprocal_of_factor(bs);
+      q0 = ordinary8_int4(x0, as, ra);
+      q1 = ordinary8_int4(x1, bs, rb);
+    } else {
+      q0 = quantise4_int4(x0.x, x0.y, inverse, a) | (quantise4_int4(x0.z, x0.w, inverse, a) << 16);
+      q1 = quantise4_int4(x1.x, x1.y, inverse, b) | (quantise4_int4(x1.z, x1.w, inverse, b) << 16);
+    }
+    if (kept) {
+      *reinterpret_cast<uint32_t *>(codes) = q0;
+      *reinterpret_cast<uint32_t *>(codes + D / 4) = q1;
+      if ((l & 1) == 0)                               // two lanes of a group, one factor each
+        factors[l & 2 ? D / 2 / kFactorGroup : 0] = uint8_t(mine);
+      if (l == 0)
+        *scale = s;
+    }
+  } else {
+    uint32_t m = max(m0, m1);
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1)
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const bool odd = __any_sync(0xffffffffu, m >= 0x7f80u);   // an infinity or a NaN in some row
+    if (odd) {
+      m = max(magnitude8_finite(x0), magnitude8_finite(x1));
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1)
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    }
+    const float most = __uint_as_float(m << 16);
+    const float s = m == 0 ? 1.f : __fmul_rn(most, kFormat == kCacheInt8 ? 1.0f / 127.0f : 1.0f / 448.0f);
+    uint2 q[2];
+    if (!odd && s > 0x1p-80f && s < 0x1p100f) {
+      const float y = __frcp_rn(s);
+      q[0] = quantise8<kFormat>(x0, s, y);
+      q[1] = quantise8<kFormat>(x1, s, y);
+    } else {
+      q[0] = quantise8_any<kFormat>(x0, s);
+      q[1] = quantise8_any<kFormat>(x1, s);
+    }
+    if (kept) {
+      *reinterpret_cast<uint2 *>(codes) = q[0];
+      *reinterpret_cast<uint2 *>(codes + D / 2) = q[1];
+      if (l == 0)
+        *scale = s;
+    }
+  }
 }
 
 constexpr int kCacheWarps = 4;
@@ -326,42 +462,9 @@ __global__ void __launch_bounds__(kCacheWarps * 32) cache_write_kernel(const Cac
         *reinterpret_cast<uint4 *>(to + kLanes * 8) = x[i][1];
       }
     } else if constexpr (kFormat == kCacheInt4) {
-      // Four lanes' pieces are a group; a row's scale is that of all its groups.
-      uint32_t mg[2] = {magnitude8(x[i][0]), magnitude8(x[i][1])};
-      const bool odd = __any_sync(0xffffffffu, max(mg[0], mg[1]) >= 0x7f80u);   // an infinity or a NaN in some row
-      if (odd) {
-        mg[0] = magnitude8_finite(x[i][0]), mg[1] = magnitude8_finite(x[i][1]);
-      }
-      uint32_t m = max(mg[0], mg[1]);
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1)
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float s = int4_scale(m);
-      if (odd) {
-        if (m > 0x7f80u)
-          x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
-        x[i][0] = bounded8(x[i][0], m), x[i][1] = bounded8(x[i][1], m);
-        mg[0] = magnitude8(x[i][0]), mg[1] = magnitude8(x[i][1]);
-      }
-#pragma unroll
-      for (int o = 2; o > 0; o >>= 1) {
-        mg[0] = max(mg[0], __shfl_xor_sync(0xffffffffu, mg[0], o));
-        mg[1] = max(mg[1], __shfl_xor_sync(0xffffffffu, mg[1], o));
-      }
-      const float inverse = m > 0x7f80u ? 1.f : __uint_as_float(0x7f000000u - __float_as_uint(s));   // 1 / s
-      const uint32_t f0 = int4_factor(mg[0], inverse), f1 = int4_factor(mg[1], inverse);
-      const uint32_t q0 = quantise8_int4(x[i][0], inverse, e4m3_value(f0)), q1 = quantise8_int4(x[i][1], inverse, e4m3_value(f1));
-      if (r < 2 * hk) {
-        uint8_t *to = static_cast<uint8_t *>(r < hk ? a.c.k : a.c.v) + (r < hk ? k_at : v_at) + (slot * (D / 2) + l * 4);
-        *reinterpret_cast<uint32_t *>(to) = q0;
-        *reinterpret_cast<uint32_t *>(to + kLanes * 4) = q1;
-        if (l % 4 == 0) {
-          uint8_t *factor = (r < hk ? a.c.kf + page * a.c.kf_page : a.c.vf + page * a.c.vf_page) + slot * (D / kFactorGroup) + l / 4;
-          factor[0] = uint8_t(f0), factor[kLanes / 4] = uint8_t(f1);
-        }
-        if (l == 0)
-          (r < hk ? k_scale : v_scale)[slot] = s;
-      }
+      uint8_t *to = static_cast<uint8_t *>(r < hk ? a.c.k : a.c.v) + (r < hk ? k_at : v_at) + (slot * (D / 2) + l * 4);
+      uint8_t *factor = (r < hk ? a.c.kf + page * a.c.kf_page : a.c.vf + page * a.c.vf_page) + slot * (D / kFactorGroup) + l / 4;
+      keep_row<kFormat, D>(x[i][0], x[i][1], l, r < 2 * hk, to, factor, (r < hk ? k_scale : v_scale) + slot);
     } else {
       uint32_t m = max(magnitude8(x[i][0]), magnitude8(x[i][1]));
 #pragma unroll
@@ -424,34 +527,49 @@ struct CacheAppendArgs {
 // squares added within a lane, then by halves of the lanes.  z is rounded to
 // bf16; q leaves in it, and k and v are quantised from it as cache_write does.
 //
-// D / 8 lanes per head row, each with four channels of either half, so that a
-// rotation's pairs meet in a lane; a warp per token and 32 kFlight / (D / 8) of
-// its head rows at a time, all loaded before the token's place is known.
+// D / 16 lanes per head row, each with eight channels of either half, so that a
+// rotation's pairs meet in a lane; a warp per token takes kFlight passes over 32 /
+// (D / 16) head rows each at a time, the first loaded before the token's place is
+// known, first of q, then of k and v.  (With few tokens blockIdx.y names the
+// passes that a warp takes.)  The square root and division of kFlight passes'
+// norms are made at once, each in lanes of its own.
 template <int kFormat, int D, int kFlight>
 __global__ void __launch_bounds__(kCacheWarps * 32) cache_append_kernel(const CacheAppendArgs a) {
-  constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+  constexpr int kLanes = D / 16, kRows = 32 / kLanes, kTaken = kRows * kFlight;
+  static_assert(kFlight <= kLanes);
   pdl_wait();
   pdl_launch_dependents();
   const int64_t row = int64_t(blockIdx.x) * kCacheWarps + (threadIdx.x >> 5);
   if (row >= a.rows)
     return;
-  const int lane = threadIdx.x & 31, l = lane % kLanes, hk = a.c.hk, heads = a.hq + 2 * hk;
-  auto fetch = [&](int first, uint2 (&x)[kFlight][2]) {
+  const int lane = threadIdx.x & 31, l = lane % kLanes, of = lane / kLanes, hk = a.c.hk;
+  const __nv_bfloat16 *source = a.qkv + row * a.row + of * a.head + l * 8;
+  const int64_t apart = kRows * a.head;              // from pass to pass
+  // The rows of kFlight passes from head `first` of `heads` on.
+  auto fetch = [&](const __nv_bfloat16 *from, int first, int heads, uint4 (&x)[kFlight][2]) {
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
-      const int r = first + i * kRows + lane / kLanes;
-      x[i][0] = x[i][1] = make_uint2(0, 0);
-      if (r < heads) {
-        const uint2 *src = reinterpret_cast<const uint2 *>(a.qkv + row * a.row + r * a.head) + l;
+      x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
+      if (first + i * kRows + of < heads) {
+        const uint4 *src = reinterpret_cast<const uint4 *>(from + i * apart);
         x[i][0] = *src;
-        x[i][1] = src[D / 8];
+        x[i][1] = src[D / 16];
       }
     }
   };
-  const int step = gridDim.y * kRows * kFlight;
-  int first = blockIdx.y * kRows * kFlight;
-  uint2 x[kFlight][2];
-  fetch(first, x);
+  // This warp's passes: all, or those of one kFlight of one kind.
+  int kind = 0, begin = 0, stop = 3;
+  bool one = false;
+  if (gridDim.y > 1) {
+    const int q_parts = (a.hq + kTaken - 1) / kTaken, kv_parts = (hk + kTaken - 1) / kTaken, part = blockIdx.y;
+    kind = part < q_parts ? 0 : part < q_parts + kv_parts ? 1 : 2;
+    begin = (part - (kind == 0 ? 0 : kind == 1 ? q_parts : q_parts + kv_parts)) * kTaken;
+    stop = kind + 1;
+    one = true;
+  }
+  auto start_of = [&](int which, int first) { return source + int64_t((which == 0 ? 0 : which == 1 ? a.hq : a.hq + hk) + first) * a.head; };
+  uint4 x[kFlight][2];
+  fetch(start_of(kind, begin), begin, kind == 0 ? a.hq : hk, x);
   const int b = sequence_of_warp(a.starts, a.batch, row);
   if (b < 0)
     return;
@@ -462,128 +580,128 @@ __global__ void __launch_bounds__(kCacheWarps * 32) cache_append_kernel(const Ca
     record_status(kStatusBadPosition);
     turn = 0;
   }
-  float2 cos[2], sin[2];
-  {
-    const float4 c = __ldg(reinterpret_cast<const float4 *>(a.cos + turn * (D / 2)) + l);
-    const float4 s = __ldg(reinterpret_cast<const float4 *>(a.sin + turn * (D / 2)) + l);
-    cos[0] = make_float2(c.x, c.y), cos[1] = make_float2(c.z, c.w);
-    sin[0] = make_float2(s.x, s.y), sin[1] = make_float2(s.z, s.w);
+  float2 cos[4], sin[4];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float4 c = __ldg(reinterpret_cast<const float4 *>(a.cos + turn * (D / 2)) + 2 * l + j);
+    const float4 s = __ldg(reinterpret_cast<const float4 *>(a.sin + turn * (D / 2)) + 2 * l + j);
+    cos[2 * j] = make_float2(c.x, c.y), cos[2 * j + 1] = make_float2(c.z, c.w);
+    sin[2 * j] = make_float2(s.x, s.y), sin[2 * j + 1] = make_float2(s.z, s.w);
   }
-  const int page = turned ? page_of(a.c, b, pos) : -1;
+  const int found = turned ? page_of(a.c, b, pos) : -1;
+  const int64_t page = max(found, 0);
   const int in_page = int(pos & ((1 << a.c.shift) - 1));
-  for (;;) {
-#pragma unroll
-    for (int i = 0; i < kFlight; ++i) {
-      const int r0 = first + i * kRows, r = r0 + lane / kLanes;
-      if (r0 >= heads)
-        break;
-      const bool is_q = r < a.hq, is_v = r >= a.hq + hk;
-      uint2 &lo = x[i][0], &hi = x[i][1];
-      if (r0 < a.hq + hk) {                       // some row of the warp is turned
-        float2 u[2] = {bf16_pair(lo.x), bf16_pair(lo.y)}, v[2] = {bf16_pair(hi.x), bf16_pair(hi.y)};
-        const __nv_bfloat16 *weight = is_q ? a.q_weight : a.k_weight;
-        const float2 p = __fadd2_rn(__fmul2_rn(u[0], u[0]), __fmul2_rn(v[0], v[0]));
-        const float2 q = __fadd2_rn(__fmul2_rn(u[1], u[1]), __fmul2_rn(v[1], v[1]));
-        const float2 pq = __fadd2_rn(p, q);
-        float sum = __fadd_rn(pq.x, pq.y);
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1)
-          sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
-        if (weight != nullptr) {
-          const float inv = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(sum * (1.f / D), a.eps)));
-          const float2 inv2 = make_float2(inv, inv);
-          const uint2 wl = __ldg(reinterpret_cast<const uint2 *>(weight) + l), wh = __ldg(reinterpret_cast<const uint2 *>(weight) + l + D / 8);
-          u[0] = __fmul2_rn(__fmul2_rn(u[0], inv2), bf16_pair(wl.x)), u[1] = __fmul2_rn(__fmul2_rn(u[1], inv2), bf16_pair(wl.y));
-          v[0] = __fmul2_rn(__fmul2_rn(v[0], inv2), bf16_pair(wh.x)), v[1] = __fmul2_rn(__fmul2_rn(v[1], inv2), bf16_pair(wh.y));
-        }
-        if (!is_v) {
-          uint32_t ww[4];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            // Single sums: a pair's would be joined with the products into FMAs.
-            const float2 uc = __fmul2_rn(u[j], cos[j]), vs = __fmul2_rn(v[j], sin[j]);
-            const float2 vc = __fmul2_rn(v[j], cos[j]), us = __fmul2_rn(u[j], sin[j]);
-            ww[j] = pack_bf16x2(__fsub_rn(uc.x, vs.x), __fsub_rn(uc.y, vs.y));
-            ww[2 + j] = pack_bf16x2(__fadd_rn(vc.x, us.x), __fadd_rn(vc.y, us.y));
-          }
-          lo = make_uint2(ww[0], ww[1]), hi = make_uint2(ww[2], ww[3]);
-          __nv_bfloat16 *to = is_q ? a.q_out + row * a.q_row + r * D : a.k_out + row * a.k_row + (r - a.hq) * D;
-          if (is_q || a.k_out != nullptr) {
-            *reinterpret_cast<uint2 *>(to + l * 4) = lo;
-            *reinterpret_cast<uint2 *>(to + D / 2 + l * 4) = hi;
-          }
-        }
-      }
-      if (r0 + kRows <= a.hq)                     // rows of q alone
-        continue;
-      const bool kept = !is_q && r < heads && page >= 0;
-      const int head = is_v ? r - a.hq - hk : r - a.hq;
-      const int slot = (max(head, 0) << a.c.shift) + in_page;
-      const int64_t page_at = int64_t(page) * (is_v ? a.c.v_page : a.c.k_page);
-      void *codes = is_v ? a.c.v : a.c.k;
-      if constexpr (kFormat == kCacheBf16) {
-        if (kept) {
-          __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(codes) + page_at + slot * D + l * 4;
-          *reinterpret_cast<uint2 *>(to) = lo;
-          *reinterpret_cast<uint2 *>(to + D / 2) = hi;
-        }
-      } else {
-        uint4 y = make_uint4(lo.x, lo.y, hi.x, hi.y);
-        uint32_t m = magnitude8(y);
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1)
-          m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const bool odd = __any_sync(0xffffffffu, m >= 0x7f80u);   // an infinity or a NaN in some row
-        if (odd) {
-          m = magnitude8_finite(y);
-#pragma unroll
-          for (int o = kLanes / 2; o > 0; o >>= 1)
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        }
-        float *scales = (is_v ? a.c.vs + int64_t(page) * a.c.vs_page : a.c.ks + int64_t(page) * a.c.ks_page);
-        if constexpr (kFormat == kCacheInt4) {
-          const float s = int4_scale(m);
-          if (odd)
-            y = m > 0x7f80u ? make_uint4(0, 0, 0, 0) : bounded8(y, m);
-          const float inverse = m > 0x7f80u ? 1.f : __uint_as_float(0x7f000000u - __float_as_uint(s));
-          // Eight lanes' channels of either half are a group.
-          uint32_t most = __vmaxu2(y.x & 0x7fff7fffu, y.y & 0x7fff7fffu), next = __vmaxu2(y.z & 0x7fff7fffu, y.w & 0x7fff7fffu);
-          most = max(most & 0xffffu, most >> 16) | (max(next & 0xffffu, next >> 16) << 16);
-#pragma unroll
-          for (int o = 4; o > 0; o >>= 1)
-            most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
-          const uint32_t f0 = int4_factor(most & 0xffffu, inverse), f1 = int4_factor(most >> 16, inverse);
-          const uint32_t q0 = quantise4_int4(y.x, y.y, inverse, e4m3_value(f0)), q1 = quantise4_int4(y.z, y.w, inverse, e4m3_value(f1));
-          if (kept) {
-            uint8_t *to = static_cast<uint8_t *>(codes) + page_at + slot * (D / 2) + l * 2;
-            *reinterpret_cast<uint16_t *>(to) = uint16_t(q0);
-            *reinterpret_cast<uint16_t *>(to + D / 4) = uint16_t(q1);
-            if (l % 8 == 0) {
-              uint8_t *factor = (is_v ? a.c.vf + int64_t(page) * a.c.vf_page : a.c.kf + int64_t(page) * a.c.kf_page) +
-                                slot * (D / kFactorGroup) + l / 8;
-              factor[0] = uint8_t(f0), factor[D / 2 / kFactorGroup] = uint8_t(f1);
-            }
-            if (l == 0)
-              scales[slot] = s;
-          }
-        } else {
-          const float most = __uint_as_float(m << 16);
-          const float s = m == 0 ? 1.f : __fmul_rn(most, kFormat == kCacheInt8 ? 1.0f / 127.0f : 1.0f / 448.0f);
-          const uint2 q = !odd && s > 0x1p-80f && s < 0x1p100f ? quantise8<kFormat>(y, s, __frcp_rn(s)) : quantise8_any<kFormat>(y, s);
-          if (kept) {
-            uint8_t *to = static_cast<uint8_t *>(codes) + page_at + slot * D + l * 4;
-            *reinterpret_cast<uint32_t *>(to) = q.x;
-            *reinterpret_cast<uint32_t *>(to + D / 2) = q.y;
-            if (l == 0)
-              scales[slot] = s;
-          }
-        }
-      }
+
+  // All passes of one kind: 0 q, 1 k, 2 v.
+  auto take = [&](auto which) {
+    constexpr int kKind = which.value;
+    constexpr bool kTurned = kKind < 2, kKept = kKind > 0;
+    const int heads = kKind == 0 ? a.hq : hk;
+    // This lane's places for head `begin + of`, and from pass to pass.
+    const int slot = ((begin + of) << a.c.shift) + in_page, slots = kRows << a.c.shift;
+    uint8_t *codes = nullptr, *factors = nullptr;
+    float *scales = nullptr;
+    if constexpr (kKept) {
+      codes = static_cast<uint8_t *>(kKind == 1 ? a.c.k : a.c.v) +
+              (kFormat == kCacheBf16 ? 2 : 1) * page * (kKind == 1 ? a.c.k_page : a.c.v_page) +
+              int64_t(slot) * code_bytes(kFormat, D) + l * code_bytes(kFormat, 8);
+      if constexpr (kFormat != kCacheBf16)
+        scales = (kKind == 1 ? a.c.ks + page * a.c.ks_page : a.c.vs + page * a.c.vs_page) + slot;
+      if constexpr (kFormat == kCacheInt4)
+        factors = (kKind == 1 ? a.c.kf + page * a.c.kf_page : a.c.vf + page * a.c.vf_page) + slot * (D / kFactorGroup) + l / 4;
     }
-    first += step;
-    if (first >= heads)
-      break;
-    fetch(first, x);
+    __nv_bfloat16 *out = nullptr;
+    if constexpr (kTurned) {
+      out = kKind == 0 ? a.q_out + row * a.q_row : a.k_out == nullptr ? nullptr : a.k_out + row * a.k_row;
+      if (out != nullptr)
+        out += (begin + of) * D + l * 8;
+    }
+    const __nv_bfloat16 *weight = kKind == 0 ? a.q_weight : kKind == 1 ? a.k_weight : nullptr;
+    uint4 wl, wh;
+    if (kTurned && weight != nullptr) {
+      wl = __ldg(reinterpret_cast<const uint4 *>(weight) + l), wh = __ldg(reinterpret_cast<const uint4 *>(weight) + l + D / 16);
+    }
+    const __nv_bfloat16 *from = start_of(kKind, begin);
+    for (int first = begin;;) {
+      float inverse[kFlight];
+      if (kTurned && weight != nullptr) {
+        float mine = 0.f;
+#pragma unroll
+        for (int i = 0; i < kFlight; ++i) {
+          // Sums of four channels and their partners, two of them per lane.
+          auto sum_of = [&](uint32_t p0, uint32_t p1, uint32_t q0, uint32_t q1) {
+            const float2 u0 = bf16_pair(p0), u1 = bf16_pair(p1), v0 = bf16_pair(q0), v1 = bf16_pair(q1);
+            const float2 p = __fadd2_rn(__fmul2_rn(u0, u0), __fmul2_rn(v0, v0)), q = __fadd2_rn(__fmul2_rn(u1, u1), __fmul2_rn(v1, v1));
+            const float2 pq = __fadd2_rn(p, q);
+            return __fadd_rn(pq.x, pq.y);
+          };
+          float s0 = sum_of(x[i][0].x, x[i][0].y, x[i][1].x, x[i][1].y), s1 = sum_of(x[i][0].z, x[i][0].w, x[i][1].z, x[i][1].w);
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) {
+            s0 = __fadd_rn(s0, __shfl_xor_sync(0xffffffffu, s0, o));
+            s1 = __fadd_rn(s1, __shfl_xor_sync(0xffffffffu, s1, o));
+          }
+          mine = l % kFlight == i ? __fadd_rn(s0, s1) : mine;
+        }
+        mine = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(mine * (1.f / D), a.eps)));
+#pragma unroll
+        for (int i = 0; i < kFlight; ++i)
+          inverse[i] = __shfl_sync(0xffffffffu, mine, of * kLanes + i);
+      }
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i) {
+        if (first + i * kRows >= heads)
+          break;
+        const bool there = first + i * kRows + of < heads;
+        uint4 y0 = x[i][0], y1 = x[i][1];
+        if constexpr (kTurned) {
+          const uint32_t lo[4] = {y0.x, y0.y, y0.z, y0.w}, hi[4] = {y1.x, y1.y, y1.z, y1.w};
+          const uint32_t wlo[4] = {wl.x, wl.y, wl.z, wl.w}, whi[4] = {wh.x, wh.y, wh.z, wh.w};
+          uint32_t z[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float2 u = bf16_pair(lo[j]), v = bf16_pair(hi[j]);
+            if (weight != nullptr) {
+              const float2 inv2 = make_float2(inverse[i], inverse[i]);
+              u = __fmul2_rn(__fmul2_rn(u, inv2), bf16_pair(wlo[j]));
+              v = __fmul2_rn(__fmul2_rn(v, inv2), bf16_pair(whi[j]));
+            }
+            // Single sums: a pair's would be joined with the products into FMAs.
+            const float2 uc = __fmul2_rn(u, cos[j]), vs = __fmul2_rn(v, sin[j]);
+            const float2 vc = __fmul2_rn(v, cos[j]), us = __fmul2_rn(u, sin[j]);
+            z[j] = pack_bf16x2(__fsub_rn(uc.x, vs.x), __fsub_rn(uc.y, vs.y));
+            z[4 + j] = pack_bf16x2(__fadd_rn(vc.x, us.x), __fadd_rn(vc.y, us.y));
+          }
+          y0 = make_uint4(z[0], z[1], z[2], z[3]), y1 = make_uint4(z[4], z[5], z[6], z[7]);
+          if (there && (kKind == 0 || out != nullptr)) {
+            *reinterpret_cast<uint4 *>(out) = y0;
+            *reinterpret_cast<uint4 *>(out + D / 2) = y1;
+          }
+          out = kKind == 0 || out != nullptr ? out + kRows * D : out;
+        }
+        if constexpr (kKept) {
+          keep_row<kFormat, D>(y0, y1, l, there && found >= 0, codes, factors, scales);
+          codes += slots * code_bytes(kFormat, D);
+          factors += slots * (D / kFactorGroup);
+          scales += slots;
+        }
+      }
+      first += kTaken;
+      if (one || first >= heads)
+        break;
+      from += kFlight * apart;
+      fetch(from, first, heads, x);
+    }
+  };
+  for (; kind < stop; ++kind) {
+    if (kind == 0)
+      take(std::integral_constant<int, 0>{});
+    else if (kind == 1)
+      take(std::integral_constant<int, 1>{});
+    else
+      take(std::integral_constant<int, 2>{});
+    if (kind + 1 < stop)
+      fetch(start_of(kind + 1, 0), 0, hk, x);
   }
 }
 
@@ -639,10 +757,16 @@ __global__ void __launch_bounds__(kCacheWarps * 32) cache_read_kernel(const Cach
       const int r = r0 + i * kRows + lane / kLanes, head = r < hk ? r : r - hk;
       uint4 y = x[i];
       if constexpr (kFormat == kCacheInt4) {
-        float f[8];
-        int4_values(x[i].x, e4m3_value(factor[i]), f);
-        y = make_uint4(pack_bf16x2(f[0] * s[i], f[1] * s[i]), pack_bf16x2(f[2] * s[i], f[3] * s[i]),
-                       pack_bf16x2(f[4] * s[i], f[5] * s[i]), pack_bf16x2(f[6] * s[i], f[7] * s[i]));
+        const float f = e4m3_value(factor[i]);
+        // A power of two (or 0), as cache_write makes them, changes no bits of the products.
+        if (__all_sync(0xffffffffu, (__float_as_uint(s[i]) & 0x807fffffu) == 0 && s[i] < 0x1p100f && (s[i] == 0.f || s[i] > 0x1p-100f) && f == f)) {
+          y = int4_to_bf16x8(x[i].x, f * s[i]);
+        } else {
+          float v[8];
+          int4_values(x[i].x, f, v);
+          y = make_uint4(pack_bf16x2(v[0] * s[i], v[1] * s[i]), pack_bf16x2(v[2] * s[i], v[3] * s[i]),
+                         pack_bf16x2(v[4] * s[i], v[5] * s[i]), pack_bf16x2(v[6] * s[i], v[7] * s[i]));
+        }
       } else if constexpr (kFormat != kCacheBf16) {
         uint32_t w[4];
 #pragma unroll
