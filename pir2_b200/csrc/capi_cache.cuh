@@ -135,8 +135,12 @@ static int launch_rows(bool write, const CacheRowsArgs &a, void *stream) {
   constexpr int kRows = 32 / (D / 16);                      // rows of a warp's load
   const int64_t grid = (a.rows + kCacheWarps - 1) / kCacheWarps;
   const int loads = (2 * a.c.hk + kRows - 1) / kRows;
-  if (!write)
-    return launch_cache("cache_read launch", cache_read_kernel<kFormat, D>, grid, 1, 1, kCacheWarps * 32, 0, stream, a);
+  if (!write) {
+    if constexpr (kFormat == kCacheInt4)
+      return launch_cache("cache_read launch", cache_read_int4_kernel<D>, grid, 1, 1, kCacheWarps * 32, 0, stream, a);
+    else
+      return launch_cache("cache_read launch", cache_read_kernel<kFormat, D>, grid, 1, 1, kCacheWarps * 32, 0, stream, a);
+  }
   if (a.rows * loads <= 4096)
     return launch_cache("cache_write launch", cache_write_kernel<kFormat, D, 1>, grid, loads, 1, kCacheWarps * 32, 0, stream, a);
   return launch_cache("cache_write launch", cache_write_kernel<kFormat, D, 4>, grid, (loads + 3) / 4, 1, kCacheWarps * 32, 0,

@@ -534,7 +534,7 @@ struct CacheAppendArgs {
 // passes that a warp takes.)  The square root and division of kFlight passes'
 // norms are made at once, each in lanes of its own.
 template <int kFormat, int D, int kFlight>
-__global__ void __launch_bounds__(kCacheWarps * 32) cache_append_kernel(const CacheAppendArgs a) {
+__global__ void __launch_bounds__(kCacheWarps * 32, 5) cache_append_kernel(const CacheAppendArgs a) {
   constexpr int kLanes = D / 16, kRows = 32 / kLanes, kTaken = kRows * kFlight;
   static_assert(kFlight <= kLanes);
   pdl_wait();
@@ -570,6 +570,13 @@ __global__ void __launch_bounds__(kCacheWarps * 32) cache_append_kernel(const Ca
   auto start_of = [&](int which, int first) { return source + int64_t((which == 0 ? 0 : which == 1 ? a.hq : a.hq + hk) + first) * a.head; };
   uint4 x[kFlight][2];
   fetch(start_of(kind, begin), begin, kind == 0 ? a.hq : hk, x);
+  if (!one)                                           // the rest of the token's rows on their way to L2
+    for (int head = lane; head < a.hq + 2 * hk; head += 32) {
+      const __nv_bfloat16 *at = a.qkv + row * a.row + head * a.head;
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+      if (D == 128)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(at + 64));
+    }
   const int b = sequence_of_warp(a.starts, a.batch, row);
   if (b < 0)
     return;
@@ -726,25 +733,17 @@ __global__ void __launch_bounds__(kCacheWarps * 32) cache_read_kernel(const Cach
   for (int r0 = 0; r0 < 2 * hk; r0 += kRows * kFlight) {
     uint4 x[kFlight];
     float s[kFlight];
-    uint32_t factor[kFlight];
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
       const int r = r0 + i * kRows + lane / kLanes, head = r < hk ? r : r - hk;
       const int64_t slot = (int64_t(head) << a.c.shift) + in_page;
-      const int64_t at = page * (r < hk ? a.c.k_page : a.c.v_page) +
-                         (kFormat == kCacheInt4 ? slot * (D / 2) + l * 4 : slot * D + l * 8);
+      const int64_t at = page * (r < hk ? a.c.k_page : a.c.v_page) + slot * D + l * 8;
       x[i] = make_uint4(0, 0, 0, 0);
       s[i] = 0.f;
-      factor[i] = 0;
       if (r < 2 * hk && page >= 0) {
         const void *codes = r < hk ? a.c.k : a.c.v;
         if constexpr (kFormat == kCacheBf16) {
           x[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(codes) + at));
-        } else if constexpr (kFormat == kCacheInt4) {
-          x[i].x = __ldg(reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(codes) + at));
-          factor[i] = __ldg((r < hk ? a.c.kf + page * a.c.kf_page : a.c.vf + page * a.c.vf_page) +
-                            slot * (D / kFactorGroup) + l / 4);
-          s[i] = __ldg((r < hk ? a.c.ks + page * a.c.ks_page : a.c.vs + page * a.c.vs_page) + slot);
         } else {
           const uint2 q = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(codes) + at));
           x[i].x = q.x, x[i].y = q.y;
@@ -756,18 +755,7 @@ __global__ void __launch_bounds__(kCacheWarps * 32) cache_read_kernel(const Cach
     for (int i = 0; i < kFlight; ++i) {
       const int r = r0 + i * kRows + lane / kLanes, head = r < hk ? r : r - hk;
       uint4 y = x[i];
-      if constexpr (kFormat == kCacheInt4) {
-        const float f = e4m3_value(factor[i]);
-        // A power of two (or 0), as cache_write makes them, changes no bits of the products.
-        if (__all_sync(0xffffffffu, (__float_as_uint(s[i]) & 0x807fffffu) == 0 && s[i] < 0x1p100f && (s[i] == 0.f || s[i] > 0x1p-100f) && f == f)) {
-          y = int4_to_bf16x8(x[i].x, f * s[i]);
-        } else {
-          float v[8];
-          int4_values(x[i].x, f, v);
-          y = make_uint4(pack_bf16x2(v[0] * s[i], v[1] * s[i]), pack_bf16x2(v[2] * s[i], v[3] * s[i]),
-                         pack_bf16x2(v[4] * s[i], v[5] * s[i]), pack_bf16x2(v[6] * s[i], v[7] * s[i]));
-        }
-      } else if constexpr (kFormat != kCacheBf16) {
+      if constexpr (kFormat != kCacheBf16) {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -779,6 +767,73 @@ __global__ void __launch_bounds__(kCacheWarps * 32) cache_read_kernel(const Cach
       }
       if (r < 2 * hk)
         *reinterpret_cast<uint4 *>((r < hk ? a.k_out : a.v_out) + (row * hk + head) * D + l * 8) = y;
+    }
+  }
+}
+
+// The same of int4 pages: D / 16 lanes per row with eight channels of either half
+// each (so that stores of a row lie side by side), k and v at once.
+template <int D>
+__global__ void __launch_bounds__(kCacheWarps * 32) cache_read_int4_kernel(const CacheRowsArgs a) {
+  constexpr int kLanes = D / 16, kRows = 32 / kLanes;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t row = int64_t(blockIdx.x) * kCacheWarps + (threadIdx.x >> 5);
+  if (row >= a.rows)
+    return;
+  const int lane = threadIdx.x & 31, l = lane % kLanes, of = lane / kLanes, hk = a.c.hk;
+  const int b = sequence_of_warp(a.starts, a.batch, row);
+  if (b < 0)
+    return;
+  const int64_t pos = row - __ldg(a.starts + b);
+  const int found = page_of(a.c, b, pos);
+  const int64_t page = max(found, 0);
+  // This lane's places, of k and of v, and from pass to pass.
+  const int slot = (of << a.c.shift) + int(pos & ((1 << a.c.shift) - 1)), slots = kRows << a.c.shift;
+  const uint8_t *codes[2] = {static_cast<const uint8_t *>(a.c.k) + page * a.c.k_page + slot * (D / 2) + l * 4,
+                             static_cast<const uint8_t *>(a.c.v) + page * a.c.v_page + slot * (D / 2) + l * 4};
+  const uint8_t *factors[2] = {a.c.kf + page * a.c.kf_page + slot * (D / kFactorGroup) + l / 4,
+                               a.c.vf + page * a.c.vf_page + slot * (D / kFactorGroup) + l / 4};
+  const float *scales[2] = {a.c.ks + page * a.c.ks_page + slot, a.c.vs + page * a.c.vs_page + slot};
+  __nv_bfloat16 *out[2] = {a.k_out + (row * hk + of) * D + l * 8, a.v_out + (row * hk + of) * D + l * 8};
+  for (int head = of; head - of < hk; head += kRows) {
+    const bool there = head < hk;
+    uint32_t x[2][2], f8[2][2];
+    float s[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x[i][0] = x[i][1] = f8[i][0] = f8[i][1] = 0;
+      s[i] = 0.f;
+      if (there && found >= 0) {
+        x[i][0] = __ldg(reinterpret_cast<const uint32_t *>(codes[i]));
+        x[i][1] = __ldg(reinterpret_cast<const uint32_t *>(codes[i] + D / 4));
+        f8[i][0] = __ldg(factors[i]), f8[i][1] = __ldg(factors[i] + D / 2 / kFactorGroup);
+        s[i] = __ldg(scales[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint4 y[2];
+      const float f[2] = {e4m3_value(f8[i][0]), e4m3_value(f8[i][1])};
+      // A power of two (or 0), as cache_write makes them, changes no bits of the products.
+      if (__all_sync(0xffffffffu, (__float_as_uint(s[i]) & 0x807fffffu) == 0 && s[i] < 0x1p100f && (s[i] == 0.f || s[i] > 0x1p-100f) &&
+                                      f[0] == f[0] && f[1] == f[1])) {
+        y[0] = int4_to_bf16x8(x[i][0], f[0] * s[i]);
+        y[1] = int4_to_bf16x8(x[i][1], f[1] * s[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float v[8];
+          int4_values(x[i][j], f[j], v);
+          y[j] = make_uint4(pack_bf16x2(v[0] * s[i], v[1] * s[i]), pack_bf16x2(v[2] * s[i], v[3] * s[i]),
+                            pack_bf16x2(v[4] * s[i], v[5] * s[i]), pack_bf16x2(v[6] * s[i], v[7] * s[i]));
+        }
+      }
+      if (there) {
+        *reinterpret_cast<uint4 *>(out[i]) = y[0];
+        *reinterpret_cast<uint4 *>(out[i] + D / 2) = y[1];
+      }
+      codes[i] += slots * (D / 2), factors[i] += slots * (D / kFactorGroup), scales[i] += slots, out[i] += kRows * D;
     }
   }
 }
