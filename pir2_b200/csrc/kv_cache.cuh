@@ -319,6 +319,31 @@ __device__ __forceinline__ int sequence_of_warp(const int *starts, int batch, in
   return r < __ldg(starts + lo + 1) ? lo : -1;
 }
 
+// What keep_row needs of rows with an infinity or a NaN among them, and of groups
+// with small factors: out of the way of the others.
+struct BoundedRow {
+  uint4 x0, x1;
+  uint32_t m, mg;       // largest finite magnitude (or a NaN's), the groups'
+};
+
+template <int kLanes>
+__device__ __noinline__ BoundedRow bounded_row(uint4 x0, uint4 x1) {
+  uint32_t m = max(magnitude8_finite(x0), magnitude8_finite(x1));
+  for (int o = kLanes / 2; o > 0; o >>= 1)
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (m > 0x7f80u)
+    x0 = x1 = make_uint4(0, 0, 0, 0);
+  x0 = bounded8(x0, m), x1 = bounded8(x1, m);
+  uint32_t mg = magnitude8(x0) | (magnitude8(x1) << 16);
+  mg = __vmaxu2(mg, __shfl_xor_sync(0xffffffffu, mg, 1));
+  mg = __vmaxu2(mg, __shfl_xor_sync(0xffffffffu, mg, 2));
+  return {x0, x1, m, mg};
+}
+
+__device__ __noinline__ uint32_t quantise8_int4_any(uint4 x, float inverse, float f) {
+  return quantise4_int4(x.x, x.y, inverse, f) | (quantise4_int4(x.z, x.w, inverse, f) << 16);
+}
+
 // A row to its slot: D / 16 lanes of it with 16 bytes of either half each (x0 from
 // l * 8 on, x1 from D / 2 + l * 8 on); `codes`, `factors` and `scale` are the lane's
 // places.  All lanes of the warp come here.
@@ -342,16 +367,8 @@ __device__ __forceinline__ void keep_row(uint4 x0, uint4 x1, int l, bool kept, u
     if (kLanes == 8)
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
     if (__any_sync(0xffffffffu, m >= 0x7f80u)) {      // an infinity or a NaN in some row
-      m = max(magnitude8_finite(x0), magnitude8_finite(x1));
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1)
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if (m > 0x7f80u)
-        x0 = x1 = make_uint4(0, 0, 0, 0);
-      x0 = bounded8(x0, m), x1 = bounded8(x1, m);
-      mg = magnitude8(x0) | (magnitude8(x1) << 16);
-      mg = __vmaxu2(mg, __shfl_xor_sync(0xffffffffu, mg, 1));
-      mg = __vmaxu2(mg, __shfl_xor_sync(0xffffffffu, mg, 2));
+      const BoundedRow bounded = bounded_row<kLanes>(x0, x1);
+      x0 = bounded.x0, x1 = bounded.x1, m = bounded.m, mg = bounded.mg;
     }
     const float s = int4_scale(m), inverse = m > 0x7f80u ? 1.f : __uint_as_float(0x7f000000u - __float_as_uint(s));   // 1 / s
     // Two lanes of a group make its first factor, two its second.
@@ -365,8 +382,8 @@ __device__ __forceinline__ void keep_row(uint4 x0, uint4 x1, int l, bool kept, u
       q0 = ordinary8_int4(x0, as, ra);
       q1 = ordinary8_int4(x1, bs, rb);
     } else {
-      q0 = quantise4_int4(x0.x, x0.y, inverse, a) | (quantise4_int4(x0.z, x0.w, inverse, a) << 16);
-      q1 = quantise4_int4(x1.x, x1.y, inverse, b) | (quantise4_int4(x1.z, x1.w, inverse, b) << 16);
+      q0 = quantise8_int4_any(x0, inverse, a);
+      q1 = quantise8_int4_any(x1, inverse, b);
     }
     if (kept) {
       *reinterpret_cast<uint32_t *>(codes) = q0;
