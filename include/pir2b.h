@@ -404,11 +404,16 @@ int pir2b_attention_causal(const void *q, const void *k, const void *v, int64_t 
  * + bias[n]), sums in fp32.  packed: [n, k / 2], two's complement codes of -8..7,
  * two to a byte with the even k in the low bits; scales: bf16 [n, k / group],
  * group 32, 64 or 128; bias: bf16 [n] or null; k a multiple of group.  x is
- * 16-byte aligned with a row stride that is a multiple of 8.  Meant for decoding:
- * the weights are read once for every 64 rows. */
+ * 16-byte aligned with a row stride that is a multiple of 8, packed and scales
+ * 16-byte aligned.  Meant for decoding: the weights are read once for every 64
+ * rows. */
 int pir2b_gemm_w4a16(const void *x, int64_t ldx, const void *packed, const void *scales, int group,
                      const void *bias, int64_t m, int64_t n, int64_t k, void *out, int64_t ldo,
-                     void *stream);
+                     void *workspace, void *stream);
+
+/* Bytes of workspace (16-byte aligned, uninitialised, written and read by the
+ * call alone) that pir2b_gemm_w4a16 needs for these shapes; may be 0. */
+int64_t pir2b_gemm_w4a16_workspace(int64_t m, int64_t n, int64_t k, int group);
 
 /* ---- ragged batches and the paged K/V cache of the text layers ----------
  *

@@ -83,7 +83,8 @@ SIGNATURES = {
     "pir2b_attention_rows": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I, _I, _F, _P],
     "pir2b_unpack_int4": [_P, _I64, _I64, _P, _P],
     "pir2b_attention_causal": [_P, _P, _P, _I64, _I64, _I, _I, _I, _F, _P, _I64, _P],
-    "pir2b_gemm_w4a16": [_P, _I64, _P, _P, _I, _P, _I64, _I64, _I64, _P, _I64, _P],
+    "pir2b_gemm_w4a16": [_P, _I64, _P, _P, _I, _P, _I64, _I64, _I64, _P, _I64, _P, _P],
+    "pir2b_gemm_w4a16_workspace": [_I64, _I64, _I64, _I],
     "pir2b_prompt_attention": [
         _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _I, _I, _F, _P, _I64, _P,
     ],
@@ -119,7 +120,7 @@ def lib():
         fn.argtypes = argtypes
         fn.restype = {
             "pir2b_last_error": ctypes.c_char_p, "pir2b_dit_ffn_workspace": _I64,
-            "pir2b_cache_attention_workspace": _I64,
+            "pir2b_cache_attention_workspace": _I64, "pir2b_gemm_w4a16_workspace": _I64,
         }.get(name, _I)
     return handle
 
@@ -174,4 +175,14 @@ def set_few_mode(mode):
     previous = lib().pir2b_set_few_mode(int(mode))
     if previous < 0:
         check(previous, "set_few_mode")
+    return previous
+
+
+def set_w4_mode(mode):
+    """Plan override for tests and measurement of gemm_w4a16: 0 lets its rules
+    choose, 1 never keeps the rows in shared memory, 2 does wherever they fit.
+    Returns the previous mode."""
+    previous = lib().pir2b_set_w4_mode(int(mode))
+    if previous < 0:
+        check(-previous, "set_w4_mode")
     return previous

@@ -688,9 +688,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
         for (int x = 0; x < 2; ++x) {
           const uint8_t *at = k_tile + h * kTile + k_off + x * kEight;
           if constexpr (KW == 4)
-            *reinterpret_cast<uint4 *>(kr[x]) = *reinterpret_cast<const uint4 *>(at);
+            load_words<4>(kr[x], at);
           else
-            *reinterpret_cast<uint2 *>(kr[x]) = *reinterpret_cast<const uint2 *>(at);
+            load_words<2>(kr[x], at);
         }
         const uint8_t *f = side + h * Shape::kBeside + q4 * (D / 4) / kFactorGroup;
         uint32_t two;
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
         for (int x = 0; x < 4; ++x) {
           const uint8_t *at = v_tile + h * kTile + (x & 1 ? v_odd : v_even) + (x >> 1) * kEight;
           if constexpr (VW == 2)
-            *reinterpret_cast<uint2 *>(vr[x]) = *reinterpret_cast<const uint2 *>(at);
+            load_words<2>(vr[x], at);
           else
             vr[x][0] = *reinterpret_cast<const uint32_t *>(at);
         }
@@ -853,7 +853,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
     for (int x = 0; x < 4; ++x) {
       const uint8_t *at = v_tile + (x & 1 ? v_odd : v_even) + (x >> 1) * kEight;
       if constexpr (VW == 2) {
-        *reinterpret_cast<uint2 *>(vr[x]) = *reinterpret_cast<const uint2 *>(at);
+        load_words<2>(vr[x], at);
       } else {
 #pragma unroll
         for (int i = 0; i < VW / 4; ++i)

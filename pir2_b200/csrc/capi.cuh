@@ -52,6 +52,7 @@ struct DeviceInfo {
   int max_smem = 0;
   bool attrs_set = false;
   bool cache_attrs_set = false;  // attributes of the paged-cache kernels
+  bool w4_attrs_set = false;     // attributes of the 4-bit weights' kernels
   void *ffn_scratch = nullptr;   // device address of g_ffn_scratch (set on first use)
 };
 

@@ -343,6 +343,19 @@ __device__ __forceinline__ void cp_async_wait_group() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// 2 or 4 words of an 8- or 16-byte aligned place at once.
+template <int kWords>
+__device__ __forceinline__ void load_words(uint32_t *w, const void *at) {
+  static_assert(kWords == 2 || kWords == 4);
+  if constexpr (kWords == 2) {
+    const uint2 v = *static_cast<const uint2 *>(at);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    const uint4 v = *static_cast<const uint4 *>(at);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  }
+}
+
 // Barrier among `count` threads (a multiple of 32) on hardware barrier `id`.
 __device__ __forceinline__ void named_barrier(uint32_t id, uint32_t count) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");

@@ -632,9 +632,12 @@ def gemm_w4a16(x, packed, scales, bias=None, *, out=None):
         raise ValueError("gemm_w4a16: out must be bf16 [rows, n] with unit column stride")
     if any(t is not None and t.get_device() != index for t in (packed, scales, bias, out)):
         raise ValueError("gemm_w4a16: all tensors must be on one device")
-    status = _lib.lib().pir2b_gemm_w4a16(
-        x.data_ptr(), x.stride(0) if m > 1 else k, packed.data_ptr(), scales.data_ptr(), k // scales.shape[1], _ptr(bias), m, n, k,
-        out.data_ptr(), out.stride(0) if m > 1 else n, _raw_stream(index),
+    lib, group = _lib.lib(), k // scales.shape[1]
+    size = lib.pir2b_gemm_w4a16_workspace(m, n, k, group) if m > 8 else 0
+    workspace = torch.empty(size, device=x.device, dtype=torch.uint8) if size > 0 else None
+    status = lib.pir2b_gemm_w4a16(
+        x.data_ptr(), x.stride(0) if m > 1 else k, packed.data_ptr(), scales.data_ptr(), group, _ptr(bias), m, n, k,
+        out.data_ptr(), out.stride(0) if m > 1 else n, None if workspace is None else workspace.data_ptr(), _raw_stream(index),
     )
     if status:
         _lib.check(status, "pir2b_gemm_w4a16")

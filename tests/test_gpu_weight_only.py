@@ -41,10 +41,18 @@ def check(out, x, packed, scales, bias=None):
     assert _lib.device_status() == 0
 
 
+@pytest.fixture(params=[0, 1, 2], ids=["chosen", "direct", "rows kept"])
+def plan(request):
+    """Both ways of running the same product."""
+    previous = _lib.set_w4_mode(request.param)
+    yield request.param
+    _lib.set_w4_mode(previous)
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("m", [1, 2, 7, 8, 9, 16, 17, 31, 33, 64, 65, 130])
 @pytest.mark.parametrize("n,pieces", [(16, 1), (1, 3), (777, 9), (4096, 16), (33, 40)])
-def test_products(group, m, n, pieces):
+def test_products(group, m, n, pieces, plan):
     k = group * pieces
     packed, scales = weights(n, k, group, seed=n + m)
     x = rows(m, k, seed=k)
@@ -55,9 +63,11 @@ def test_products(group, m, n, pieces):
     assert torch.equal(out, ops.gemm_w4a16(x, packed, scales, bias))
 
 
-@pytest.mark.parametrize("group", [32, 128])
-@pytest.mark.parametrize("m,n,k", [(1, 2048, 6144), (4, 20011, 2048), (32, 12288, 2048), (3, 40, 65536), (50, 1001, 8192)])
-def test_large_products(group, m, n, k):
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize(
+    "m,n,k", [(1, 2048, 6144), (8, 2050, 8192), (4, 20011, 2048), (32, 12288, 2048), (3, 40, 65536), (50, 1001, 8192), (12, 8001, 2304)]
+)
+def test_large_products(group, m, n, k, plan):
     packed, scales = weights(n, k, group, seed=2)
     x = rows(m, k, seed=3)
     check(ops.gemm_w4a16(x, packed, scales), x, packed, scales)
@@ -80,22 +90,29 @@ def test_every_code_and_strides(m):
     assert (store[:, 0] == 9).all() and (store[:, n + 1 :] == 9).all()
 
 
-def test_rows_that_are_not_finite_stay_alone():
+@pytest.mark.parametrize("m", [6, 12])
+def test_rows_that_are_not_finite_stay_alone(m, plan):
     packed, scales = weights(100, 256, 32, seed=6)
-    x = rows(12, 256, seed=7)
-    clean = ops.gemm_w4a16(x, packed, scales)
-    x[3, 200], x[9, 0] = float("nan"), float("inf")
+    x = rows(m, 256, seed=7)
+    x[3, 200], x[5, 8] = float("nan"), -float("inf")
+    x[4, 77] = 2.0**120                                      # finite, and so are its products
+    x[1] *= 2.0**-110
     out = ops.gemm_w4a16(x, packed, scales)
-    assert torch.isnan(out[3]).all() and not torch.isfinite(out[9]).any()
-    keep = [i for i in range(12) if i not in (3, 9)]
-    assert torch.equal(out[keep], clean[keep])
+    assert torch.isnan(out[3]).all()
+    # An infinity gives infinities, and NaN where the weight is 0.
+    w = dense(packed, scales)[:, 8]
+    assert torch.equal(torch.isnan(out[5]), w == 0)
+    assert torch.equal(out[5][w != 0], torch.where(w[w != 0] > 0, -float("inf"), float("inf")).to(torch.bfloat16))
+    keep = [i for i in range(m) if i not in (3, 5)]
+    check(out[keep], x[keep], packed, scales)
 
 
-def test_another_stream_and_a_replayed_graph_with_new_weights():
+@pytest.mark.parametrize("m", [5, 20])
+def test_another_stream_and_a_replayed_graph_with_new_weights(m, plan):
     packed, scales = weights(300, 512, 128, seed=8)
     other, other_scales = weights(300, 512, 128, seed=9)
-    x = rows(5, 512, seed=10)
-    out = torch.empty(5, 300, device="cuda", dtype=torch.bfloat16)
+    x = rows(m, 512, seed=10)
+    out = torch.empty(m, 300, device="cuda", dtype=torch.bfloat16)
     ops.gemm_w4a16(x, packed, scales, out=out)
     want = ops.gemm_w4a16(x, other, other_scales)
     graph = torch.cuda.CUDAGraph()
@@ -111,9 +128,10 @@ def test_another_stream_and_a_replayed_graph_with_new_weights():
     assert torch.equal(out, want)
 
 
-def test_weights_written_right_before_the_call():
+@pytest.mark.parametrize("m", [2, 30])
+def test_weights_written_right_before_the_call(m, plan):
     """Nothing of the weights is read before the launches ahead of the call end."""
-    x = rows(2, 2048, seed=11)
+    x = rows(m, 2048, seed=11)
     sets = [weights(4096, 2048, 128, seed=s) for s in (20, 21)]
     wants = [ops.gemm_w4a16(x, *s) for s in sets]
     packed, scales = (t.clone() for t in sets[0])
@@ -165,6 +183,8 @@ def test_refusals():
     ):
         with pytest.raises(ValueError, match=message):
             ops.gemm_w4a16(*args)
+    with pytest.raises(ValueError, match="mode"):
+        _lib.set_w4_mode(3)
     with pytest.raises(ValueError, match="out"):
         ops.gemm_w4a16(x, packed, scales, out=torch.empty(2, 31, device="cuda", dtype=torch.bfloat16))
     assert ops.gemm_w4a16(x[:0], packed, scales).shape == (0, 32)

@@ -10,10 +10,10 @@ from int4_reference import unpack
 
 def test_arguments_that_are_refused():
     lib = _lib.lib()
-    good = [4096, 256, 4096, 4096, 64, None, 2, 32, 256, 4096, 32, None]
+    good = [4096, 256, 4096, 4096, 64, None, 2, 32, 256, 4096, 32, None, None]
     for at, value, status in (
         (0, None, _lib.EINVAL), (0, 4104, _lib.EALIGN), (1, 248, _lib.EINVAL), (1, 260, _lib.EALIGN), (2, None, _lib.EINVAL),
-        (2, 4100, _lib.EALIGN), (3, None, _lib.EINVAL), (3, 4097, _lib.EALIGN), (4, 48, _lib.EINVAL), (4, 0, _lib.EINVAL),
+        (2, 4100, _lib.EALIGN), (3, None, _lib.EINVAL), (3, 4100, _lib.EALIGN), (4, 48, _lib.EINVAL), (4, 0, _lib.EINVAL),
         (5, 4097, _lib.EALIGN), (6, -1, _lib.EINVAL), (7, 0, _lib.EINVAL), (8, 0, _lib.EINVAL), (8, 200, _lib.EINVAL),
         (8, 1 << 21, _lib.EINVAL), (9, None, _lib.EINVAL), (9, 4097, _lib.EALIGN), (10, 31, _lib.EINVAL),
     ):
