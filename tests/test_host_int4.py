@@ -78,6 +78,74 @@ def test_seventh_parts_round_to_the_nearest_factor():
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("places", [-3, -2, -1, 1, 2, 3])
+def test_codes_from_a_reciprocal_that_is_off(places):
+    """The same codes where 1 / f is off by some places of its last bit, as an
+    approximate reciprocal may be: the sum q + 1.5 2^23 rounds as the kernel's does."""
+    f32 = np.float32
+    for top in range(8, 16):
+        f = f32(top / 8)
+        y = (f32(1) / f).view(np.int32) + np.int32(places)
+        y = y.view(f32)
+        for exponent in range(-4, 4):
+            v = (np.arange(128, 256) / 128 * 2.0**exponent).astype(f32)
+            q = v * y
+            rest = (v.astype(np.float64) - q.astype(np.float64) * float(f)).astype(f32)
+            q = (q.astype(np.float64) + rest.astype(np.float64) * float(y)).astype(f32)
+            a, b = (v.astype(np.float64) * 2**11).astype(np.int64), int(f * 8) * 2**8
+            low, rest = a // b, a % b
+            true = low + ((2 * rest > b) | ((2 * rest == b) & (low % 2 == 1)))
+            assert np.array_equal(((q + f32(12582912)) - f32(12582912)).astype(np.int64), true)
+
+
+def test_seventh_parts_by_a_product_and_one_step():
+    """q = m fl(1/7), q + (m - 7 q) fl(1/7) is the correctly rounded m / 7 for every bf16 m."""
+    f32 = np.float32
+    m, y = np.arange(128, 256).astype(f32), f32(1) / f32(7)
+    q = m * y
+    rest = (m.astype(np.float64) - 7 * q.astype(np.float64)).astype(f32)
+    q = (q.astype(np.float64) + rest.astype(np.float64) * float(y)).astype(f32)
+    assert np.array_equal(q, m / f32(7))
+
+
+@pytest.mark.parametrize(
+    "changes,text",
+    [
+        ({"hq": 0}, b"query heads"),
+        ({"hq": 1025}, b"query heads"),
+        ({"eps": -1e-6}, b"eps"),
+        ({"eps": float("inf")}, b"eps"),
+        ({"eps": float("nan")}, b"eps"),
+        ({"cos": None}, b"cos"),
+        ({"sin": None}, b"cos"),
+        ({"turns": 0}, b"cos"),
+        ({"sin": 4100}, b"aligned"),
+        ({"q_weight": 4098}, b"aligned"),
+        ({"k_weight": 4104}, b"aligned"),
+        ({"qkv": None}, b"qkv"),
+        ({"qkv": 4104}, b"qkv"),
+        ({"row": 32 * 128 + 4}, b"qkv"),
+        ({"head": 12}, b"qkv"),
+        ({"q_out": None}, b"q"),
+        ({"q_row": 16 * 128 - 8}, b"q"),
+        ({"k_out": 4104}, b"k"),
+        ({"k_row": 8 * 128 - 8, "k_out": 4096}, b"k"),
+        ({"rows": -1}, b"rows"),
+    ],
+)
+def test_appends_that_are_refused(changes, text):
+    args = dict(qkv=4096, row=32 * 128, head=128, rows=2, hq=16, q_weight=4096, k_weight=4096, eps=1e-6, cos=4096, sin=4096,
+                turns=512, positions=None, q_out=4096, q_row=16 * 128, k_out=None, k_row=0)
+    args.update(changes)
+    lib, p = _lib.lib(), pages()
+    s = _lib.SequencesStruct(starts=4096, lengths=4096, table=4096, table_stride=4, batch=2, table_width=4)
+    order = ("qkv", "row", "head", "rows", "hq", "q_weight", "k_weight", "eps", "cos", "sin", "turns", "positions")
+    status = lib.pir2b_cache_append(*[args[x] for x in order], ctypes.byref(p), ctypes.byref(s), args["q_out"], args["q_row"],
+                                    args["k_out"], args["k_row"], None)
+    assert status in (_lib.EINVAL, _lib.EALIGN)
+    assert text in lib.pir2b_last_error()
+
+
 def test_plain_form_of_the_format():
     x = torch.randn(5, 3, 128, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
     packed, scale, factor = quantise4(x)
