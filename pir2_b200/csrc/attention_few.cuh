@@ -673,69 +673,217 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
       const uint8_t *k_tile = ring + stage * 4 * kTile, *v_tile = k_tile + 2 * kTile;
       const uint8_t *side = beside + stage * 2 * Shape::kBeside;
       auto work = [&](auto some_hidden) {
-      constexpr bool kMasked = some_hidden.value;
-      float sc[2][kNT][4] = {};
-      uint4 qs[kNT][KS / 2];
+        constexpr bool kMasked = some_hidden.value;
+        float sc[2][kNT][4] = {};
+        uint4 qs[kNT][KS / 2];
 #pragma unroll
-      for (int t = 0; t < kNT; ++t)
+        for (int t = 0; t < kNT; ++t)
 #pragma unroll
-        for (int s = 0; s < KS / 2; ++s)
-          qs[t][s] = query[(t * (KS / 2) + s) * 32];
+          for (int s = 0; s < KS / 2; ++s)
+            qs[t][s] = query[(t * (KS / 2) + s) * 32];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t kr[2][KW];                         // K rows mine, mine + 8
+        for (int h = 0; h < 2; ++h) {
+          uint32_t kr[2][KW];                         // K rows mine, mine + 8
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const uint8_t *at = k_tile + h * kTile + k_off + x * kEight;
-          if constexpr (KW == 4)
-            load_words<4>(kr[x], at);
-          else
-            load_words<2>(kr[x], at);
+          for (int x = 0; x < 2; ++x) {
+            const uint8_t *at = k_tile + h * kTile + k_off + x * kEight;
+            if constexpr (KW == 4)
+              load_words<4>(kr[x], at);
+            else
+              load_words<2>(kr[x], at);
+          }
+          const uint8_t *f = side + h * Shape::kBeside + q4 * (D / 4) / kFactorGroup;
+          uint32_t two;
+          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(two) : "h"(uint16_t(f[mine * kGroups] | (f[(mine + 8) * kGroups] << 8))));
+          const Int4Factors lo = int4_factors(__byte_perm(two, two, 0x1010)), hi = int4_factors(__byte_perm(two, two, 0x3232));
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            uint32_t af[4];
+            if (s & 1) {
+              int4_to_half<1>(kr[0][s / 2], lo, masks, af[0], af[2]);
+              int4_to_half<1>(kr[1][s / 2], hi, masks, af[1], af[3]);
+            } else {
+              int4_to_half<0>(kr[0][s / 2], lo, masks, af[0], af[2]);
+              int4_to_half<0>(kr[1][s / 2], hi, masks, af[1], af[3]);
+            }
+#pragma unroll
+            for (int t = 0; t < kNT; ++t)
+              mma_half_16816(sc[h][t], af, s & 1 ? qs[t][s / 2].z : qs[t][s / 2].x, s & 1 ? qs[t][s / 2].w : qs[t][s / 2].y);
+          }
+          const float *k_scale = reinterpret_cast<const float *>(side + h * Shape::kBeside + 128) + mine;
+          const float k_lo = k_scale[0], k_hi = k_scale[8];
+#pragma unroll
+          for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              // The factors first: a large key's scale alone could overflow the product.
+              float v = sc[h][t][e] * ((e < 2 ? k_lo : k_hi) * to_log2[t][e & 1]);
+              if (kMasked && key0 + h * 16 + mine + (e & 2) * 4 > limit[t][e & 1])
+                v = -INFINITY;
+              sc[h][t][e] = v;
+            }
+          }
         }
-        const uint8_t *f = side + h * Shape::kBeside + q4 * (D / 4) / kFactorGroup;
-        uint32_t two;
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(two) : "h"(uint16_t(f[mine * kGroups] | (f[(mine + 8) * kGroups] << 8))));
-        const Int4Factors lo = int4_factors(__byte_perm(two, two, 0x1010)), hi = int4_factors(__byte_perm(two, two, 0x3232));
+        bool raise = false;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          uint32_t af[4];
-          if (s & 1) {
-            int4_to_half<1>(kr[0][s / 2], lo, masks, af[0], af[2]);
-            int4_to_half<1>(kr[1][s / 2], hi, masks, af[1], af[3]);
-          } else {
-            int4_to_half<0>(kr[0][s / 2], lo, masks, af[0], af[2]);
-            int4_to_half<0>(kr[1][s / 2], hi, masks, af[1], af[3]);
+        for (int t = 0; t < kNT; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            raise |= fmaxf(fmaxf(sc[0][t][e], sc[0][t][e + 2]), fmaxf(sc[1][t][e], sc[1][t][e + 2])) > top[t][e] + 8.f;
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+          for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float m = fmaxf(fmaxf(top[t][e], fmaxf(sc[0][t][e], sc[0][t][e + 2])), fmaxf(sc[1][t][e], sc[1][t][e + 2]));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+              const float keep = top[t][e] == -INFINITY ? 1.f : exp2_fast(top[t][e] - m);   // nothing summed yet: keep it
+              top[t][e] = m;
+              mu[t][e] = m == -INFINITY ? 0.f : m;
+              l[t][e] *= keep;
+#pragma unroll
+              for (int s = 0; s < KS; ++s) {
+                o[t][s][e] *= keep;
+                o[t][s][e + 2] *= keep;
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t vr[4][VW];                         // V rows 2 q4, odd, and 8 after them
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint8_t *at = v_tile + h * kTile + (x & 1 ? v_odd : v_even) + (x >> 1) * kEight;
+            if constexpr (VW == 2)
+              load_words<2>(vr[x], at);
+            else
+              vr[x][0] = *reinterpret_cast<const uint32_t *>(at);
+          }
+          const uint8_t *f = side + h * Shape::kBeside + 64 + g * (D / 8) / kFactorGroup;
+          uint32_t vf[2], minus_24vf[2];              // of keys 2 q4 and odd, and 8 after them
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            vf[x] = factor_pair_bf16(f[(2 * q4 + 8 * x) * kGroups], f[(odd + 8 * x) * kGroups], minus_24vf[x]);
+          const float *v_scale = reinterpret_cast<const float *>(side + h * Shape::kBeside + 192) + mine;
+          const float vsc[2] = {v_scale[0], v_scale[8]};
+          uint32_t pf[kNT][2];
+#pragma unroll
+          for (int t = 0; t < kNT; ++t) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = exp2_fast(sc[h][t][e] - mu[t][e & 1]);
+              l[t][e & 1] += x;
+              // A hidden key's scale may be anything.
+              w[e] = kMasked && sc[h][t][e] == -INFINITY ? 0.f : x * vsc[e >> 1];
+            }
+            pf[t][0] = transpose_8x8(pack_bf16x2(w[0], w[1]));
+            pf[t][1] = transpose_8x8(pack_bf16x2(w[2], w[3]));
           }
 #pragma unroll
-          for (int t = 0; t < kNT; ++t)
-            mma_half_16816(sc[h][t], af, s & 1 ? qs[t][s / 2].z : qs[t][s / 2].x, s & 1 ? qs[t][s / 2].w : qs[t][s / 2].y);
+          for (int j = 0; j < VW; ++j) {
+            // Channels 0-3 of the two keys in one word, 4-7 in the next.
+            uint32_t af[4][4];
+#pragma unroll
+            for (int x = 0; x < 2; ++x)      // keys 2 q4 .. and 2 q4 + 8 ..
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const uint32_t y = __byte_perm(vr[2 * x][j], vr[2 * x + 1][j], c ? 0x7632 : 0x5410);
+                af[2 * c][2 * x] = int4_to_bf16<0>(y, vf[x], minus_24vf[x], masks);
+                af[2 * c][2 * x + 1] = int4_to_bf16<1>(y, vf[x], minus_24vf[x], masks);
+                af[2 * c + 1][2 * x] = int4_to_bf16<2>(y, vf[x], minus_24vf[x], masks);
+                af[2 * c + 1][2 * x + 1] = int4_to_bf16<3>(y, vf[x], minus_24vf[x], masks);
+              }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int t = 0; t < kNT; ++t)
+                mma_bf16_16816(o[t][4 * j + i], af[i], pf[t][0], pf[t][1]);
+          }
         }
-        const float *k_scale = reinterpret_cast<const float *>(side + h * Shape::kBeside + 128) + mine;
-        const float k_lo = k_scale[0], k_hi = k_scale[8];
+      };
+      // Few steps have positions that some row does not see.
+      if (key0 + 32 > all_see)
+        work(std::true_type{});
+      else
+        work(std::false_type{});
+    }
+  }
+  if constexpr (!kInt4) {
+    for (; done < count; ++done) {
+      const int step = step0 + done * kFewWarps, stage = done % kStages;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], uint32_t((done / kStages) & 1), kStatusTimeoutProducer)))
+        break;
+      const uint8_t *k_tile = ring + stage * 2 * kTile, *v_tile = k_tile + kTile;
+      uint32_t kr[2][KW], vr[4][VW];                  // K rows mine, mine + 8; V rows 2 q4, odd, and 8 after them
+#pragma unroll
+      for (int i = 0; i < KW / 4; ++i) {
+        const uint8_t *at = k_tile + (i >> 1) * 2048 + (i & 1 ? k_off ^ 64 : k_off);
+        *reinterpret_cast<uint4 *>(&kr[0][i * 4]) = *reinterpret_cast<const uint4 *>(at);
+        *reinterpret_cast<uint4 *>(&kr[1][i * 4]) = *reinterpret_cast<const uint4 *>(at + kEight);
+      }
+      float ksc[2] = {1.f, 1.f}, vsc[2] = {1.f, 1.f};
+      if constexpr (!kBf16) {
+        const float *s = scales + stage * 32 + mine;
+        ksc[0] = s[0], ksc[1] = s[8], vsc[0] = s[16], vsc[1] = s[24];
+      }
+      float sc[kNT][4] = {};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        uint32_t af[4];
+        if constexpr (kBf16) {
+          af[0] = kr[0][2 * s], af[1] = kr[1][2 * s], af[2] = kr[0][2 * s + 1], af[3] = kr[1][2 * s + 1];
+        } else {
+          codes_to_half<kFormat>(kr[0][s], af[0], af[2]);
+          codes_to_half<kFormat>(kr[1][s], af[1], af[3]);
+        }
 #pragma unroll
         for (int t = 0; t < kNT; ++t) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            // The factors first: a large key's scale alone could overflow the product.
-            float v = sc[h][t][e] * ((e < 2 ? k_lo : k_hi) * to_log2[t][e & 1]);
-            if (kMasked && key0 + h * 16 + mine + (e & 2) * 4 > limit[t][e & 1])
-              v = -INFINITY;
-            sc[h][t][e] = v;
-          }
+          if constexpr (kBf16)
+            mma_bf16_16816(sc[t], af, qf[t][s][0], qf[t][s][1]);
+          else
+            mma_half_16816(sc[t], af, qf[t][s][0], qf[t][s][1]);
         }
       }
+      const float k_lo = ksc[0], k_hi = ksc[1];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint8_t *at = v_tile + (x & 1 ? v_odd : v_even) + (x >> 1) * kEight;
+        if constexpr (VW == 2) {
+          load_words<2>(vr[x], at);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VW / 4; ++i)
+            *reinterpret_cast<uint4 *>(&vr[x][i * 4]) = *reinterpret_cast<const uint4 *>(at + i * 2048);
+        }
+      }
+      __syncwarp();
+      if (done + kStages < count)
+        copy(done + kStages);
+      const int key0 = step << 4;
+      const bool masked = key0 + 16 > all_see;
       bool raise = false;
 #pragma unroll
-      for (int t = 0; t < kNT; ++t)
+      for (int t = 0; t < kNT; ++t) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          raise |= fmaxf(fmaxf(sc[0][t][e], sc[0][t][e + 2]), fmaxf(sc[1][t][e], sc[1][t][e + 2])) > top[t][e] + 8.f;
+        for (int e = 0; e < 4; ++e) {
+          // The factors first: a large key's scale alone could overflow the product.
+          float v = sc[t][e] * (kBf16 ? a.scale_log2 : (e < 2 ? k_lo : k_hi) * to_log2[t][e & 1]);
+          if (masked && key0 + mine + (e & 2) * 4 > limit[t][e & 1])
+            v = -INFINITY;
+          sc[t][e] = v;
+          raise |= v > top[t][e & 1] + 8.f;
+        }
+      }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
         for (int t = 0; t < kNT; ++t) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float m = fmaxf(fmaxf(top[t][e], fmaxf(sc[0][t][e], sc[0][t][e + 2])), fmaxf(sc[1][t][e], sc[1][t][e + 2]));
+            float m = fmaxf(top[t][e], fmaxf(sc[t][e], sc[t][e + 2]));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
@@ -751,261 +899,114 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
           }
         }
       }
+      uint32_t pf[kNT][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t vr[4][VW];                         // V rows 2 q4, odd, and 8 after them
+      for (int t = 0; t < kNT; ++t) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const uint8_t *at = v_tile + h * kTile + (x & 1 ? v_odd : v_even) + (x >> 1) * kEight;
-          if constexpr (VW == 2)
-            load_words<2>(vr[x], at);
-          else
-            vr[x][0] = *reinterpret_cast<const uint32_t *>(at);
+        for (int e = 0; e < 4; ++e) {
+          const float w = exp2_fast(sc[t][e] - mu[t][e & 1]);
+          l[t][e & 1] += w;
+          // A hidden key's scale may be anything.
+          sc[t][e] = kBf16 ? w : masked && sc[t][e] == -INFINITY ? 0.f : w * vsc[e >> 1];
         }
-        const uint8_t *f = side + h * Shape::kBeside + 64 + g * (D / 8) / kFactorGroup;
-        uint32_t vf[2], minus_24vf[2];              // of keys 2 q4 and odd, and 8 after them
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          vf[x] = factor_pair_bf16(f[(2 * q4 + 8 * x) * kGroups], f[(odd + 8 * x) * kGroups], minus_24vf[x]);
-        const float *v_scale = reinterpret_cast<const float *>(side + h * Shape::kBeside + 192) + mine;
-        const float vsc[2] = {v_scale[0], v_scale[8]};
-        uint32_t pf[kNT][2];
-#pragma unroll
-        for (int t = 0; t < kNT; ++t) {
-          float w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = exp2_fast(sc[h][t][e] - mu[t][e & 1]);
-            l[t][e & 1] += x;
-            // A hidden key's scale may be anything.
-            w[e] = kMasked && sc[h][t][e] == -INFINITY ? 0.f : x * vsc[e >> 1];
-          }
-          pf[t][0] = transpose_8x8(pack_bf16x2(w[0], w[1]));
-          pf[t][1] = transpose_8x8(pack_bf16x2(w[2], w[3]));
-        }
+        pf[t][0] = transpose_8x8(pack_bf16x2(sc[t][0], sc[t][1]));
+        pf[t][1] = transpose_8x8(pack_bf16x2(sc[t][2], sc[t][3]));
+      }
+      // Pairs (key, key + 1) of a column for the two halves of an M tile pair.
+      auto product = [&](const uint32_t (&pp)[kNT][2]) {
 #pragma unroll
         for (int j = 0; j < VW; ++j) {
-          // Channels 0-3 of the two keys in one word, 4-7 in the next.
-          uint32_t af[4][4];
-#pragma unroll
-          for (int x = 0; x < 2; ++x)      // keys 2 q4 .. and 2 q4 + 8 ..
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const uint32_t y = __byte_perm(vr[2 * x][j], vr[2 * x + 1][j], c ? 0x7632 : 0x5410);
-              af[2 * c][2 * x] = int4_to_bf16<0>(y, vf[x], minus_24vf[x], masks);
-              af[2 * c][2 * x + 1] = int4_to_bf16<1>(y, vf[x], minus_24vf[x], masks);
-              af[2 * c + 1][2 * x] = int4_to_bf16<2>(y, vf[x], minus_24vf[x], masks);
-              af[2 * c + 1][2 * x + 1] = int4_to_bf16<3>(y, vf[x], minus_24vf[x], masks);
-            }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
+          if constexpr (kBf16) {
+            const uint32_t af[4] = {__byte_perm(vr[0][j], vr[1][j], 0x5410), __byte_perm(vr[0][j], vr[1][j], 0x7632),
+                                    __byte_perm(vr[2][j], vr[3][j], 0x5410), __byte_perm(vr[2][j], vr[3][j], 0x7632)};
 #pragma unroll
             for (int t = 0; t < kNT; ++t)
-              mma_bf16_16816(o[t][4 * j + i], af[i], pf[t][0], pf[t][1]);
-        }
-      }
-      };
-      // Few steps have positions that some row does not see.
-      if (key0 + 32 > all_see)
-        work(std::true_type{});
-      else
-        work(std::false_type{});
-    }
-  }
-  if constexpr (!kInt4)
-  for (; done < count; ++done) {
-    const int step = step0 + done * kFewWarps, stage = done % kStages;
-    if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], uint32_t((done / kStages) & 1), kStatusTimeoutProducer)))
-      break;
-    const uint8_t *k_tile = ring + stage * 2 * kTile, *v_tile = k_tile + kTile;
-    uint32_t kr[2][KW], vr[4][VW];                  // K rows mine, mine + 8; V rows 2 q4, odd, and 8 after them
+              mma_bf16_16816(o[t][j], af, pp[t][0], pp[t][1]);
+          } else {
+            uint32_t af[2][4];
 #pragma unroll
-    for (int i = 0; i < KW / 4; ++i) {
-      const uint8_t *at = k_tile + (i >> 1) * 2048 + (i & 1 ? k_off ^ 64 : k_off);
-      *reinterpret_cast<uint4 *>(&kr[0][i * 4]) = *reinterpret_cast<const uint4 *>(at);
-      *reinterpret_cast<uint4 *>(&kr[1][i * 4]) = *reinterpret_cast<const uint4 *>(at + kEight);
-    }
-    float ksc[2] = {1.f, 1.f}, vsc[2] = {1.f, 1.f};
-    if constexpr (!kBf16) {
-      const float *s = scales + stage * 32 + mine;
-      ksc[0] = s[0], ksc[1] = s[8], vsc[0] = s[16], vsc[1] = s[24];
-    }
-    float sc[kNT][4] = {};
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      uint32_t af[4];
-      if constexpr (kBf16) {
-        af[0] = kr[0][2 * s], af[1] = kr[1][2 * s], af[2] = kr[0][2 * s + 1], af[3] = kr[1][2 * s + 1];
-      } else {
-        codes_to_half<kFormat>(kr[0][s], af[0], af[2]);
-        codes_to_half<kFormat>(kr[1][s], af[1], af[3]);
-      }
-#pragma unroll
-      for (int t = 0; t < kNT; ++t) {
-        if constexpr (kBf16)
-          mma_bf16_16816(sc[t], af, qf[t][s][0], qf[t][s][1]);
-        else
-          mma_half_16816(sc[t], af, qf[t][s][0], qf[t][s][1]);
-      }
-    }
-    const float k_lo = ksc[0], k_hi = ksc[1];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const uint8_t *at = v_tile + (x & 1 ? v_odd : v_even) + (x >> 1) * kEight;
-      if constexpr (VW == 2) {
-        load_words<2>(vr[x], at);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VW / 4; ++i)
-          *reinterpret_cast<uint4 *>(&vr[x][i * 4]) = *reinterpret_cast<const uint4 *>(at + i * 2048);
-      }
-    }
-    __syncwarp();
-    if (done + kStages < count)
-      copy(done + kStages);
-    const int key0 = step << 4;
-    const bool masked = key0 + 16 > all_see;
-    bool raise = false;
-#pragma unroll
-    for (int t = 0; t < kNT; ++t) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // The factors first: a large key's scale alone could overflow the product.
-        float v = sc[t][e] * (kBf16 ? a.scale_log2 : (e < 2 ? k_lo : k_hi) * to_log2[t][e & 1]);
-        if (masked && key0 + mine + (e & 2) * 4 > limit[t][e & 1])
-          v = -INFINITY;
-        sc[t][e] = v;
-        raise |= v > top[t][e & 1] + 8.f;
-      }
-    }
-    if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-      for (int t = 0; t < kNT; ++t) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float m = fmaxf(top[t][e], fmaxf(sc[t][e], sc[t][e + 2]));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-          const float keep = top[t][e] == -INFINITY ? 1.f : exp2_fast(top[t][e] - m);   // nothing summed yet: keep it
-          top[t][e] = m;
-          mu[t][e] = m == -INFINITY ? 0.f : m;
-          l[t][e] *= keep;
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            o[t][s][e] *= keep;
-            o[t][s][e + 2] *= keep;
-          }
-        }
-      }
-    }
-    uint32_t pf[kNT][2];
-#pragma unroll
-    for (int t = 0; t < kNT; ++t) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float w = exp2_fast(sc[t][e] - mu[t][e & 1]);
-        l[t][e & 1] += w;
-        // A hidden key's scale may be anything.
-        sc[t][e] = kBf16 ? w : masked && sc[t][e] == -INFINITY ? 0.f : w * vsc[e >> 1];
-      }
-      pf[t][0] = transpose_8x8(pack_bf16x2(sc[t][0], sc[t][1]));
-      pf[t][1] = transpose_8x8(pack_bf16x2(sc[t][2], sc[t][3]));
-    }
-    // Pairs (key, key + 1) of a column for the two halves of an M tile pair.
-    auto product = [&](const uint32_t (&pp)[kNT][2]) {
-#pragma unroll
-      for (int j = 0; j < VW; ++j) {
-        if constexpr (kBf16) {
-          const uint32_t af[4] = {__byte_perm(vr[0][j], vr[1][j], 0x5410), __byte_perm(vr[0][j], vr[1][j], 0x7632),
-                                  __byte_perm(vr[2][j], vr[3][j], 0x5410), __byte_perm(vr[2][j], vr[3][j], 0x7632)};
-#pragma unroll
-          for (int t = 0; t < kNT; ++t)
-            mma_bf16_16816(o[t][j], af, pp[t][0], pp[t][1]);
-        } else {
-          uint32_t af[2][4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {   // keys 2 q4 .. and 2 q4 + 8 ..
-            const uint32_t x = __byte_perm(vr[2 * h][j], vr[2 * h + 1][j], 0x5140);
-            const uint32_t y = __byte_perm(vr[2 * h][j], vr[2 * h + 1][j], 0x7362);
-            codes_to_bf16<kFormat>(x, af[0][2 * h], af[0][2 * h + 1]);
-            codes_to_bf16<kFormat>(y, af[1][2 * h], af[1][2 * h + 1]);
-          }
-#pragma unroll
-          for (int t = 0; t < kNT; ++t) {
-            mma_bf16_16816(o[t][2 * j], af[0], pp[t][0], pp[t][1]);
-            mma_bf16_16816(o[t][2 * j + 1], af[1], pp[t][0], pp[t][1]);
-          }
-        }
-      }
-    };
-    if constexpr (kBf16) {
-      if (masked) {
-        // Hidden values must not enter a product, not even times 0: positions
-        // no row sees become 0 here, and where a position hidden from some
-        // rows holds a value that is not finite the rows go one at a time.
-        bool spoiled = false;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int key = key0 + (x & 1 ? odd : 2 * q4) + (x & 2) * 4;
-#pragma unroll
-          for (int j = 0; j < VW; ++j) {
-            if (key >= keys)
-              vr[x][j] = 0;
-            else if (key >= all_see)
-              spoiled |= pair_not_finite(vr[x][j]);
-          }
-        }
-        if (__any_sync(0xffffffffu, spoiled)) {
-          uint32_t kept[4][VW];
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-#pragma unroll
-            for (int j = 0; j < VW; ++j)
-              kept[x][j] = vr[x][j];
-#pragma unroll 1
-          for (int r = 0; r < kRows; ++r) {
-            const int last = r0 + r < r1 ? first_new + (r0 + r) / group : -1;
-            uint32_t one[kNT][2];
+            for (int h = 0; h < 2; ++h) {   // keys 2 q4 .. and 2 q4 + 8 ..
+              const uint32_t x = __byte_perm(vr[2 * h][j], vr[2 * h + 1][j], 0x5140);
+              const uint32_t y = __byte_perm(vr[2 * h][j], vr[2 * h + 1][j], 0x7362);
+              codes_to_bf16<kFormat>(x, af[0][2 * h], af[0][2 * h + 1]);
+              codes_to_bf16<kFormat>(y, af[1][2 * h], af[1][2 * h + 1]);
+            }
 #pragma unroll
             for (int t = 0; t < kNT; ++t) {
-              one[t][0] = t * 8 + g == r ? pf[t][0] : 0;
-              one[t][1] = t * 8 + g == r ? pf[t][1] : 0;
+              mma_bf16_16816(o[t][2 * j], af[0], pp[t][0], pp[t][1]);
+              mma_bf16_16816(o[t][2 * j + 1], af[1], pp[t][0], pp[t][1]);
             }
-            // The product runs on columns of zeros for the other rows, so a
-            // value that this row sees must not reach them either: it is
-            // added to this row alone, below.
+          }
+        }
+      };
+      if constexpr (kBf16) {
+        if (masked) {
+          // Hidden values must not enter a product, not even times 0: positions
+          // no row sees become 0 here, and where a position hidden from some
+          // rows holds a value that is not finite the rows go one at a time.
+          bool spoiled = false;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int key = key0 + (x & 1 ? odd : 2 * q4) + (x & 2) * 4;
+          for (int x = 0; x < 4; ++x) {
+            const int key = key0 + (x & 1 ? odd : 2 * q4) + (x & 2) * 4;
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+              if (key >= keys)
+                vr[x][j] = 0;
+              else if (key >= all_see)
+                spoiled |= pair_not_finite(vr[x][j]);
+            }
+          }
+          if (__any_sync(0xffffffffu, spoiled)) {
+            uint32_t kept[4][VW];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
 #pragma unroll
               for (int j = 0; j < VW; ++j)
-                vr[x][j] = key > last ? 0 : kept[x][j];
+                kept[x][j] = vr[x][j];
+#pragma unroll 1
+            for (int r = 0; r < kRows; ++r) {
+              const int last = r0 + r < r1 ? first_new + (r0 + r) / group : -1;
+              uint32_t one[kNT][2];
+#pragma unroll
+              for (int t = 0; t < kNT; ++t) {
+                one[t][0] = t * 8 + g == r ? pf[t][0] : 0;
+                one[t][1] = t * 8 + g == r ? pf[t][1] : 0;
+              }
+              // The product runs on columns of zeros for the other rows, so a
+              // value that this row sees must not reach them either: it is
+              // added to this row alone, below.
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const int key = key0 + (x & 1 ? odd : 2 * q4) + (x & 2) * 4;
+#pragma unroll
+                for (int j = 0; j < VW; ++j)
+                  vr[x][j] = key > last ? 0 : kept[x][j];
+              }
+              float saved[kNT][KS][4];
+#pragma unroll
+              for (int t = 0; t < kNT; ++t)
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    saved[t][s][e] = o[t][s][e];
+              product(one);
+              // Columns of O^T are rows: keep the new sums of row r only.
+#pragma unroll
+              for (int t = 0; t < kNT; ++t)
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    if (t * 8 + 2 * q4 + (e & 1) != r)
+                      o[t][s][e] = saved[t][s][e];
             }
-            float saved[kNT][KS][4];
-#pragma unroll
-            for (int t = 0; t < kNT; ++t)
-#pragma unroll
-              for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  saved[t][s][e] = o[t][s][e];
-            product(one);
-            // Columns of O^T are rows: keep the new sums of row r only.
-#pragma unroll
-            for (int t = 0; t < kNT; ++t)
-#pragma unroll
-              for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (t * 8 + 2 * q4 + (e & 1) != r)
-                    o[t][s][e] = saved[t][s][e];
+            continue;
           }
-          continue;
         }
       }
+      product(pf);
     }
-    product(pf);
   }
 
   // No copy is in flight past this point (at once, unless a wait gave up).
