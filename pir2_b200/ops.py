@@ -610,8 +610,9 @@ def gemm_w4a16(x, packed, scales, bias=None, *, out=None):
     x: bf16 [rows, k] with unit column stride and a row stride that is a multiple
     of 8; packed: uint8 [n, k / 2] codes of -8..7 (two's complement, the even k in
     the low bits); scales: bf16 [n, k / group], group 32, 64 or 128; bias: bf16
-    [n].  Sums in fp32, rounded once.  The weights are read once for every 64
-    rows (`weight_only.WeightOnlyLinear` makes them from a Linear).
+    [n].  x, packed and scales must be 16-byte aligned.  Sums in fp32, rounded
+    once.  The weights are read once for every 64 rows
+    (`weight_only.WeightOnlyLinear` makes them from a Linear).
     """
     if x.dtype != torch.bfloat16 or not x.is_cuda or x.ndim != 2 or x.stride(1) != 1:
         raise ValueError("gemm_w4a16: x must be CUDA bf16 [rows, k] with unit column stride")
