@@ -107,6 +107,40 @@ def test_rows_that_are_not_finite_stay_alone(m, plan):
     check(out[keep], x[keep], packed, scales)
 
 
+@pytest.mark.parametrize("m", [5, 12, 40])
+def test_rows_of_any_range(m, plan):
+    """Small values count beside large ones where the codes of those are 0."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    packed, scales = weights(200, 512, 64, seed=12)
+    x = torch.randn(m, 512, generator=g, device="cuda")
+    x = torch.ldexp(x, torch.randint(-50, 51, x.shape, generator=g, device="cuda")).to(torch.bfloat16)
+    x[1] = 0
+    x[1, 7], x[1, 300] = 2.0**90, 2.0**-30
+    codes = unpack(packed)
+    codes[:, 7] = 0
+    packed = pack(codes)
+    check(ops.gemm_w4a16(x, packed, scales), x, packed, scales)
+
+
+@pytest.mark.parametrize("m", [4, 40])
+def test_two_streams_at_once(m):
+    """Each call has rows and a workspace of its own."""
+    sets = [weights(6400, 1024, 64, seed=s) for s in (30, 31)]
+    xs = [rows(m, 1024, seed=s) for s in (32, 33)]
+    wants = [ops.gemm_w4a16(x, *w) for x, w in zip(xs, sets)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream())
+    outs = [[], []]
+    for _ in range(30):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                outs[i].append(ops.gemm_w4a16(xs[i], *sets[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for mine, want in zip(outs, wants) for out in mine)
+    assert _lib.device_status() == 0
+
+
 @pytest.mark.parametrize("m", [5, 20])
 def test_another_stream_and_a_replayed_graph_with_new_weights(m, plan):
     packed, scales = weights(300, 512, 128, seed=8)
