@@ -220,6 +220,15 @@ __device__ __forceinline__ void cp_async_ca(uint32_t dst, const void *src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
 }
 
+// Codes of a block's units `from` to `to` on their way to L2 while the launch before
+// this one ends; nothing is read of them yet.
+__device__ __forceinline__ void w4_prefetch(const W4Args &a, int block, int from, int to) {
+  const int row = block * 16 + (threadIdx.x & 15);
+  if (row < a.n)
+    for (int unit = from + ((threadIdx.x >> 4) & 1); unit < to; unit += 2)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.w + int64_t(row) * (a.k >> 1) + unit * 128));
+}
+
 template <int kGroup>
 __global__ void __launch_bounds__(W4Staged::kWarps * 32, 1) gemm_w4_staged_kernel(const W4Args a) {
   using Shape = W4Staged;
@@ -235,6 +244,7 @@ __global__ void __launch_bounds__(W4Staged::kWarps * 32, 1) gemm_w4_staged_kerne
   // Block blockIdx + gridDim i of 16 channels is the CTA's i-th.
   const int blocks = (a.n + 15) >> 4, stride = gridDim.x * wc;
   const Int4Masks masks = int4_masks();
+  w4_prefetch(a, int(blockIdx.x + gridDim.x * which), begin, min(begin + 2, end));
   pdl_wait();
   pdl_launch_dependents();
 
@@ -449,6 +459,8 @@ __global__ void __launch_bounds__(W4Wide<kTiles>::kWarps * 32, 1) gemm_w4_wide_k
     fence_barrier_init();
   }
   __syncthreads();
+  const int units0 = min(a.slab, a.k) >> 8, block0 = int(blockIdx.x + gridDim.x * which);
+  w4_prefetch(a, block0, part * units0 / wk, (part + 1) * units0 / wk);
   pdl_wait();
   pdl_launch_dependents();
 
