@@ -19,10 +19,10 @@ static std::atomic<int> g_w4_mode{0};
 //    8 rows  4096 x 2048 3.7 (4.9) 4.9 (5.2)   2048 x 6144 5.0 (6.8) 7.8 (6.8)
 //            6144 x 1536 5.2 (6.0) 5.1 (5.3)   12288 x 2048 8.4 (12.0) 7.7 (8.3)
 //            151936 x 2048 68 (119) 36 (41)
-//   16       4096 x 1024 3.6 4.7               4096 x 2048 6.2 (6.0) 5.6 (5.9)
-//   32       2048 x 6144 10.2 (13.1) 13.2 (13.9)   4096 x 1024 4.7 5.8
-//            4096 x 2048 7.5 (11.7) 7.1 (8.3)  6144 x 1024 7.8 6.5
-//            12288 x 2048 19.8 (24.1) 12.9 (14.6)   151936 x 2048 198 (222) 97 (108)
+//   16       4096 x 1024 3.6 4.7               4096 x 2048 6.2 (6.0) 5.5 (5.8)
+//   32       2048 x 6144 10.2 (13.1) 12.8 (13.3)   4096 x 1024 4.7 5.8
+//            4096 x 2048 7.5 (11.7) 7.1 (7.8)  6144 x 1024 7.8 6.5
+//            12288 x 2048 19.8 (24.1) 12.9 (14.1)   151936 x 2048 198 (222) 99 (106)
 static bool w4_keeps_rows(int64_t m, int64_t n, int64_t k) {
   const int mode = g_w4_mode.load();
   if (mode == 1 || k % 256 != 0)
@@ -33,7 +33,8 @@ static bool w4_keeps_rows(int64_t m, int64_t n, int64_t k) {
 }
 
 // Warps that split K: the fewest rounds of chunks of 128, a round's meeting counted
-// as `meeting` more.
+// as `meeting` more (wide, 32 rows of 4096 -> 20000: 33-36 us with 4 to 16, 36-39 with
+// 2, 43-45 with 1).
 static int w4_split(int64_t blocks, int64_t ctas, int warps, int slabs, int units, int meeting) {
   int best = 1;
   int64_t least = INT64_MAX;
@@ -73,7 +74,7 @@ static int launch_w4_wide(W4Args a, void *workspace, const DeviceInfo *dev, void
   while (Shape::bytes(a.slab) > kW4Smem)
     a.slab = (a.slab / 2 + 255) / 256 * 256;
   const int64_t blocks = (a.n + 15) / 16, grid = std::min<int64_t>(dev->sms, blocks);
-  a.wk = w4_split(blocks, grid, Shape::kWarps, (a.k + a.slab - 1) / a.slab, a.slab / 256, 2);
+  a.wk = w4_split(blocks, grid, Shape::kWarps, (a.k + a.slab - 1) / a.slab, a.slab / 256, 4);
   return launch_cache("gemm_w4a16 launch", gemm_w4_wide_kernel<kGroup, kTiles>, grid, 1, 1, Shape::kWarps * 32,
                       size_t(Shape::bytes(a.slab)), stream, a, static_cast<const uint4 *>(rows));
 }

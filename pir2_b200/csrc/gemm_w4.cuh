@@ -13,11 +13,13 @@
 // of one group each, so a product step stays in a group, whose sums are scaled in
 // fp32.  The only other rounding is that of the output.
 //
-// What bounds it: up to 16 rows the start of a launch and the latency of the loads
-// where weights are few (2048 -> 4096, one row: 2.9 us, the weights' bytes alone 0.7),
-// the instructions that bring codes into bf16 where they are many (2048 -> 151936, 4
-// rows: 36 us, bytes 25, 4.5 TB/s); more rows the rate of the MMAs themselves, 8
-// cycles of a quarter SM each (32 rows of 2048 -> 12288: 14.5 us, MMAs 8, bytes 2.3).
+// What bounds it: the start of a launch and the latency of the loads where weights
+// are few (2048 -> 4096, one row: 2.9 us, the weights' bytes alone 0.7); the
+// instructions that bring codes into bf16 where they are many (2048 -> 151936, 4 rows:
+// 35.5 us, bytes 25, 4.6 TB/s); with more rows shared memory as well, from which every
+// 16 channels read all rows (32 rows of 2048 -> 151936: 99 us, of them 50 of shared
+// memory, 34 of MMAs at 8 cycles of a quarter SM each; of 2048 -> 12288 13.9, bytes
+// 2.3).
 #pragma once
 #include "attention_few.cuh"
 
