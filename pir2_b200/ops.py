@@ -621,9 +621,10 @@ def gemm_w4a16(x, packed, scales, bias=None, *, out=None):
     if packed.dtype != torch.uint8 or packed.ndim != 2 or packed.shape[1] * 2 != k or not packed.is_contiguous():
         raise ValueError("gemm_w4a16: packed must be contiguous uint8 [n, k / 2]")
     n = packed.shape[0]
-    if scales.dtype != torch.bfloat16 or scales.ndim != 2 or scales.shape[0] != n or scales.shape[1] < 1 or not scales.is_contiguous():
+    if scales.dtype != torch.bfloat16 or scales.ndim != 2 or scales.shape[0] != n or not scales.is_contiguous():
         raise ValueError("gemm_w4a16: scales must be contiguous bf16 [n, k / group]")
-    if k % scales.shape[1]:
+    groups = scales.shape[1]
+    if groups < 1 or k % groups:
         raise ValueError("gemm_w4a16: k must be a multiple of the group")
     if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (n,) or not bias.is_contiguous()):
         raise ValueError("gemm_w4a16: bias must be contiguous bf16 [n]")
@@ -631,9 +632,10 @@ def gemm_w4a16(x, packed, scales, bias=None, *, out=None):
         out = x.new_empty((m, n))
     elif out.shape != (m, n) or out.dtype != torch.bfloat16 or out.stride(1) != 1:
         raise ValueError("gemm_w4a16: out must be bf16 [rows, n] with unit column stride")
-    if any(t is not None and t.get_device() != index for t in (packed, scales, bias, out)):
+    if (packed.get_device() != index or scales.get_device() != index or out.get_device() != index
+            or (bias is not None and bias.get_device() != index)):
         raise ValueError("gemm_w4a16: all tensors must be on one device")
-    lib, group = _lib.lib(), k // scales.shape[1]
+    lib, group = _lib.lib(), k // groups
     size = lib.pir2b_gemm_w4a16_workspace(m, n, k, group) if m > 8 else 0
     workspace = torch.empty(size, device=x.device, dtype=torch.uint8) if size > 0 else None
     status = lib.pir2b_gemm_w4a16(
@@ -772,8 +774,9 @@ def cache_append(qkv, pages, sequences, cos, sin, *, q_weight=None, k_weight=Non
     index = qkv.get_device()
     if pages.index != index or sequences.index != index:
         raise ValueError("cache_append: rows, pages and sequences must be on one device")
+    turns = cos.shape
     for t in (cos, sin):
-        if t.dtype != torch.float32 or t.ndim != 2 or t.shape != cos.shape or t.shape[1] != d // 2 or not t.is_contiguous() or t.get_device() != index:
+        if t.dtype != torch.float32 or t.shape != turns or not t.is_contiguous() or t.get_device() != index or len(turns) != 2 or turns[1] != d // 2:
             raise ValueError("cache_append: cos and sin must be contiguous fp32 [positions, head_dim / 2] on the rows' device")
     for t in (q_weight, k_weight):
         if t is not None and (t.dtype != torch.bfloat16 or t.shape != (d,) or not t.is_contiguous() or t.get_device() != index):
@@ -781,15 +784,16 @@ def cache_append(qkv, pages, sequences, cos, sin, *, q_weight=None, k_weight=Non
     if positions is not None and (positions.dtype != torch.int32 or positions.shape != (rows,) or not positions.is_contiguous()
                                   or positions.get_device() != index):
         raise ValueError("cache_append: positions must be contiguous int32 [rows] on the rows' device")
-    if out is None:
+    given = out is not None
+    if not given:
         out = qkv.new_empty((rows, hq, d))
-    for t, count in ((out, hq), (k_out, hk)):
+    for t, count in ((out if given else None, hq), (k_out, hk)):
         if t is not None and (t.shape != (rows, count, d) or t.dtype != torch.bfloat16 or t.get_device() != index or t.stride(2) != 1
                               or (count > 1 and t.stride(1) != d)):
             raise ValueError("cache_append: outputs must be bf16 [rows, heads, head_dim] with contiguous heads on the rows' device")
     status = _lib.lib().pir2b_cache_append(
-        qkv.data_ptr(), row, head, rows, hq, _ptr(q_weight), _ptr(k_weight), eps, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-        _ptr(positions), pages.address, sequences.address, out.data_ptr(), out.stride(0) if rows > 1 else hq * d, _ptr(k_out),
+        qkv.data_ptr(), row, head, rows, hq, _ptr(q_weight), _ptr(k_weight), eps, cos.data_ptr(), sin.data_ptr(), turns[0],
+        _ptr(positions), pages.address, sequences.address, out.data_ptr(), out.stride(0) if given and rows > 1 else hq * d, _ptr(k_out),
         0 if k_out is None else k_out.stride(0) if rows > 1 else hk * d, _raw_stream(index),
     )
     if status:
