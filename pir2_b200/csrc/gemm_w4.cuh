@@ -13,6 +13,12 @@
 // of one group each, so a product step stays in a group, whose sums are scaled in
 // fp32.  The only other rounding is that of the output.
 //
+// Sums are kept at 2^-10 of themselves, which the same instruction gives the codes:
+// a group's are not scaled yet and may be 8 * 128 times the largest row value, which
+// must not overflow where the scale brings it back.  Powers of two change no bits of
+// ordinary sums; an addition below 2^-116 may lose half of 2^-139 (fp32's smallest
+// step, 2^10 times), a 64th of bf16's smallest number.
+//
 // What bounds it: the start of a launch and the latency of the loads where weights
 // are few (2048 -> 4096, one row: 2.9 us, the weights' bytes alone 0.7); the
 // instructions that bring codes into bf16 where they are many (2048 -> 151936, 4 rows:
@@ -39,11 +45,14 @@ struct W4Args {
   int pairs;                     // output channels may be stored two at a time
 };
 
-// Code kAt of each half of a word as a bf16 pair.
+// What brings a sum back.
+constexpr float kW4Up = 1024.f;
+
+// Code kAt of each half of a word as a bf16 pair, times 2^-10: (16 + u) 2^-10 - 24 2^-10.
 template <int kAt>
 __device__ __forceinline__ uint32_t w4_pair(uint32_t w, const Int4Masks &m) {
   const uint32_t t = kAt == 0 ? w << 3 : w >> (kAt == 0 ? 0 : 4 * kAt - 3);
-  return bf162_fma(masked_xor<0x41c041c0u>(t, m.mantissa), 0x3f803f80u, 0xc1c0c1c0u);
+  return bf162_fma(masked_xor<0x41c041c0u>(t, m.mantissa), 0x3a803a80u, 0xbcc0bcc0u);
 }
 
 // Eight values of x in the order in which w4_pair brings the codes.
@@ -188,9 +197,8 @@ __global__ void __launch_bounds__(kWarps * 32) gemm_w4_kernel(const W4Args a) {
 #pragma unroll
       for (int x = 0; x < kWarps; ++x)              // in order of K
         sum += red[(x * kCols + token) * kRow + c];
-      if (a.bias != nullptr)
-        sum += __bfloat162float(a.bias[channel]);
-      a.out[token * a.ldo + channel] = __float2bfloat16_rn(sum);
+      const float bias = a.bias != nullptr ? __bfloat162float(a.bias[channel]) : 0.f;
+      a.out[token * a.ldo + channel] = __float2bfloat16_rn(fmaf(sum, kW4Up, bias));
     }
     if (block + gridDim.x < blocks)
       __syncthreads();
@@ -372,8 +380,7 @@ __global__ void __launch_bounds__(W4Staged::kWarps * 32, 1) gemm_w4_staged_kerne
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float b = h ? b1 : b0;              // token g, channels 2 q4 and 2 q4 + 1 of the half
-          const uint32_t y = transpose_8x8(
-              pack_bf16x2(acc[2 * h] + b, acc[2 * h + 1] + b));
+          const uint32_t y = transpose_8x8(pack_bf16x2(fmaf(acc[2 * h], kW4Up, b), fmaf(acc[2 * h + 1], kW4Up, b)));
           const int c = c0 + h * 8 + 2 * q4;
           uint16_t *out = reinterpret_cast<uint16_t *>(a.out + g * a.ldo + c);
           const bool one = g < a.m && c < a.n, two = g < a.m && c + 1 < a.n;
@@ -400,9 +407,8 @@ __global__ void __launch_bounds__(W4Staged::kWarps * 32, 1) gemm_w4_staged_kerne
       float sum = 0.f;
       for (int x = 0; x < wk; ++x)                  // in order of K
         sum += red[((of * wk + x) * kCols + token) * Shape::kRedRow + c];
-      if (a.bias != nullptr)
-        sum += __bfloat162float(a.bias[channel]);
-      a.out[token * a.ldo + channel] = __float2bfloat16_rn(sum);
+      const float bias = a.bias != nullptr ? __bfloat162float(a.bias[channel]) : 0.f;
+      a.out[token * a.ldo + channel] = __float2bfloat16_rn(fmaf(sum, kW4Up, bias));
     }
     __syncthreads();
   }
@@ -586,9 +592,8 @@ __global__ void __launch_bounds__(W4Wide<kTiles>::kWarps * 32, 1) gemm_w4_wide_k
       float sum = 0.f;
       for (int x = 0; x < wk; ++x)                  // in order of K
         sum += red[((of * wk + x) * kCols + token) * Shape::kRedRow + c];
-      if (a.bias != nullptr)
-        sum += __bfloat162float(a.bias[channel]);
-      a.out[token * a.ldo + channel] = __float2bfloat16_rn(sum);
+      const float bias = a.bias != nullptr ? __bfloat162float(a.bias[channel]) : 0.f;
+      a.out[token * a.ldo + channel] = __float2bfloat16_rn(fmaf(sum, kW4Up, bias));
     }
     __syncthreads();
   }
