@@ -103,6 +103,12 @@ class _Routes:
     def _by_thread(mine, plain):
         return lambda *args, **kwargs: mine.get(threading.get_ident(), plain)(*args, **kwargs)
 
+    def installed(self, module):
+        """The module's own instance attribute, whichever runs there are."""
+        with self.lock:
+            routed = self.modules.get(id(module))
+            return module.__dict__.get("forward") if routed is None else routed[0]
+
     @contextmanager
     def routed(self, modules, forwards):
         """In this thread, and within the block, module i's forward is
@@ -143,10 +149,12 @@ class PackedTextDecoder:
     `append`: norm, rotation and cache write of a layer are one launch
     (`ops.cache_append`), in fp32 with one rounding, where the layers' own
     arithmetic rounds each step to bf16: results differ in the last bits.
-    `weight_only` (weight_only.TextProjections): the projections, SwiGLU and
-    output layer of calls with few rows, in 4-bit weights.  While anything is
-    installed in a layer's projections, norms or the layer itself (quantised
-    projections, fusions), its layers run as installed."""
+    `weight_only` (weight_only.TextProjections, packed from this backbone): the
+    projections, SwiGLU and output layer of calls with few rows, in 4-bit weights.
+    While anything is installed in a layer's projections, MLP, norms or the layer
+    itself (quantised projections, fusions, hooks), or their weights are not those
+    that were packed, all layers and the output layer run as they are; the output
+    layer alone does while the embeddings are not those that were packed."""
 
     def __init__(self, backbone, cache, *, controller=None, bits=None, append=False, weight_only=None):
         self.backbone, self.cache, self.controller = backbone, cache, controller
@@ -167,16 +175,18 @@ class PackedTextDecoder:
                         self.groups[precision, id(attn)] = group
         if weight_only is not None and len(weight_only.qkv) != len(self.attentions):
             raise ValueError("weight_only must have the backbone's layers")
+        if weight_only is not None and any(a is not b for a, b in zip(weight_only.layers, backbone.layers)):
+            raise ValueError("weight_only must be packed from the backbone's layers")
         self.rope = self.turns = None
 
     def _narrow(self, rows):
         """Whether the 4-bit projections take a call of so many rows."""
-        if self.weight_only is None or rows > self.weight_only.rows:
+        if self.weight_only is None or rows > self.weight_only.rows or not self.weight_only.holds(self.backbone):
             return False
-        return not any("forward" in module.__dict__ for layer in self.backbone.layers for module in (
-            layer, layer.input_layernorm, layer.post_attention_layernorm, layer.self_attn.q_proj, layer.self_attn.k_proj,
-            layer.self_attn.v_proj, layer.self_attn.o_proj, layer.mlp.gate_proj, layer.mlp.up_proj, layer.mlp.down_proj,
-        ))
+        return not any(
+            "forward" in module.__dict__ for layer in self.backbone.layers
+            for module in (layer, layer.input_layernorm, layer.post_attention_layernorm)
+        ) and all(_ROUTES.installed(layer.mlp) is None for layer in self.backbone.layers)
 
     def _project(self, attn, x):
         mode = None if self.controller is None else self.controller.mode
@@ -234,17 +244,20 @@ class PackedTextDecoder:
         sequence after the other, new[b] of them for sequence b.  Returns the
         last layer's [rows, hidden].  Where a layer raises, the cache is as it
         was before the call."""
+        return self._run(hidden, new, self._narrow(hidden.shape[0]))
+
+    def _run(self, hidden, new, narrow):
         if hidden.ndim != 2 or hidden.shape[0] != sum(new):
             raise ValueError("run: hidden must hold the new tokens' rows")
         past = list(self.cache.tokens)
         try:
             self.cache.extend(new)
-            return self._layers(hidden, past, new) if hidden.shape[0] else hidden
+            return self._layers(hidden, past, new, narrow) if hidden.shape[0] else hidden
         except BaseException:
             self.cache.rewind(past)      # rows that no layer may have written
             raise
 
-    def _layers(self, hidden, past, new):
+    def _layers(self, hidden, past, new, narrow):
         prompts = all(p == 0 for p, n in zip(past, new) if n)   # every sequence of the batch starts with this call
         if self.append:
             cos = sin = None                                     # positions are looked up on the device
@@ -252,7 +265,6 @@ class PackedTextDecoder:
         else:
             positions = [p + i for p, n in zip(past, new) for i in range(n)]
             cos, sin = self._rope(positions, hidden.device, hidden.dtype)
-        narrow = self._narrow(hidden.shape[0])
         modules = list(self.attentions)
         forwards = [partial(self._attend, index, prompts, narrow) for index in range(len(self.attentions))]
         if narrow:
@@ -272,9 +284,10 @@ class PackedTextDecoder:
         embed = self.backbone.embed_tokens.weight
         tokens = []
         for _ in range(steps):
-            narrow = self.weight_only is not None and last_hidden.shape[0] <= self.weight_only.rows
-            logits = self.weight_only.vocabulary(last_hidden) if narrow else last_hidden @ embed.T
+            narrow = self._narrow(last_hidden.shape[0])      # of the whole step
+            packed = narrow and self.weight_only.holds_vocabulary(self.backbone)
+            logits = self.weight_only.vocabulary(last_hidden) if packed else last_hidden @ embed.T
             ids = logits.argmax(-1)
             tokens.append(ids)
-            last_hidden = self.run(embed[ids], [1] * self.cache.batch)
+            last_hidden = self._run(embed[ids], [1] * self.cache.batch, narrow)
         return torch.stack(tokens, dim=1)

@@ -8,6 +8,8 @@ so here the weights alone are narrow, with a bf16 scale for every group of 32, 6
 or 128 of a channel's weights.
 """
 
+from functools import partial
+
 import torch
 import torch.nn.functional as F
 
@@ -66,17 +68,30 @@ class WeightOnlyLinear(torch.nn.Module):
         return ops.gemm_w4a16(rows, self.packed_weight, self.weight_scale, self.bias).view(*x.shape[:-1], self.out_features)
 
 
+def _mark(tensor):
+    """What changes when a tensor's memory is replaced or written to.  (Inference
+    tensors count no versions.)"""
+    return None if tensor is None else (tensor.data_ptr(), None if tensor.is_inference() else tensor._version)
+
+
 class TextProjections:
     """A text backbone's projections in 4 bits, beside its own, for decoding:
     q|k|v and gate|up of a layer merged, o and down, and the output layer over the
     input embeddings.  `PackedTextDecoder` takes them where a call has at most
-    `rows` new rows; longer ones (prompts, camera views) keep the layers' own."""
+    `rows` new rows; longer ones (prompts, camera views) keep the layers' own.
+
+    They stand for the weights at the time of packing.  A backbone whose Linears or
+    weights are others since (`holds`), or whose embeddings are
+    (`holds_vocabulary`), runs its own until it is packed again.  Weights that
+    are written to through `.data` or as inference tensors do not show it."""
 
     def __init__(self, backbone, *, group=128, rows=64):
         def of(*linears):
             return WeightOnlyLinear.from_linear(*linears, group=group)
 
         self.rows = rows
+        self.layers = list(backbone.layers)
+        self.sources = []       # (owner, name, module, its class, [(how to get a weight or bias, it, its mark)])
         self.qkv, self.o, self.gate_up, self.down = [], [], [], []
         for layer in backbone.layers:
             attn, mlp = layer.self_attn, layer.mlp
@@ -86,7 +101,40 @@ class TextProjections:
             self.o.append(of(attn.o_proj))
             self.gate_up.append(of(mlp.gate_proj, mlp.up_proj))
             self.down.append(of(mlp.down_proj))
-        self.vocabulary = WeightOnlyLinear(*quantize_groups(backbone.embed_tokens.weight, group))
+            self.sources += [(layer, name, module, type(module), None) for name, module in (("self_attn", attn), ("mlp", mlp))]
+            for owner, name in [(attn, part + "_proj") for part in "qkvo"] + [(mlp, name) for name, _ in mlp.named_children()]:
+                module = getattr(owner, name)
+                held = []
+                for part in ("weight", "bias"):
+                    tensor = getattr(module, part, None)
+                    get = partial(module._parameters.get if tensor is module._parameters.get(part) else partial(getattr, module), part, None)
+                    held.append((get, tensor, _mark(tensor)))
+                self.sources.append((owner, name, module, type(module), held))
+        self.embedding = backbone.embed_tokens.weight
+        self.vocabulary = WeightOnlyLinear(*quantize_groups(self.embedding, group))
+        self.embedding_mark = _mark(self.embedding)
+
+    def holds(self, backbone):
+        """Whether the backbone's projections are those that were packed, with
+        nothing installed in them."""
+        if len(backbone.layers) != len(self.layers) or any(a is not b for a, b in zip(backbone.layers, self.layers)):
+            return False
+        for owner, name, module, kind, held in self.sources:
+            if owner._modules.get(name) is not module or type(module) is not kind:
+                return False
+            if held is None:    # self_attn, mlp: their hooks run, their own forwards are the caller's matter
+                continue
+            if "forward" in module.__dict__ or module._forward_hooks or module._forward_pre_hooks:
+                return False
+            for get, was, mark in held:
+                if get() is not was or (was is not None and _mark(was) != mark):
+                    return False
+        return True
+
+    def holds_vocabulary(self, backbone):
+        """The same of the embeddings."""
+        weight = backbone.embed_tokens.weight
+        return weight is self.embedding and _mark(weight) == self.embedding_mark
 
     def feed(self, index, x):
         """Layer `index`'s SwiGLU."""
