@@ -29,7 +29,7 @@ def quantize_groups(weight, group):
         raise ValueError("Weights must be finite")
     w = w.unflatten(1, (-1, group))
     most = w.abs().amax(-1)
-    scales = (most / 7).to(torch.bfloat16)
+    scales = (most / torch.full_like(most, 7)).to(torch.bfloat16)   # by a number: a product with its reciprocal
     scales = torch.where(scales == 0, torch.ones_like(scales), scales)
     codes = torch.round(w / scales.float()[..., None]).clamp(-7, 7).flatten(1).to(torch.int8)
     u = codes.view(torch.uint8) & 15
