@@ -266,12 +266,14 @@ static bool by_length(const RaggedArgs &a, int64_t grid, int resident, int parts
 template <int kFormat, int D, int kNT>
 static int launch_attention_few(const FewPlan &p, RaggedArgs a, void *stream) {
   a.ordered = by_length(a, p.grid, FewShape<kFormat, D, kNT>::kCtas, std::max(p.cluster, 1));
-  constexpr int kBytes = kFormat == kCacheBf16 ? 2 : 1, kWide = code_bytes(kFormat, D) / kBytes;
-  CUtensorMap tm_k, tm_v;
-  if (int r = make_pages_map(&tm_k, a.c.k, a.c, kWide, a.c.k_page, kBytes, 16, kWide > 32))
-    return r;
-  if (int r = make_pages_map(&tm_v, a.c.v, a.c, kWide, a.c.v_page, kBytes, 16, kWide > 32))
-    return r;
+  CUtensorMap tm_k = {}, tm_v = {};
+  if constexpr (kFormat != kCacheInt4) {            // int4 pages are copied without maps
+    constexpr int kBytes = kFormat == kCacheBf16 ? 2 : 1;
+    if (int r = make_pages_map(&tm_k, a.c.k, a.c, D, a.c.k_page, kBytes, 16, true))
+      return r;
+    if (int r = make_pages_map(&tm_v, a.c.v, a.c, D, a.c.v_page, kBytes, 16, true))
+      return r;
+  }
   return launch_cache("cache_attention launch", attention_few_kernel<kFormat, D, kNT>, p.grid, 1, std::max(p.cluster, 1), kFewWarps * 32,
                       FewShape<kFormat, D, kNT>::kSmem, stream, a, tm_k, tm_v);
 }
