@@ -17,6 +17,20 @@ from . import ops
 
 GROUPS = (32, 64, 128)
 
+# Rows up to which a backbone's 4-bit projections take its calls.  Graph replays on
+# one B200, us, the layers' own bf16 Linears (q|k|v three, gate|up two of them)
+# against the 4-bit ones in groups of 128:
+#   rows                         1            8            16           32           48           64
+#   q|k|v     2048 -> 4096       23.1  3.2    20.4  3.7    19.1  5.5    17.6  7.2    16.3 10.3    16.3 10.9
+#   o         2048 -> 2048       8.4   2.1    7.1   2.3    5.6   3.4    5.6   4.5    5.7   6.5    5.7   7.5
+#   gate|up   2048 -> 12288      13.9  7.0    13.6  7.4    14.7 10.0    15.1 13.0    14.7 23.7    14.1 25.5
+#   down      6144 -> 2048       16.8  4.1    16.1  4.8    10.4  6.4    10.4 10.0    10.4 15.4    10.6 18.4
+#   output    2048 -> 151936     101  35      103  35      105  70      106 101      105 203      106 221
+# (In groups of 32 down takes 12.9 at 32 rows and the output layer 106.)  The device
+# is busy for 1.91 ms a token of 16 such layers in bf16 and 1.14 in 4 bits for one
+# sequence, 2.13 and 1.96 for 32, 2.16 and 2.59 for 64.
+NARROW_ROWS = 32
+
 
 def quantize_groups(weight, group):
     """(packed uint8 [n, k / 2], scales bf16 [n, k / group]) of weights [n, k]:
@@ -85,7 +99,7 @@ class TextProjections:
     (`holds_vocabulary`), runs its own until it is packed again.  Weights that
     are written to through `.data` or as inference tensors do not show it."""
 
-    def __init__(self, backbone, *, group=128, rows=64):
+    def __init__(self, backbone, *, group=128, rows=NARROW_ROWS):
         def of(*linears):
             return WeightOnlyLinear.from_linear(*linears, group=group)
 

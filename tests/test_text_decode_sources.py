@@ -197,3 +197,10 @@ def test_rows_that_are_not_one_per_sequence(made, narrow):
     projections.rows = 8 if narrow else 0
     with pytest.raises(ValueError, match="rows"):
         decoder.decode(torch.randn(1, 128), 1)
+
+
+def test_rows_at_which_4_bit_weights_stop_by_themselves(made):
+    """Above these the layers' own Linears are faster, and exact."""
+    backbone, _, _ = made
+    decoder = PackedTextDecoder(backbone, Cache(2), weight_only=weight_only.TextProjections(backbone))
+    assert decoder._narrow(32) and not decoder._narrow(33)
