@@ -442,8 +442,10 @@ int64_t pir2b_gemm_w4a16_workspace(int64_t m, int64_t n, int64_t k, int group);
  * scale per token and head; value = code * factor * scale.  With m the row's
  * largest finite magnitude: s = 2^(floor(log2 m) - 10), at least 2^-126, 1 for a
  * row of zeros; factor = E4M3(m_group / s / 7); code = v / s / factor rounded to
- * nearest even and clamped, 0 where the factor is 0.  An infinity counts as m; a
- * row with a NaN gets codes and factors of 0 and a NaN scale. */
+ * nearest even and clamped, 0 where the factor is 0.  An infinity counts as m, so
+ * a row of infinities and zeros alone holds zeros (int8 and E4M3: the largest code
+ * under a scale of 1); a row with a NaN gets codes and factors of 0 and a NaN
+ * scale. */
 #define PIR2B_CACHE_BF16 16
 #define PIR2B_CACHE_INT8 8
 #define PIR2B_CACHE_E4M3 9

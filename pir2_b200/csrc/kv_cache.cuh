@@ -20,8 +20,9 @@
 // f rounded to nearest even and clamped, 0 where f is 0.  s is a power of two
 // so that the quotients are those of numbers of 8 and of 4 bits, which lie on a
 // border of the rounding or far from it: any exact division gives these codes.
-// m / s is below 2048, so f is below 304.  An infinity counts as m; a row with
-// a NaN gets codes and factors of 0 and the NaN as its scale.
+// m / s is below 2048, so f is below 304.  An infinity counts as m (as 0 where
+// no other value but zeros is finite); a row with a NaN gets codes and factors of 0
+// and the NaN as its scale.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
