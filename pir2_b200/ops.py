@@ -1,6 +1,7 @@
 """Torch-facing wrappers of the C ABI: allocate outputs, validate, launch.
 
-Every function runs on the current CUDA stream of the input's device, never
+Every function runs on the current CUDA stream of the input's device, which has
+to be the current device (others are refused: kernels are launched there), never
 synchronizes and allocates only through torch's caching allocator, so all of
 them can be captured in CUDA graphs (after the library has been loaded once).
 Errors from the library are raised as ValueError (argument/alignment) or
@@ -33,7 +34,16 @@ def _ptr(t):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index)
+
+
+def _raw_stream(index):
+    """The current stream of device `index` as the library takes it.  The library
+    launches on the current device: with another device's default stream, which
+    has the same handle, its kernels would run there on memory of this one."""
+    if torch._C._cuda_getDevice() != index:
+        raise ValueError(f"tensors are on cuda:{index}, which is not the current device (torch.cuda.device makes it that)")
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _rows(x):
@@ -671,11 +681,6 @@ def attention_rows(q, k, v, *, batch, heads, head_dim, scale=None, out=None):
     )
     _lib.check(status, "pir2b_attention_rows")
     return out
-
-
-def _raw_stream(index):
-    """The current stream of device `index` as the library takes it."""
-    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _head_rows(x, what):
