@@ -15,10 +15,16 @@ static std::atomic<int> g_w4_mode{0};
 // Whether the rows are kept in shared memory (the staged kernel up to eight, the
 // wide one above) while weights stream past them.  That costs a start, which many
 // channels pay back; more than eight rows pay a launch more as well.  Graph replays,
-// us, the direct kernel against the one that keeps rows, in groups of 128 (32):
-//    8 rows  4096 x 2048 3.7 (4.9) 4.9 (5.2)   2048 x 6144 5.0 (6.8) 7.8 (6.8)
-//            6144 x 1536 5.2 (6.0) 5.1 (5.3)   12288 x 2048 8.4 (12.0) 7.7 (8.3)
-//            151936 x 2048 68 (119) 36 (41)
+// us, the direct kernel against the one that keeps rows, in groups of 128 (32), channels
+// x K:
+//    1 row   6144 x 1024 3.6 (4.0) 3.4 (3.7)   6144 x 2048 4.5 (7.3) 4.7 (5.2)
+//            4096 x 2048 3.2 (4.3) 4.0 (4.3)   12288 x 2048 7.1 (10.8) 7.0 (7.7)
+//            4096 x 4096 5.9 (8.1) 5.6 (6.2)   4096 x 6144 7.4 (11.3) 6.9 (7.4)
+//            2048 x 6144 4.1 (6.1) 5.1 (5.4)   8192 x 4096 10.2 (14.4) 8.0 (8.7)
+//    8 rows  4096 x 2048 3.7 (4.8) 4.2 (4.6)   2048 x 6144 4.8 (6.6) 6.7 (6.4)
+//            6144 x 1536 5.1 (5.9) 4.5 (4.8)   12288 x 2048 8.4 (12.0) 7.3 (8.0)
+//            4096 x 4096 6.7 (8.9) 6.4 (6.5)   4096 x 6144 8.8 (12.6) 8.6 (8.5)
+//            151936 x 2048 69 (121) 36 (40)
 //   16       4096 x 1024 3.6 4.7               4096 x 2048 6.2 (6.0) 5.5 (5.8)
 //   32       2048 x 6144 10.2 (13.1) 12.8 (13.3)   4096 x 1024 4.7 5.8
 //            4096 x 2048 7.5 (11.7) 7.1 (7.8)  6144 x 1024 7.8 6.5
@@ -28,7 +34,7 @@ static bool w4_keeps_rows(int64_t m, int64_t n, int64_t k) {
   if (mode == 1 || k % 256 != 0)
     return false;
   if (m <= 8)
-    return W4Staged::bytes(k) <= kW4Smem && (mode == 2 || n >= 6144);
+    return W4Staged::bytes(k) <= kW4Smem && (mode == 2 || n >= 6144 || (n >= 4096 && k >= 4096));
   return mode == 2 || (n >= 4096 && n * k >= (int64_t(6) << 20));
 }
 
