@@ -37,13 +37,18 @@ def _stream(device):
     return _raw_stream(device.index)
 
 
+# Bound once: a call of a few microseconds asks both.
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _raw_stream(index):
     """The current stream of device `index` as the library takes it.  The library
     launches on the current device: with another device's default stream, which
     has the same handle, its kernels would run there on memory of this one."""
-    if torch._C._cuda_getDevice() != index:
+    if _current_device() != index:
         raise ValueError(f"tensors are on cuda:{index}, which is not the current device (torch.cuda.device makes it that)")
-    return torch._C._cuda_getCurrentRawStream(index)
+    return _current_raw_stream(index)
 
 
 def _rows(x):
