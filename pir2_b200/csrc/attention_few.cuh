@@ -16,15 +16,21 @@
 // its range) exactly in registers; the scales multiply scores and weights in
 // fp32.  P is transposed between the products by movmatrix.  The running maximum of a row
 // moves only when a score passes it by more than 8 (in log2), so that most
-// steps have one vote and no rescaling; sums and maxima are fp32.
+// steps have one vote and no rescaling; sums and maxima are fp32.  The weights, times
+// V's scales, are rounded to bf16 for their product (error against 64 bits 0.0018 to
+// 0.0023 of the result, with weights in fp32 0.0017, bf16's own rounding): a second
+// product for what the rounding leaves would double V's MMAs.
 //
 // What bounds it, one new token per sequence, 16 query and 8 kv heads of 128,
 // replayed from a graph (called in a loop): bf16 over four histories of
 // 29000-32700, 85 us (87), 6150 GB/s, 94 % of a copy's rate.  int8 over 64
 // histories of 500-4000, 62 us (65), 4710 GB/s: instructions, a third of them the
 // conversion of codes, which no warp-level MMA takes beside 16-bit weights.  int4
-// over the same, 47 us (48), 23 of them bytes: instructions, 391 per 16 keys.  Its
-// steps are of 32 keys, whose six small pieces all lanes copy by 16 bytes (copies of
+// over the same, 47 us (48), 23 of them bytes: 391 instructions per 16 keys and a
+// quarter as many at starts and ends issue in 54 % of the cycles; for 14 % of the time
+// an SM has no CTA yet or none any more; in the rest its 15 warps all wait, for a busy
+// math pipe or its dispatch (24 % of a warp's time), for the result before (17 %), at
+// barriers and for loads (6 % each).  Its steps are of 32 keys, whose six small pieces all lanes copy by 16 bytes (copies of
 // one lane in bulk: 67 us), with the hidden positions' steps apart; q's fragments
 // are read from shared memory, for which four CTAs of 128 registers stay on an SM
 // (three, with q in registers: four histories of 29000-32700 42 us for 45, the 64
@@ -1016,11 +1022,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewShape<kFormat, D, kNT>::kCt
   }
 
   // No copy is in flight past this point (at once, unless a wait gave up).
-  if constexpr (kInt4)
+  if constexpr (kInt4) {
     cp_async_wait_group<0>();
-  else
-  for (int i = done; i < min(done + kStages, count); ++i)
-    mbar_wait(&full[i % kStages], uint32_t((i / kStages) & 1), kStatusTimeoutProducer);
+  } else {
+    for (int i = done; i < min(done + kStages, count); ++i)
+      mbar_wait(&full[i % kStages], uint32_t((i / kStages) & 1), kStatusTimeoutProducer);
+  }
   __syncthreads();
   // The warps' partial sums, added in warp order.
   float *so = reinterpret_cast<float *>(few_sm);                // [warps][rows][D + 4]

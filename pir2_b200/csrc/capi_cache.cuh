@@ -161,7 +161,12 @@ static int launch_rows(bool write, int format, int d, const CacheRowsArgs &a, vo
   }
 }
 
-// Few tokens are spread over more warps, as in launch_rows.
+// Few tokens are spread over more warps, as in launch_rows: each pass then looks up
+// its token and angles for itself.  Spread against not, us, 16 query and 8 kv heads of
+// 128 (8 passes): one token to int4 2.6 6.2, bf16 2.3 4.5; 512 int4 5.2 6.8, int8 5.1
+// 6.3, bf16 4.7 4.9; 768 6.8 7.4, 6.5 6.9, 5.9 5.7; 1024 7.7 7.5, 7.5 7.0, 6.8 5.8;
+// 4096 24.9 19.4, 24.2 17.8, 21.9 16.6.  12 and 4 of 64 (4 passes): 1024 int4 5.0 5.1,
+// bf16 4.5 4.2; 2048 7.5 7.3, 6.5 5.6.
 template <int kFormat, int D>
 static int launch_append(const CacheAppendArgs &a, void *stream) {
   constexpr int kRows = 32 / (D / 16);
@@ -181,7 +186,8 @@ static int launch_append(int d, const CacheAppendArgs &a, void *stream) {
 // reads the keys once per 16 rows, the tile kernel once per 128 or 256.  Over
 // 1000 tokens of 64 sequences: 16 rows 50 us against 55 (bf16) and 50 against
 // 110 (int8, whose tiles are converted first), 24 rows 80 against 56 and 84
-// against 111, 34 rows 115 against 55 and 125 against 110.
+// against 111, 34 rows 115 against 55 and 125 against 110.  int4: 16 rows 39 against
+// 108, 32 74 against 107, 34 103 against 108, 64 129 against 107.
 constexpr int kFewRowsBf16 = 16, kFewRows8Bit = 32;
 
 // How the few-row kernel covers a call: a cluster of CTAs per unit of rows,
@@ -196,6 +202,7 @@ struct FewPlan {
   int64_t bytes(int hk, int d) const { return cluster ? 0 : grid * 8 * nt * (d * 4 + 8) + slots * hk * 8; }
 };
 
+// (Lengths are counted in steps of 16 keys in every format; a step of int4 is 32.)
 static FewPlan plan_few(int64_t rows, int hq, int hk, int batch, int64_t positions, int format, int d, int sms) {
   FewPlan p = {};
   const int group = hq / hk;
@@ -212,12 +219,18 @@ static FewPlan plan_few(int64_t rows, int hq, int hk, int batch, int64_t positio
   // cluster against pieces, one token: one int8 sequence of 2000 8.8 us against
   // 10.2, of 8000 17.7 against 13.9, of 30000 50 against 22; two tokens in a group
   // of four, eight bf16 sequences: of 2000-4000 20.5 against 22.9, of 3000-6000
-  // 32.3 against 34.9.
+  // 32.3 against 34.9.  int4: one sequence of 578 6.9 against 9.3, of 2000 8.3 against
+  // 9.8, of 3000 9.1 against 10.2, of 4000 9.8 against 10.3, of 8000 13.2 against 12.5,
+  // of 30000 33 against 20; eight of 2000 12.0 against 13.8, of 4000 17.5 against 19.6,
+  // of 12000 36 either way.
   if (4 * units >= places || longest <= (8 * units > places ? 96 : 40)) {
     // One round of CTAs; a second only where each has 1280 keys or more (eight
     // bf16 sequences of 1000-2000 12.1 us with four to a unit, 18.2 with eight;
     // 64 int8 ones of 500-4000 62 with two, 74 with four; 64 of 2000-4000, group
-    // of four, 80 with two, 102 with one).
+    // of four, 80 with two, 102 with one; int4: eight of 1000-2000 13.0 with four,
+    // 11.4 with eight, 64 of 500-4000 51 with two, 66 with four, 69 with one, 64 of
+    // 2000-4000, group of four, 67 with two, 74 with one, 28 of 660-1320 18.5 with
+    // one, 18.4 with two, 23.5 with four).
     p.cluster = 1;
     while (p.cluster < 8 && 2 * p.cluster <= longest && p.cluster * units < places &&
            (2 * p.cluster * units <= places || positions >= 1280 * 2 * p.cluster))

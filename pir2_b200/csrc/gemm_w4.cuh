@@ -20,12 +20,15 @@
 // step, 2^10 times), a 64th of bf16's smallest number.
 //
 // What bounds it: the start of a launch and the latency of the loads where weights
-// are few (2048 -> 4096, one row: 2.9 us, the weights' bytes alone 0.7); the
-// instructions that bring codes into bf16 where they are many (2048 -> 151936, 4 rows:
-// 35.5 us, bytes 25, 4.6 TB/s); with more rows shared memory as well, from which every
-// 16 channels read all rows (32 rows of 2048 -> 151936: 99 us, of them 50 of shared
-// memory, 34 of MMAs at 8 cycles of a quarter SM each; of 2048 -> 12288 13.9, bytes
-// 2.3).
+// are few (2048 -> 4096, one row: 3.2 us, the weights' bytes alone 0.7); where they are
+// many, the pipes that bring codes into bf16 (2048 -> 151936, 4 rows: 35.5 us, bytes
+// 25, 4.6 TB/s; the schedulers issue in 63 % of the cycles, and of a warp's time 27 %
+// goes to a busy math pipe or its dispatch, 24 % to other warps' turns, 12 % to the
+// result before, 9 % to loads); with more rows shared memory as well, from which every
+// 16 channels read all rows (32 rows of 2048 -> 151936: 101 us, of them 50 of shared
+// memory, 34 of MMAs at 8 cycles of a quarter SM each), and the start and the meetings
+// (of 2048 -> 12288 in groups of 32: 14.1, bytes 2.3; 38 % of the cycles issue, 22 % of
+// a warp's time is at barriers, 20 % at loads).
 #pragma once
 #include "attention_few.cuh"
 
@@ -208,9 +211,9 @@ __global__ void __launch_bounds__(kWarps * 32) gemm_w4_kernel(const W4Args a) {
 // Up to eight rows and many channels: a persistent CTA keeps the rows in shared
 // memory, as the lanes take them, and streams the weights of its blocks of 16
 // channels through a ring per warp; `wk` warps split K, and their sums meet in
-// shared memory.  Two stages of two chunks a warp and as many warps as fit keep 111
-// KB in flight on an SM (2048 -> 151936, 4 rows: 16 warps 4 us longer, four stages
-// of one chunk 3).
+// shared memory.  One of a warp's two stages of two chunks is on its way while the
+// other is read: with as many warps as fit up to 55 KB on an SM (2048 -> 151936, 4
+// rows: 16 warps 4 us longer, four stages of one chunk 3).
 struct W4Staged {
   static constexpr int kWarps = 24;
   static constexpr int kCols = 8;
