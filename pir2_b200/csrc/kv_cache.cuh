@@ -466,54 +466,19 @@ __global__ void __launch_bounds__(kCacheWarps * 32) cache_write_kernel(const Cac
   if (page < 0)
     return;
   const int in_page = int(pos & ((1 << a.c.shift) - 1));
-  const int64_t k_at = page * a.c.k_page, v_at = page * a.c.v_page;
+  constexpr int kUnit = kFormat == kCacheBf16 ? 2 : 1;       // bytes that page strides count
+  const int64_t k_at = int64_t(kUnit) * page * a.c.k_page, v_at = int64_t(kUnit) * page * a.c.v_page;
   float *k_scale = a.c.ks + page * a.c.ks_page, *v_scale = a.c.vs + page * a.c.vs_page;
 #pragma unroll
   for (int i = 0; i < kFlight; ++i) {
     const int r = r0 + i * kRows, head = r < hk ? r : r - hk;
     const int slot = (head << a.c.shift) + in_page;          // below 2^17
-    const int64_t at = (r < hk ? k_at : v_at) + (slot * D + l * 8);
-    if constexpr (kFormat == kCacheBf16) {
-      if (r < 2 * hk) {
-        __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(r < hk ? a.c.k : a.c.v) + at;
-        *reinterpret_cast<uint4 *>(to) = x[i][0];
-        *reinterpret_cast<uint4 *>(to + kLanes * 8) = x[i][1];
-      }
-    } else if constexpr (kFormat == kCacheInt4) {
-      uint8_t *to = static_cast<uint8_t *>(r < hk ? a.c.k : a.c.v) + (r < hk ? k_at : v_at) + (slot * (D / 2) + l * 4);
-      uint8_t *factor = (r < hk ? a.c.kf + page * a.c.kf_page : a.c.vf + page * a.c.vf_page) + slot * (D / kFactorGroup) + l / 4;
-      keep_row<kFormat, D>(x[i][0], x[i][1], l, r < 2 * hk, to, factor, (r < hk ? k_scale : v_scale) + slot);
-    } else {
-      uint32_t m = max(magnitude8(x[i][0]), magnitude8(x[i][1]));
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1)
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const bool odd = __any_sync(0xffffffffu, m >= 0x7f80u);   // an infinity or a NaN in some row
-      if (odd) {
-        m = max(magnitude8_finite(x[i][0]), magnitude8_finite(x[i][1]));
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1)
-          m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      }
-      const float most = __uint_as_float(m << 16);
-      const float s = m == 0 ? 1.f : __fmul_rn(most, kFormat == kCacheInt8 ? 1.0f / 127.0f : 1.0f / 448.0f);
-      uint2 q[2];
-      if (!odd && s > 0x1p-80f && s < 0x1p100f) {
-        const float y = __frcp_rn(s);
-        q[0] = quantise8<kFormat>(x[i][0], s, y);
-        q[1] = quantise8<kFormat>(x[i][1], s, y);
-      } else {
-        q[0] = quantise8_any<kFormat>(x[i][0], s);
-        q[1] = quantise8_any<kFormat>(x[i][1], s);
-      }
-      if (r < 2 * hk) {
-        uint8_t *to = static_cast<uint8_t *>(r < hk ? a.c.k : a.c.v) + at;
-        *reinterpret_cast<uint2 *>(to) = q[0];
-        *reinterpret_cast<uint2 *>(to + kLanes * 8) = q[1];
-        if (l == 0)
-          (r < hk ? k_scale : v_scale)[slot] = s;
-      }
-    }
+    uint8_t *codes = static_cast<uint8_t *>(r < hk ? a.c.k : a.c.v) +
+                     ((r < hk ? k_at : v_at) + (slot * code_bytes(kFormat, D) + l * code_bytes(kFormat, 8)));
+    uint8_t *factor = nullptr;
+    if constexpr (kFormat == kCacheInt4)
+      factor = (r < hk ? a.c.kf + page * a.c.kf_page : a.c.vf + page * a.c.vf_page) + slot * (D / kFactorGroup) + l / 4;
+    keep_row<kFormat, D>(x[i][0], x[i][1], l, r < 2 * hk, codes, factor, (r < hk ? k_scale : v_scale) + slot);
   }
 }
 
